@@ -598,6 +598,56 @@ struct AttnOutArgs {          // second attention pass: global softmax and p.V p
   int C;                      // channels-last kernels (_nhwc): C (multiple of 8); unused otherwise
 };
 
+struct PagedAppendArgs {      // paged.hip: rotate q and k, write k and v into the pages of their sequences
+  const void* q;              // [N, H, D]; rows and heads strided (q_rs, q_hs elements), dims contiguous
+  const void* k;              // [N, KVH, D]
+  const void* v;
+  void* k_pages;              // row r of page p, head h: p * page_stride + h * head_stride + r * row_stride
+  void* v_pages;
+  void* q_out;                // [N, H, D]
+  const int* table;           // [B, M]
+  const int* q_start;         // [B + 1]
+  const int* kv_len;          // [B]
+  const float* inv_freq;      // [R / 2]
+  long long q_rs, q_hs, k_rs, k_hs, v_rs, v_hs;
+  long long page_stride, head_stride, row_stride;
+  long long pages;
+  int N, B, M, H, KVH, D, R, page_size;
+  float scaling;
+  int dtype;
+};
+
+struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over paged K and V
+  const void* q;              // [N, H, D]; rows and heads strided
+  const void* k_pages;
+  const void* v_pages;
+  void* out;                  // [N, H, D]
+  const int* table;           // [B, M]
+  const int* q_start;         // [B + 1]
+  const int* kv_len;          // [B]
+  long long q_rs, q_hs;
+  long long page_stride, head_stride, row_stride;
+  long long pages;
+  int N, B, M, H, KVH, D, page_size;
+  float scale;
+  int dtype;
+  int pad;
+};
+
+struct SampleArgs {           // sample.hip: one token per row of logits [rows, vocab]
+  const void* logits;
+  const float* temperature;   // [rows] each
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* u;
+  long long* out;             // [rows]
+  int rows;
+  int vocab;
+  int dtype;
+  int shift;                  // weights are integers of 2^-shift; vocab << shift < 2^63
+};
+
 // host and device (the rotary sincos below is also built into a host test helper)
 #ifdef __HIPCC__
 #define HS_HD __host__ __device__
@@ -621,12 +671,11 @@ HS_HD inline TilePos tile_order(unsigned lin, unsigned gx, unsigned gy, unsigned
   return TilePos{first + t3 % width, t3 / width, kz};
 }
 
-// sin and cos of an fp32 angle (|x| < 2^30), branch-free and table-free so that no load or
+// sin and cos of an angle (|x| < 2^31), branch-free and table-free so that no load or
 // wait enters the caller's critical path: Cody-Waite reduction by pi/2 in double (k*pi/2 with
 // a two-part pi/2), Taylor polynomials in double on |r| <= pi/4 (truncation error < 1e-17),
-// quadrant by selects, then one rounding to fp32.
-HS_HD inline void sincos_rot(float xf, float* s_out, float* c_out) {
-  const double x = (double)xf;
+// quadrant by selects, then one rounding to fp32. sincos_rot: of an fp32 angle.
+HS_HD inline void sincos_rot_d(double x, float* s_out, float* c_out) {
   const double q = __builtin_rint(x * 0.63661977236758134308);   // 2/pi
   double r = __builtin_fma(-q, 1.57079632679489655800e+00, x);     // pi/2, high part
   r = __builtin_fma(-q, 6.12323399573676603587e-17, r);             // pi/2, low part
@@ -654,6 +703,7 @@ HS_HD inline void sincos_rot(float xf, float* s_out, float* c_out) {
   *s_out = (float)((k & 2) ? -sv : sv);
   *c_out = (float)(((k + 1) & 2) ? -cv : cv);
 }
+HS_HD inline void sincos_rot(float xf, float* s_out, float* c_out) { sincos_rot_d((double)xf, s_out, c_out); }
 
 #ifdef __HIPCC__
 // ---------------------------------------------------------------- device helpers

@@ -400,6 +400,9 @@ size_t hs_argsize(const char* s) {
   HS_SZ(CombineArgs)
   HS_SZ(PersistArgs)
   HS_SZ(DecodeLayerPtrs)
+  HS_SZ(PagedAppendArgs)
+  HS_SZ(PagedAttnArgs)
+  HS_SZ(SampleArgs)
 #undef HS_SZ
   return 0;
 }

@@ -10,6 +10,7 @@ that node to the CPU instead of failing at compile time.
 from __future__ import annotations
 
 from hip_compiler.codegen import EW_OPS
+from hip_compiler.serving import LOWERINGS as SERVING
 
 _HIP_SUPPORTED_OPS: set[str] = {
     # GEMM-shaped
@@ -28,7 +29,7 @@ _HIP_SUPPORTED_OPS: set[str] = {
     "aten.alias.default", "aten.detach.default", "aten.detach_.default", "aten.dropout.default",
     "<built-in function getitem>", "aten.t.default", "aten.expand.default", "aten.slice.Tensor",
     "aten.select.int", "aten.transpose.int", "aten.permute.default", "aten._assert_tensor_metadata.default",
-} | set(EW_OPS)
+} | set(EW_OPS) | set(SERVING)
 
 
 def is_hip_op_supported(op_type: str, attrs: dict | None = None) -> bool:

@@ -32,6 +32,7 @@ from hip_compiler.codegen import MAX_CHAIN_INPUTS, VEC, ChainOp, generate_chain,
 from hip_compiler.op_classify import OpCategory, classify_op
 from hip_compiler.program import (DTYPE_CODE, ELEM_SIZE, FLOAT_DTYPES, LaunchStep, Ref, Storage, TView,
                                   contiguous_strides, numel)
+from hip_compiler.serving import LOWERINGS as SERVING
 from npu_compiler.ir_reader import IRGraph, OpNode
 
 HS_BF16, HS_F16 = DTYPE_CODE["bfloat16"], DTYPE_CODE["float16"]
@@ -1554,22 +1555,29 @@ class Lowering:
                 expect = t * s
         return st if st is not None else 0
 
+    def inplace_or_copy(self, self_t, out) -> TView:
+        """Where an op that updates part of ``self_t`` writes: the tensor itself when it is a whole graph input that
+        nothing else reads (a cache), else a copy of it."""
+        tv = self.view(self_t.name)
+        st = self.storages[tv.storage]
+        if (self.inplace_inputs and st.kind == "input" and len(self.consumers.get(self_t.name, [])) == 1
+                and tv.is_contiguous() and tv.offset == 0 and tv.numel * tv.itemsize == st.nbytes
+                and self_t.name not in self.graph_output_names):
+            self.flush_chains_reading(tv.storage)
+            self.mutated_inputs.add(tv.storage)
+            self.views[out.name] = tv
+            return tv
+        dst = self.new_storage(out.name, out.shape, out.dtype)
+        self.emit_copy(tv, dst, [self_t.name], [out.name])
+        self.views[out.name] = dst
+        return dst
+
     def lower_index_copy(self, node: OpNode) -> None:
         self_t, idx_t, src_t = node.inputs[0], node.inputs[1], node.inputs[2]
         out = node.outputs[0]
         dim = int(node.attrs.get("dim", 0)) % len(self_t.shape)
-        tv = self.view(self_t.name)
-        st = self.storages[tv.storage]
-        inplace = (self.inplace_inputs and st.kind == "input" and len(self.consumers.get(self_t.name, [])) == 1
-                   and tv.is_contiguous() and tv.offset == 0 and tv.numel * tv.itemsize == st.nbytes
-                   and self_t.name not in self.graph_output_names)
-        if inplace:
-            self.flush_chains_reading(tv.storage)
-            dst = tv
-            self.mutated_inputs.add(tv.storage)
-        else:
-            dst = self.new_storage(out.name, out.shape, out.dtype)
-            self.emit_copy(tv, dst, [self_t.name], [out.name])
+        dst = self.inplace_or_copy(self_t, out)
+        tv, inplace = dst, dst.storage in self.mutated_inputs
         src = self.view(src_t.name)
         shape = list(tv.shape)
         outer = numel(shape[:dim])
@@ -1700,6 +1708,8 @@ class Lowering:
             "aten.adaptive_avg_pool2d.default": self.lower_adaptive_avg_pool2d,
         }
         fn = table.get(op)
+        if fn is None and op in SERVING:
+            return SERVING[op](self, node)
         if fn is None:
             raise NotImplementedError(f"HIP backend has no lowering for {op} (node {node.name})")
         fn(node)

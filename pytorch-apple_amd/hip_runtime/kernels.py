@@ -127,6 +127,17 @@ _struct("DecodeAttnArgs", [("q", P), ("k", P), ("v", P), ("mask", P), ("out", P)
                            ("S", LL), ("q_head_stride", LL), ("kv_head_stride", LL),
                            ("mask_stride", LL), ("H", I), ("KVH", I), ("D", I), ("ntiles", I), ("scale", F),
                            ("mask_dtype", I), ("add_dtype", I), ("dtype", I)])
+_struct("PagedAppendArgs", [("q", P), ("k", P), ("v", P), ("k_pages", P), ("v_pages", P), ("q_out", P), ("table", P),
+                            ("q_start", P), ("kv_len", P), ("inv_freq", P), ("q_rs", LL), ("q_hs", LL), ("k_rs", LL),
+                            ("k_hs", LL), ("v_rs", LL), ("v_hs", LL), ("page_stride", LL), ("head_stride", LL),
+                            ("row_stride", LL), ("pages", LL), ("N", I), ("B", I), ("M", I), ("H", I), ("KVH", I),
+                            ("D", I), ("R", I), ("page_size", I), ("scaling", F), ("dtype", I)])
+_struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), ("table", P), ("q_start", P),
+                          ("kv_len", P), ("q_rs", LL), ("q_hs", LL), ("page_stride", LL), ("head_stride", LL),
+                          ("row_stride", LL), ("pages", LL), ("N", I), ("B", I), ("M", I), ("H", I), ("KVH", I), ("D", I),
+                          ("page_size", I), ("scale", F), ("dtype", I), ("pad", I)])
+_struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
+                       ("rows", I), ("vocab", I), ("dtype", I), ("shift", I)])
 
 
 def check_layouts() -> dict[str, tuple[int, int]]:

@@ -80,7 +80,7 @@ class IRBuilder:
     def op(self, op_type: str, inputs: list[T], attrs: dict | None = None, n_out: int = 1,
            base: str | None = None, out_dtype: str | None = None):
         if base is None:
-            base = op_type.split(".")[1] if op_type.startswith("aten.") else op_type
+            base = op_type.split(".")[1] if op_type.startswith(("aten.", "serving.")) else op_type
             base = base.lstrip("_")
         name = self._fresh(base)
         outs = [{"name": name if n_out == 1 else f"{name}_out{i}", "shape": [], "dtype": out_dtype or "float32",

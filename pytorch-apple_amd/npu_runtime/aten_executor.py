@@ -16,6 +16,7 @@ from ``node.inputs`` in schema order and every other argument taken from
   ``"torch.float32"`` are mapped to ``torch.dtype``; device, layout and
   memory-format values are host-neutralised), falling back to the schema default,
   or, for a missing ``size``/``shape``, to the node's declared output shape;
+* ``serving.<op>.<overload>`` nodes (``npu_runtime.serving_ops``) run the same way, from ``torch.ops.serving``;
 * three non-ATen node kinds have fixed meanings: ``<built-in function getitem>``
   selects ``inputs[attrs.index]``; ``wrap_with_set_grad_enabled`` is the rotary
   embedding of HF ``Qwen2RotaryEmbedding.forward`` (fp32 ``inv_freq @ position``,
@@ -28,6 +29,8 @@ from __future__ import annotations
 from typing import Any
 
 import torch
+
+from npu_runtime import serving_ops  # noqa: F401  (defines torch.ops.serving)
 
 TORCH_DTYPES: dict[str, torch.dtype] = {
     "float32": torch.float32, "float": torch.float32, "float16": torch.float16, "half": torch.float16,
@@ -56,9 +59,9 @@ def resolve_aten(op_type: str):
     if op is not None:
         return op
     parts = op_type.split(".")
-    if len(parts) != 3 or parts[0] != "aten":
-        raise NotImplementedError(f"not an ATen op: {op_type}")
-    op = getattr(getattr(torch.ops.aten, parts[1]), parts[2])
+    if len(parts) != 3 or parts[0] not in ("aten", "serving"):
+        raise NotImplementedError(f"not an ATen or serving op: {op_type}")
+    op = getattr(getattr(getattr(torch.ops, parts[0]), parts[1]), parts[2])
     _OP_CACHE[op_type] = op
     return op
 
