@@ -628,9 +628,15 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   long long q_rs, q_hs;
   long long page_stride, head_stride, row_stride;
   long long pages;
+  float* part_o;              // split tiles: [slot][row of the tile][D] unnormalised outputs, 32-row tiles' slots first
+  float* part_ml;             // [slot][row of the tile][2] running maximum of the raw scores, sum of exponentials
   int N, B, M, H, KVH, D, page_size;
   float scale;
   int dtype;
+  int page_groups;            // page_size / 16
+  unsigned group_magic;       // ceil(2^32 / page_groups); 0 where page_groups is 1
+  int grid_wide;              // workgroups of the wide tiles (the first ones), the rest take narrow tiles
+  int narrow_slots;           // partial slots of narrow tiles
   int pad;
 };
 

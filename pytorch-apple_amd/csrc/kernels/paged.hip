@@ -120,3 +120,745 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
     if (i * 64 + lane < a.D)
       st_f(a.out, ((long long)row * a.H + h) * a.D + i * 64 + lane, a.dtype, l == 0.f ? 0.f : o[i] / l);
 }
+
+// ------------------------------------------------------------------ attention on matrix cores
+//
+// Types of 16 bits, head sizes 64 and 128, pages of a multiple of 16 positions. The G = H / KVH query heads of a K/V
+// head are packed with the tokens into rows (row = token * G + head), so K and V are read once for all of them. A
+// wave holds 32 rows: S^T = K Q^T on v_mfma_f32_32x32x16 leaves each lane the scores of ONE row, so maximum, exponentials
+// and the rescaling of that row's outputs stay in the lane (two lanes, 32 apart, share a row's positions), and
+// O^T += V^T P^T takes P as it lies. Two forms of a workgroup of four waves:
+//   * narrow tile, sequences of up to 32 rows (decoding, a few speculated tokens): the four waves hold the SAME rows
+//     and take every fourth block of positions, each streaming K and V through LDS of its own with no barrier: while a
+//     block's scores are taken the next K is on its way, while its outputs are, the next V. Bound by memory.
+//   * wide tile, longer chunks: 128 rows, each wave 32 of them, all sharing blocks of 64 positions staged one block
+//     ahead. Bound by the matrix cores and the softmax's vector instructions.
+// K and V go from the pages to LDS directly (a load covers 4 or 8 rows of one page), K swizzled for the fragment
+// reads, V for the transposing ones.
+//
+// Work is dealt out on the device: lengths are tensors, the launch is the same for every batch. Each workgroup sums the
+// sequences' tiles and blocks, splits tiles longer than an even share of all blocks, and takes items of the list that
+// follows. A split tile leaves unnormalised outputs with their maximum and sum; k_paged_combine_* joins them.
+// Wide items are dealt to the XCDs in ranges of equal cost, so the tiles that read the same blocks share an L2.
+
+#define PT_MAXB 1024             // sequences
+#define PT_NARROW 32             // rows
+#define PT_WIDE 128
+#define PT_NARROW_ITEMS 2048     // items that narrow tiles are split towards: several per CU, of uneven length
+#define PT_WIDE_ITEMS 480        // wide: one round of two workgroups per CU
+#define PT_NARROW_MIN 8          // fewest blocks of a split
+#define PT_WIDE_MIN 8
+
+typedef __attribute__((ext_vector_type(16))) float pt_f32x16;
+typedef __attribute__((ext_vector_type(4))) short pt_s16x4;
+
+template <int DT>
+__device__ __forceinline__ pt_f32x16 pt_mfma(const uint4 a, const uint4 b, pt_f32x16 c) {
+  if constexpr (DT == HS_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(__attribute__((ext_vector_type(8))) __bf16, a),
+                                                   __builtin_bit_cast(__attribute__((ext_vector_type(8))) __bf16, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(__attribute__((ext_vector_type(8))) _Float16, a),
+                                                  __builtin_bit_cast(__attribute__((ext_vector_type(8))) _Float16, b), c,
+                                                  0, 0, 0);
+}
+
+// lanes 32-63 of a and lanes 0-31 of b change places
+__device__ __forceinline__ void pt_swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+
+// Transposing LDS read: lanes 4r + c of each 16-lane group address row r, columns 4c .. 4c + 3 (8 bytes);
+// lane i gets column i of rows 0 .. 3.
+__device__ __forceinline__ uint2 pt_read_tr(const char* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) pt_s16x4*)(__attribute__((address_space(3))) char*)p));
+}
+
+// uniform load from memory that no kernel in flight writes
+__device__ __forceinline__ int pt_ldc(const int* p, long long i) {
+  return ((const __attribute__((address_space(4))) int*)p)[i];
+}
+
+// A sequence's share of the work: rows, tiles of R rows, blocks of PB positions that its last tile needs. Batches that
+// name rows outside the tensor have none.
+struct PtSeq {
+  int start, n, kv, tiles, blocks;
+};
+template <int R, int PB>
+__device__ __forceinline__ PtSeq pt_seq(const PagedAttnArgs& a, int b, int s0, int s1, int kv, int lo, int hi) {
+  PtSeq q{s0, s1 - s0, max(kv, -(1 << 30)), 0, 0};
+  const int G = a.H / a.KVH;
+  const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.N;
+  const long long rows = ok ? (long long)q.n * G : 0;
+  if (rows <= lo || rows > hi) {
+    q.n = 0;
+    return q;
+  }
+  q.tiles = (int)((rows + R - 1) / R);
+  const long long end = min((long long)max(kv, 0), (long long)a.M * a.page_size);
+  q.blocks = (int)((end + PB - 1) / PB);
+  return q;
+}
+
+// The list of items of one form of tile, in LDS: for each sequence the items, split slots and cost (JOIN: rows and
+// heads of split tiles) up to and with it.
+struct PtList {
+  int items[PT_MAXB];
+  int slots[PT_MAXB];
+  int cost[PT_MAXB];
+  int red[3][4];
+  int share;   // blocks per split
+};
+
+// inclusive scans of three values over 256 threads, added to the running totals
+__device__ __forceinline__ void pt_scan3(int (&v)[3], int (&total)[3], int (&red)[3][4]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int w = __shfl_up(v[j], o, 64);
+      if (lane >= o) v[j] += w;
+    }
+  __syncthreads();
+  if (lane == 63)
+#pragma unroll
+    for (int j = 0; j < 3; ++j) red[j][wave] = v[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    int base = total[j], all = total[j];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      base += w < wave ? red[j][w] : 0;
+      all += red[j][w];
+    }
+    v[j] += base;
+    total[j] = all;
+  }
+}
+
+// splits of a sequence's tiles
+__device__ __forceinline__ int pt_splits(const PtSeq& q, int share) { return max(1, (q.blocks + share - 1) / share); }
+
+// Builds the list (by 256 threads; ends with a barrier) and returns the number of items. lo < rows <= hi.
+template <int R, int PB, int ITEMS, int LEAST, bool JOIN = false>
+__device__ __forceinline__ int pt_build(const PagedAttnArgs& a, PtList& t, int lo, int hi, int* cost) {
+  const int tid = threadIdx.x;
+  int work[3] = {0, 0, 0};   // blocks of all tiles, in units of 256 and the rest
+  for (int b = tid; b < a.B; b += 256) {
+    const PtSeq q = pt_seq<R, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], lo, hi);
+    const long long w = (long long)q.tiles * q.blocks * a.KVH;
+    work[0] += (int)(w >> 8);
+    work[1] += (int)(w & 255);
+  }
+  int total[3] = {0, 0, 0};
+  pt_scan3(work, total, t.red);
+  const long long all = ((long long)total[0] << 8) + total[1];
+  const int share = (int)max((all + ITEMS - 1) / ITEMS, (long long)LEAST);
+  total[0] = total[1] = total[2] = 0;
+  for (int c = 0; c < a.B; c += 256) {
+    const int b = c + tid;
+    int v[3] = {0, 0, 0};
+    if (b < a.B) {
+      const PtSeq q = pt_seq<R, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], lo, hi);
+      const int S = pt_splits(q, share);
+      v[0] = q.tiles * S * a.KVH;
+      v[1] = S > 1 ? v[0] : 0;
+      // cost of an item, in blocks: the mean of the first and the last tile's, and 2 for starting and ending it
+      v[2] = JOIN ? (S > 1 ? q.n * a.H : 0) : v[0] * (max(0, q.blocks - q.n / PB / 2) / S + 2);
+    }
+    pt_scan3(v, total, t.red);
+    if (b < a.B) t.items[b] = v[0], t.slots[b] = v[1], t.cost[b] = v[2];
+  }
+  if (tid == 0) t.share = share;
+  __syncthreads();
+  *cost = total[2];
+  return total[0];
+}
+
+// first sequence whose running sum passes x (the sums are non-decreasing)
+__device__ __forceinline__ int pt_find(const int* sums, int B, int x) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] > x) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+struct PtItem {
+  PtSeq q;
+  int b, h, tile, split, splits, slot;   // slot: of the partial output, -1 for a whole tile
+};
+template <int R, int PB>
+__device__ __forceinline__ PtItem pt_item(const PagedAttnArgs& a, const PtList& t, int item, int lo, int hi) {
+  PtItem it;
+  it.b = __builtin_amdgcn_readfirstlane(pt_find(t.items, a.B, item));
+  const int s0 = pt_ldc(a.q_start, it.b), s1 = pt_ldc(a.q_start, it.b + 1), kv = pt_ldc(a.kv_len, it.b);
+  it.q = pt_seq<R, PB>(a, it.b, s0, s1, kv, lo, hi);
+  it.splits = pt_splits(it.q, t.share);
+  const int first = it.b ? t.items[it.b - 1] : 0;
+  const int i = __builtin_amdgcn_readfirstlane(item - first);   // (head, split, tile from the last)
+  it.tile = it.q.tiles - 1 - i % it.q.tiles;
+  it.split = i / it.q.tiles % it.splits;
+  it.h = i / it.q.tiles / it.splits;
+  const int base = it.b ? t.slots[it.b - 1] : 0;
+  it.slot = it.splits > 1 ? __builtin_amdgcn_readfirstlane(base + (it.h * it.q.tiles + it.tile) * it.splits + it.split) : -1;
+  return it;
+}
+
+// Rows' swizzles: chunk c (16 bytes) of row r lies in slot c ^ x(r). K: the 32 rows x 2 chunks of a fragment read hit
+// every bank; V: so do the transposing reads of 4 rows.
+template <int D>
+__device__ __forceinline__ int pt_xk(int r) {
+  return D == 128 ? r & 15 : (r >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int pt_xv(int r) {
+  return (D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
+}
+
+// The state of a wave's 32 rows over the positions seen so far.
+template <int DT, int D>
+struct PtWave {
+  static constexpr int RB = 2 * D;         // bytes of a row
+  static constexpr int TD = D / 32;        // output tiles of 32 dims
+  uint4 qf[D / 16];                        // B operand of S^T: row fr, dims 16 ks + 8 hi .. + 8
+  pt_f32x16 o[TD];                         // O^T: dims 32 t + 8 i + 4 hi + r, row fr
+  float m, l;                              // running maximum of the raw scores; the lane's own sum
+  float c;                                 // |scale| log2(e)
+  int pos;                                 // position of row fr, -1: none open
+  int lane, fr, hi;
+
+  __device__ __forceinline__ void init(const PagedAttnArgs& a, const PtItem& it, int row0) {
+    lane = threadIdx.x & 63, fr = lane & 31, hi = lane >> 5;
+    const int G = a.H / a.KVH, rows = it.q.n * G, r = min(row0 + fr, rows - 1), t = r / G;
+    pos = it.q.kv - it.q.n + t;
+    const long long last = (long long)a.M * a.page_size - 1;
+    pos = pos > last ? (int)last : pos;
+    const uint16_t* p = (const uint16_t*)a.q + (long long)(it.q.start + t) * a.q_rs + (long long)(it.h * G + r - t * G) * a.q_hs;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // a negative scale: of -q
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint4 v = *(const uint4*)(p + ks * 16 + hi * 8);
+      qf[ks] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+    }
+#pragma unroll
+    for (int t2 = 0; t2 < TD; ++t2)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[t2][e] = 0.f;
+    m = -INFINITY, l = 0.f;
+    c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);   // (0: every score counts alike)
+  }
+
+  // scores of 32 NB positions from Kt
+  template <int NB>
+  __device__ __forceinline__ void scores(const char* Kt, pt_f32x16 (&s)[NB]) const {
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[sb][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint4 k = *(const uint4*)(Kt + (sb * 32 + fr) * RB + (((2 * ks + hi) ^ pt_xk<D>(fr)) * 16));
+        s[sb] = pt_mfma<DT>(k, qf[ks], s[sb]);
+      }
+    }
+  }
+
+  // closed positions' scores to -inf: behind the row, or in one of the 16-position groups of `bad`
+  template <int NB>
+  __device__ __forceinline__ void mask(pt_f32x16 (&s)[NB], int p0, unsigned bad) const {
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = sb * 32 + 8 * (e >> 2) + 4 * hi + (e & 3);
+        if (p0 + j > pos || ((bad >> (j >> 4)) & 1)) s[sb][e] = -INFINITY;
+      }
+  }
+
+  // maximum, exponentials (left in s), sums. Outputs are rescaled when a row's maximum has grown by more than 8 in
+  // the exponent, not at every new maximum: the exponentials stay below 2^8, as exact as below 1, and of 32 rows some
+  // row's maximum grows in nearly every block.
+  template <int NB>
+  __device__ __forceinline__ void softmax(pt_f32x16 (&s)[NB]) {
+    float bm = -INFINITY;
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bm = fmaxf(bm, s[sb][e]);
+    {
+      uint32_t u = __float_as_uint(bm), w = u;
+      pt_swap32(u, w);
+      bm = fmaxf(__uint_as_float(u), __uint_as_float(w));
+    }
+    if (__ballot((bm - m) * c > 8.f) != 0ull) {
+      const float mn = fmaxf(m, bm);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < TD; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+    }
+    const float mc = m == -INFINITY ? 0.f : -m * c;   // nothing open yet: every score is -inf
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[sb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sb][e], c, mc));
+        l += s[sb][e];
+      }
+  }
+
+  __device__ __forceinline__ uint4 vfrag(const char* Vt, int sb, int hf, int t) const {
+    // rows 8 hi + 4 q + vr of the half block's 16, dims 32 t + 16 g + 4 c
+    const int vr = (lane & 15) >> 2, r = sb * 32 + hf * 16 + 8 * hi + vr;
+    const int ch = 4 * t + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const char* p = Vt + r * RB + (lane & 1) * 8;
+    const uint2 lo = pt_read_tr(p + ((ch ^ pt_xv<D>(vr)) * 16));
+    const uint2 up = pt_read_tr(p + 4 * RB + ((ch ^ pt_xv<D>(vr + 4)) * 16));
+    return make_uint4(lo.x, lo.y, up.x, up.y);
+  }
+
+  // P in the B operand's layout: lane half 0 needs positions 0-7 / 16-23 of 32, half 1 8-15 / 24-31
+  template <int NB>
+  __device__ __forceinline__ void pack(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) const {
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb) {
+      uint32_t g[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        g[i][0] = gm_pack2<DT>(s[sb][4 * i], s[sb][4 * i + 1]);
+        g[i][1] = gm_pack2<DT>(s[sb][4 * i + 2], s[sb][4 * i + 3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        pt_swap32(g[i][0], g[i + 1][0]);
+        pt_swap32(g[i][1], g[i + 1][1]);
+        p[2 * sb + i / 2] = make_uint4(g[i][0], g[i][1], g[i + 1][0], g[i + 1][1]);
+      }
+    }
+  }
+
+  template <int NB>
+  __device__ __forceinline__ void outputs(const char* Vt, const uint4 (&p)[2 * NB]) {
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int t = 0; t < TD; ++t) o[t] = pt_mfma<DT>(vfrag(Vt, sb, hf, t), p[2 * sb + hf], o[t]);
+  }
+
+  // Outputs of a block with closed positions: a value there may be anything (stale memory, a later token's NaN), and
+  // 0 x NaN is NaN. Values that are not finite are taken as 0 in the product and, where there are any, added position
+  // by position to the rows that have it open.
+  template <int NB>
+  __device__ __forceinline__ void outputs_masked(const char* Vt, const uint4 (&p)[2 * NB], int p0, unsigned bad) {
+    constexpr uint32_t EXP = DT == HS_BF16 ? 0x7f80u : 0x7c00u;
+    bool odd = false;
+    auto clean = [&](uint32_t w) {
+      const bool l0 = (w & EXP) == EXP, h0 = ((w >> 16) & EXP) == EXP;
+      odd = odd || l0 || h0;
+      return (l0 ? 0u : w & 0xffffu) | (h0 ? 0u : w & 0xffff0000u);
+    };
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int t = 0; t < TD; ++t) {
+          const uint4 v = vfrag(Vt, sb, hf, t);
+          o[t] = pt_mfma<DT>(make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)), p[2 * sb + hf], o[t]);
+        }
+    if (__ballot(odd) == 0ull) return;
+#pragma unroll
+    for (int q = 0; q < 2 * NB; ++q)
+#pragma unroll 1
+      for (int j = 0; j < 16; ++j) {   // position 16 q + j of the block: the only one left in the operand
+        const bool open = p0 + 16 * q + j <= pos && !((bad >> q) & 1);
+#pragma unroll
+        for (int t = 0; t < TD; ++t) {
+          const uint4 v = vfrag(Vt, q >> 1, q & 1, t);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t k[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t l0 = w[i] & 0xffffu, h0 = w[i] >> 16;
+            k[i] = (8 * hi + 2 * i == j && (l0 & EXP) == EXP ? l0 : 0u) |
+                   (8 * hi + 2 * i + 1 == j && (h0 & EXP) == EXP ? h0 << 16 : 0u);
+          }
+          pt_f32x16 z;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[e] = 0.f;
+          z = pt_mfma<DT>(make_uint4(k[0], k[1], k[2], k[3]), p[q], z);
+          if (open)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[t][e] += z[e];
+        }
+      }
+  }
+
+  // both lanes' sum of the row
+  __device__ __forceinline__ float row_sum() const {
+    uint32_t u = __float_as_uint(l), w = u;
+    pt_swap32(u, w);
+    return __uint_as_float(u) + __uint_as_float(w);
+  }
+};
+
+// Pages of a block's groups of 16 positions: ids (0 where there is none) and which have none.
+template <int NG>
+struct PtPages {
+  int id[NG];
+  unsigned bad;
+};
+template <int NG>
+__device__ __forceinline__ PtPages<NG> pt_pages(const PagedAttnArgs& a, int b, int p0) {
+  PtPages<NG> r;
+  r.bad = 0;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const unsigned grp = (unsigned)(p0 >> 4) + g;
+    const unsigned at = a.group_magic ? __umulhi(grp, a.group_magic) : grp;
+    const int id = pt_ldc(a.table, (long long)b * a.M + min(at, (unsigned)a.M - 1));
+    const bool ok = at < (unsigned)a.M && (unsigned)id < (unsigned)a.pages;
+    r.id[g] = ok ? id : 0;
+    r.bad |= ok ? 0u : 1u << g;
+  }
+  return r;
+}
+// byte address of the 16-position group at p0 (K/V head h) in a pool
+__device__ __forceinline__ const char* pt_group(const PagedAttnArgs& a, const void* pool, int id, int h, int p0) {
+  const unsigned grp = (unsigned)(p0 >> 4);
+  const unsigned in = a.group_magic ? grp - __umulhi(grp, a.group_magic) * a.page_groups : 0;
+  return (const char*)pool + 2 * (id * a.page_stride + h * a.head_stride + (long long)(in * 16) * a.row_stride);
+}
+
+// One 1 KiB load of a group to LDS: rows i * (1024 / RB) .. of its 16, swizzled
+template <int D, bool V>
+__device__ __forceinline__ void pt_load(const char* group, unsigned row_bytes, int i, unsigned lds, int lane) {
+  constexpr int RB = 2 * D, PER = 1024 / RB, SL = RB / 16;   // rows per load, slots of a row
+  const int r = i * PER + lane / SL, ch = (lane % SL) ^ (V ? pt_xv<D>(r) : pt_xk<D>(r));
+  gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
+}
+
+// ------------------------------------------------------------------ narrow tiles
+
+template <int DT, int D>
+struct PtNarrow {
+  static constexpr int PB = 8192 / (2 * D), NB = PB / 32, NG = PB / 16;   // positions of a block: 8 KiB of K, 8 of V
+  static constexpr int LPG = 2 * D * 16 / 1024;                             // loads per group
+  static constexpr int OLD = 64 + 4;                                        // output row in LDS (floats)
+};
+
+template <int DT, int D>
+__device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32]) {
+  using C = PtNarrow<DT, D>;
+  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, OLD = C::OLD;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.H / a.KVH, rows = it.q.n * G, row0 = it.tile * 32;
+  PtWave<DT, D> w;
+  const unsigned row_bytes = (unsigned)(2 * a.row_stride);
+  char* Kt = lds + wave * 16384;
+  char* Vt = Kt + 8192;
+  const unsigned k0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)Kt, v0 = k0 + 8192;
+  // blocks of this tile (up to its last row's position), this split's, this wave's
+  const int tlast = min(row0 + 31, rows - 1) / G;
+  const int need = min(it.q.blocks, (it.q.kv - it.q.n + tlast) / PB + 1);
+  const int nblk = it.q.kv - it.q.n + tlast < 0 ? 0 : need;
+  const int b0 = (int)((long long)nblk * it.split / it.splits), b1 = (int)((long long)nblk * (it.split + 1) / it.splits);
+  auto load_k = [&](const PtPages<NG>& pg, int blk) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const char* p = pt_group(a, a.k_pages, pg.id[g], it.h, blk * PB + 16 * g);
+#pragma unroll
+      for (int i = 0; i < LPG; ++i) pt_load<D, false>(p, row_bytes, i, k0 + (g * LPG + i) * 1024, lane);
+    }
+  };
+  auto load_v = [&](const PtPages<NG>& pg, int blk) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const char* p = pt_group(a, a.v_pages, pg.id[g], it.h, blk * PB + 16 * g);
+#pragma unroll
+      for (int i = 0; i < LPG; ++i) pt_load<D, true>(p, row_bytes, i, v0 + (g * LPG + i) * 1024, lane);
+    }
+  };
+  int blk = b0 + wave;
+  PtPages<NG> pg, next;
+  if (blk < b1) {
+    pg = pt_pages<NG>(a, it.b, blk * PB);
+    load_k(pg, blk);
+    load_v(pg, blk);
+  }
+  w.init(a, it, row0);
+  // the queries are waited for here: at their first use the wait would cover the loads in flight of every block
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
+  const int pmin = __builtin_amdgcn_readfirstlane(w.pos);   // the tile's first row
+  for (; blk < b1; blk += 4) {
+    const bool more = blk + 4 < b1;
+    if (more) next = pt_pages<NG>(a, it.b, (blk + 4) * PB);
+    const bool open = blk * PB + PB - 1 <= pmin && pg.bad == 0;
+    gm_vmcnt<8>();   // K has landed; V's eight loads may be on their way
+    asm volatile("" ::: "memory");
+    pt_f32x16 s[NB];
+    w.template scores<NB>(Kt, s);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's rows are in registers
+    if (more) load_k(next, blk + 4);
+    if (!open) w.template mask<NB>(s, blk * PB, pg.bad);
+    w.template softmax<NB>(s);
+    uint4 p[2 * NB];
+    w.template pack<NB>(s, p);
+    if (more) gm_vmcnt<8>();   // V has landed; the next K's eight loads may be on their way
+    else gm_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    if (open) w.template outputs<NB>(Vt, p);
+    else w.template outputs_masked<NB>(Vt, p, blk * PB, pg.bad);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) load_v(next, blk + 4);
+    pg = next;
+  }
+  // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
+  const float l = w.row_sum();
+  if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
+  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - M) * w.c);
+  float* ob = (float*)lds;
+  const int valid = min(32, rows - row0);
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half) {   // dims 64 half .. + 64
+    if (half) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const pt_f32x16& o = w.o[2 * half + t];
+        float4 v;
+        v.x = o[4 * i] * f, v.y = o[4 * i + 1] * f, v.z = o[4 * i + 2] * f, v.w = o[4 * i + 3] * f;
+        *(float4*)&ob[(wave * 32 + w.fr) * OLD + t * 32 + 8 * i + 4 * w.hi] = v;
+      }
+    __syncthreads();
+    for (int idx = tid; idx < valid * 8; idx += 256) {   // (row, 8 dims)
+      const int ch = idx & 7, r = idx >> 3;
+      float Mr = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Mr = fmaxf(Mr, ml[i][0][r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        L += ml[i][0][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i][0][r] - Mr) * w.c) * ml[i][1][r];
+      float x[8] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4* p = (const float4*)&ob[(i * 32 + r) * OLD + 8 * ch];
+        const float4 u = p[0], v = p[1];
+        x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w;
+        x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
+      }
+      if (it.slot >= 0) {
+        float* po = a.part_o + ((long long)it.slot * 32 + r) * D + 64 * half + 8 * ch;
+        *(float4*)po = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(po + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        if (half == 0 && ch == 0) *(float2*)(a.part_ml + ((long long)it.slot * 32 + r) * 2) = make_float2(Mr, L);
+      } else {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int row = row0 + r, t = row / G;
+        uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + 64 * half + 8 * ch;
+        *(uint4*)out = make_uint4(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv),
+                                  gm_pack2<DT>(x[4] * inv, x[5] * inv), gm_pack2<DT>(x[6] * inv, x[7] * inv));
+      }
+    }
+  }
+  __syncthreads();   // the next item's loads go to the same LDS
+}
+
+// ------------------------------------------------------------------ wide tiles
+
+template <int DT, int D>
+__device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds) {
+  constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V
+  constexpr int LPG = RB * 16 / 1024;                                   // loads per group: each wave takes its group's
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.H / a.KVH, rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
+  const unsigned row_bytes = (unsigned)(2 * a.row_stride);
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+  const int first = it.q.kv - it.q.n;   // position of token 0
+  const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
+  const int nblk = first + tlast < 0 ? 0 : min(it.q.blocks, (first + tlast) / PB + 1);
+  const int b0 = (int)((long long)nblk * it.split / it.splits), b1 = (int)((long long)nblk * (it.split + 1) / it.splits);
+  auto issue = [&](const PtPages<NG>& pg, int blk) {
+    const unsigned dst = lds0 + (unsigned)(blk & 1) * 2 * BYTES + (unsigned)wave * LPG * 1024;
+    const int id = wave == 0 ? pg.id[0] : wave == 1 ? pg.id[1] : wave == 2 ? pg.id[2] : pg.id[3];
+    const char* k = pt_group(a, a.k_pages, id, it.h, blk * PB + 16 * wave);
+    const char* v = pt_group(a, a.v_pages, id, it.h, blk * PB + 16 * wave);
+#pragma unroll
+    for (int i = 0; i < LPG; ++i) pt_load<D, false>(k, row_bytes, i, dst + i * 1024, lane);
+#pragma unroll
+    for (int i = 0; i < LPG; ++i) pt_load<D, true>(v, row_bytes, i, dst + BYTES + i * 1024, lane);
+  };
+  PtPages<NG> pg, next;
+  if (b0 < b1) {
+    pg = pt_pages<NG>(a, it.b, b0 * PB);
+    issue(pg, b0);
+    next = pt_pages<NG>(a, it.b, (b0 + 1) * PB);
+  }
+  PtWave<DT, D> w;
+  w.init(a, it, row0);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
+  // positions that every row of the wave has open, and that any has
+  const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
+  const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
+  for (int blk = b0; blk < b1; ++blk) {
+    gm_vmcnt<0>();
+    __syncthreads();   // the block is in LDS, and every wave is done with the other stage
+    const unsigned bad = pg.bad;
+    if (blk + 1 < b1) {
+      issue(next, blk + 1);
+      pg = next;
+      next = pt_pages<NG>(a, it.b, (blk + 2) * PB);
+    }
+    if (blk * PB > pmax) continue;   // wave-uniform
+    const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
+    const char* Kt = lds + (blk & 1) * 2 * BYTES;
+    const char* Vt = Kt + BYTES;
+    pt_f32x16 s[NB];
+    w.template scores<NB>(Kt, s);
+    if (!open) w.template mask<NB>(s, blk * PB, bad);
+    w.template softmax<NB>(s);
+    uint4 p[2 * NB];
+    w.template pack<NB>(s, p);
+    if (open) w.template outputs<NB>(Vt, p);
+    else w.template outputs_masked<NB>(Vt, p, blk * PB, bad);
+  }
+  const float l = w.row_sum();
+  const int row = row0 + w.fr;
+  if (row < rows) {
+    if (it.slot >= 0) {
+      const long long at = (long long)a.narrow_slots * 32 + (long long)it.slot * PT_WIDE + row - tile0;
+      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
+              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t0 = row / G;
+      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
+              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
+                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
+    }
+  }
+  __syncthreads();   // the next item's loads go to the same LDS
+}
+
+// ------------------------------------------------------------------ kernels
+
+// all: rows of any number on narrow tiles (launches whose batches are nearly all single tokens)
+template <int DT, int D>
+__device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
+  using C = PtNarrow<DT, D>;
+  constexpr int ANY = 0x7fffffff;
+  __shared__ __attribute__((aligned(1024))) char lds[65536];
+  __shared__ float ml[4][2][32];
+  __shared__ PtList t;
+  const int nw = a.grid_wide;
+  int cost;
+  if ((int)blockIdx.x >= nw) {
+    const int hi = nw ? PT_NARROW : ANY;
+    const int n = pt_build<PT_NARROW, C::PB, PT_NARROW_ITEMS, PT_NARROW_MIN>(a, t, 0, hi, &cost);
+    for (int item = blockIdx.x - nw; item < n; item += gridDim.x - nw)
+      pt_narrow<DT, D>(a, pt_item<PT_NARROW, C::PB>(a, t, item, 0, hi), lds, ml);
+    return;
+  }
+  const int n = pt_build<PT_WIDE, 64, PT_WIDE_ITEMS, PT_WIDE_MIN>(a, t, PT_NARROW, ANY, &cost);
+  // XCD x (workgroups x, x + 8, ...) takes the items whose running cost falls into its eighth of the whole
+  auto bound = [&](int x) {
+    if (x >= 8) return n;
+    const int at = (int)((long long)cost * x / 8);
+    const int b = pt_find(t.cost, a.B, at);
+    const int c0 = b ? t.cost[b - 1] : 0, i0 = b ? t.items[b - 1] : 0;
+    const int ci = t.cost[b] - c0, ii = t.items[b] - i0;
+    return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
+  };
+  const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
+  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3)
+    pt_wide<DT, D>(a, pt_item<PT_WIDE, 64>(a, t, item, PT_NARROW, ANY), lds);
+}
+
+// k_paged_combine: joins the partial outputs of split tiles, a wave per row, and zeroes the rows of no sequence.
+template <int DT, int D, bool WIDE>
+__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, PtList& t, int me, int waves) {
+  constexpr int R = WIDE ? PT_WIDE : PT_NARROW, PB = WIDE ? 64 : PtNarrow<DT, D>::PB, ANY = 0x7fffffff, E = D / 64;
+  constexpr int ITEMS = WIDE ? PT_WIDE_ITEMS : PT_NARROW_ITEMS, LEAST = WIDE ? PT_WIDE_MIN : PT_NARROW_MIN;
+  const int lo = WIDE ? PT_NARROW : 0, hi = WIDE || !a.grid_wide ? ANY : PT_NARROW, lane = threadIdx.x & 63;
+  const int G = a.H / a.KVH;
+  const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
+  int rows;
+  pt_build<R, PB, ITEMS, LEAST, true>(a, t, lo, hi, &rows);
+  for (int u = me; u < rows; u += waves) {   // (sequence, head, row)
+    const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
+    const PtSeq q = pt_seq<R, PB>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), lo, hi);
+    const int S = pt_splits(q, t.share), i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
+    const int slot = (b ? t.slots[b - 1] : 0) + (h * q.tiles + row / R) * S;
+    const long long p = (WIDE ? (long long)a.narrow_slots * PT_NARROW : 0) + (long long)slot * R + row % R;
+    float M = -INFINITY, L = 0.f, x[E] = {};
+    for (int s = 0; s < S; ++s) M = fmaxf(M, a.part_ml[(p + (long long)s * R) * 2]);
+    for (int s = 0; s < S; ++s) {
+      const long long ps = p + (long long)s * R;
+      const float m = a.part_ml[ps * 2], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c);
+      L += f * a.part_ml[ps * 2 + 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += f * a.part_o[ps * D + lane * E + e];
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int tk = row / G;
+    uint16_t* out = (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = gm_pack<DT>(x[e] * inv);
+  }
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
+  __shared__ PtList t;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = gridDim.x * 4, me = blockIdx.x * 4 + wave;
+  pt_join<DT, D, false>(a, t, me, waves);
+  if (a.grid_wide) {
+    __syncthreads();
+    pt_join<DT, D, true>(a, t, me, waves);
+  }
+  const int s0 = a.q_start[0], s1 = a.q_start[a.B];
+  for (int row = me; row < a.N; row += waves) {
+    if (row >= s0 && row < s1) continue;
+    uint4* out = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
+    for (int i = lane; i < a.H * D / 8; i += 64) out[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+#define PT_KERNELS(NAME, DT, D)                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_##NAME(const PagedAttnArgs a) { pt_attn_body<DT, D>(a); }     \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_combine_##NAME(const PagedAttnArgs a) { pt_combine_body<DT, D>(a); }
+PT_KERNELS(bf16_d128, HS_BF16, 128)
+PT_KERNELS(bf16_d64, HS_BF16, 64)
+PT_KERNELS(f16_d128, HS_F16, 128)
+PT_KERNELS(f16_d64, HS_F16, 64)

@@ -9,6 +9,10 @@ from npu_compiler.ir_reader import OpNode
 from npu_runtime.serving_ops import check_paged_append, check_paged_attention, check_sample
 
 PAGED_ANY_MAX_D = 256          # paged.hip PG_ANY_D
+# paged.hip: sequences of an item list, rows of a tile, items that tiles are split towards, fewest blocks of a split
+PT_MAXB, PT_NARROW, PT_WIDE = 1024, 32, 128
+PT_NARROW_ITEMS, PT_WIDE_ITEMS, PT_NARROW_MIN, PT_WIDE_MIN = 2048, 480, 8, 8
+PT_GRID_NARROW = 4096          # workgroups of narrow items, which take more than one each past it
 SAMPLE_MAX_PIECES = 4096 * 64  # sample.hip SM_GROUPS groups of 64 pieces of 16 bytes
 
 
@@ -33,6 +37,41 @@ def _check_i32(op: str, **sizes) -> None:
     for name, n in sizes.items():
         if n >= 2 ** 31:
             raise NotImplementedError(f"{op}: {name} = {n} does not fit 32 bits")
+
+
+def _aligned_rows(low, name: str, v: TView) -> TView:
+    """``v`` when its rows and heads start on 16-byte boundaries, else a contiguous copy of it."""
+    per = 16 // ELEM_SIZE[v.dtype]
+    if v.offset % per == 0 and all(s % per == 0 for n, s in zip(v.shape[:2], v.strides[:2]) if n > 1):
+        return v
+    out = low.new_storage(name + ".rows", v.shape, v.dtype)
+    low.emit_copy(v, out, [name], [name + ".rows"])
+    return out
+
+
+def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_size: int, dtype: str) -> dict | None:
+    """Launch of the tiled attention kernels (paged.hip), None where they do not apply: other types or head sizes,
+    pages that are no multiple of 16 positions, more sequences than the item list holds, or sizes whose item
+    counts could pass 32 bits. Wide tiles are left out where the rows average at most two tokens per sequence: a
+    decode step's batches then need no workgroups that look for chunks, and a longer chunk in one takes several
+    narrow tiles."""
+    if dtype not in ("bfloat16", "float16") or D not in (64, 128) or page_size % 16 or not 0 < B <= PT_MAXB or M < 1 or P < 1:
+        return None
+    G, block = H // KVH, 8192 // (2 * D)
+    blocks = -(-M * page_size // block)
+    tiles = lambda R: KVH * (N * G // R + min(N, B))
+    if (tiles(PT_NARROW) + 2 * PT_NARROW_ITEMS) * (blocks + 3) >= 2 ** 31 or M * page_size * page_size >= 2 ** 40 \
+            or KVH * page_size * D >= 2 ** 30:
+        return None
+    wide = N > 2 * B and N * G > PT_NARROW
+    # a split sequence has ceil(blocks / share) < 2 blocks / share slots per tile, all together under twice the items
+    # aimed at; nor can a tile have more than its blocks allow
+    slots = lambda R, items, least: min(2 * items, tiles(R) * -(-blocks // least))
+    return {"grid_wide": min(512, 8 * -(-(tiles(PT_WIDE) + PT_WIDE_ITEMS) // 8)) if wide else 0,
+            "grid_narrow": min(tiles(PT_NARROW) + PT_NARROW_ITEMS, PT_GRID_NARROW,
+                               tiles(PT_NARROW) * max(1, -(-blocks // PT_NARROW_MIN))),
+            "narrow_slots": slots(PT_NARROW, PT_NARROW_ITEMS, PT_NARROW_MIN),
+            "wide_slots": slots(PT_WIDE, PT_WIDE_ITEMS, PT_WIDE_MIN) if wide else 0}
 
 
 def _batch(low, table, q_start, kv_len) -> dict:
@@ -80,14 +119,34 @@ def lower_paged_attention(low, node: OpNode) -> None:
     low.views[node.outputs[0].name] = out
     if N == 0:
         return
+    B, M, P = int(kv_len.shape[0]), int(table.shape[1]), int(kp.shape[0])
+    tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype)
+    if tiled:
+        qv = _aligned_rows(low, q.name, qv)
+    args = dict(q=low.ref(qv), k_pages=low.ref(kv), v_pages=low.ref(vv), out=low.ref(out), part_o=None, part_ml=None,
+                **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
+                **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
+                scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
+                narrow_slots=0, pad=0)
+    params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
+    ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
+    if tiled is None:
+        low.emit(LaunchStep(kind="paged_attention", kernel="k_paged_attn_any", module="paged", arg_struct="PagedAttnArgs",
+                            args=args, grid=(N, H, 1), block=(64, 1, 1), inputs=ins, outputs=outs, params=params))
+        return
+    groups = ps // 16
+    part_rows = tiled["narrow_slots"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
+    args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
+                part_ml=low.scratch(outs[0] + ".part_ml", 8 * part_rows), page_groups=groups,
+                group_magic=0 if groups == 1 else -(-2 ** 32 // groups), grid_wide=tiled["grid_wide"],
+                narrow_slots=tiled["narrow_slots"])
+    name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
-        kind="paged_attention", kernel="k_paged_attn_any", module="paged", arg_struct="PagedAttnArgs",
-        args=dict(q=low.ref(qv), k_pages=low.ref(kv), v_pages=low.ref(vv), out=low.ref(out),
-                  **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
-                  **_pool_strides(kp.shape, layout), pages=int(kp.shape[0]), N=N, H=H, KVH=KVH, D=D, page_size=ps,
-                  scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], pad=0),
-        grid=(N, H, 1), block=(64, 1, 1), inputs=[t.name for t in node.inputs], outputs=[node.outputs[0].name],
-        params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D}))
+        kind="paged_attention", kernel="k_paged_attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
+        grid=(tiled["grid_wide"] + tiled["grid_narrow"], 1, 1), inputs=ins, outputs=outs, params={**params, "mfma": True}))
+    low.emit(LaunchStep(
+        kind="paged_attention", kernel="k_paged_combine_" + name, module="paged", arg_struct="PagedAttnArgs",
+        args=dict(args), grid=(min(1024, -(-N * H // 4)), 1, 1), inputs=ins, outputs=outs, params=params))
 
 
 def lower_sample(low, node: OpNode) -> None:

@@ -134,8 +134,10 @@ _struct("PagedAppendArgs", [("q", P), ("k", P), ("v", P), ("k_pages", P), ("v_pa
                             ("D", I), ("R", I), ("page_size", I), ("scaling", F), ("dtype", I)])
 _struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), ("table", P), ("q_start", P),
                           ("kv_len", P), ("q_rs", LL), ("q_hs", LL), ("page_stride", LL), ("head_stride", LL),
-                          ("row_stride", LL), ("pages", LL), ("N", I), ("B", I), ("M", I), ("H", I), ("KVH", I), ("D", I),
-                          ("page_size", I), ("scale", F), ("dtype", I), ("pad", I)])
+                          ("row_stride", LL), ("pages", LL), ("part_o", P), ("part_ml", P), ("N", I), ("B", I), ("M", I),
+                          ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
+                          ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("narrow_slots", I),
+                          ("pad", I)])
 _struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
                        ("rows", I), ("vocab", I), ("dtype", I), ("shift", I)])
 
