@@ -458,53 +458,28 @@ struct PtWave {
         for (int t = 0; t < TD; ++t) o[t] = pt_mfma<DT>(vfrag(Vt, sb, hf, t), p[2 * sb + hf], o[t]);
   }
 
-  // Outputs of a block with closed positions: a value there may be anything (stale memory, a later token's NaN), and
-  // 0 x NaN is NaN. Values that are not finite are taken as 0 in the product and, where there are any, added position
-  // by position to the rows that have it open.
+  // Closed positions have probability 0, but a value there may be anything, and 0 x NaN is NaN. Those that are closed to
+  // every row of the tile (behind its last row's position `end`, or without a page: stale or foreign memory) are zeroed
+  // in LDS; for the rest see bad_output.
   template <int NB>
-  __device__ __forceinline__ void outputs_masked(const char* Vt, const uint4 (&p)[2 * NB], int p0, unsigned bad) {
-    constexpr uint32_t EXP = DT == HS_BF16 ? 0x7f80u : 0x7c00u;
-    bool odd = false;
-    auto clean = [&](uint32_t w) {
-      const bool l0 = (w & EXP) == EXP, h0 = ((w >> 16) & EXP) == EXP;
-      odd = odd || l0 || h0;
-      return (l0 ? 0u : w & 0xffffu) | (h0 ? 0u : w & 0xffff0000u);
-    };
-#pragma unroll
-    for (int sb = 0; sb < NB; ++sb)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int t = 0; t < TD; ++t) {
-          const uint4 v = vfrag(Vt, sb, hf, t);
-          o[t] = pt_mfma<DT>(make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w)), p[2 * sb + hf], o[t]);
-        }
-    if (__ballot(odd) == 0ull) return;
-#pragma unroll
-    for (int q = 0; q < 2 * NB; ++q)
+  __device__ __forceinline__ void clear_closed(char* Vt, int p0, int end, unsigned bad) const {
+    constexpr int SL = RB / 16;
 #pragma unroll 1
-      for (int j = 0; j < 16; ++j) {   // position 16 q + j of the block: the only one left in the operand
-        const bool open = p0 + 16 * q + j <= pos && !((bad >> q) & 1);
+    for (int i = lane; i < NB * 32 * SL; i += 64) {
+      const int j = i / SL;
+      if (p0 + j > end || ((bad >> (j >> 4)) & 1)) *(uint4*)(Vt + i * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  // Whether an output of the wave is not finite: it may come from a position that is open to other rows only
+  // (pt_row then takes the rows one by one).
+  __device__ __forceinline__ bool bad_output() const {
+    bool odd = false;
 #pragma unroll
-        for (int t = 0; t < TD; ++t) {
-          const uint4 v = vfrag(Vt, q >> 1, q & 1, t);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t k[4];
+    for (int t = 0; t < TD; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t l0 = w[i] & 0xffffu, h0 = w[i] >> 16;
-            k[i] = (8 * hi + 2 * i == j && (l0 & EXP) == EXP ? l0 : 0u) |
-                   (8 * hi + 2 * i + 1 == j && (h0 & EXP) == EXP ? h0 << 16 : 0u);
-          }
-          pt_f32x16 z;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) z[e] = 0.f;
-          z = pt_mfma<DT>(make_uint4(k[0], k[1], k[2], k[3]), p[q], z);
-          if (open)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[t][e] += z[e];
-        }
-      }
+      for (int e = 0; e < 16; ++e) odd = odd || (__float_as_uint(o[t][e]) & 0x7f800000u) == 0x7f800000u;
+    return __ballot(odd) != 0ull;
   }
 
   // both lanes' sum of the row
@@ -549,6 +524,71 @@ __device__ __forceinline__ void pt_load(const char* group, unsigned row_bytes, i
   constexpr int RB = 2 * D, PER = 1024 / RB, SL = RB / 16;   // rows per load, slots of a row
   const int r = i * PER + lane / SL, ch = (lane % SL) ^ (V ? pt_xv<D>(r) : pt_xk<D>(r));
   gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
+}
+
+// One row over positions p0 .. p1 - 1 by a wave, 64 at a time, reading open positions only: the row's maximum of the raw
+// scores, sum of exponentials and the lane's outputs (dims lane * E ..). For tiles whose product is not finite.
+template <int DT, int D>
+__device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it, int row, int p0, int p1, float& m,
+                                       float& l, float (&x)[D / 64]) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, G = a.H / a.KVH, t = row / G;
+  const float flip = a.scale < 0.f ? -1.f : 1.f, c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
+  const uint16_t* q = (const uint16_t*)a.q + (long long)(it.q.start + t) * a.q_rs + (long long)(it.h * G + row - t * G) * a.q_hs;
+  m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.f;
+  const int end = min(p1, it.q.kv - it.q.n + t + 1);
+#pragma unroll 1
+  for (; p0 < end; p0 += 64) {
+    const int pos = p0 + lane, page = pos < end ? pg_page(a.table, it.b, a.M, a.page_size, a.pages, pos) : -1;
+    const long long at = page < 0 ? 0 : page * a.page_stride + it.h * a.head_stride + (pos % a.page_size) * a.row_stride;
+    float s = 0.f;
+    if (page >= 0)
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) s = fmaf(gm_ld<DT>(q, d), gm_ld<DT>(a.k_pages, at + d), s);
+    s = page < 0 ? -INFINITY : s * flip;
+    const float mn = fmaxf(m, wave_max(s)), mc = mn == -INFINITY ? 0.f : -mn * c;
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
+    const float e = page < 0 ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, mc));
+    m = mn;
+    l = l * alpha + wave_sum(e);
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] *= alpha;
+#pragma unroll 1
+    for (int j = 0; j < min(64, end - p0); ++j) {
+      const long long aj = __shfl(at, j, 64);
+      const float ej = __shfl(e, j, 64);
+      if (__shfl(page, j, 64) < 0) continue;
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = fmaf(ej, gm_ld<DT>(a.v_pages, aj + lane * E + i), x[i]);
+    }
+  }
+}
+
+// rows r0, r0 + step, ... of a tile one by one, written as the tile's rows are (part: index of its first partial row)
+template <int DT, int D>
+__device__ __forceinline__ void pt_rows(const PagedAttnArgs& a, const PtItem& it, int tile0, int r0, int r1, int step, int p0,
+                                     int p1, long long part) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, G = a.H / a.KVH;
+#pragma unroll 1
+  for (int row = r0; row < r1; row += step) {
+    float m, l, x[E];
+    pt_row<DT, D>(a, it, row, p0, p1, m, l, x);
+    if (it.slot >= 0) {
+      const long long at = part + row - tile0;
+      if (lane == 0) *(float2*)(a.part_ml + at * 2) = make_float2(m, l);
+#pragma unroll
+      for (int i = 0; i < E; ++i) a.part_o[at * D + lane * E + i] = x[i];
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t = row / G;
+      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + lane * E;
+#pragma unroll
+      for (int i = 0; i < E; ++i) out[i] = gm_pack<DT>(x[i] * inv);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ narrow tiles
@@ -603,7 +643,8 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
   // the queries are waited for here: at their first use the wait would cover the loads in flight of every block
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
-  const int pmin = __builtin_amdgcn_readfirstlane(w.pos);   // the tile's first row
+  // positions that the tile's first row has open, and its last
+  const int pmin = __builtin_amdgcn_readfirstlane(w.pos), pend = __builtin_amdgcn_readlane(w.pos, 31);
   for (; blk < b1; blk += 4) {
     const bool more = blk + 4 < b1;
     if (more) next = pt_pages<NG>(a, it.b, (blk + 4) * PB);
@@ -621,8 +662,8 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
     if (more) gm_vmcnt<8>();   // V has landed; the next K's eight loads may be on their way
     else gm_vmcnt<0>();
     asm volatile("" ::: "memory");
-    if (open) w.template outputs<NB>(Vt, p);
-    else w.template outputs_masked<NB>(Vt, p, blk * PB, pg.bad);
+    if (blk * PB + PB - 1 > pend || pg.bad) w.template clear_closed<NB>(Vt, blk * PB, pend, pg.bad);
+    w.template outputs<NB>(Vt, p);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) load_v(next, blk + 4);
     pg = next;
@@ -630,7 +671,11 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
   // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
   const float l = w.row_sum();
   if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
-  __syncthreads();
+  if (__syncthreads_or(w.bad_output())) {
+    pt_rows<DT, D>(a, it, row0, row0 + wave, min(row0 + 32, rows), 4, b0 * PB, b1 * PB, (long long)it.slot * 32);
+    __syncthreads();
+    return;
+  }
   float M = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
@@ -720,6 +765,7 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
   // positions that every row of the wave has open, and that any has
   const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
   const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
+  const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's
   for (int blk = b0; blk < b1; ++blk) {
     gm_vmcnt<0>();
     __syncthreads();   // the block is in LDS, and every wave is done with the other stage
@@ -731,22 +777,25 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     }
     if (blk * PB > pmax) continue;   // wave-uniform
     const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
-    const char* Kt = lds + (blk & 1) * 2 * BYTES;
-    const char* Vt = Kt + BYTES;
+    char* Kt = lds + (blk & 1) * 2 * BYTES;
+    char* Vt = Kt + BYTES;
     pt_f32x16 s[NB];
     w.template scores<NB>(Kt, s);
     if (!open) w.template mask<NB>(s, blk * PB, bad);
     w.template softmax<NB>(s);
     uint4 p[2 * NB];
     w.template pack<NB>(s, p);
-    if (open) w.template outputs<NB>(Vt, p);
-    else w.template outputs_masked<NB>(Vt, p, blk * PB, bad);
+    if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
+    w.template outputs<NB>(Vt, p);
   }
   const float l = w.row_sum();
   const int row = row0 + w.fr;
-  if (row < rows) {
+  const long long part = (long long)a.narrow_slots * 32 + (long long)it.slot * PT_WIDE;
+  if (row0 < rows && w.bad_output()) {
+    pt_rows<DT, D>(a, it, tile0, row0, min(row0 + 32, rows), 1, b0 * PB, b1 * PB, part);
+  } else if (row < rows) {
     if (it.slot >= 0) {
-      const long long at = (long long)a.narrow_slots * 32 + (long long)it.slot * PT_WIDE + row - tile0;
+      const long long at = part + row - tile0;
       if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
