@@ -136,18 +136,18 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
 // K and V go from the pages to LDS directly (a load covers 4 or 8 rows of one page), K swizzled for the fragment
 // reads, V for the transposing ones.
 //
-// Work is dealt out on the device: lengths are tensors, the launch is the same for every batch. Each workgroup sums the
-// sequences' tiles and blocks, splits tiles longer than an even share of all blocks, and takes items of the list that
-// follows. A split tile leaves unnormalised outputs with their maximum and sum; k_paged_combine_* joins them.
-// Wide items are dealt to the XCDs in ranges of equal cost, so the tiles that read the same blocks share an L2.
+// Work is dealt out on the device: lengths are tensors, the launch is the same for every batch. Narrow tiles' blocks form
+// one list (sequence, head, tile, block), of which every workgroup takes an equal range, so that at most the tiles at
+// its ends are split. Wide tiles longer than an even share of all blocks are split evenly; their items are dealt to the
+// XCDs in ranges of equal cost, so that the tiles that read the same blocks share an L2. A part of a split tile leaves
+// unnormalised outputs with their maximum and sum; k_paged_combine_* joins them.
 
 #define PT_MAXB 1024             // sequences
 #define PT_NARROW 32             // rows
 #define PT_WIDE 128
-#define PT_NARROW_ITEMS 2048     // items that narrow tiles are split towards: several per CU, of uneven length
-#define PT_WIDE_ITEMS 480        // wide: one round of two workgroups per CU
-#define PT_NARROW_MIN 8          // fewest blocks of a split
-#define PT_WIDE_MIN 8
+#define PT_NARROW_LEAST 4        // fewest blocks of a narrow workgroup: one per wave
+#define PT_WIDE_ITEMS 480        // items that wide tiles are split towards: one round of two workgroups per CU
+#define PT_WIDE_LEAST 8          // fewest blocks of a split
 
 typedef __attribute__((ext_vector_type(16))) float pt_f32x16;
 typedef __attribute__((ext_vector_type(4))) short pt_s16x4;
@@ -177,6 +177,21 @@ __device__ __forceinline__ uint2 pt_read_tr(const char* p) {
                                        (__attribute__((address_space(3))) pt_s16x4*)(__attribute__((address_space(3))) char*)p));
 }
 
+// Order of N matrix instructions with RD LDS reads each: the reads of four go ahead. (Left alone, the compiler reads one
+// operand, waits for it, multiplies, and reads the next into the same registers: 2.9 us for a wave's 32 x 64 block
+// of 32 matrix instructions, of which those are 0.4.)
+template <int N, int RD>
+__device__ __forceinline__ void pt_feed() {
+  constexpr int AHEAD = 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RD, 0);   // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);          // matrix instruction
+    __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 // uniform load from memory that no kernel in flight writes
 __device__ __forceinline__ int pt_ldc(const int* p, long long i) {
   return ((const __attribute__((address_space(4))) int*)p)[i];
@@ -198,13 +213,13 @@ __device__ __forceinline__ PtSeq pt_seq(const PagedAttnArgs& a, int b, int s0, i
     return q;
   }
   q.tiles = (int)((rows + R - 1) / R);
-  const long long end = min((long long)max(kv, 0), (long long)a.M * a.page_size);
-  q.blocks = (int)((end + PB - 1) / PB);
+  const long long end = min((long long)max(kv, 1), (long long)a.M * a.page_size);
+  q.blocks = (int)((end + PB - 1) / PB);   // (at least one: a tile without positions writes its zeros)
   return q;
 }
 
-// The list of items of one form of tile, in LDS: for each sequence the items, split slots and cost (JOIN: rows and
-// heads of split tiles) up to and with it.
+// The sequences' work, in LDS: running sums over them. Narrow: blocks in items, rows and heads in cost. Wide: items,
+// partial slots, and cost (JOIN: rows and heads of split tiles).
 struct PtList {
   int items[PT_MAXB];
   int slots[PT_MAXB];
@@ -244,27 +259,51 @@ __device__ __forceinline__ void pt_scan3(int (&v)[3], int (&total)[3], int (&red
 // splits of a sequence's tiles
 __device__ __forceinline__ int pt_splits(const PtSeq& q, int share) { return max(1, (q.blocks + share - 1) / share); }
 
-// Builds the list (by 256 threads; ends with a barrier) and returns the number of items. lo < rows <= hi.
-template <int R, int PB, int ITEMS, int LEAST, bool JOIN = false>
-__device__ __forceinline__ int pt_build(const PagedAttnArgs& a, PtList& t, int lo, int hi, int* cost) {
+// Narrow sequences' blocks (by 256 threads; ends with a barrier); returns their number, and that of rows and heads.
+template <int PB>
+__device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t, int hi, int* rows) {
+  int total[3] = {0, 0, 0};
+  for (int c = 0; c < a.B; c += 256) {
+    const int b = c + threadIdx.x;
+    int v[3] = {0, 0, 0};
+    if (b < a.B) {
+      const PtSeq q = pt_seq<PT_NARROW, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], 0, hi);
+      v[0] = q.tiles * q.blocks * a.KVH;
+      v[1] = q.n * a.H;
+    }
+    pt_scan3(v, total, t.red);
+    if (b < a.B) t.items[b] = v[0], t.cost[b] = v[1];
+  }
+  __syncthreads();
+  *rows = total[1];
+  return total[0];
+}
+
+// Workgroups that share `all` narrow blocks, of at most `most`, and the first block of workgroup w
+__device__ __forceinline__ int pt_workers(int all, int most) {
+  return max(1, min(most, (all + PT_NARROW_LEAST - 1) / PT_NARROW_LEAST));
+}
+__device__ __forceinline__ int pt_first(int all, int workers, int w) { return (int)((long long)all * w / workers); }
+
+// Wide sequences' items (by 256 threads; ends with a barrier); returns their number.
+template <bool JOIN>
+__device__ __forceinline__ int pt_build_wide(const PagedAttnArgs& a, PtList& t, int* cost) {
+  constexpr int PB = 64, ANY = 0x7fffffff;
   const int tid = threadIdx.x;
-  int work[3] = {0, 0, 0};   // blocks of all tiles, in units of 256 and the rest
+  int work[3] = {0, 0, 0};
   for (int b = tid; b < a.B; b += 256) {
-    const PtSeq q = pt_seq<R, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], lo, hi);
-    const long long w = (long long)q.tiles * q.blocks * a.KVH;
-    work[0] += (int)(w >> 8);
-    work[1] += (int)(w & 255);
+    const PtSeq q = pt_seq<PT_WIDE, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], PT_NARROW, ANY);
+    work[0] += q.tiles * q.blocks * a.KVH;
   }
   int total[3] = {0, 0, 0};
   pt_scan3(work, total, t.red);
-  const long long all = ((long long)total[0] << 8) + total[1];
-  const int share = (int)max((all + ITEMS - 1) / ITEMS, (long long)LEAST);
+  const int share = max((total[0] + PT_WIDE_ITEMS - 1) / PT_WIDE_ITEMS, PT_WIDE_LEAST);
   total[0] = total[1] = total[2] = 0;
   for (int c = 0; c < a.B; c += 256) {
     const int b = c + tid;
     int v[3] = {0, 0, 0};
     if (b < a.B) {
-      const PtSeq q = pt_seq<R, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], lo, hi);
+      const PtSeq q = pt_seq<PT_WIDE, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], PT_NARROW, ANY);
       const int S = pt_splits(q, share);
       v[0] = q.tiles * S * a.KVH;
       v[1] = S > 1 ? v[0] : 0;
@@ -291,24 +330,48 @@ __device__ __forceinline__ int pt_find(const int* sums, int B, int x) {
   return lo;
 }
 
+// One item: blocks b0 .. b1 - 1 of a tile (of those that its rows see). slot: of the partial output, -1 for a whole tile.
 struct PtItem {
   PtSeq q;
-  int b, h, tile, split, splits, slot;   // slot: of the partial output, -1 for a whole tile
+  int b, h, tile, b0, b1, slot;
 };
+
+// blocks that tile `tile` of R rows sees
 template <int R, int PB>
-__device__ __forceinline__ PtItem pt_item(const PagedAttnArgs& a, const PtList& t, int item, int lo, int hi) {
+__device__ __forceinline__ int pt_seen(const PagedAttnArgs& a, const PtSeq& q, int tile) {
+  const int G = a.H / a.KVH, last = q.kv - q.n + min(tile * R + R - 1, q.n * G - 1) / G;
+  return last < 0 ? 0 : min(q.blocks, last / PB + 1);
+}
+
+// the item of workgroup w that starts at block `at` of all narrow blocks; `end`: of its range. Returns the next start.
+template <int PB>
+__device__ __forceinline__ int pt_item_narrow(const PagedAttnArgs& a, const PtList& t, int w, int at, int end, int hi, PtItem& it) {
+  it.b = __builtin_amdgcn_readfirstlane(pt_find(t.items, a.B, at));
+  it.q = pt_seq<PT_NARROW, PB>(a, it.b, pt_ldc(a.q_start, it.b), pt_ldc(a.q_start, it.b + 1), pt_ldc(a.kv_len, it.b), 0, hi);
+  const int i = at - (it.b ? __builtin_amdgcn_readfirstlane(t.items[it.b - 1]) : 0), tl = i / it.q.blocks;
+  it.tile = tl % it.q.tiles, it.h = tl / it.q.tiles;
+  it.b0 = i % it.q.blocks, it.b1 = min(it.q.blocks, it.b0 + end - at);
+  const int next = at + it.b1 - it.b0;
+  // the first part of a split tile ends its workgroup's range (slot 2 w + 1), the others begin theirs (2 w)
+  it.slot = it.b0 > 0 ? 2 * w : it.b1 < it.q.blocks ? 2 * w + 1 : -1;
+  const int seen = pt_seen<PT_NARROW, PB>(a, it.q, it.tile);
+  it.b0 = min(it.b0, seen), it.b1 = min(it.b1, seen);
+  return next;
+}
+
+__device__ __forceinline__ PtItem pt_item_wide(const PagedAttnArgs& a, const PtList& t, int item) {
   PtItem it;
   it.b = __builtin_amdgcn_readfirstlane(pt_find(t.items, a.B, item));
-  const int s0 = pt_ldc(a.q_start, it.b), s1 = pt_ldc(a.q_start, it.b + 1), kv = pt_ldc(a.kv_len, it.b);
-  it.q = pt_seq<R, PB>(a, it.b, s0, s1, kv, lo, hi);
-  it.splits = pt_splits(it.q, t.share);
-  const int first = it.b ? t.items[it.b - 1] : 0;
-  const int i = __builtin_amdgcn_readfirstlane(item - first);   // (head, split, tile from the last)
+  it.q = pt_seq<PT_WIDE, 64>(a, it.b, pt_ldc(a.q_start, it.b), pt_ldc(a.q_start, it.b + 1), pt_ldc(a.kv_len, it.b),
+                             PT_NARROW, 0x7fffffff);
+  const int S = pt_splits(it.q, __builtin_amdgcn_readfirstlane(t.share));
+  const int i = item - (it.b ? __builtin_amdgcn_readfirstlane(t.items[it.b - 1]) : 0);   // (head, split, tile from the last)
   it.tile = it.q.tiles - 1 - i % it.q.tiles;
-  it.split = i / it.q.tiles % it.splits;
-  it.h = i / it.q.tiles / it.splits;
-  const int base = it.b ? t.slots[it.b - 1] : 0;
-  it.slot = it.splits > 1 ? __builtin_amdgcn_readfirstlane(base + (it.h * it.q.tiles + it.tile) * it.splits + it.split) : -1;
+  const int split = i / it.q.tiles % S;
+  it.h = i / it.q.tiles / S;
+  it.slot = S > 1 ? (it.b ? __builtin_amdgcn_readfirstlane(t.slots[it.b - 1]) : 0) + (it.h * it.q.tiles + it.tile) * S + split : -1;
+  const int seen = pt_seen<PT_WIDE, 64>(a, it.q, it.tile);
+  it.b0 = (int)((long long)seen * split / S), it.b1 = (int)((long long)seen * (split + 1) / S);
   return it;
 }
 
@@ -356,17 +419,24 @@ struct PtWave {
     c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);   // (0: every score counts alike)
   }
 
-  // scores of 32 NB positions from Kt
+  // scores of 32 NB positions from Kt; the operands are read eight (D = 64: four) ahead
   template <int NB>
   __device__ __forceinline__ void scores(const char* Kt, pt_f32x16 (&s)[NB]) const {
+    constexpr int KS = D / 16;
+    uint4 k[KS];
+    auto read = [&](int sb, int ks) { return *(const uint4*)(Kt + (sb * 32 + fr) * RB + (((2 * ks + hi) ^ pt_xk<D>(fr)) * 16)); };
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k[ks] = read(0, ks);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[sb][e] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint4 k = *(const uint4*)(Kt + (sb * 32 + fr) * RB + (((2 * ks + hi) ^ pt_xk<D>(fr)) * 16));
-        s[sb] = pt_mfma<DT>(k, qf[ks], s[sb]);
+      for (int ks = 0; ks < KS; ++ks) {
+        s[sb] = pt_mfma<DT>(k[ks], qf[ks], s[sb]);
+        if (sb + 1 < NB) k[ks] = read(sb + 1, ks);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -409,13 +479,15 @@ struct PtWave {
         for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
     }
     const float mc = m == -INFINITY ? 0.f : -m * c;   // nothing open yet: every score is -inf
+    float sum[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[sb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sb][e], c, mc));
-        l += s[sb][e];
+        sum[e & 3] += s[sb][e];
       }
+    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
 
   __device__ __forceinline__ uint4 vfrag(const char* Vt, int sb, int hf, int t) const {
@@ -456,6 +528,7 @@ struct PtWave {
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int t = 0; t < TD; ++t) o[t] = pt_mfma<DT>(vfrag(Vt, sb, hf, t), p[2 * sb + hf], o[t]);
+    pt_feed<2 * NB * TD, 2>();
   }
 
   // Closed positions have probability 0, but a value there may be anything, and 0 x NaN is NaN. Those that are closed to
@@ -611,11 +684,7 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
   char* Kt = lds + wave * 16384;
   char* Vt = Kt + 8192;
   const unsigned k0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)Kt, v0 = k0 + 8192;
-  // blocks of this tile (up to its last row's position), this split's, this wave's
-  const int tlast = min(row0 + 31, rows - 1) / G;
-  const int need = min(it.q.blocks, (it.q.kv - it.q.n + tlast) / PB + 1);
-  const int nblk = it.q.kv - it.q.n + tlast < 0 ? 0 : need;
-  const int b0 = (int)((long long)nblk * it.split / it.splits), b1 = (int)((long long)nblk * (it.split + 1) / it.splits);
+  const int b0 = it.b0, b1 = it.b1;
   auto load_k = [&](const PtPages<NG>& pg, int blk) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -740,8 +809,7 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
   const int first = it.q.kv - it.q.n;   // position of token 0
   const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
-  const int nblk = first + tlast < 0 ? 0 : min(it.q.blocks, (first + tlast) / PB + 1);
-  const int b0 = (int)((long long)nblk * it.split / it.splits), b1 = (int)((long long)nblk * (it.split + 1) / it.splits);
+  const int b0 = it.b0, b1 = it.b1;
   auto issue = [&](const PtPages<NG>& pg, int blk) {
     const unsigned dst = lds0 + (unsigned)(blk & 1) * 2 * BYTES + (unsigned)wave * LPG * 1024;
     const int id = wave == 0 ? pg.id[0] : wave == 1 ? pg.id[1] : wave == 2 ? pg.id[2] : pg.id[3];
@@ -790,7 +858,7 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
   }
   const float l = w.row_sum();
   const int row = row0 + w.fr;
-  const long long part = (long long)a.narrow_slots * 32 + (long long)it.slot * PT_WIDE;
+  const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
   if (row0 < rows && w.bad_output()) {
     pt_rows<DT, D>(a, it, tile0, row0, min(row0 + 32, rows), 1, b0 * PB, b1 * PB, part);
   } else if (row < rows) {
@@ -821,86 +889,125 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 
 // ------------------------------------------------------------------ kernels
 
-// all: rows of any number on narrow tiles (launches whose batches are nearly all single tokens)
+// grid_wide = 0: sequences of any number of rows on narrow tiles (batches that are nearly all single tokens)
 template <int DT, int D>
 __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
-  using C = PtNarrow<DT, D>;
-  constexpr int ANY = 0x7fffffff;
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
   __shared__ float ml[4][2][32];
   __shared__ PtList t;
   const int nw = a.grid_wide;
-  int cost;
+  int x;
   if ((int)blockIdx.x >= nw) {
-    const int hi = nw ? PT_NARROW : ANY;
-    const int n = pt_build<PT_NARROW, C::PB, PT_NARROW_ITEMS, PT_NARROW_MIN>(a, t, 0, hi, &cost);
-    for (int item = blockIdx.x - nw; item < n; item += gridDim.x - nw)
-      pt_narrow<DT, D>(a, pt_item<PT_NARROW, C::PB>(a, t, item, 0, hi), lds, ml);
+    const int hi = nw ? PT_NARROW : ANY, w = blockIdx.x - nw;
+    const int all = pt_build_narrow<NPB>(a, t, hi, &x), workers = pt_workers(all, gridDim.x - nw);
+    if (w >= workers) return;
+    const int end = pt_first(all, workers, w + 1);
+    for (int at = pt_first(all, workers, w); at < end;) {
+      PtItem it;
+      at = pt_item_narrow<NPB>(a, t, w, at, end, hi, it);
+      pt_narrow<DT, D>(a, it, lds, ml);
+    }
     return;
   }
-  const int n = pt_build<PT_WIDE, 64, PT_WIDE_ITEMS, PT_WIDE_MIN>(a, t, PT_NARROW, ANY, &cost);
-  // XCD x (workgroups x, x + 8, ...) takes the items whose running cost falls into its eighth of the whole
-  auto bound = [&](int x) {
-    if (x >= 8) return n;
-    const int at = (int)((long long)cost * x / 8);
+  const int n = pt_build_wide<false>(a, t, &x);
+  // XCD i (workgroups i, i + 8, ...) takes the items whose running cost falls into its eighth of the whole
+  auto bound = [&](int i) {
+    if (i >= 8) return n;
+    const int at = (int)((long long)x * i / 8);
     const int b = pt_find(t.cost, a.B, at);
     const int c0 = b ? t.cost[b - 1] : 0, i0 = b ? t.items[b - 1] : 0;
     const int ci = t.cost[b] - c0, ii = t.items[b] - i0;
     return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
   };
   const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
-  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3)
-    pt_wide<DT, D>(a, pt_item<PT_WIDE, 64>(a, t, item, PT_NARROW, ANY), lds);
+  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds);
 }
 
-// k_paged_combine: joins the partial outputs of split tiles, a wave per row, and zeroes the rows of no sequence.
-template <int DT, int D, bool WIDE>
-__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, PtList& t, int me, int waves) {
-  constexpr int R = WIDE ? PT_WIDE : PT_NARROW, PB = WIDE ? 64 : PtNarrow<DT, D>::PB, ANY = 0x7fffffff, E = D / 64;
-  constexpr int ITEMS = WIDE ? PT_WIDE_ITEMS : PT_NARROW_ITEMS, LEAST = WIDE ? PT_WIDE_MIN : PT_NARROW_MIN;
-  const int lo = WIDE ? PT_NARROW : 0, hi = WIDE || !a.grid_wide ? ANY : PT_NARROW, lane = threadIdx.x & 63;
-  const int G = a.H / a.KVH;
+// Joins S parts of one row (by a wave): row `p` of the slots that at(s) gives.
+template <int DT, int D, int R, typename F>
+__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long base, int r, int S, F at, uint16_t* out) {
+  // a load covers PER parts: lane (part, 4 dims)
+  constexpr int LN = D / 4, PER = 64 / LN;
+  const int lane = threadIdx.x & 63;
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
-  int rows;
-  pt_build<R, PB, ITEMS, LEAST, true>(a, t, lo, hi, &rows);
-  for (int u = me; u < rows; u += waves) {   // (sequence, head, row)
-    const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
-    const PtSeq q = pt_seq<R, PB>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), lo, hi);
-    const int S = pt_splits(q, t.share), i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
-    const int slot = (b ? t.slots[b - 1] : 0) + (h * q.tiles + row / R) * S;
-    const long long p = (WIDE ? (long long)a.narrow_slots * PT_NARROW : 0) + (long long)slot * R + row % R;
-    float M = -INFINITY, L = 0.f, x[E] = {};
-    for (int s = 0; s < S; ++s) M = fmaxf(M, a.part_ml[(p + (long long)s * R) * 2]);
-    for (int s = 0; s < S; ++s) {
-      const long long ps = p + (long long)s * R;
-      const float m = a.part_ml[ps * 2], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c);
-      L += f * a.part_ml[ps * 2 + 1];
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += f * a.part_o[ps * D + lane * E + e];
+  float M = -INFINITY;
+  for (int s = lane; s < S; s += 64) M = fmaxf(M, a.part_ml[(base + (long long)at(s) * R + r) * 2]);
+  M = wave_max(M);
+  float L = 0.f, x[4] = {};
+  for (int s0 = 0; s0 < S; s0 += 64) {
+    const int n = min(64, S - s0);
+    float f = 0.f;
+    if (lane < n) {
+      const float2 v = *(const float2*)(a.part_ml + (base + (long long)at(s0 + lane) * R + r) * 2);
+      f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v.x - M) * c);
+      L += f * v.y;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int tk = row / G;
-    uint16_t* out = (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D + lane * E;
+    for (int j = 0; j < n; j += 8 * PER) {   // eight loads in flight; past the last part: it again, weighed 0
+      float4 v[8];
+      float g[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = gm_pack<DT>(x[e] * inv);
+      for (int i = 0; i < 8; ++i) {
+        const int k = j + i * PER + lane / LN, s = min(k, n - 1);
+        const float fs = __shfl(f, s, 64);
+        g[i] = k < n ? fs : 0.f;
+        v[i] = *(const float4*)(a.part_o + (base + (long long)at(s0 + s) * R + r) * D + (lane % LN) * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[0] += g[i] * v[i].x, x[1] += g[i] * v[i].y, x[2] += g[i] * v[i].z, x[3] += g[i] * v[i].w;
+    }
   }
+  L = wave_sum(L);
+#pragma unroll
+  for (int o = LN; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o, 64);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (lane < LN) *(uint2*)(out + lane * 4) = make_uint2(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv));
 }
 
+// k_paged_combine: joins the parts of split tiles, a wave per row and head, and zeroes the rows of no sequence.
+// (A part without open positions has maximum -inf and outputs of zero.)
 template <int DT, int D>
 __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ PtList t;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = gridDim.x * 4, me = blockIdx.x * 4 + wave;
-  pt_join<DT, D, false>(a, t, me, waves);
+  const int G = a.H / a.KVH, waves = gridDim.x * 4, me = blockIdx.x * 4 + wave, hi = a.grid_wide ? PT_NARROW : ANY;
+  auto out = [&](const PtSeq& q, int h, int row) {
+    const int tk = row / G;
+    return (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D;
+  };
+  int rows;
+  const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers(all, a.grid_narrow);
+  for (int u = me; u < rows; u += waves) {   // (sequence, head, row)
+    const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
+    const PtSeq q = pt_seq<PT_NARROW, NPB>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), 0, hi);
+    const int i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
+    const int g0 = (b ? t.items[b - 1] : 0) + (h * q.tiles + row / PT_NARROW) * q.blocks;
+    // workgroups that hold its first and last block
+    const int w0 = (int)((((long long)g0 + 1) * workers - 1) / all);
+    const int w1 = (int)((((long long)g0 + q.blocks) * workers - 1) / all);
+    if (w0 == w1) continue;
+    pt_join<DT, D, PT_NARROW>(a, 0, row % PT_NARROW, w1 - w0 + 1, [&](int s) { return 2 * (w0 + s) + (s == 0); }, out(q, h, row));
+  }
   if (a.grid_wide) {
     __syncthreads();
-    pt_join<DT, D, true>(a, t, me, waves);
+    pt_build_wide<true>(a, t, &rows);
+    for (int u = me; u < rows; u += waves) {
+      const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
+      const PtSeq q = pt_seq<PT_WIDE, 64>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), PT_NARROW, ANY);
+      const int S = pt_splits(q, t.share), i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
+      const int slot = (b ? t.slots[b - 1] : 0) + (h * q.tiles + row / PT_WIDE) * S;
+      pt_join<DT, D, PT_WIDE>(a, (long long)2 * a.grid_narrow * PT_NARROW, row % PT_WIDE, S, [&](int s) { return slot + s; },
+                              out(q, h, row));
+    }
   }
   const int s0 = a.q_start[0], s1 = a.q_start[a.B];
   for (int row = me; row < a.N; row += waves) {
     if (row >= s0 && row < s1) continue;
-    uint4* out = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
-    for (int i = lane; i < a.H * D / 8; i += 64) out[i] = make_uint4(0, 0, 0, 0);
+    uint4* o = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
+    for (int i = lane; i < a.H * D / 8; i += 64) o[i] = make_uint4(0, 0, 0, 0);
   }
 }
 

@@ -9,10 +9,10 @@ from npu_compiler.ir_reader import OpNode
 from npu_runtime.serving_ops import check_paged_append, check_paged_attention, check_sample
 
 PAGED_ANY_MAX_D = 256          # paged.hip PG_ANY_D
-# paged.hip: sequences of an item list, rows of a tile, items that tiles are split towards, fewest blocks of a split
-PT_MAXB, PT_NARROW, PT_WIDE = 1024, 32, 128
-PT_NARROW_ITEMS, PT_WIDE_ITEMS, PT_NARROW_MIN, PT_WIDE_MIN = 2048, 480, 8, 8
-PT_GRID_NARROW = 4096          # workgroups of narrow items, which take more than one each past it
+# paged.hip: sequences of a list, rows of a tile, fewest blocks of a narrow workgroup and of a wide tile's split, items
+# that wide tiles are split towards
+PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
+PT_GRID = 512                  # two workgroups per CU
 SAMPLE_MAX_PIECES = 4096 * 64  # sample.hip SM_GROUPS groups of 64 pieces of 16 bytes
 
 
@@ -60,18 +60,16 @@ def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_s
     G, block = H // KVH, 8192 // (2 * D)
     blocks = -(-M * page_size // block)
     tiles = lambda R: KVH * (N * G // R + min(N, B))
-    if (tiles(PT_NARROW) + 2 * PT_NARROW_ITEMS) * (blocks + 3) >= 2 ** 31 or M * page_size * page_size >= 2 ** 40 \
+    if (tiles(PT_NARROW) + 2 * PT_GRID) * (2 * blocks + 3) >= 2 ** 31 or M * page_size * page_size >= 2 ** 40 \
             or KVH * page_size * D >= 2 ** 30:
         return None
     wide = N > 2 * B and N * G > PT_NARROW
-    # a split sequence has ceil(blocks / share) < 2 blocks / share slots per tile, all together under twice the items
-    # aimed at; nor can a tile have more than its blocks allow
-    slots = lambda R, items, least: min(2 * items, tiles(R) * -(-blocks // least))
-    return {"grid_wide": min(512, 8 * -(-(tiles(PT_WIDE) + PT_WIDE_ITEMS) // 8)) if wide else 0,
-            "grid_narrow": min(tiles(PT_NARROW) + PT_NARROW_ITEMS, PT_GRID_NARROW,
-                               tiles(PT_NARROW) * max(1, -(-blocks // PT_NARROW_MIN))),
-            "narrow_slots": slots(PT_NARROW, PT_NARROW_ITEMS, PT_NARROW_MIN),
-            "wide_slots": slots(PT_WIDE, PT_WIDE_ITEMS, PT_WIDE_MIN) if wide else 0}
+    # a split tile has ceil(blocks / share) < 2 blocks / share parts, all together under twice the items aimed at;
+    # nor can a tile have more than its blocks allow
+    slots = min(2 * PT_WIDE_ITEMS, tiles(PT_WIDE) * -(-blocks // PT_WIDE_LEAST))
+    return {"grid_wide": min(PT_GRID, 8 * -(-(tiles(PT_WIDE) + PT_WIDE_ITEMS) // 8)) if wide else 0,
+            "grid_narrow": min(PT_GRID, -(-tiles(PT_NARROW) * blocks // PT_NARROW_LEAST)),
+            "wide_slots": slots if wide else 0}
 
 
 def _batch(low, table, q_start, kv_len) -> dict:
@@ -127,7 +125,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
                 scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
-                narrow_slots=0, pad=0)
+                grid_narrow=0, pad=0)
     params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
     ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
     if tiled is None:
@@ -135,11 +133,11 @@ def lower_paged_attention(low, node: OpNode) -> None:
                             args=args, grid=(N, H, 1), block=(64, 1, 1), inputs=ins, outputs=outs, params=params))
         return
     groups = ps // 16
-    part_rows = tiled["narrow_slots"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
+    part_rows = 2 * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
                 part_ml=low.scratch(outs[0] + ".part_ml", 8 * part_rows), page_groups=groups,
                 group_magic=0 if groups == 1 else -(-2 ** 32 // groups), grid_wide=tiled["grid_wide"],
-                narrow_slots=tiled["narrow_slots"])
+                grid_narrow=tiled["grid_narrow"])
     name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
         kind="paged_attention", kernel="k_paged_attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),

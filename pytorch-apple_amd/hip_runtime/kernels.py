@@ -136,7 +136,7 @@ _struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), 
                           ("kv_len", P), ("q_rs", LL), ("q_hs", LL), ("page_stride", LL), ("head_stride", LL),
                           ("row_stride", LL), ("pages", LL), ("part_o", P), ("part_ml", P), ("N", I), ("B", I), ("M", I),
                           ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
-                          ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("narrow_slots", I),
+                          ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
                           ("pad", I)])
 _struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
                        ("rows", I), ("vocab", I), ("dtype", I), ("shift", I)])
