@@ -563,32 +563,43 @@ struct PtWave {
   }
 };
 
-// Pages of a block's groups of 16 positions: ids (0 where there is none) and which have none.
-template <int NG>
-struct PtPages {
-  int id[NG];
-  unsigned bad;
+// The places of 64 consecutive groups of 16 positions, a lane each: byte offset in a pool of the K/V head's row (of page
+// 0 where there is no page), and which have a page. Looked up once for 16 (or 32) blocks: a scalar load per block left its
+// latency, 700 cycles, in every block's way. The next window's page ids are on their way to the wave's slot of LDS
+// meanwhile (to registers, the compiler's wait for them would cover the K and V loads in flight).
+struct PtWindow {
+  uint32_t lo, hi;
+  unsigned long long ok;
 };
-template <int NG>
-__device__ __forceinline__ PtPages<NG> pt_pages(const PagedAttnArgs& a, int b, int p0) {
-  PtPages<NG> r;
-  r.bad = 0;
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const unsigned grp = (unsigned)(p0 >> 4) + g;
-    const unsigned at = a.group_magic ? __umulhi(grp, a.group_magic) : grp;
-    const int id = pt_ldc(a.table, (long long)b * a.M + min(at, (unsigned)a.M - 1));
-    const bool ok = at < (unsigned)a.M && (unsigned)id < (unsigned)a.pages;
-    r.id[g] = ok ? id : 0;
-    r.bad |= ok ? 0u : 1u << g;
-  }
-  return r;
+__device__ __forceinline__ unsigned pt_page_of(const PagedAttnArgs& a, int group) {   // may lie past the table
+  const unsigned grp = (unsigned)group + (threadIdx.x & 63);
+  return a.group_magic ? __umulhi(grp, a.group_magic) : grp;
 }
-// byte address of the 16-position group at p0 (K/V head h) in a pool
-__device__ __forceinline__ const char* pt_group(const PagedAttnArgs& a, const void* pool, int id, int h, int p0) {
-  const unsigned grp = (unsigned)(p0 >> 4);
-  const unsigned in = a.group_magic ? grp - __umulhi(grp, a.group_magic) * a.page_groups : 0;
-  return (const char*)pool + 2 * (id * a.page_stride + h * a.head_stride + (long long)(in * 16) * a.row_stride);
+__device__ __forceinline__ PtWindow pt_window(const PagedAttnArgs& a, const PtItem& it, int group, int id) {
+  PtWindow w;
+  const unsigned grp = (unsigned)group + (threadIdx.x & 63), at = pt_page_of(a, group);
+  const bool ok = at < (unsigned)a.M && (unsigned long long)(long long)id < (unsigned long long)a.pages;
+  const unsigned long long off = 2ull * ((ok ? id : 0) * a.page_stride + it.h * a.head_stride +
+                                         (ok ? (long long)((grp - at * a.page_groups) * 16) * a.row_stride : 0));
+  w.lo = (uint32_t)off, w.hi = (uint32_t)(off >> 32);
+  w.ok = __ballot(ok);
+  return w;
+}
+__device__ __forceinline__ PtWindow pt_window(const PagedAttnArgs& a, const PtItem& it, int group) {
+  return pt_window(a, it, group, a.table[(long long)it.b * a.M + min(pt_page_of(a, group), (unsigned)a.M - 1)]);
+}
+// page ids of a window to slot[64]
+__device__ __forceinline__ void pt_fetch(const PagedAttnArgs& a, const PtItem& it, int group, int* slot) {
+  const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) int*)slot;
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(
+                   min(pt_page_of(a, group), (unsigned)a.M - 1) * 4u),
+               "s"(a.table + (long long)it.b * a.M), "s"(lds)
+               : "memory", "m0");
+}
+
+// offset of group i of the window (uniform)
+__device__ __forceinline__ unsigned long long pt_place(const PtWindow& w, int i) {
+  return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(w.hi, i) << 32) | (uint32_t)__builtin_amdgcn_readlane(w.lo, i);
 }
 
 // One 1 KiB load of a group to LDS: rows i * (1024 / RB) .. of its 16, swizzled
@@ -666,6 +677,13 @@ __device__ __forceinline__ void pt_rows(const PagedAttnArgs& a, const PtItem& it
 
 // ------------------------------------------------------------------ narrow tiles
 
+struct PtK {
+  static constexpr bool value = false;
+};
+struct PtV {
+  static constexpr bool value = true;
+};
+
 template <int DT, int D>
 struct PtNarrow {
   static constexpr int PB = 8192 / (2 * D), NB = PB / 32, NG = PB / 16;   // positions of a block: 8 KiB of K, 8 of V
@@ -674,7 +692,7 @@ struct PtNarrow {
 };
 
 template <int DT, int D>
-__device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32]) {
+__device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32], int (*slots)[64]) {
   using C = PtNarrow<DT, D>;
   constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, OLD = C::OLD;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -685,28 +703,36 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
   char* Vt = Kt + 8192;
   const unsigned k0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)Kt, v0 = k0 + 8192;
   const int b0 = it.b0, b1 = it.b1;
-  auto load_k = [&](const PtPages<NG>& pg, int blk) {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const char* p = pt_group(a, a.k_pages, pg.id[g], it.h, blk * PB + 16 * g);
-#pragma unroll
-      for (int i = 0; i < LPG; ++i) pt_load<D, false>(p, row_bytes, i, k0 + (g * LPG + i) * 1024, lane);
+  constexpr int WB = 64 / NG;   // blocks of a window
+  PtWindow cur;
+  int* ids = slots[wave];
+  int wi;                       // window of cur
+  unsigned bad = 0, bad_next;   // groups of the present and the next block without a page
+  auto seek = [&](int blk) {    // cur: the block's window
+    if (blk / WB != wi) {
+      ++wi;
+      cur = pt_window(a, it, wi * 64, ids[lane]);
+      pt_fetch(a, it, (wi + 1) * 64, ids);
     }
+    return ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
   };
-  auto load_v = [&](const PtPages<NG>& pg, int blk) {
+  auto load = [&](auto v, int blk) {
+    constexpr bool V = decltype(v)::value;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const char* p = pt_group(a, a.v_pages, pg.id[g], it.h, blk * PB + 16 * g);
+      const char* p = (const char*)(V ? a.v_pages : a.k_pages) + pt_place(cur, blk % WB * NG + g);
 #pragma unroll
-      for (int i = 0; i < LPG; ++i) pt_load<D, true>(p, row_bytes, i, v0 + (g * LPG + i) * 1024, lane);
+      for (int i = 0; i < LPG; ++i) pt_load<D, V>(p, row_bytes, i, (V ? v0 : k0) + (g * LPG + i) * 1024, lane);
     }
   };
   int blk = b0 + wave;
-  PtPages<NG> pg, next;
   if (blk < b1) {
-    pg = pt_pages<NG>(a, it.b, blk * PB);
-    load_k(pg, blk);
-    load_v(pg, blk);
+    wi = blk / WB;
+    cur = pt_window(a, it, wi * 64);
+    pt_fetch(a, it, (wi + 1) * 64, ids);
+    bad = seek(blk);
+    load(PtK{}, blk);
+    load(PtV{}, blk);
   }
   w.init(a, it, row0);
   // the queries are waited for here: at their first use the wait would cover the loads in flight of every block
@@ -716,26 +742,28 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
   const int pmin = __builtin_amdgcn_readfirstlane(w.pos), pend = __builtin_amdgcn_readlane(w.pos, 31);
   for (; blk < b1; blk += 4) {
     const bool more = blk + 4 < b1;
-    if (more) next = pt_pages<NG>(a, it.b, (blk + 4) * PB);
-    const bool open = blk * PB + PB - 1 <= pmin && pg.bad == 0;
+    const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
     gm_vmcnt<8>();   // K has landed; V's eight loads may be on their way
     asm volatile("" ::: "memory");
     pt_f32x16 s[NB];
     w.template scores<NB>(Kt, s);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's rows are in registers
-    if (more) load_k(next, blk + 4);
-    if (!open) w.template mask<NB>(s, blk * PB, pg.bad);
+    if (more) {
+      bad_next = seek(blk + 4);
+      load(PtK{}, blk + 4);
+    }
+    if (!open) w.template mask<NB>(s, blk * PB, bad);
     w.template softmax<NB>(s);
     uint4 p[2 * NB];
     w.template pack<NB>(s, p);
     if (more) gm_vmcnt<8>();   // V has landed; the next K's eight loads may be on their way
     else gm_vmcnt<0>();
     asm volatile("" ::: "memory");
-    if (blk * PB + PB - 1 > pend || pg.bad) w.template clear_closed<NB>(Vt, blk * PB, pend, pg.bad);
+    if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
     w.template outputs<NB>(Vt, p);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) load_v(next, blk + 4);
-    pg = next;
+    if (more) load(PtV{}, blk + 4);
+    bad = bad_next;
   }
   // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
   const float l = w.row_sum();
@@ -800,7 +828,7 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
 // ------------------------------------------------------------------ wide tiles
 
 template <int DT, int D>
-__device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds) {
+__device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V
   constexpr int LPG = RB * 16 / 1024;                                   // loads per group: each wave takes its group's
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -810,21 +838,30 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
   const int first = it.q.kv - it.q.n;   // position of token 0
   const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
   const int b0 = it.b0, b1 = it.b1;
-  auto issue = [&](const PtPages<NG>& pg, int blk) {
+  constexpr int WB = 64 / NG;   // blocks of a window
+  PtWindow cur;
+  int* ids = slots[wave];
+  int wi = b0 / WB;             // window of cur
+  unsigned bad = 0, bad_next = 0;   // groups of the present and the next block without a page
+  auto issue = [&](int blk) {
+    if (blk / WB != wi) {
+      ++wi;
+      cur = pt_window(a, it, wi * 64, ids[lane]);
+      pt_fetch(a, it, (wi + 1) * 64, ids);
+    }
+    bad_next = ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
     const unsigned dst = lds0 + (unsigned)(blk & 1) * 2 * BYTES + (unsigned)wave * LPG * 1024;
-    const int id = wave == 0 ? pg.id[0] : wave == 1 ? pg.id[1] : wave == 2 ? pg.id[2] : pg.id[3];
-    const char* k = pt_group(a, a.k_pages, id, it.h, blk * PB + 16 * wave);
-    const char* v = pt_group(a, a.v_pages, id, it.h, blk * PB + 16 * wave);
+    const unsigned long long at = pt_place(cur, blk % WB * NG + wave);
+    const char *k = (const char*)a.k_pages + at, *v = (const char*)a.v_pages + at;
 #pragma unroll
     for (int i = 0; i < LPG; ++i) pt_load<D, false>(k, row_bytes, i, dst + i * 1024, lane);
 #pragma unroll
     for (int i = 0; i < LPG; ++i) pt_load<D, true>(v, row_bytes, i, dst + BYTES + i * 1024, lane);
   };
-  PtPages<NG> pg, next;
   if (b0 < b1) {
-    pg = pt_pages<NG>(a, it.b, b0 * PB);
-    issue(pg, b0);
-    next = pt_pages<NG>(a, it.b, (b0 + 1) * PB);
+    cur = pt_window(a, it, wi * 64);
+    pt_fetch(a, it, (wi + 1) * 64, ids);
+    issue(b0);
   }
   PtWave<DT, D> w;
   w.init(a, it, row0);
@@ -837,12 +874,8 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
   for (int blk = b0; blk < b1; ++blk) {
     gm_vmcnt<0>();
     __syncthreads();   // the block is in LDS, and every wave is done with the other stage
-    const unsigned bad = pg.bad;
-    if (blk + 1 < b1) {
-      issue(next, blk + 1);
-      pg = next;
-      next = pt_pages<NG>(a, it.b, (blk + 2) * PB);
-    }
+    bad = bad_next;
+    if (blk + 1 < b1) issue(blk + 1);
     if (blk * PB > pmax) continue;   // wave-uniform
     const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
     char* Kt = lds + (blk & 1) * 2 * BYTES;
@@ -895,6 +928,7 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
   constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
   __shared__ float ml[4][2][32];
+  __shared__ int ids[4][64];
   __shared__ PtList t;
   const int nw = a.grid_wide;
   int x;
@@ -906,7 +940,7 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     for (int at = pt_first(all, workers, w); at < end;) {
       PtItem it;
       at = pt_item_narrow<NPB>(a, t, w, at, end, hi, it);
-      pt_narrow<DT, D>(a, it, lds, ml);
+      pt_narrow<DT, D>(a, it, lds, ml, ids);
     }
     return;
   }
@@ -921,7 +955,7 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
   };
   const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
-  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds);
+  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
 }
 
 // Joins S parts of one row (by a wave): row `p` of the slots that at(s) gives.
