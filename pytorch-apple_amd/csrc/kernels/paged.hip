@@ -177,21 +177,6 @@ __device__ __forceinline__ uint2 pt_read_tr(const char* p) {
                                        (__attribute__((address_space(3))) pt_s16x4*)(__attribute__((address_space(3))) char*)p));
 }
 
-// Order of N matrix instructions with RD LDS reads each: the reads of four go ahead. (Left alone, the compiler reads one
-// operand, waits for it, multiplies, and reads the next into the same registers: 2.9 us for a wave's 32 x 64 block
-// of 32 matrix instructions, of which those are 0.4.)
-template <int N, int RD>
-__device__ __forceinline__ void pt_feed() {
-  constexpr int AHEAD = 4;
-  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RD, 0);   // LDS reads
-#pragma unroll
-  for (int i = 0; i < N - AHEAD; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);          // matrix instruction
-    __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-}
-
 // uniform load from memory that no kernel in flight writes
 __device__ __forceinline__ int pt_ldc(const int* p, long long i) {
   return ((const __attribute__((address_space(4))) int*)p)[i];
@@ -453,7 +438,7 @@ struct PtWave {
       }
   }
 
-  // maximum, exponentials (left in s), sums. Outputs are rescaled when a row's maximum has grown by more than 8 in
+  // Maximum and exponentials (left in s). Outputs are rescaled when a row's maximum has grown by more than 8 in
   // the exponent, not at every new maximum: the exponentials stay below 2^8, as exact as below 1, and of 32 rows some
   // row's maximum grows in nearly every block.
   template <int NB>
@@ -479,15 +464,10 @@ struct PtWave {
         for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
     }
     const float mc = m == -INFINITY ? 0.f : -m * c;   // nothing open yet: every score is -inf
-    float sum[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[sb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sb][e], c, mc));
-        sum[e & 3] += s[sb][e];
-      }
-    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int e = 0; e < 16; ++e) s[sb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sb][e], c, mc));
   }
 
   __device__ __forceinline__ uint4 vfrag(const char* Vt, int sb, int hf, int t) const {
@@ -520,15 +500,27 @@ struct PtWave {
     }
   }
 
+  // Outputs, and the sums of the exponentials s. The operands are read four ahead, in an order that the compiler keeps:
+  // left alone it read one, waited for it, multiplied and read the next (98 us for a long chunk's wide tiles; 94 so), or
+  // not, depending on code elsewhere.
   template <int NB>
-  __device__ __forceinline__ void outputs(const char* Vt, const uint4 (&p)[2 * NB]) {
+  __device__ __forceinline__ void outputs(const char* Vt, const uint4 (&p)[2 * NB], const pt_f32x16 (&s)[NB]) {
+    constexpr int N = 2 * NB * TD, EL = NB * 16 / N;
+    auto read = [&](int i) { return vfrag(Vt, i / TD / 2, i / TD % 2, i % TD); };
+    uint4 v[4];
+    float sum[2] = {l, 0.f};
 #pragma unroll
-    for (int sb = 0; sb < NB; ++sb)
+    for (int i = 0; i < 4; ++i) v[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+    for (int i = 0; i < N; ++i) {
+      o[i % TD] = pt_mfma<DT>(v[i % 4], p[i / TD], o[i % TD]);
+      if (i + 4 < N) v[i % 4] = read(i + 4);
 #pragma unroll
-        for (int t = 0; t < TD; ++t) o[t] = pt_mfma<DT>(vfrag(Vt, sb, hf, t), p[2 * sb + hf], o[t]);
-    pt_feed<2 * NB * TD, 2>();
+      for (int e = i * EL; e < i * EL + EL; ++e) sum[e & 1] += s[e / 16][e % 16];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l = sum[0] + sum[1];
   }
 
   // Closed positions have probability 0, but a value there may be anything, and 0 x NaN is NaN. Those that are closed to
@@ -760,7 +752,7 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
     else gm_vmcnt<0>();
     asm volatile("" ::: "memory");
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
-    w.template outputs<NB>(Vt, p);
+    w.template outputs<NB>(Vt, p, s);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) load(PtV{}, blk + 4);
     bad = bad_next;
@@ -883,11 +875,13 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     pt_f32x16 s[NB];
     w.template scores<NB>(Kt, s);
     if (!open) w.template mask<NB>(s, blk * PB, bad);
+    __builtin_amdgcn_s_setprio(1);   // vector instructions first: the other workgroup's matrix instructions run on beside them
     w.template softmax<NB>(s);
     uint4 p[2 * NB];
     w.template pack<NB>(s, p);
+    __builtin_amdgcn_s_setprio(0);
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
-    w.template outputs<NB>(Vt, p);
+    w.template outputs<NB>(Vt, p, s);
   }
   const float l = w.row_sum();
   const int row = row0 + w.fr;

@@ -253,3 +253,10 @@ def _special(backend, x, par):
     for k, t in {"logits": x, **par}.items():
         _SPECIAL["bufs"][k].native_handle.copy_(t)
     return _SPECIAL["dag"].execute(_SPECIAL["bufs"])[_SPECIAL["out"]].to_torch().cpu()
+
+
+@pytest.mark.parametrize("H,KVH,D,page", [(12, 2, 128, 16), (4, 4, 64, 32), (8, 1, 128, 48)])
+@pytest.mark.parametrize("new,kv", [(40, 3958), (70, 2040), (1, 9000), (2, 4095)])
+def test_paged_attention_of_long_tiles(backend, H, KVH, D, page, new, kv):
+    """Tiles split along their positions: parts that begin at the last block of a window of page ids, and at every other."""
+    _attention(backend, R.batch([new, 1], [kv, 77], page, seed=new), H, KVH, D, "bfloat16", page, "hnd")
