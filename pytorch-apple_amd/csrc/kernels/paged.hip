@@ -21,6 +21,9 @@ __device__ __forceinline__ int pg_page(const int* table, int b, int M, int page_
 }
 
 // ------------------------------------------------------------------ append
+
+#define PG_APPEND_R 256   // rotated dims of k_paged_append_bf16, _f16
+
 //
 // k_paged_append_any: one workgroup per row, one element pair (or one element past R) per thread and step; any
 // type, head size and strides. x'_j = x_j c - x_{j + R/2} d, x'_{j + R/2} = x_{j + R/2} c + x_j d with c, d the scaled
@@ -67,6 +70,70 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_any(const Paged
     st_f(a.v_pages, slot + h * a.head_stride + d, a.dtype, ld_f(a.v, row * a.v_rs + h * a.v_hs + d, a.dtype));
   }
 }
+
+// k_paged_append_*: rows of 16-byte pieces (16-bit types, whole pieces on both sides of every rotated pair, 16-byte
+// aligned rows). A wave per row, or the four waves of a workgroup where rows are few (_row): one row's chain of lookups
+// (q_start, kv_len, block_table, each waiting for the one before) is what it takes then, and its heads are done in one
+// step instead of three. Cosines and sines are taken once per row, for all heads, by a lane each. Bound by the bytes: each
+// row is read once and written once (5963 rows of 32 + 8 heads, 147 MB: %s).
+template <int DT, int WAVES>
+__device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
+  constexpr int ROWS = 4 / WAVES, TH = 64 * WAVES;
+  __shared__ __attribute__((aligned(16))) float cs[ROWS][2][PG_APPEND_R / 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = wave / WAVES, tid = (wave % WAVES) * 64 + lane;
+  const int row = blockIdx.x * ROWS + mine, half = a.R / 2;
+  const bool in = row < a.N;
+  const int b = in ? pg_sequence(a.q_start, a.B, row, lane) : a.B;
+  const bool real = b < a.B && row >= a.q_start[0];
+  const int pos = real ? a.kv_len[b] - a.q_start[b + 1] + row : 0;
+  const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
+  if (real)
+    for (int j = tid; j < half; j += TH) {
+      float s, c;
+      sincos_rot_d((double)pos * (double)a.inv_freq[j], &s, &c);
+      cs[mine][0][j] = c * a.scaling, cs[mine][1][j] = s * a.scaling;
+    }
+  __syncthreads();
+  if (!in) return;
+  const long long slot = page < 0 ? 0 : page * a.page_stride + (pos % a.page_size) * a.row_stride;
+  // steps: pairs of pieces, then the pieces past R, then v's
+  const int pairs = half / 8, rest = (a.D - a.R) / 8, qk = a.H + a.KVH;
+  const int n0 = qk * pairs, n1 = n0 + qk * rest, n2 = n1 + a.KVH * (a.D / 8);
+  for (int i = tid; i < n2; i += TH) {
+    const bool pair = i < n0, v = i >= n1;
+    const int k = pair ? i : v ? i - n1 : i - n0, per = pair ? pairs : v ? a.D / 8 : rest;
+    const int h = k / per, e = (pair ? 0 : v ? 0 : a.R) + k % per * 8;
+    const bool isq = !v && h < a.H;
+    if (!isq && page < 0) continue;
+    const int hk = v ? h : h - a.H;
+    const uint16_t* src = isq ? (const uint16_t*)a.q + row * a.q_rs + h * a.q_hs
+                         : v  ? (const uint16_t*)a.v + row * a.v_rs + hk * a.v_hs
+                              : (const uint16_t*)a.k + row * a.k_rs + hk * a.k_hs;
+    uint16_t* dst = isq ? (uint16_t*)a.q_out + ((long long)row * a.H + h) * a.D
+                        : (uint16_t*)(v ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
+    const uint4 x = *(const uint4*)(src + e);
+    if (!pair) {
+      *(uint4*)(dst + e) = real ? x : make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const uint4 y = *(const uint4*)(src + half + e);
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    uint32_t lo[4], up[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 c = *(const float2*)&cs[mine][0][e + 2 * j], d = *(const float2*)&cs[mine][1][e + 2 * j];
+      const float x0 = gm_lo<DT>(xw[j]), x1 = gm_hi<DT>(xw[j]), y0 = gm_lo<DT>(yw[j]), y1 = gm_hi<DT>(yw[j]);
+      lo[j] = real ? gm_pack2<DT>(x0 * c.x - y0 * d.x, x1 * c.y - y1 * d.y) : 0u;
+      up[j] = real ? gm_pack2<DT>(y0 * c.x + x0 * d.x, y1 * c.y + x1 * d.y) : 0u;
+    }
+    *(uint4*)(dst + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *(uint4*)(dst + half + e) = make_uint4(up[0], up[1], up[2], up[3]);
+  }
+}
+extern "C" __global__ void __launch_bounds__(256) k_paged_append_bf16(const PagedAppendArgs a) { append_body<HS_BF16, 1>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_append_bf16_row(const PagedAppendArgs a) { append_body<HS_BF16, 4>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16(const PagedAppendArgs a) { append_body<HS_F16, 1>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16_row(const PagedAppendArgs a) { append_body<HS_F16, 4>(a); }
 
 // ------------------------------------------------------------------ attention
 //

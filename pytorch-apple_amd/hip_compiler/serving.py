@@ -9,6 +9,8 @@ from npu_compiler.ir_reader import OpNode
 from npu_runtime.serving_ops import check_paged_append, check_paged_attention, check_sample
 
 PAGED_ANY_MAX_D = 256          # paged.hip PG_ANY_D
+PAGED_APPEND_MAX_R = 256       # paged.hip PG_APPEND_R
+PAGED_APPEND_ROW_N = 1024      # up to this many rows a workgroup per row, past it a wave
 # paged.hip: sequences of a list, rows of a tile, fewest blocks of a narrow workgroup and of a wide tile's split, items
 # that wide tiles are split towards
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
@@ -90,15 +92,22 @@ def lower_paged_append(low, node: OpNode) -> None:
     pools = [low.inplace_or_copy(t, o) for t, o in ((kp, node.outputs[1]), (vp, node.outputs[2]))]
     if N == 0:
         return
+    kernel, grid = "k_paged_append_any", N
+    R = 2 * int(inv.shape[0])
+    if q.dtype in ("bfloat16", "float16") and D % 8 == 0 and R % 16 == 0 and R <= PAGED_APPEND_MAX_R:
+        qv, kv, vv = (_aligned_rows(low, t.name, v) for t, v in ((q, qv), (k, kv), (v, vv)))
+        few = N <= PAGED_APPEND_ROW_N
+        kernel = f"k_paged_append_{'bf16' if q.dtype == 'bfloat16' else 'f16'}" + ("_row" if few else "")
+        grid = N if few else -(-N // 4)
     low.emit(LaunchStep(
-        kind="paged_append", kernel="k_paged_append_any", module="paged", arg_struct="PagedAppendArgs",
+        kind="paged_append", kernel=kernel, module="paged", arg_struct="PagedAppendArgs",
         args=dict(q=low.ref(qv), k=low.ref(kv), v=low.ref(vv), k_pages=low.ref(pools[0]), v_pages=low.ref(pools[1]),
                   q_out=low.ref(q_out), **_batch(low, table, q_start, kv_len),
                   inv_freq=low.ref(low.contiguous(inv.name)), q_rs=qv.strides[0], q_hs=qv.strides[1], k_rs=kv.strides[0],
                   k_hs=kv.strides[1], v_rs=vv.strides[0], v_hs=vv.strides[1], **_pool_strides(kp.shape, layout),
-                  pages=int(kp.shape[0]), N=N, H=H, KVH=KVH, D=D, R=2 * int(inv.shape[0]), page_size=ps,
+                  pages=int(kp.shape[0]), N=N, H=H, KVH=KVH, D=D, R=R, page_size=ps,
                   scaling=float(node.attrs.get("attention_scaling", 1.0)), dtype=DTYPE_CODE[q.dtype]),
-        grid=(N, 1, 1), inputs=[t.name for t in node.inputs], outputs=[o.name for o in node.outputs],
+        grid=(grid, 1, 1), inputs=[t.name for t in node.inputs], outputs=[o.name for o in node.outputs],
         params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D}))
 
 
