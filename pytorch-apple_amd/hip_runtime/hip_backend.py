@@ -102,9 +102,9 @@ class HIPBuffer(DeviceBuffer):
 
     def to_torch(self) -> torch.Tensor:
         """The device tensor with the logical shape (no copy)."""
-        n = int(np.prod(self._shape)) if self._shape else 1
-        if tuple(self._t.shape) == self._shape:
+        if self._t.shape == self._shape:   # (a torch.Size is a tuple; the product below costs 2 us)
             return self._t
+        n = int(np.prod(self._shape)) if self._shape else 1
         return self._t.reshape(-1)[:n].reshape(self._shape)
 
     def write_from_numpy(self, data, spec=None) -> None:

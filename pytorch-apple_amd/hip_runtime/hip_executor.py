@@ -22,6 +22,7 @@ graph inputs updated in place (KV caches) are the input buffers themselves.
 from __future__ import annotations
 
 import ctypes as C
+import itertools
 import operator
 import os
 from collections import OrderedDict
@@ -332,9 +333,11 @@ class HIPExecutor:
                 self._w_src, self._w_snap, self._w_key = weights, tuple(weights.values()), wk
         else:
             wk = self._w_key
-        bufs = tuple(self._lookup(n, inputs, weights) for n in self._in_names)
+        bufs = tuple(map(inputs.get, self._in_names))
+        if any(map(operator.is_, bufs, itertools.repeat(None))):
+            bufs = tuple(self._lookup(n, inputs, weights) for n in self._in_names)
         last = self._last_bufs
-        if last is not None and all(b is c for b, c in zip(bufs, last)):
+        if last is not None and all(map(operator.is_, bufs, last)):
             return (wk, self._last_in_key)
         ids = tuple(map(id, bufs))
         hit = self._in_cache.get(ids)
