@@ -640,6 +640,17 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   int pad;
 };
 
+struct SampleRow {            // sample.hip: what k_sample_merge finds out about a row
+  unsigned long long best;    // key of the first ranked token
+  double ahead;               // weight of the bins before kb, in units
+  double base;                // weight of the bins before plo
+  double total;               // weight of all tokens, where top-k cuts nothing
+  int mode;                   // 0: the first ranked, 1: every token, 2: a cut within the listed bins, 3: not binned
+  int kb, kr;                 // bin of the k-th token (-1: no cut) and its rank there, from 1
+  int plo, phi;               // bins in which the last kept token lies
+  int pad;
+};
+
 struct SampleArgs {           // sample.hip: one token per row of logits [rows, vocab]
   const void* logits;
   const float* temperature;   // [rows] each
@@ -648,10 +659,19 @@ struct SampleArgs {           // sample.hip: one token per row of logits [rows, 
   const float* min_p;
   const float* u;
   long long* out;             // [rows]
+  unsigned long long* best;   // [rows, parts] key of each part's first ranked token; null: no parts, k_sample_pick alone
+  unsigned* cnt;              // [rows, parts, bins] tokens
+  unsigned long long* wts;    // [rows, parts, bins] weights, relative to the part's largest
+  SampleRow* row;             // [rows]
+  unsigned long long* groups; // [rows, groups] weights of the kept tokens of 64 pieces
+  unsigned* listed;           // [rows] length of the row's list
+  unsigned long long* list;   // [rows, SM_LIST] keys of the tokens in the bins where the cuts lie
   int rows;
   int vocab;
   int dtype;
   int shift;                  // weights are integers of 2^-shift; vocab << shift < 2^63
+  int parts;
+  int ngroups;                // row stride of groups
 };
 
 // host and device (the rotary sincos below is also built into a host test helper)

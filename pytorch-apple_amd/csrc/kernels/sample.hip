@@ -1,26 +1,32 @@
 // One token per row of logits from a given uniform number, after temperature, top-k, top-p and min-p.
 //
-// k_sample_*: one workgroup of 1024 threads per row. With w = exp((l - max) / T), tokens ranked by (logit descending,
-// index ascending), the kept ones are those not after the k-th, not after the last whose preceding weights sum to less
-// than top_p of them all, and of w >= min_p; the token is the first by index at which the running sum of the kept
-// weights passes u times their sum.
+// With w = exp((l - max) / T), tokens ranked by (logit descending, index ascending), the kept ones are those not after
+// the k-th, not after the last whose preceding weights sum to less than top_p of them all, and of w >= min_p; the token
+// is the first by index at which the running sum of the kept weights passes u times their sum.
 //   * Weights are integers: w rounded to 2^-shift (2^-44 up to 2^18 tokens), from a double exponential of relative
 //     error below 2^-42. Their sums are exact in any order, so threads, waves and atomics add in whichever order they
 //     come and a call gives the same token every time; in 32-bit floats a border between two tokens would move by 1e-7
 //     of the sum, and with 150,000 borders a row in a thousand draws another token.
 //   * No sort. A token's rank is its 64-bit key, the logit's order-preserving bits over the inverted index (no two
-//     alike). The rows's first pass takes the largest; the second counts and weighs tokens in 2048 bins of (max - l)
-//     covering 32 T, where weights end (e^-32 rounds to 0: what lies past is in the last bin and weighs nothing). The
-//     bin in which the k-th token or the top-p sum falls is then split again by key, 2048 ways a pass, until at most
-//     1024 tokens are in it: those are gathered and ranked against each other. Typical rows need no second split; rows
-//     of equal logits take two more.
-//   * The last passes weigh the kept tokens in groups of 64 sixteen-byte pieces, find the group by a scan and the
-//     token within the group by one wave.
+//     alike). A cut is a key; what is needed of the row to find it are the tokens near it.
+//   * Rows are read twice, by many workgroups each, in four launches: _hist counts and weighs each part's tokens in
+//     512 bins of l of width T / 16, on one grid for all parts of a row and down from the part's largest (after 32 T
+//     weights round to 0, so the bins hold all that weigh); _merge adds the parts up and finds the bins in which the
+//     k-th token and the top-p sum lie; _collect sums the weights that are kept for sure in groups of 64 sixteen-byte
+//     pieces and lists the tokens of those bins; _pick ranks the listed ones (a few hundred to a few thousand), adds
+//     the kept ones to their groups, finds the group by a scan and the token in it by one wave.
+//   * _pick alone does a row of few tokens, and one that the bins do not tell apart (more than SM_LIST tokens in a
+//     bin: equal logits; infinite ones): it splits the range of keys 2048 ways a pass over the row until at most 256
+//     tokens are left around the cut.
 #include "common.h"
 
-#define SM_T 1024              // threads
-#define SM_BINS 2048
-#define SM_LIST 1024           // tokens ranked against each other
+#define SM_T 1024              // threads of _pick
+#define SM_TH 256              // of the others
+#define SM_BINS 512            // of width T / 16
+#define SM_PART 2048           // pieces of a part: 8 per thread, which stay in registers
+#define SM_LIST 4096           // tokens of the bins around the cuts
+#define SM_RANK 256            // tokens ranked against each other: n^2 reads of LDS, 4 us at 256
+#define SM_SPLIT 2048
 #define SM_GROUPS 4096         // groups of 64 pieces: vocab <= SM_GROUPS * 64 * (4 | 8)
 
 typedef unsigned long long u64;
@@ -62,7 +68,10 @@ struct SmRow {
   float max;
   double inv_t2;   // log2(e) / T
   int shift;
-  float bin_scale;
+  float scale;     // bins per unit of l
+  __device__ __forceinline__ void init(float largest, float T, int sh) {
+    max = largest, inv_t2 = 1.4426950408889634074 / (double)T, shift = sh, scale = 16.f / T;
+  }
   __device__ __forceinline__ double weight(float v) const {
     // (equal to the largest, also where both are infinite: 1)
     return v == max ? 1.0 : sm_exp2(((double)v - (double)max) * inv_t2);
@@ -72,11 +81,20 @@ struct SmRow {
     const double s = w * __builtin_bit_cast(double, (u64)(1023 + shift) << 52) + 4503599627370496.0;
     return __builtin_bit_cast(u64, s) & 0xFFFFFFFFFFFFFull;
   }
-  __device__ __forceinline__ int bin(float v) const {
-    const float d = v == max ? 0.f : (max - v) * bin_scale;
-    return d < (float)(SM_BINS - 1) ? (int)d : SM_BINS - 1;   // NaN too: the last
+  // whether the grid tells values apart. Below 2^20 v * scale is off by at most a 16th of a bin, and what is SM_BINS
+  // bins from the largest (e^-32 of it) still rounds to 0. A part's own bound is twice the row's, so that every part
+  // that reaches into a row's bins has its own.
+  __device__ __forceinline__ bool binned(float most) const {
+    return scale > 0.f && scale < INFINITY && fabsf(max * scale) < most;
+  }
+  __device__ __forceinline__ int grid(float v) const {   // non-decreasing in v
+    return (int)fminf(fmaxf(floorf(v * scale), -536870912.f), 536870912.f);
   }
 };
+// whether the row's first ranked token is the answer
+__device__ __forceinline__ bool sm_greedy(float max, float T, int top_k, float top_p) {
+  return !(T > 0.f) || max == -INFINITY || top_k == 1 || top_p <= 0.f;
+}
 
 __device__ __forceinline__ u64 sm_wave_sum(u64 v) {
 #pragma unroll
@@ -92,30 +110,33 @@ __device__ __forceinline__ u64 sm_wave_max(u64 v) {
   return v;
 }
 // inclusive scan over the wave
-__device__ __forceinline__ u64 sm_wave_scan(u64 v, int lane) {
+template <typename N>
+__device__ __forceinline__ N sm_wave_scan(N v, int lane) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(v, o, 64);
+    const N w = __shfl_up(v, o, 64);
     if (lane >= o) v += w;
   }
   return v;
 }
-// exclusive scan over the workgroup, and the total; red: 16 words
-__device__ __forceinline__ u64 sm_block_scan(u64 v, u64* red, u64* total) {
+// exclusive scan over TH threads, and the total; red: TH / 64 words
+template <int TH, typename N>
+__device__ __forceinline__ N sm_block_scan(N v, N* red, N* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 inc = sm_wave_scan(v, lane);
+  const N inc = sm_wave_scan(v, lane);
   __syncthreads();
   if (lane == 63) red[wave] = inc;
   __syncthreads();
-  u64 base = 0, all = 0;
+  N base = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < SM_T / 64; ++w) {
+  for (int w = 0; w < TH / 64; ++w) {
     base += w < wave ? red[w] : 0;
     all += red[w];
   }
   *total = all;
   return base + inc - v;
 }
+template <int TH>
 __device__ __forceinline__ u64 sm_block_max(u64 v, u64* red) {
   v = sm_wave_max(v);
   __syncthreads();
@@ -123,12 +144,12 @@ __device__ __forceinline__ u64 sm_block_max(u64 v, u64* red) {
   __syncthreads();
   v = 0;
 #pragma unroll
-  for (int w = 0; w < SM_T / 64; ++w) v = red[w] > v ? red[w] : v;
+  for (int w = 0; w < TH / 64; ++w) v = red[w] > v ? red[w] : v;
   return v;
 }
 
-// Pieces of 16 bytes of a row, aligned in memory whatever the vocabulary: piece c holds tokens c * E - skew ..,
-// those outside the row given as -inf with an index past 2^31 (key below every token's).
+// Pieces of 16 bytes of a row, aligned in memory whatever the vocabulary: piece c holds tokens c * E - skew .., those
+// outside the row given as -inf.
 template <int DT>
 struct SmPieces {
   static constexpr int E = DT == HS_F32 ? 4 : 8;
@@ -143,226 +164,466 @@ struct SmPieces {
     count = (skew + vocab + E - 1) / E;
   }
   __device__ __forceinline__ int first(int c) const { return c * E - skew; }
-  __device__ __forceinline__ void load(int c, float (&v)[E]) const {
-    const int i0 = first(c);
-    if (i0 >= 0 && i0 + E <= vocab) {
-      const uint4 q = *(const uint4*)(base + (long long)c * 16);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-      if constexpr (DT == HS_F32) {
+  __device__ __forceinline__ bool whole(int c) const { return c < count && first(c) >= 0 && first(c) + E <= vocab; }
+  // the piece's bits; a piece at the row's ends comes token by token, and nothing past them is read
+  __device__ __forceinline__ uint4 bits(int c) const {
+    if (whole(c)) return *(const uint4*)(base + (long long)c * 16);
+    constexpr uint32_t NINF = DT == HS_F32 ? 0xff800000u : DT == HS_BF16 ? 0xff80u : 0xfc00u;
+    uint32_t w[4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[2 * j] = gm_lo<DT>(w[j]), v[2 * j + 1] = gm_hi<DT>(w[j]);
-      }
-    } else {   // the row's ends, and nothing past them
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int i = i0 + j;
-        v[j] = i >= 0 && i < vocab ? ld_f(base, (long long)c * E + j, DT) : -INFINITY;
-      }
+    for (int j = 0; j < E; ++j) {
+      const int i = first(c) + j;
+      const bool in = c < count && i >= 0 && i < vocab;
+      if constexpr (DT == HS_F32) w[j] = in ? ((const uint32_t*)base)[(long long)c * E + j] : NINF;
+      else w[j / 2] |= (in ? (uint32_t)((const uint16_t*)base)[(long long)c * E + j] : NINF) << (16 * (j & 1));
     }
-#pragma unroll
-    for (int j = 0; j < E; ++j) v[j] = v[j] != v[j] ? -INFINITY : v[j];
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // f(value, index) for every token of the row, by all threads
+  __device__ __forceinline__ static void values(uint4 q, float (&v)[E]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      float x;
+      if constexpr (DT == HS_F32) x = __uint_as_float(w[j]);
+      else x = j & 1 ? gm_hi<DT>(w[j / 2]) : gm_lo<DT>(w[j / 2]);
+      v[j] = x != x ? -INFINITY : x;
+    }
+  }
+  __device__ __forceinline__ bool in(int i) const { return i >= 0 && i < vocab; }
+  // f(value, index) for every token of the row, by SM_T threads
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     for (int c = threadIdx.x; c < count; c += SM_T) {
       float v[E];
-      load(c, v);
-      const int i0 = first(c);
+      values(bits(c), v);
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (i0 + j >= 0 && i0 + j < vocab) f(v[j], i0 + j);
+        if (in(first(c) + j)) f(v[j], first(c) + j);
     }
   }
 };
 
+// ------------------------------------------------------------------ counts and weights of a part, by bins
+
+// grid (parts, rows). The part stays in registers between its maximum and its bins.
 template <int DT>
-__device__ __forceinline__ void sample_body(const SampleArgs& a) {
-  __shared__ u64 red[16];
-  __shared__ u64 wsum[SM_GROUPS];        // bins' weights, then groups'
+__device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
+  constexpr int E = SmPieces<DT>::E, N = SM_PART / SM_TH;
+  __shared__ u64 red[SM_TH / 64];
   __shared__ unsigned cnt[SM_BINS];
-  __shared__ u64 lkey[SM_LIST], lw[SM_LIST];
-  __shared__ unsigned ln;
-  __shared__ u64 pick[3];
-  static_assert(SM_GROUPS >= SM_BINS, "");
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ u64 wts[SM_BINS];
+  const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const SmPieces<DT> x(a, row);
-
-  u64 best = 0;
-  x.each([&](float v, int i) {
-    const u64 k = sm_key(v, i);
-    best = k > best ? k : best;
-  });
-  best = sm_block_max(best, red);
-  const float T = a.temperature[row], top_p = a.top_p[row], min_p = a.min_p[row], u = a.u[row];
+  uint4 q[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = x.bits(part * SM_PART + i * SM_TH + tid);
+  const float T = a.temperature[row], top_p = a.top_p[row];
   const int top_k = a.top_k[row];
+  if (part == 0 && tid == 0) a.listed[row] = 0;
+#pragma unroll
+  for (int i = 0; i < SM_BINS / SM_TH; ++i) cnt[i * SM_TH + tid] = 0, wts[i * SM_TH + tid] = 0;
+  u64 best = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float v[E];
+    x.values(q[i], v);
+    float m = v[0];
+    int at = 0;
+#pragma unroll
+    for (int j = 1; j < E; ++j)
+      if (v[j] > m) m = v[j], at = j;
+    // (a token outside the row, -inf, wins over none that is in it)
+    const int i0 = x.first(part * SM_PART + i * SM_TH + tid);
+    if (m == -INFINITY) at = max(0, -i0);
+    const u64 k = x.in(i0 + at) ? sm_key(m, i0 + at) : 0;
+    best = k > best ? k : best;
+  }
+  best = sm_block_max<SM_TH>(best, red);
+  const long long me = (long long)row * a.parts + part;
+  if (tid == 0) a.best[me] = best;
   SmRow r;
-  r.max = sm_value((uint32_t)(best >> 32));
-  if (!(T > 0.f) || r.max == -INFINITY) {   // the first ranked
-    if (tid == 0) a.out[row] = (int)~(uint32_t)best;
-    return;
-  }
-  r.inv_t2 = 1.4426950408889634074 / (double)T;
-  r.shift = a.shift;
-  r.bin_scale = (float)SM_BINS / 32.f / T;
-
-  u64 cut = 0;   // kept: keys >= cut
-  // One threshold: the smallest key with fewer than `need` before it (counting tokens or weights, of those above the
-  // present cut).
-  auto threshold = [&](bool weigh, u64 need) {
-    // first split, by bins of (max - l); later ones by key bits: members are keys in [lo, hi], bin (hi - key) >> sh
-    u64 lo = 0, hi = best, before = 0;
-    int sh = -1;
-    while (true) {
-      for (int i = tid; i < SM_BINS; i += SM_T) cnt[i] = 0, wsum[i] = 0;
-      __syncthreads();
-      x.each([&](float v, int i) {
-        const u64 k = sm_key(v, i);
-        if (k < cut || k < lo || k > hi) return;
-        const int bin = sh < 0 ? r.bin(v) : (int)((hi - k) >> sh);
-        atomicAdd(&cnt[bin], 1u);
-        if (weigh) {
-          const u64 w = r.units(r.weight(v));
-          if (w) atomicAdd(&wsum[bin], w);
-        }
-      });
-      __syncthreads();
-      const u64 c0 = cnt[2 * tid], c1 = cnt[2 * tid + 1], w0 = wsum[2 * tid], w1 = wsum[2 * tid + 1];
-      const u64 v0 = weigh ? w0 : c0, v1 = weigh ? w1 : c1;
-      u64 total;
-      const u64 ex = before + sm_block_scan(v0 + v1, red, &total);
-      if (tid == 0) pick[0] = ~0ull;
-      __syncthreads();
-      if (ex < need && ex + v0 >= need) pick[0] = 2 * tid, pick[1] = ex, pick[2] = c0;
-      else if (ex + v0 < need && ex + v0 + v1 >= need) pick[0] = 2 * tid + 1, pick[1] = ex + v0, pick[2] = c1;
-      __syncthreads();
-      const u64 bin = pick[0], at = pick[1], members = pick[2];
-      // none, or the last bin, whose tokens weigh nothing: all stay
-      if (bin == ~0ull || (sh < 0 && bin == SM_BINS - 1)) return;
-      before = at;
-      auto in = [&](float v, u64 k) {
-        return k >= cut && k >= lo && k <= hi && (sh < 0 ? (u64)r.bin(v) : (hi - k) >> sh) == bin;
-      };
-      if (members <= SM_LIST) {
-        if (tid == 0) ln = 0;
-        __syncthreads();
-        x.each([&](float v, int i) {
-          const u64 k = sm_key(v, i);
-          if (!in(v, k)) return;
-          const unsigned s = atomicAdd(&ln, 1u);
-          lkey[s] = k;
-          lw[s] = weigh ? r.units(r.weight(v)) : 1;
-        });
-        __syncthreads();
-        u64 mine = ~0ull;   // the largest of the inverted keys that stay
-        const int n = (int)ln;
-        if (tid < n) {
-          u64 b = before;
-          const u64 k = lkey[tid];
-          for (int j = 0; j < n; ++j) b += lkey[j] > k ? lw[j] : 0;
-          if (b < need) mine = k;
-        }
-        // the smallest key that stays
-        const u64 m = ~sm_block_max(~mine, red);
-        cut = m > cut ? m : cut;
-        return;
-      }
-      // the bin's range of keys, and the next split of it
-      u64 kmax = 0, kmin = 0;
-      x.each([&](float v, int i) {
-        const u64 k = sm_key(v, i);
-        if (!in(v, k)) return;
-        kmax = k > kmax ? k : kmax;
-        kmin = ~k > kmin ? ~k : kmin;
-      });
-      kmax = sm_block_max(kmax, red);
-      kmin = ~sm_block_max(kmin, red);
-      lo = kmin, hi = kmax;
-      const int bits = 64 - __builtin_clzll((hi - lo) | 1);
-      sh = bits > 11 ? bits - 11 : 0;
-    }
-  };
-  if (top_k > 0 && top_k < a.vocab) threshold(false, (u64)top_k);
-  // groups of 64 pieces: the weights of their kept tokens
-  const int groups = (x.count + 63) / 64;
-  const double floor_w = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
-  auto kept = [&](float v, int i, double least) -> u64 {
-    if (i < 0 || i >= a.vocab || sm_key(v, i) < cut) return 0;
-    const double w = r.weight(v);
-    return w >= least ? r.units(w) : 0;
-  };
-  auto weigh_groups = [&](double least) {
-    __syncthreads();
-    for (int g = wave; g < groups; g += SM_T / 64) {
-      u64 s = 0;
-      const int c = g * 64 + lane;
-      if (c < x.count) {
-        float v[SmPieces<DT>::E];
-        x.load(c, v);
+  r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
+  const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
+  if (sm_greedy(r.max, T, top_k, top_p) || !(k || p) || !r.binned(2097152.f)) return;
+  const int top = r.grid(r.max);
 #pragma unroll
-        for (int j = 0; j < SmPieces<DT>::E; ++j) s += kept(v[j], x.first(c) + j, least);
-      }
-      s = sm_wave_sum(s);
-      if (lane == 0) wsum[g] = s;
-    }
-    __syncthreads();
-  };
-  auto group_total = [&](u64& ex, u64 (&g)[SM_GROUPS / SM_T]) {
-    u64 s = 0, total;
+  for (int i = 0; i < N; ++i) {
+    float v[E];
+    x.values(q[i], v);
 #pragma unroll
-    for (int j = 0; j < SM_GROUPS / SM_T; ++j) {
-      const int i = tid * (SM_GROUPS / SM_T) + j;
-      g[j] = i < groups ? wsum[i] : 0;
-      s += g[j];
-    }
-    ex = sm_block_scan(s, red, &total);
-    return total;
-  };
-  u64 ex, g[SM_GROUPS / SM_T];
-  if (top_p < 1.f) {
-    if (!(top_p > 0.f)) {
-      cut = best;
-    } else {
-      weigh_groups(0.0);
-      const u64 total = group_total(ex, g);
-      const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
-      __syncthreads();
-      if (need < total) threshold(true, need);
+    for (int j = 0; j < E; ++j) {
+      const int bin = top - r.grid(v[j]);
+      if (bin >= SM_BINS) continue;   // (-inf, and so those outside the row, too)
+      atomicAdd(&cnt[bin], 1u);
+      if (p) atomicAdd(&wts[bin], r.units(r.weight(v[j])));
     }
   }
-  weigh_groups(floor_w);
-  const u64 total = group_total(ex, g);
-  const double t = (double)u * (double)total;
-  const u64 target = t > 0.0 ? (t < (double)total ? min((u64)t, total - 1) : total - 1) : 0;
-  if (tid == 0) pick[0] = 0, pick[1] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < SM_GROUPS / SM_T; ++j) {
-    if (ex <= target && ex + g[j] > target) pick[0] = tid * (SM_GROUPS / SM_T) + j, pick[1] = ex;
+  for (int i = 0; i < SM_BINS / SM_TH; ++i) {
+    a.cnt[me * SM_BINS + i * SM_TH + tid] = cnt[i * SM_TH + tid];
+    if (p) a.wts[me * SM_BINS + i * SM_TH + tid] = wts[i * SM_TH + tid];
+  }
+}
+
+// ------------------------------------------------------------------ the bins of the cuts
+
+// grid (rows). Thread i holds bins 2 i and 2 i + 1 of the row's, which count down from its largest value's.
+extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_merge(const SampleArgs a) {
+  static_assert(SM_BINS == 2 * SM_TH, "");
+  __shared__ u64 red[SM_TH / 64];
+  __shared__ unsigned redc[SM_TH / 64];
+  __shared__ double redw[SM_TH / 64];
+  __shared__ int kb, kr, plo, phi;
+  __shared__ double ahead, in_kb, base;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const u64* keys = a.best + (long long)row * a.parts;
+  u64 best = 0;
+  for (int p = tid; p < a.parts; p += SM_TH) best = keys[p] > best ? keys[p] : best;
+  best = sm_block_max<SM_TH>(best, red);
+  const float T = a.temperature[row], top_p = a.top_p[row];
+  const int top_k = a.top_k[row];
+  SmRow r;
+  r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
+  const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
+  SampleRow s;
+  s.best = best, s.ahead = s.base = s.total = 0.0, s.kb = -1, s.kr = 0, s.plo = s.phi = -1, s.pad = 0;
+  s.mode = sm_greedy(r.max, T, top_k, top_p) ? 0 : !r.binned(1048576.f) ? 3 : k || p ? 2 : 1;
+  if (s.mode != 2) {
+    if (tid == 0) a.row[row] = s;
+    return;
+  }
+  const int top = r.grid(r.max);
+  unsigned c[2] = {0, 0};
+  double w[2] = {0.0, 0.0};
+  for (int q = 0; q < a.parts; ++q) {
+    const u64 key = keys[q];
+    const float m = sm_value((uint32_t)(key >> 32));
+    if (key == 0 || m == -INFINITY) continue;
+    const int off = top - r.grid(m);   // the part's first bin, in the row's
+    const double f = r.weight(m);
+    const long long at = ((long long)row * a.parts + q) * SM_BINS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int bin = 2 * tid + i - off;
+      if (bin < 0) continue;
+      c[i] += a.cnt[at + bin];
+      if (p) w[i] += f * (double)a.wts[at + bin];
+    }
+  }
+  if (tid == 0) kb = -1, kr = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
+  unsigned call;
+  double wall;
+  const unsigned c0 = sm_block_scan<SM_TH>(c[0] + c[1], redc, &call);
+  const double w0 = sm_block_scan<SM_TH>(w[0] + w[1], redw, &wall);
+  if (k) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned before = c0 + (i ? c[0] : 0);
+      if (before < (unsigned)top_k && before + c[i] >= (unsigned)top_k) {
+        kb = 2 * tid + i, kr = top_k - (int)before;
+        ahead = w0 + (i ? w[0] : 0.0);
+        // the bin's first kr tokens weigh at least their share of it, and at most all
+        in_kb = w[i], base = w[i] * (double)kr / (double)c[i];
+      }
+    }
+  }
+  __syncthreads();
+  s.kb = kb, s.kr = kr, s.ahead = ahead, s.total = wall;
+  s.plo = s.phi = kb;
+  if (p) {
+    // (the slack covers weights rounded to a part's units here and to the row's there)
+    const double lo = kb < 0 ? wall : ahead + base, up = kb < 0 ? wall : ahead + in_kb;
+    const double plow = (double)top_p * lo * (1.0 - 1e-9), pup = (double)top_p * up * (1.0 + 1e-9);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const double before = w0 + (i ? w[0] : 0.0), after = w0 + w[0] + (i ? w[1] : 0.0);
+      if (before < plow && after >= plow) atomicMin(&plo, 2 * tid + i);
+      if (before < pup && after >= pup) atomicMin(&phi, 2 * tid + i);
+    }
+    __syncthreads();
+    const int last = kb < 0 ? SM_BINS - 1 : kb;
+    s.plo = min(plo, last), s.phi = min(phi, last);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (2 * tid + i == s.plo) base = w0 + (i ? w[0] : 0.0);
+    __syncthreads();
+    s.base = base;
+  } else if (kb < 0) {
+    s.mode = 1;   // (fewer tokens weigh anything than k)
+  }
+  if (tid == 0) a.row[row] = s;
+}
+
+// ------------------------------------------------------------------ kept weights by groups, tokens near the cuts
+
+// grid (parts, rows): wave i of a part takes its groups i, i + 4, ..., all loads in flight together.
+template <int DT>
+__device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
+  constexpr int E = SmPieces<DT>::E, N = SM_PART / SM_TH, CAP = 1024;
+  __shared__ u64 list[CAP];
+  __shared__ unsigned n, at;
+  const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const SmPieces<DT> x(a, row);
+  const int c0 = part * SM_PART + wave * 64 + lane;
+  uint4 q[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = x.bits(c0 + i * SM_TH);
+  const SampleRow s = a.row[row];
+  if (s.mode == 0 || s.mode == 3) return;
+  const float T = a.temperature[row], min_p = a.min_p[row];
+  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
+  SmRow r;
+  r.init(sm_value((uint32_t)(s.best >> 32)), T, a.shift);
+  const int top = r.grid(r.max), sure = s.mode == 1 ? SM_BINS : s.plo;
+  if (tid == 0) n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = c0 + i * SM_TH;
+    float v[E];
+    x.values(q[i], v);
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int bin = top - r.grid(v[j]);   // (outside the row: -inf, past every bin)
+      if (bin < sure) {
+        const double w = r.weight(v[j]);
+        sum += w >= least ? r.units(w) : 0;
+      } else if (s.mode == 2 && bin < SM_BINS && (bin <= s.phi || bin == s.kb)) {
+        const unsigned k = atomicAdd(&n, 1u);
+        if (k < CAP) list[k] = sm_key(v[j], x.first(c) + j);
+      }
+    }
+    sum = sm_wave_sum(sum);
+    const int g = (part * SM_PART + i * SM_TH) / 64 + wave;
+    if (lane == 0 && g < a.ngroups) a.groups[(long long)row * a.ngroups + g] = sum;
+  }
+  __syncthreads();
+  if (n == 0) return;
+  // (more than CAP: the row's count goes past SM_LIST, and k_sample_pick does it without the list)
+  if (tid == 0) at = atomicAdd(&a.listed[row], n > CAP ? SM_LIST + 1 : n);
+  __syncthreads();
+  for (int i = tid; i < (int)min(n, (unsigned)CAP); i += SM_TH)
+    if (at + i < SM_LIST) a.list[(long long)row * SM_LIST + at + i] = list[i];
+}
+
+// ------------------------------------------------------------------ the token
+
+struct SmCut {
+  u64 red[SM_T / 64];
+  unsigned cnt[SM_SPLIT];
+  u64 sum[SM_SPLIT];
+  u64 key[SM_RANK], w[SM_RANK];
+  unsigned n;
+  u64 pick[3];
+};
+
+// The smallest key in [lo, hi] with less than `need` before it: `before`, and the weights (1 each where `weigh` is
+// false) of the larger keys in [lo, hi]. each(f) calls f(key) for the keys of its thread; 0: none has it.
+template <typename F>
+__device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool weigh, u64 need, u64 before, u64 lo, u64 hi) {
+  const int tid = threadIdx.x;
+  auto units = [&](u64 k) { return weigh ? r.units(r.weight(sm_value((uint32_t)(k >> 32)))) : 1ull; };
+  u64 least = ~0ull, most = 0, members = 0;
+  each([&](u64 k) {
+    if (k < lo || k > hi) return;
+    least = k < least ? k : least, most = k > most ? k : most, ++members;
+  });
+  sm_block_scan<SM_T>(members, t.red, &members);
+  lo = ~sm_block_max<SM_T>(~least, t.red), hi = sm_block_max<SM_T>(most, t.red);
+  if (members == 0) return 0;
+  while (members > SM_RANK) {
+    const int bits = 64 - __builtin_clzll((hi - lo) | 1), sh = max(bits - 11, 0);
+    for (int i = tid; i < SM_SPLIT; i += SM_T) t.cnt[i] = 0, t.sum[i] = 0;
+    __syncthreads();
+    each([&](u64 k) {
+      if (k < lo || k > hi) return;
+      const int bin = (int)((hi - k) >> sh);
+      atomicAdd(&t.cnt[bin], 1u);
+      const u64 w = weigh ? units(k) : 0;
+      if (w) atomicAdd(&t.sum[bin], w);
+    });
+    __syncthreads();
+    const u64 c0 = t.cnt[2 * tid], c1 = t.cnt[2 * tid + 1];
+    const u64 v0 = weigh ? t.sum[2 * tid] : c0, v1 = weigh ? t.sum[2 * tid + 1] : c1;
+    u64 total;
+    const u64 ex = before + sm_block_scan<SM_T>(v0 + v1, t.red, &total);
+    if (tid == 0) t.pick[0] = ~0ull;
+    __syncthreads();
+    if (ex < need && ex + v0 >= need) t.pick[0] = 2 * tid, t.pick[1] = ex, t.pick[2] = c0;
+    else if (ex + v0 < need && ex + v0 + v1 >= need) t.pick[0] = 2 * tid + 1, t.pick[1] = ex + v0, t.pick[2] = c1;
+    __syncthreads();
+    const u64 bin = t.pick[0];
+    if (bin == ~0ull) return 0;
+    members = t.pick[2];
+    before = t.pick[1];
+    const u64 h = hi - (bin << sh);
+    lo = hi - lo >= ((bin + 1) << sh) ? h - ((1ull << sh) - 1) : lo;
+    hi = h;
+    __syncthreads();
+  }
+  if (tid == 0) t.n = 0;
+  __syncthreads();
+  each([&](u64 k) {
+    if (k < lo || k > hi) return;
+    const unsigned s = atomicAdd(&t.n, 1u);
+    t.key[s] = k;
+    t.w[s] = units(k);
+  });
+  __syncthreads();
+  u64 mine = ~0ull;
+  const int n = (int)t.n;
+  if (tid < n) {
+    u64 b = before;
+    const u64 k = t.key[tid];
+    for (int j = 0; j < n; ++j) b += t.key[j] > k ? t.w[j] : 0;
+    if (b < need) mine = k;
+  }
+  const u64 found = ~sm_block_max<SM_T>(~mine, t.red);
+  return found == ~0ull ? 0 : found;
+}
+
+// grid (rows)
+template <int DT>
+__device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
+  constexpr int E = SmPieces<DT>::E, PER = SM_GROUPS / SM_T;
+  __shared__ SmCut t;
+  __shared__ u64 groups[SM_GROUPS];
+  __shared__ u64 list[SM_LIST];
+  static_assert(SM_SPLIT == 2 * SM_T && SM_RANK <= SM_T, "");
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const SmPieces<DT> x(a, row);
+  const float T = a.temperature[row], top_p = a.top_p[row], min_p = a.min_p[row], u = a.u[row];
+  const int top_k = a.top_k[row];
+  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.0;
+  const bool k = top_k > 0 && top_k < a.vocab;
+  SampleRow s;
+  unsigned n = 0;
+  if (a.best) {
+    s = a.row[row];
+    n = a.listed[row];
+  } else {
+    u64 best = 0;
+    x.each([&](float v, int i) {
+      const u64 key = sm_key(v, i);
+      best = key > best ? key : best;
+    });
+    s.best = sm_block_max<SM_T>(best, t.red);
+    s.mode = sm_greedy(sm_value((uint32_t)(s.best >> 32)), T, top_k, top_p) ? 0 : 3;
+  }
+  if (s.mode == 0) {
+    if (tid == 0) a.out[row] = (int)~(uint32_t)s.best;
+    return;
+  }
+  SmRow r;
+  r.init(sm_value((uint32_t)(s.best >> 32)), T, a.shift);
+  const int ng = (x.count + 63) / 64;
+  u64 cut = 0;   // kept: keys >= cut
+  auto kept = [&](float v, int i, double at_least) -> u64 {
+    if (!x.in(i) || sm_key(v, i) < cut) return 0;
+    const double w = r.weight(v);
+    return w >= at_least ? r.units(w) : 0;
+  };
+  const bool listed = s.mode == 1 || (s.mode == 2 && n <= SM_LIST);
+  if (listed) {
+    for (int g = tid; g < ng; g += SM_T) groups[g] = a.groups[(long long)row * a.ngroups + g];
+    if (s.mode == 2) {
+      for (int i = tid; i < (int)n; i += SM_T) list[i] = a.list[(long long)row * SM_LIST + i];
+      __syncthreads();
+      const int top = r.grid(r.max);
+      auto each = [&](int b0, int b1, auto f) {   // keys of bins b0 .. b1
+        for (int i = tid; i < (int)n; i += SM_T) {
+          const int bin = top - r.grid(sm_value((uint32_t)(list[i] >> 32)));
+          if (bin >= b0 && bin <= b1) f(list[i]);
+        }
+      };
+      double total = s.total;
+      if (s.kb >= 0) {
+        cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, 0, s.best);
+        if (top_p < 1.f) {
+          u64 w = 0, all;
+          each(s.kb, s.kb, [&](u64 key) { w += key >= cut ? r.units(r.weight(sm_value((uint32_t)(key >> 32)))) : 0; });
+          sm_block_scan<SM_T>(w, t.red, &all);
+          total = s.ahead + (double)all;
+        }
+      }
+      if (top_p < 1.f) {
+        const u64 need = (u64)__builtin_ceil((double)top_p * total);
+        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, (u64)(s.base + 0.5), cut, s.best);
+        cut = c > cut ? c : cut;
+      }
+      __syncthreads();
+      for (int i = tid; i < (int)n; i += SM_T) {
+        const int idx = (int)~(uint32_t)list[i];
+        const u64 w = kept(sm_value((uint32_t)(list[i] >> 32)), idx, least);
+        if (w) atomicAdd(&groups[(idx + x.skew) / E / 64], w);
+      }
+    }
+  } else {
+    auto each = [&](auto f) { x.each([&](float v, int i) { f(sm_key(v, i)); }); };
+    auto weigh = [&](double at_least) {
+      __syncthreads();
+      for (int g = wave; g < ng; g += SM_T / 64) {
+        u64 w = 0;
+        float v[E];
+        x.values(x.bits(g * 64 + lane), v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) w += kept(v[j], x.first(g * 64 + lane) + j, at_least);
+        w = sm_wave_sum(w);
+        if (lane == 0) groups[g] = w;
+      }
+      __syncthreads();
+    };
+    if (k) cut = sm_cut(t, each, r, false, (u64)top_k, 0, 0, s.best);
+    if (top_p < 1.f) {
+      weigh(0.0);
+      u64 w = 0, total;
+      for (int g = tid; g < ng; g += SM_T) w += groups[g];
+      sm_block_scan<SM_T>(w, t.red, &total);
+      const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
+      const u64 c = sm_cut(t, each, r, true, need, 0, cut, s.best);
+      cut = c > cut ? c : cut;
+    }
+    weigh(least);
+  }
+  __syncthreads();
+  // the group in which the running sum passes u times the whole, and the token in it
+  u64 g[PER], w = 0, total;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) w += g[j] = tid * PER + j < ng ? groups[tid * PER + j] : 0;
+  u64 ex = sm_block_scan<SM_T>(w, t.red, &total);
+  const double want = (double)u * (double)total;
+  const u64 target = want > 0.0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;
+  if (tid == 0) t.pick[0] = 0, t.pick[1] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (ex <= target && ex + g[j] > target) t.pick[0] = tid * PER + j, t.pick[1] = ex;
     ex += g[j];
   }
   __syncthreads();
   if (wave == 0) {
-    const int c = (int)pick[0] * 64 + lane;
-    u64 w[SmPieces<DT>::E] = {}, s = 0;
-    if (c < x.count) {
-      float v[SmPieces<DT>::E];
-      x.load(c, v);
+    const int c = (int)t.pick[0] * 64 + lane;
+    float v[E];
+    x.values(x.bits(c), v);
+    u64 p[E], sum = 0;
 #pragma unroll
-      for (int j = 0; j < SmPieces<DT>::E; ++j) s += w[j] = kept(v[j], x.first(c) + j, floor_w);
-    }
-    u64 run = pick[1] + sm_wave_scan(s, lane) - s;
+    for (int j = 0; j < E; ++j) sum += p[j] = kept(v[j], x.first(c) + j, least);
+    u64 run = t.pick[1] + sm_wave_scan(sum, lane) - sum;
 #pragma unroll
-    for (int j = 0; j < SmPieces<DT>::E; ++j) {
-      if (run <= target && run + w[j] > target) a.out[row] = x.first(c) + j;
-      run += w[j];
+    for (int j = 0; j < E; ++j) {
+      if (run <= target && run + p[j] > target) a.out[row] = x.first(c) + j;
+      run += p[j];
     }
   }
 }
 
-extern "C" __global__ void __launch_bounds__(SM_T) k_sample_f32(const SampleArgs a) { sample_body<HS_F32>(a); }
-extern "C" __global__ void __launch_bounds__(SM_T) k_sample_f16(const SampleArgs a) { sample_body<HS_F16>(a); }
-extern "C" __global__ void __launch_bounds__(SM_T) k_sample_bf16(const SampleArgs a) { sample_body<HS_BF16>(a); }
+#define SM_KERNELS(NAME, DT)                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_hist_##NAME(const SampleArgs a) { sample_hist_body<DT>(a); }     \
+  extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_collect_##NAME(const SampleArgs a) { sample_collect_body<DT>(a); } \
+  extern "C" __global__ void __launch_bounds__(SM_T) k_sample_pick_##NAME(const SampleArgs a) { sample_pick_body<DT>(a); }
+SM_KERNELS(f32, HS_F32)
+SM_KERNELS(f16, HS_F16)
+SM_KERNELS(bf16, HS_BF16)

@@ -403,6 +403,7 @@ size_t hs_argsize(const char* s) {
   HS_SZ(PagedAppendArgs)
   HS_SZ(PagedAttnArgs)
   HS_SZ(SampleArgs)
+  HS_SZ(SampleRow)
 #undef HS_SZ
   return 0;
 }

@@ -15,7 +15,9 @@ PAGED_APPEND_ROW_N = 1024      # up to this many rows a workgroup per row, past 
 # that wide tiles are split towards
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
 PT_GRID = 512                  # two workgroups per CU
-SAMPLE_MAX_PIECES = 4096 * 64  # sample.hip SM_GROUPS groups of 64 pieces of 16 bytes
+# sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, pieces of a part, bins, tokens of a list
+SAMPLE_MAX_PIECES, SAMPLE_PART, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 2048, 512, 4096
+SAMPLE_PICK_PIECES = 1024      # up to this many pieces k_sample_pick alone
 
 
 def _rows_view(low, name: str) -> TView:
@@ -160,22 +162,36 @@ def lower_sample(low, node: OpNode) -> None:
     x, temperature, top_k, top_p, min_p, u = node.inputs
     check_sample(x, temperature, top_k, top_p, min_p, u)
     B, V = (int(s) for s in x.shape)
-    if V > (SAMPLE_MAX_PIECES - 1) * (16 // ELEM_SIZE[x.dtype]):
-        raise NotImplementedError(f"{node.op_type}: a vocabulary of {V} is over the kernel's {SAMPLE_MAX_PIECES} pieces")
+    if V > (SAMPLE_MAX_PIECES - 1) * (16 // ELEM_SIZE[x.dtype]) or B > 65535:
+        raise NotImplementedError(f"{node.op_type}: {B} rows of {V}: over 65,535 rows, or over the kernel's {SAMPLE_MAX_PIECES} "
+                                  f"pieces of the vocabulary")
     xv = low.aligned16(low.contiguous(x.name), x.name)
     out = low.new_storage(node.outputs[0].name, [B], "int64")
     low.views[node.outputs[0].name] = out
     if B == 0:
         return
-    low.emit(LaunchStep(
-        kind="sample", kernel={"float32": "k_sample_f32", "float16": "k_sample_f16",
-                               "bfloat16": "k_sample_bf16"}[x.dtype], module="sample", arg_struct="SampleArgs",
-        args=dict(logits=low.ref(xv), temperature=low.ref(low.contiguous(temperature.name)),
-                  top_k=low.ref(low.contiguous(top_k.name)), top_p=low.ref(low.contiguous(top_p.name)),
-                  min_p=low.ref(low.contiguous(min_p.name)), u=low.ref(low.contiguous(u.name)), out=low.ref(out), rows=B,
-                  vocab=V, dtype=DTYPE_CODE[x.dtype], shift=min(44, 62 - V.bit_length())),
-        grid=(B, 1, 1), block=(1024, 1, 1), inputs=[t.name for t in node.inputs], outputs=[node.outputs[0].name],
-        params={"rows": B, "vocab": V}))
+    per = 16 // ELEM_SIZE[x.dtype]
+    pieces = (V + per - 2) // per + 1   # most that a row, wherever it starts, can touch
+    parts, groups = -(-pieces // SAMPLE_PART), -(-pieces // 64)
+    binned = pieces > SAMPLE_PICK_PIECES
+    name = node.outputs[0].name
+    ws = (lambda what, nbytes: low.scratch(f"{name}.{what}", nbytes)) if binned else (lambda what, nbytes: None)
+    args = dict(logits=low.ref(xv), temperature=low.ref(low.contiguous(temperature.name)),
+                top_k=low.ref(low.contiguous(top_k.name)), top_p=low.ref(low.contiguous(top_p.name)),
+                min_p=low.ref(low.contiguous(min_p.name)), u=low.ref(low.contiguous(u.name)), out=low.ref(out),
+                best=ws("best", 8 * B * parts), cnt=ws("cnt", 4 * B * parts * SAMPLE_BINS),
+                wts=ws("wts", 8 * B * parts * SAMPLE_BINS), row=ws("row", 56 * B), groups=ws("groups", 8 * B * groups),
+                listed=ws("listed", 4 * B), list=ws("list", 8 * B * SAMPLE_LIST), rows=B, vocab=V,
+                dtype=DTYPE_CODE[x.dtype], shift=min(44, 62 - V.bit_length()), parts=parts, ngroups=groups)
+    dt = {"float32": "f32", "float16": "f16", "bfloat16": "bf16"}[x.dtype]
+    launches = [("k_sample_pick_" + dt, (B, 1, 1), 1024)]
+    if binned:
+        launches = [("k_sample_hist_" + dt, (parts, B, 1), 256), ("k_sample_merge", (B, 1, 1), 256),
+                    ("k_sample_collect_" + dt, (parts, B, 1), 256)] + launches
+    for kernel, grid, threads in launches:
+        low.emit(LaunchStep(kind="sample", kernel=kernel, module="sample", arg_struct="SampleArgs", args=dict(args),
+                            grid=grid, block=(threads, 1, 1), inputs=[t.name for t in node.inputs], outputs=[name],
+                            params={"rows": B, "vocab": V}))
 
 
 LOWERINGS = {"serving.paged_append.default": lower_paged_append,
