@@ -672,6 +672,8 @@ struct SampleArgs {           // sample.hip: one token per row of logits [rows, 
   int shift;                  // weights are integers of 2^-shift; vocab << shift < 2^63
   int parts;
   int ngroups;                // row stride of groups
+  int per;                    // a part is 256 * per pieces
+  int pad;
 };
 
 // host and device (the rotary sincos below is also built into a host test helper)

@@ -21,9 +21,10 @@
 #include "common.h"
 
 #define SM_T 1024              // threads of _pick
-#define SM_TH 256              // of the others
+#define SM_TH 256              // of _hist and _collect
+#define SM_MAX_PARTS 1024      // of a row
 #define SM_BINS 512            // of width T / 16
-#define SM_PART 2048           // pieces of a part: 8 per thread, which stay in registers
+#define SM_MAX_PER 8           // pieces of a part per thread, which stay in registers (SampleArgs.per)
 #define SM_LIST 4096           // tokens of the bins around the cuts
 #define SM_RANK 256            // tokens ranked against each other: n^2 reads of LDS, 4 us at 256
 #define SM_SPLIT 2048
@@ -208,15 +209,17 @@ struct SmPieces {
 // grid (parts, rows). The part stays in registers between its maximum and its bins.
 template <int DT>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
-  constexpr int E = SmPieces<DT>::E, N = SM_PART / SM_TH;
+  constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER;
   __shared__ u64 red[SM_TH / 64];
   __shared__ unsigned cnt[SM_BINS];
   __shared__ u64 wts[SM_BINS];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const SmPieces<DT> x(a, row);
+  const int c0 = part * a.per * SM_TH + tid;
   uint4 q[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = x.bits(part * SM_PART + i * SM_TH + tid);
+  for (int i = 0; i < N; ++i)
+    if (i < a.per) q[i] = x.bits(c0 + i * SM_TH);
   const float T = a.temperature[row], top_p = a.top_p[row];
   const int top_k = a.top_k[row];
   if (part == 0 && tid == 0) a.listed[row] = 0;
@@ -225,6 +228,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
   u64 best = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    if (i >= a.per) break;
     float v[E];
     x.values(q[i], v);
     float m = v[0];
@@ -233,7 +237,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
     for (int j = 1; j < E; ++j)
       if (v[j] > m) m = v[j], at = j;
     // (a token outside the row, -inf, wins over none that is in it)
-    const int i0 = x.first(part * SM_PART + i * SM_TH + tid);
+    const int i0 = x.first(c0 + i * SM_TH);
     if (m == -INFINITY) at = max(0, -i0);
     const u64 k = x.in(i0 + at) ? sm_key(m, i0 + at) : 0;
     best = k > best ? k : best;
@@ -248,6 +252,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
   const int top = r.grid(r.max);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    if (i >= a.per) break;
     float v[E];
     x.values(q[i], v);
 #pragma unroll
@@ -268,21 +273,24 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
 
 // ------------------------------------------------------------------ the bins of the cuts
 
-// grid (rows). Thread i holds bins 2 i and 2 i + 1 of the row's, which count down from its largest value's.
-extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_merge(const SampleArgs a) {
-  static_assert(SM_BINS == 2 * SM_TH, "");
-  __shared__ u64 red[SM_TH / 64];
-  __shared__ unsigned redc[SM_TH / 64];
-  __shared__ double redw[SM_TH / 64];
+// grid (rows). Threads i and 512 + i hold the row's bin i, which counts down from its largest value's: one adds up the
+// even parts, the other the odd ones, sixteen parts' loads in flight (one at a time takes 0.7 us a part).
+extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleArgs a) {
+  static_assert(SM_T == 2 * SM_BINS && SM_MAX_PARTS <= SM_T, "");
+  __shared__ u64 red[SM_T / 64];
+  __shared__ unsigned redc[SM_T / 64];
+  __shared__ double redw[SM_T / 64];
+  __shared__ int off[SM_MAX_PARTS + 32];    // the parts' first bins, in the row's
+  __shared__ double f[SM_MAX_PARTS + 32];   // their largest tokens' weights
+  __shared__ unsigned oddc[SM_BINS];
+  __shared__ double oddw[SM_BINS];
   __shared__ int kb, kr, plo, phi;
   __shared__ double ahead, in_kb, base;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const u64* keys = a.best + (long long)row * a.parts;
-  u64 best = 0;
-  for (int p = tid; p < a.parts; p += SM_TH) best = keys[p] > best ? keys[p] : best;
-  best = sm_block_max<SM_TH>(best, red);
+  const int row = blockIdx.x, tid = threadIdx.x, bin = tid & (SM_BINS - 1), odd = tid / SM_BINS;
+  const u64 key = tid < a.parts ? a.best[(long long)row * a.parts + tid] : 0;
   const float T = a.temperature[row], top_p = a.top_p[row];
   const int top_k = a.top_k[row];
+  const u64 best = sm_block_max<SM_T>(key, red);
   SmRow r;
   r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
   const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
@@ -294,39 +302,41 @@ extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_merge(const SampleA
     return;
   }
   const int top = r.grid(r.max);
-  unsigned c[2] = {0, 0};
-  double w[2] = {0.0, 0.0};
-  for (int q = 0; q < a.parts; ++q) {
-    const u64 key = keys[q];
-    const float m = sm_value((uint32_t)(key >> 32));
-    if (key == 0 || m == -INFINITY) continue;
-    const int off = top - r.grid(m);   // the part's first bin, in the row's
-    const double f = r.weight(m);
-    const long long at = ((long long)row * a.parts + q) * SM_BINS;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int bin = 2 * tid + i - off;
-      if (bin < 0) continue;
-      c[i] += a.cnt[at + bin];
-      if (p) w[i] += f * (double)a.wts[at + bin];
-    }
-  }
+  const float most = sm_value((uint32_t)(key >> 32));
+  const bool any = key != 0 && most != -INFINITY;
+  off[tid] = any ? min(top - r.grid(most), SM_BINS) : SM_BINS;
+  f[tid] = any ? r.weight(most) : 0.0;
+  if (tid < 32) off[SM_MAX_PARTS + tid] = SM_BINS, f[SM_MAX_PARTS + tid] = 0.0;
   if (tid == 0) kb = -1, kr = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
+  __syncthreads();
+  unsigned c = 0;
+  double w = 0.0;
+  for (int q0 = odd; q0 < a.parts; q0 += 32) {
+    unsigned n[16];
+    u64 m[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {   // (a part that does not reach the bin is read at its first and left out)
+      const long long at = ((long long)row * a.parts + min(q0 + 2 * j, a.parts - 1)) * SM_BINS;
+      const int i = max(bin - off[q0 + 2 * j], 0);
+      n[j] = a.cnt[at + i];
+      m[j] = p ? a.wts[at + i] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (bin >= off[q0 + 2 * j]) c += n[j], w += f[q0 + 2 * j] * (double)m[j];
+  }
+  if (odd) oddc[bin] = c, oddw[bin] = w;
+  __syncthreads();
+  c = odd ? 0 : c + oddc[bin];
+  w = odd ? 0.0 : w + oddw[bin];
   unsigned call;
   double wall;
-  const unsigned c0 = sm_block_scan<SM_TH>(c[0] + c[1], redc, &call);
-  const double w0 = sm_block_scan<SM_TH>(w[0] + w[1], redw, &wall);
-  if (k) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const unsigned before = c0 + (i ? c[0] : 0);
-      if (before < (unsigned)top_k && before + c[i] >= (unsigned)top_k) {
-        kb = 2 * tid + i, kr = top_k - (int)before;
-        ahead = w0 + (i ? w[0] : 0.0);
-        // the bin's first kr tokens weigh at least their share of it, and at most all
-        in_kb = w[i], base = w[i] * (double)kr / (double)c[i];
-      }
-    }
+  const unsigned c0 = sm_block_scan<SM_T>(c, redc, &call);
+  const double w0 = sm_block_scan<SM_T>(w, redw, &wall);
+  if (k && c0 < (unsigned)top_k && c0 + c >= (unsigned)top_k) {
+    kb = bin, kr = top_k - (int)c0, ahead = w0;
+    // the bin's first kr tokens weigh at least their share of it, and at most all
+    in_kb = w, base = w * (double)kr / (double)c;
   }
   __syncthreads();
   s.kb = kb, s.kr = kr, s.ahead = ahead, s.total = wall;
@@ -335,19 +345,12 @@ extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_merge(const SampleA
     // (the slack covers weights rounded to a part's units here and to the row's there)
     const double lo = kb < 0 ? wall : ahead + base, up = kb < 0 ? wall : ahead + in_kb;
     const double plow = (double)top_p * lo * (1.0 - 1e-9), pup = (double)top_p * up * (1.0 + 1e-9);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const double before = w0 + (i ? w[0] : 0.0), after = w0 + w[0] + (i ? w[1] : 0.0);
-      if (before < plow && after >= plow) atomicMin(&plo, 2 * tid + i);
-      if (before < pup && after >= pup) atomicMin(&phi, 2 * tid + i);
-    }
+    if (!odd && w0 < plow && w0 + w >= plow) atomicMin(&plo, bin);
+    if (!odd && w0 < pup && w0 + w >= pup) atomicMin(&phi, bin);
     __syncthreads();
     const int last = kb < 0 ? SM_BINS - 1 : kb;
     s.plo = min(plo, last), s.phi = min(phi, last);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (2 * tid + i == s.plo) base = w0 + (i ? w[0] : 0.0);
+    if (tid == s.plo) base = w0;
     __syncthreads();
     s.base = base;
   } else if (kb < 0) {
@@ -361,15 +364,16 @@ extern "C" __global__ void __launch_bounds__(SM_TH) k_sample_merge(const SampleA
 // grid (parts, rows): wave i of a part takes its groups i, i + 4, ..., all loads in flight together.
 template <int DT>
 __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
-  constexpr int E = SmPieces<DT>::E, N = SM_PART / SM_TH, CAP = 1024;
+  constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER, CAP = 1024;
   __shared__ u64 list[CAP];
   __shared__ unsigned n, at;
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const SmPieces<DT> x(a, row);
-  const int c0 = part * SM_PART + wave * 64 + lane;
+  const int c0 = part * a.per * SM_TH + tid;
   uint4 q[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = x.bits(c0 + i * SM_TH);
+  for (int i = 0; i < N; ++i)
+    if (i < a.per) q[i] = x.bits(c0 + i * SM_TH);
   const SampleRow s = a.row[row];
   if (s.mode == 0 || s.mode == 3) return;
   const float T = a.temperature[row], min_p = a.min_p[row];
@@ -381,6 +385,7 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    if (i >= a.per) break;
     const int c = c0 + i * SM_TH;
     float v[E];
     x.values(q[i], v);
@@ -397,7 +402,7 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
       }
     }
     sum = sm_wave_sum(sum);
-    const int g = (part * SM_PART + i * SM_TH) / 64 + wave;
+    const int g = (part * a.per + i) * (SM_TH / 64) + wave;
     if (lane == 0 && g < a.ngroups) a.groups[(long long)row * a.ngroups + g] = sum;
   }
   __syncthreads();
@@ -427,13 +432,26 @@ __device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool wei
   const int tid = threadIdx.x;
   auto units = [&](u64 k) { return weigh ? r.units(r.weight(sm_value((uint32_t)(k >> 32)))) : 1ull; };
   u64 least = ~0ull, most = 0, members = 0;
+  __syncthreads();
   each([&](u64 k) {
     if (k < lo || k > hi) return;
     least = k < least ? k : least, most = k > most ? k : most, ++members;
   });
-  sm_block_scan<SM_T>(members, t.red, &members);
-  lo = ~sm_block_max<SM_T>(~least, t.red), hi = sm_block_max<SM_T>(most, t.red);
+  members = sm_wave_sum(members), least = ~sm_wave_max(~least), most = sm_wave_max(most);
+  if ((tid & 63) == 0) {
+    const int w = tid >> 6;
+    t.key[w] = least, t.key[SM_T / 64 + w] = most, t.w[w] = members;
+  }
+  __syncthreads();
+  members = 0;
+#pragma unroll
+  for (int w = 0; w < SM_T / 64; ++w) {
+    least = t.key[w] < least ? t.key[w] : least, most = t.key[SM_T / 64 + w] > most ? t.key[SM_T / 64 + w] : most;
+    members += t.w[w];
+  }
   if (members == 0) return 0;
+  lo = least, hi = most;
+  __syncthreads();
   while (members > SM_RANK) {
     const int bits = 64 - __builtin_clzll((hi - lo) | 1), sh = max(bits - 11, 0);
     for (int i = tid; i < SM_SPLIT; i += SM_T) t.cnt[i] = 0, t.sum[i] = 0;
@@ -473,13 +491,18 @@ __device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool wei
     t.w[s] = units(k);
   });
   __syncthreads();
+  // four threads a key, each over a quarter of the others
+  static_assert(SM_T == 4 * SM_RANK, "");
   u64 mine = ~0ull;
-  const int n = (int)t.n;
-  if (tid < n) {
-    u64 b = before;
-    const u64 k = t.key[tid];
-    for (int j = 0; j < n; ++j) b += t.key[j] > k ? t.w[j] : 0;
-    if (b < need) mine = k;
+  const int n = (int)t.n, me = tid >> 2;
+  if (me < n) {
+    u64 b = 0;
+    const u64 k = t.key[me];
+#pragma unroll 4
+    for (int j = tid & 3; j < n; j += 4) b += t.key[j] > k ? t.w[j] : 0;
+    b += __shfl_xor(b, 1, 64);
+    b += __shfl_xor(b, 2, 64);
+    if (before + b < need) mine = k;
   }
   const u64 found = ~sm_block_max<SM_T>(~mine, t.red);
   return found == ~0ull ? 0 : found;

@@ -15,8 +15,8 @@ PAGED_APPEND_ROW_N = 1024      # up to this many rows a workgroup per row, past 
 # that wide tiles are split towards
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
 PT_GRID = 512                  # two workgroups per CU
-# sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, pieces of a part, bins, tokens of a list
-SAMPLE_MAX_PIECES, SAMPLE_PART, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 2048, 512, 4096
+# sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, bins, tokens of a list
+SAMPLE_MAX_PIECES, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 512, 4096
 SAMPLE_PICK_PIECES = 1024      # up to this many pieces k_sample_pick alone
 
 
@@ -170,9 +170,15 @@ def lower_sample(low, node: OpNode) -> None:
     low.views[node.outputs[0].name] = out
     if B == 0:
         return
-    per = 16 // ELEM_SIZE[x.dtype]
-    pieces = (V + per - 2) // per + 1   # most that a row, wherever it starts, can touch
-    parts, groups = -(-pieces // SAMPLE_PART), -(-pieces // 64)
+    width = 16 // ELEM_SIZE[x.dtype]
+    pieces = (V + width - 2) // width + 1   # most that a row, wherever it starts, can touch
+    # Pieces a thread: few, so that few rows take many workgroups, but not over 32 parts, whose bins one workgroup adds
+    # up at 0.25 us a part. One row of 151,936 in bf16 is 10 parts of 8 (15 + 10 + 15 us), 19 of 4 (TBD) or
+    # 75 of 1 (5 + 23 + 5); 256 rows take 8.
+    def parts_of(per):
+        return -(-pieces // (256 * per))
+    per = next((p for p in (1, 2, 4) if parts_of(p) <= 32 and B * parts_of(p) <= 1024), 8)
+    parts, groups = parts_of(per), -(-pieces // 64)
     binned = pieces > SAMPLE_PICK_PIECES
     name = node.outputs[0].name
     ws = (lambda what, nbytes: low.scratch(f"{name}.{what}", nbytes)) if binned else (lambda what, nbytes: None)
@@ -182,11 +188,11 @@ def lower_sample(low, node: OpNode) -> None:
                 best=ws("best", 8 * B * parts), cnt=ws("cnt", 4 * B * parts * SAMPLE_BINS),
                 wts=ws("wts", 8 * B * parts * SAMPLE_BINS), row=ws("row", 56 * B), groups=ws("groups", 8 * B * groups),
                 listed=ws("listed", 4 * B), list=ws("list", 8 * B * SAMPLE_LIST), rows=B, vocab=V,
-                dtype=DTYPE_CODE[x.dtype], shift=min(44, 62 - V.bit_length()), parts=parts, ngroups=groups)
+                dtype=DTYPE_CODE[x.dtype], shift=min(44, 62 - V.bit_length()), parts=parts, ngroups=groups, per=per)
     dt = {"float32": "f32", "float16": "f16", "bfloat16": "bf16"}[x.dtype]
     launches = [("k_sample_pick_" + dt, (B, 1, 1), 1024)]
     if binned:
-        launches = [("k_sample_hist_" + dt, (parts, B, 1), 256), ("k_sample_merge", (B, 1, 1), 256),
+        launches = [("k_sample_hist_" + dt, (parts, B, 1), 256), ("k_sample_merge", (B, 1, 1), 1024),
                     ("k_sample_collect_" + dt, (parts, B, 1), 256)] + launches
     for kernel, grid, threads in launches:
         low.emit(LaunchStep(kind="sample", kernel=kernel, module="sample", arg_struct="SampleArgs", args=dict(args),

@@ -142,7 +142,8 @@ _struct("SampleRow", [("best", LL), ("ahead", C.c_double), ("base", C.c_double),
                       ("kb", I), ("kr", I), ("plo", I), ("phi", I), ("pad", I)])
 _struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
                        ("best", P), ("cnt", P), ("wts", P), ("row", P), ("groups", P), ("listed", P), ("list", P),
-                       ("rows", I), ("vocab", I), ("dtype", I), ("shift", I), ("parts", I), ("ngroups", I)])
+                       ("rows", I), ("vocab", I), ("dtype", I), ("shift", I), ("parts", I), ("ngroups", I),
+                       ("per", I), ("pad", I)])
 
 
 def check_layouts() -> dict[str, tuple[int, int]]:
