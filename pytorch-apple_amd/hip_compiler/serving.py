@@ -110,7 +110,8 @@ def lower_paged_append(low, node: OpNode) -> None:
                   pages=int(kp.shape[0]), N=N, H=H, KVH=KVH, D=D, R=R, page_size=ps,
                   scaling=float(node.attrs.get("attention_scaling", 1.0)), dtype=DTYPE_CODE[q.dtype]),
         grid=(grid, 1, 1), inputs=[t.name for t in node.inputs], outputs=[o.name for o in node.outputs],
-        params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D}))
+        params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D,
+                "pieces16": [] if kernel == "k_paged_append_any" else ["q", "k", "v", "k_pages", "v_pages"]}))
 
 
 def lower_paged_attention(low, node: OpNode) -> None:
@@ -143,6 +144,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
         low.emit(LaunchStep(kind="paged_attention", kernel="k_paged_attn_any", module="paged", arg_struct="PagedAttnArgs",
                             args=args, grid=(N, H, 1), block=(64, 1, 1), inputs=ins, outputs=outs, params=params))
         return
+    params["pieces16"] = ["q", "k_pages", "v_pages"]
     groups = ps // 16
     part_rows = 2 * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),

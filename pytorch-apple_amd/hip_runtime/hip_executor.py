@@ -171,6 +171,9 @@ class HIPExecutor:
             r.kernarg_size = C.sizeof(s)
             r.kernarg = C.addressof(s)
         self._n = n
+        # external storages that some kernel reads or writes 16 bytes at a time
+        self._pieces16 = {v.storage for st in program.steps for f in st.params.get("pieces16", ())
+                      if isinstance(v := st.args[f], Ref) and v.storage in self._ext_names}
         self._ext_key: tuple | None = None        # external pointers packed into the kernargs now
         # external storages bound to weights (checked once per weights dict) and to graph inputs
         # (checked once per set of buffer objects)
@@ -305,7 +308,11 @@ class HIPExecutor:
         if t.numel() * t.element_size() < spec_st.nbytes:
             raise ValueError(f"HIPExecutor: '{name}' holds {t.numel() * t.element_size()} bytes, "
                              f"program needs {spec_st.nbytes}")
-        return t.data_ptr()
+        ptr = t.data_ptr()
+        if name in self._pieces16 and ptr % 16:
+            raise ValueError(f"HIPExecutor: '{name}' starts {ptr % 16} bytes after a 16-byte boundary, and a kernel reads "
+                             f"it in pieces of 16; pass a copy")
+        return ptr
 
     def _lookup(self, name: str, inputs: dict, weights: dict):
         buf = inputs.get(name)

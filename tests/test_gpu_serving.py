@@ -260,3 +260,138 @@ def _special(backend, x, par):
 def test_paged_attention_of_long_tiles(backend, H, KVH, D, page, new, kv):
     """Tiles split along their positions: parts that begin at the last block of a window of page ids, and at every other."""
     _attention(backend, R.batch([new, 1], [kv, 77], page, seed=new), H, KVH, D, "bfloat16", page, "hnd")
+
+
+# ---------------------------------------------------------------- rows that bins do not split well, and other grids
+
+@pytest.mark.parametrize("dtype,spread,shift", [
+    ("float32", 0.3, 0.0),       # thousands of tokens in a bin: more than a row's list holds
+    ("float32", 1.0, 0.0), ("bfloat16", 1.0, 0.0), ("float16", 0.01, 0.0),
+    ("float32", 3.0, 3e4), ("float32", 3.0, -6e4),   # near and past the bound of the grid
+    ("float32", 100.0, 1e7),     # past it
+    ("float32", 40.0, 0.0)])     # most tokens weigh nothing, and whole parts
+def test_sample_of_dense_and_distant_rows(backend, dtype, spread, shift):
+    x = (spread * _rand(7, 8, 120011) + shift).to(R.DT[dtype])
+    x[0, 0], x[1, -1] = float("inf"), float("nan")
+    par = _params(8, 3, T=(0.3, 1.0, 8.0), k=(0, 50, 3000), p=(1.0, 0.95, 0.5), m=(0.0, 0.01))
+    assert torch.equal(_sample(backend, x, par, dtype), R.sample64(x, **par))
+
+
+@pytest.mark.parametrize("B,V,dtype", [(1, 151936, "bfloat16"), (1, 4097, "float32"), (3, 8200, "float16"),
+                                       (300, 9001, "float32"), (1100, 4500, "float32"), (2, 500009, "bfloat16")])
+def test_sample_over_parts_of_every_size(backend, B, V, dtype):
+    x = (2.0 * _rand(B + V, B, V)).to(R.DT[dtype])
+    par = _params(B, V + 1, T=(0.7, 1.0), k=(0, 40), p=(1.0, 0.9), m=(0.0, 0.03))
+    assert torch.equal(_sample(backend, x, par, dtype), R.sample64(x, **par))
+
+
+@pytest.mark.parametrize("D,page,dtype", [(128, 1, "bfloat16"), (80, 7, "float16"), (64, 24, "bfloat16"), (48, 16, "float32"),
+                                          (256, 32, "float16"), (1, 3, "float32")])
+def test_paged_attention_of_other_pages_and_heads(backend, D, page, dtype):
+    _attention(backend, R.batch([1, 0, 5, 33, 0, 1], [1, 0, 5, 70, 9, 130], page, pad=3, seed=D), 6, 2, D, dtype, page, "nhd")
+
+
+@pytest.mark.parametrize("seqs", [1000, 1100])
+def test_paged_attention_of_many_sequences(backend, seqs):
+    """As many as the list of a tiled launch holds, and more."""
+    r = np.random.default_rng(seqs)
+    kv = r.integers(0, 60, seqs)
+    _attention(backend, R.batch([min(int(k), 1) for k in kv], [int(k) for k in kv], 16, pad=5), 4, 1, 64, "bfloat16", 16, "hnd")
+
+
+# ---------------------------------------------------------------- together, captured, on other streams
+
+def _step_graph(N, B, P, page, M, H, KVH, D, V, dtype):
+    """Append, attention and sampling from a projection of its output, as one program."""
+    from irgen.builder import IRBuilder
+    from irgen.serving import batch_inputs, paged_append, paged_attention, pool_shape, sampling_inputs
+
+    b = IRBuilder("ServingStep")
+    q, k, v = (b.input(n, [N, h, D], dtype) for n, h in (("q", H), ("k", KVH), ("v", KVH)))
+    kp, vp = (b.input(n, pool_shape(P, page, KVH, D), dtype) for n in ("k_pages", "v_pages"))
+    batch = batch_inputs(b, B, M)
+    inv = b.input("inv_freq", [D // 2], "float32")
+    w = b.input("w", [V, H * D], dtype)
+    last = b.input("last_rows", [B], "int64")
+    par = sampling_inputs(b, B)
+    q, kp, vp = paged_append(b, q, k, v, kp, vp, batch, inv)
+    o = b.op("aten.reshape.default", [paged_attention(b, q, kp, vp, batch, D ** -0.5)], {"shape": [N, H * D]})
+    l = b.op("aten.linear.default", [b.op("aten.embedding.default", [o, last]), w])
+    b.output(b.op("serving.sample.default", [l, *par]), o, kp, vp)
+    return b.to_dict()
+
+
+def _step_inputs(seed, bt, H, KVH, D, V, page, dtype):
+    N, B, dt = bt["rows"], len(bt["kv_len"]), R.DT[dtype]
+    kp, vp = R.pools(bt, KVH, page, D, dtype, seed=seed)
+    g = lambda i, *s: _rand(seed * 10 + i, *s).to(dt)   # noqa: E731
+    last = (bt["q_start"][1:].long() - 1).clamp(min=0)
+    return {"q": g(0, N, H, D), "k": g(1, N, KVH, D), "v": g(2, N, KVH, D), "k_pages": kp, "v_pages": vp, **_meta(bt),
+            "inv_freq": _inv(D // 2), "w": (0.3 * _rand(seed, V, H * D)).to(dt), "last_rows": last,
+            **_params(B, seed, T=(0.0, 1.0), k=(0, 50), p=(1.0, 0.9), m=(0.0,))}
+
+
+@pytest.mark.parametrize("news,kvs", [([1, 1, 1, 1], [9, 700, 1, 64]), ([40, 1, 0, 200], [40, 300, 5, 260])])
+def test_a_step_captured_and_replayed(backend, news, kvs):
+    """One program under the caller's capture, replayed with other inputs, eager calls and synchronisations between, on
+    the stream of the capture and on another: every output equals the eager one, rows and pages of no sequence too."""
+    H, KVH, D, V, page, dtype = 8, 2, 128, 5000, 16, "bfloat16"
+    bt = R.batch(news, kvs, page, pad=4, seed=1)
+    sets = [_step_inputs(s, bt, H, KVH, D, V, page, dtype) for s in (1, 2, 3)]
+    bufs = {k: backend.allocate_buffer(t.cuda()) for k, t in sets[0].items()}
+    ir = _step_graph(bt["rows"], len(news), sets[0]["k_pages"].shape[0], page, bt["block_table"].shape[1], H, KVH, D, V, dtype)
+    dag, other = _dag(ir, backend), _dag(ir, backend)
+    names = [o["name"] for o in ir["graph_outputs"]]
+    print(f"[case] {news} {kvs}", flush=True)
+
+    def fill(s):
+        for k, t in s.items():
+            bufs[k].native_handle.copy_(t)
+
+    def read(y):
+        torch.cuda.synchronize()
+        return [y[n].to_torch().clone() for n in names]
+
+    want = []
+    for s in sets:
+        fill(s)
+        want.append(read(dag.execute(bufs)))
+        for _ in range(2):   # (appending the same rows again changes nothing)
+            assert all(torch.equal(a, b) for a, b in zip(read(dag.execute(bufs)), want[-1]))
+    pad = want[0][1][int(bt["q_start"][-1]):]
+    assert pad.shape[0] == 4 and pad.eq(0).all()
+    g, h = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out = dag.execute(bufs)
+    with torch.cuda.graph(h):
+        out2 = other.execute(bufs)
+    side = torch.cuda.Stream()
+    for rep in range(2):
+        for s, w in zip(sets, want):
+            fill(s)
+            g.replay()
+            assert all(torch.equal(a, b) for a, b in zip(read(out), w))
+            assert all(torch.equal(a, b) for a, b in zip(read(dag.execute(bufs)), w))
+            h.replay()
+            g.replay()
+            assert all(torch.equal(a, b) for a, b in zip(read(out2), w))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                y = dag.execute(bufs)
+            assert all(torch.equal(a, b) for a, b in zip(read(y), w))
+
+
+def test_a_pool_that_starts_between_pieces_is_refused(backend):
+    from irgen.serving import build_paged_attention_ir
+
+    bt = R.batch([1], [20], 16)
+    kp, vp = R.pools(bt, 2, 16, 128, "bfloat16")
+    t = {"q": _rand(1, bt["rows"], 4, 128).to(torch.bfloat16), "k_pages": kp, "v_pages": vp, **_meta(bt)}
+    bufs = {k: backend.allocate_buffer(x.cuda()) for k, x in t.items()}
+    dag = _dag(build_paged_attention_ir(bt["rows"], 1, kp.shape[0], 16, bt["block_table"].shape[1], 4, 2, 128), backend)
+    dag.execute(bufs)
+    odd = torch.empty(vp.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(vp.shape)
+    odd.copy_(vp)
+    with pytest.raises(ValueError, match="16"):
+        dag.execute({**bufs, "v_pages": backend.allocate_buffer(odd)})
