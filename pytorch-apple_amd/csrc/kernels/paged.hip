@@ -1019,37 +1019,45 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
   for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
 }
 
-// Joins S parts of one row (by a wave): row `p` of the slots that at(s) gives.
+// Joins S parts of one row (by a wave): part s lies `rel(s)` slots of R rows after row `first` of the parts.
 template <int DT, int D, int R, typename F>
-__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long base, int r, int S, F at, uint16_t* out) {
-  // a load covers PER parts: lane (part, 4 dims)
+__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out) {
+  // a load covers PER parts: lane (part, 4 dims); a batch is eight of them
   constexpr int LN = D / 4, PER = 64 / LN;
   const int lane = threadIdx.x & 63;
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
-  float M = -INFINITY;
-  for (int s = lane; s < S; s += 64) M = fmaxf(M, a.part_ml[(base + (long long)at(s) * R + r) * 2]);
-  M = wave_max(M);
-  float L = 0.f, x[4] = {};
+  const float* mls = a.part_ml + first * 2;
+  const float* os = a.part_o + first * D;
+  float M = -INFINITY, L = 0.f, x[4] = {};
   for (int s0 = 0; s0 < S; s0 += 64) {
     const int n = min(64, S - s0);
-    float f = 0.f;
-    if (lane < n) {
-      const float2 v = *(const float2*)(a.part_ml + (base + (long long)at(s0 + lane) * R + r) * 2);
-      f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v.x - M) * c);
-      L += f * v.y;
-    }
-    for (int j = 0; j < n; j += 8 * PER) {   // eight loads in flight; past the last part: it again, weighed 0
-      float4 v[8];
-      float g[8];
+    const float2 ml = *(const float2*)(mls + rel(s0 + min(lane, n - 1)) * R * 2);
+    float4 v[8];
+    auto fetch = [&](int j) {   // (past the last part: it again, weighed 0)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int k = j + i * PER + lane / LN, s = min(k, n - 1);
-        const float fs = __shfl(f, s, 64);
-        g[i] = k < n ? fs : 0.f;
-        v[i] = *(const float4*)(a.part_o + (base + (long long)at(s0 + s) * R + r) * D + (lane % LN) * 4);
+        if (j + i * PER >= n) break;
+        const int s = min(j + i * PER + lane / LN, n - 1);
+        v[i] = *(const float4*)(os + rel(s0 + s) * R * D + (lane % LN) * 4);
       }
+    };
+    fetch(0);   // in flight with the statistics
+    const float m = lane < n ? ml.x : -INFINITY, most = fmaxf(M, wave_max(m));
+    const float old = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - most) * c);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
+    M = most;
+    L = L * old + (lane < n ? f * ml.y : 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[0] += g[i] * v[i].x, x[1] += g[i] * v[i].y, x[2] += g[i] * v[i].z, x[3] += g[i] * v[i].w;
+    for (int e = 0; e < 4; ++e) x[e] *= old;
+    for (int j = 0; j < n; j += 8 * PER) {
+      if (j) fetch(j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (j + i * PER >= n) break;
+        const int k = j + i * PER + lane / LN;
+        const float fs = __shfl(f, min(k, n - 1), 64), g = k < n ? fs : 0.f;
+        x[0] += g * v[i].x, x[1] += g * v[i].y, x[2] += g * v[i].z, x[3] += g * v[i].w;
+      }
     }
   }
   L = wave_sum(L);
@@ -1067,38 +1075,67 @@ template <int DT, int D>
 __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
   constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ PtList t;
+  __shared__ int start[PT_MAXB + 1], kv[PT_MAXB];   // (a row looks its sequence up in LDS: from memory it is 1 us)
+  for (int b = threadIdx.x; b <= a.B; b += 256) {
+    start[b] = a.q_start[b];
+    if (b < a.B) kv[b] = a.kv_len[b];
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.H / a.KVH, waves = gridDim.x * 4, me = blockIdx.x * 4 + wave, hi = a.grid_wide ? PT_NARROW : ANY;
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  // Each wave takes a run of rows and looks up where they lie only where a sequence, head or tile begins: looked up
+  // row by row (binary search, divisions) a batch of 7,100 rows takes 18 us rather than TBD.
+  auto runs = [&](int rows, auto seq, auto tile, auto join) {
+    const int per = (rows + waves - 1) / waves, end = min(rows, (me + 1) * per);
+    for (int u = me * per; u < end;) {
+      const int b = uniform(pt_find(t.cost, a.B, u));
+      const int s0 = uniform(start[b]), i = u - (b ? uniform(t.cost[b - 1]) : 0);
+      const PtSeq q = seq(b, s0, uniform(start[b + 1]), uniform(kv[b]));
+      const int of = q.n * G, stop = min(end, u - i + of * a.KVH);   // (rows of the sequence, per head)
+      int h = i / of, row = i - h * of;
+      bool fresh = true;
+      for (; u < stop; ++u, ++row) {
+        if (row == of) row = 0, ++h, fresh = true;
+        if (fresh || tile(row)) join(b, q, h, row, true);
+        else join(b, q, h, row, false);
+        fresh = false;
+      }
+    }
+  };
   auto out = [&](const PtSeq& q, int h, int row) {
     const int tk = row / G;
     return (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D;
   };
   int rows;
   const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers(all, a.grid_narrow);
-  for (int u = me; u < rows; u += waves) {   // (sequence, head, row)
-    const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
-    const PtSeq q = pt_seq<PT_NARROW, NPB>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), 0, hi);
-    const int i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
-    const int g0 = (b ? t.items[b - 1] : 0) + (h * q.tiles + row / PT_NARROW) * q.blocks;
-    // workgroups that hold its first and last block
-    const int w0 = (int)((((long long)g0 + 1) * workers - 1) / all);
-    const int w1 = (int)((((long long)g0 + q.blocks) * workers - 1) / all);
-    if (w0 == w1) continue;
-    pt_join<DT, D, PT_NARROW>(a, 0, row % PT_NARROW, w1 - w0 + 1, [&](int s) { return 2 * (w0 + s) + (s == 0); }, out(q, h, row));
-  }
+  int w0 = 0, w1 = 0;   // workgroups that hold the tile's first and last block
+  runs(
+      uniform(rows), [&](int b, int s0, int s1, int kv) { return pt_seq<PT_NARROW, NPB>(a, b, s0, s1, kv, 0, hi); },
+      [](int row) { return row % PT_NARROW == 0; },
+      [&](int b, const PtSeq& q, int h, int row, bool fresh) {
+        if (fresh) {
+          const int g0 = (b ? uniform(t.items[b - 1]) : 0) + (h * q.tiles + row / PT_NARROW) * q.blocks;
+          w0 = uniform((int)((((long long)g0 + 1) * workers - 1) / all));
+          w1 = uniform((int)((((long long)g0 + q.blocks) * workers - 1) / all));
+        }
+        if (w0 != w1)
+          pt_join<DT, D, PT_NARROW>(a, (long long)2 * w0 * PT_NARROW + row % PT_NARROW, w1 - w0 + 1,
+                                    [](int s) { return 2 * s + (s == 0); }, out(q, h, row));
+      });
   if (a.grid_wide) {
     __syncthreads();
     pt_build_wide<true>(a, t, &rows);
-    for (int u = me; u < rows; u += waves) {
-      const int b = __builtin_amdgcn_readfirstlane(pt_find(t.cost, a.B, u));
-      const PtSeq q = pt_seq<PT_WIDE, 64>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), PT_NARROW, ANY);
-      const int S = pt_splits(q, t.share), i = u - (b ? t.cost[b - 1] : 0), h = i / (q.n * G), row = i % (q.n * G);
-      const int slot = (b ? t.slots[b - 1] : 0) + (h * q.tiles + row / PT_WIDE) * S;
-      pt_join<DT, D, PT_WIDE>(a, (long long)2 * a.grid_narrow * PT_NARROW, row % PT_WIDE, S, [&](int s) { return slot + s; },
-                              out(q, h, row));
-    }
+    const int share = uniform(t.share);
+    runs(
+        uniform(rows), [&](int b, int s0, int s1, int kv) { return pt_seq<PT_WIDE, 64>(a, b, s0, s1, kv, PT_NARROW, ANY); },
+        [](int) { return false; },
+        [&](int b, const PtSeq& q, int h, int row, bool) {
+          const int S = pt_splits(q, share), slot = (b ? uniform(t.slots[b - 1]) : 0) + (h * q.tiles + row / PT_WIDE) * S;
+          pt_join<DT, D, PT_WIDE>(a, (long long)(2 * a.grid_narrow * PT_NARROW) + (long long)slot * PT_WIDE + row % PT_WIDE, S,
+                                  [](int s) { return s; }, out(q, h, row));
+        });
   }
-  const int s0 = a.q_start[0], s1 = a.q_start[a.B];
+  const int s0 = start[0], s1 = start[a.B];
   for (int row = me; row < a.N; row += waves) {
     if (row >= s0 && row < s1) continue;
     uint4* o = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
