@@ -642,9 +642,6 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
 
 struct SampleRow {            // sample.hip: what k_sample_merge finds out about a row
   unsigned long long best;    // key of the first ranked token
-  double ahead;               // weight of the bins before kb, in units
-  double base;                // weight of the bins before plo
-  double total;               // weight of all tokens, where top-k cuts nothing
   int mode;                   // 0: the first ranked, 1: every token, 2: a cut within the listed bins, 3: not binned
   int kb, kr;                 // bin of the k-th token (-1: no cut) and its rank there, from 1
   int plo, phi;               // bins in which the last kept token lies
@@ -660,10 +657,10 @@ struct SampleArgs {           // sample.hip: one token per row of logits [rows, 
   const float* u;
   long long* out;             // [rows]
   unsigned long long* best;   // [rows, parts] key of each part's first ranked token; null: no parts, k_sample_pick alone
-  unsigned* cnt;              // [rows, parts, bins] tokens
-  unsigned long long* wts;    // [rows, parts, bins] weights, relative to the part's largest
+  unsigned long long* bins;   // [rows, parts, bins] number of tokens, and weights relative to the part's largest
   SampleRow* row;             // [rows]
   unsigned long long* groups; // [rows, groups] weights of the kept tokens of 64 pieces
+  unsigned long long* sums;   // [rows, 2] weights of the tokens before bin plo, and before bin kb (-1: of all)
   unsigned* listed;           // [rows] length of the row's list
   unsigned long long* list;   // [rows, SM_LIST] keys of the tokens in the bins where the cuts lie
   int rows;

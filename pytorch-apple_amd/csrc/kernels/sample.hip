@@ -11,8 +11,9 @@
 //     alike). A cut is a key; what is needed of the row to find it are the tokens near it.
 //   * Rows are read twice, by many workgroups each, in four launches: _hist counts and weighs each part's tokens in
 //     512 bins of l of width T / 16, on one grid for all parts of a row and down from the part's largest (after 32 T
-//     weights round to 0, so the bins hold all that weigh); _merge adds the parts up and finds the bins in which the
-//     k-th token and the top-p sum lie; _collect sums the weights that are kept for sure in groups of 64 sixteen-byte
+//     weights round to 0, so the bins hold all that weigh), near enough to say where a cut lies; _merge adds the parts
+//     up and finds the bins in which the k-th token and the end of the top-p sum lie; _collect sums the weights before
+//     those bins, those that are kept for sure also in groups of 64 sixteen-byte
 //     pieces and lists the tokens of those bins; _pick ranks the listed ones (a few hundred to a few thousand), adds
 //     the kept ones to their groups, finds the group by a scan and the token in it by one wave.
 //   * _pick alone does a row of few tokens, and one that the bins do not tell apart (more than SM_LIST tokens in a
@@ -206,13 +207,21 @@ struct SmPieces {
 
 // ------------------------------------------------------------------ counts and weights of a part, by bins
 
-// grid (parts, rows). The part stays in registers between its maximum and its bins.
+// A token of weight w (<= 1) as what it adds to its bin: 1 above 49 bits for the sum of weights in units of 2^-34, at
+// most SM_MAX_PER * SM_TH * 8 = 2^14 tokens of them. (Adding 2^52 + 2^49 rounds to an integer in the mantissa's low bits.)
+__device__ __forceinline__ u64 sm_pack(float w) {
+  const double s = __builtin_fma((double)w, 17179869184.0, 4503599627370496.0 + 562949953421312.0);
+  return __builtin_bit_cast(u64, s) & 0xFFFFFFFFFFFFFull;
+}
+
+// grid (parts, rows). The part stays in registers between its maximum and its bins. The bins' weights only say where
+// the cuts lie, so 32-bit exponentials do (arguments to -46, 4e-6 off; rounded to 2^-35, at most 2^14 times against a
+// largest of 1: 5e-7): one atomic a token, and half the instructions of a double.
 template <int DT>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
   constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER;
   __shared__ u64 red[SM_TH / 64];
-  __shared__ unsigned cnt[SM_BINS];
-  __shared__ u64 wts[SM_BINS];
+  __shared__ u64 bins[SM_BINS];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const SmPieces<DT> x(a, row);
   const int c0 = part * a.per * SM_TH + tid;
@@ -222,9 +231,9 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
     if (i < a.per) q[i] = x.bits(c0 + i * SM_TH);
   const float T = a.temperature[row], top_p = a.top_p[row];
   const int top_k = a.top_k[row];
-  if (part == 0 && tid == 0) a.listed[row] = 0;
+  if (part == 0 && tid == 0) a.listed[row] = 0, a.sums[2 * row] = a.sums[2 * row + 1] = 0;
 #pragma unroll
-  for (int i = 0; i < SM_BINS / SM_TH; ++i) cnt[i * SM_TH + tid] = 0, wts[i * SM_TH + tid] = 0;
+  for (int i = 0; i < SM_BINS / SM_TH; ++i) bins[i * SM_TH + tid] = 0;
   u64 best = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -250,6 +259,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
   const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
   if (sm_greedy(r.max, T, top_k, top_p) || !(k || p) || !r.binned(2097152.f)) return;
   const int top = r.grid(r.max);
+  const float c = 1.44269504088896340736f / T;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (i >= a.per) break;
@@ -258,17 +268,12 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs& a) {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int bin = top - r.grid(v[j]);
-      if (bin >= SM_BINS) continue;   // (-inf, and so those outside the row, too)
-      atomicAdd(&cnt[bin], 1u);
-      if (p) atomicAdd(&wts[bin], r.units(r.weight(v[j])));
+      if (bin < SM_BINS) atomicAdd(&bins[bin], sm_pack(__builtin_amdgcn_exp2f((v[j] - r.max) * c)));
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < SM_BINS / SM_TH; ++i) {
-    a.cnt[me * SM_BINS + i * SM_TH + tid] = cnt[i * SM_TH + tid];
-    if (p) a.wts[me * SM_BINS + i * SM_TH + tid] = wts[i * SM_TH + tid];
-  }
+  for (int i = 0; i < SM_BINS / SM_TH; ++i) a.bins[me * SM_BINS + i * SM_TH + tid] = bins[i * SM_TH + tid];
 }
 
 // ------------------------------------------------------------------ the bins of the cuts
@@ -295,7 +300,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
   const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
   SampleRow s;
-  s.best = best, s.ahead = s.base = s.total = 0.0, s.kb = -1, s.kr = 0, s.plo = s.phi = -1, s.pad = 0;
+  s.best = best, s.kb = -1, s.kr = 0, s.plo = s.phi = -1, s.pad = 0;
   s.mode = sm_greedy(r.max, T, top_k, top_p) ? 0 : !r.binned(1048576.f) ? 3 : k || p ? 2 : 1;
   if (s.mode != 2) {
     if (tid == 0) a.row[row] = s;
@@ -312,18 +317,16 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   unsigned c = 0;
   double w = 0.0;
   for (int q0 = odd; q0 < a.parts; q0 += 32) {
-    unsigned n[16];
-    u64 m[16];
+    u64 n[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {   // (a part that does not reach the bin is read at its first and left out)
       const long long at = ((long long)row * a.parts + min(q0 + 2 * j, a.parts - 1)) * SM_BINS;
       const int i = max(bin - off[q0 + 2 * j], 0);
-      n[j] = a.cnt[at + i];
-      m[j] = p ? a.wts[at + i] : 0;
+      n[j] = a.bins[at + i];
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (bin >= off[q0 + 2 * j]) c += n[j], w += f[q0 + 2 * j] * (double)m[j];
+      if (bin >= off[q0 + 2 * j]) c += (unsigned)(n[j] >> 49), w += f[q0 + 2 * j] * (double)(n[j] & ((1ull << 49) - 1));
   }
   if (odd) oddc[bin] = c, oddw[bin] = w;
   __syncthreads();
@@ -339,20 +342,17 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
     in_kb = w, base = w * (double)kr / (double)c;
   }
   __syncthreads();
-  s.kb = kb, s.kr = kr, s.ahead = ahead, s.total = wall;
+  s.kb = kb, s.kr = kr;
   s.plo = s.phi = kb;
   if (p) {
-    // (the slack covers weights rounded to a part's units here and to the row's there)
+    // (the slack is several times the error of the bins' weights)
     const double lo = kb < 0 ? wall : ahead + base, up = kb < 0 ? wall : ahead + in_kb;
-    const double plow = (double)top_p * lo * (1.0 - 1e-9), pup = (double)top_p * up * (1.0 + 1e-9);
+    const double plow = (double)top_p * lo * (1.0 - 2e-5), pup = (double)top_p * up * (1.0 + 2e-5);
     if (!odd && w0 < plow && w0 + w >= plow) atomicMin(&plo, bin);
     if (!odd && w0 < pup && w0 + w >= pup) atomicMin(&phi, bin);
     __syncthreads();
     const int last = kb < 0 ? SM_BINS - 1 : kb;
     s.plo = min(plo, last), s.phi = min(phi, last);
-    if (tid == s.plo) base = w0;
-    __syncthreads();
-    s.base = base;
   } else if (kb < 0) {
     s.mode = 1;   // (fewer tokens weigh anything than k)
   }
@@ -367,6 +367,7 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
   constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER, CAP = 1024;
   __shared__ u64 list[CAP];
   __shared__ unsigned n, at;
+  __shared__ u64 red[2 * SM_TH / 64];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const SmPieces<DT> x(a, row);
   const int c0 = part * a.per * SM_TH + tid;
@@ -381,6 +382,10 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
   SmRow r;
   r.init(sm_value((uint32_t)(s.best >> 32)), T, a.shift);
   const int top = r.grid(r.max), sure = s.mode == 1 ? SM_BINS : s.plo;
+  // top-p needs the weights of the bins before plo, and of those before the k-th token's
+  const bool p = s.mode == 2 && a.top_p[row] < 1.f;
+  const int before = !p ? sure : s.kb < 0 ? SM_BINS : s.kb;   // (>= sure)
+  u64 base = 0, ahead = 0;
   if (tid == 0) n = 0;
   __syncthreads();
 #pragma unroll
@@ -393,10 +398,13 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int bin = top - r.grid(v[j]);   // (outside the row: -inf, past every bin)
-      if (bin < sure) {
+      if (bin < before) {
         const double w = r.weight(v[j]);
-        sum += w >= least ? r.units(w) : 0;
-      } else if (s.mode == 2 && bin < SM_BINS && (bin <= s.phi || bin == s.kb)) {
+        const u64 in = r.units(w);
+        ahead += in;
+        if (bin < sure) base += in, sum += w >= least ? in : 0;
+      }
+      if (bin >= sure && s.mode == 2 && bin < SM_BINS && (bin <= s.phi || bin == s.kb)) {
         const unsigned k = atomicAdd(&n, 1u);
         if (k < CAP) list[k] = sm_key(v[j], x.first(c) + j);
       }
@@ -405,7 +413,17 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
     const int g = (part * a.per + i) * (SM_TH / 64) + wave;
     if (lane == 0 && g < a.ngroups) a.groups[(long long)row * a.ngroups + g] = sum;
   }
+  if (p) {
+    base = sm_wave_sum(base), ahead = sm_wave_sum(ahead);
+    if (lane == 0) red[wave] = base, red[SM_TH / 64 + wave] = ahead;
+  }
   __syncthreads();
+  if (p && tid < 2) {
+    u64 w = 0;
+#pragma unroll
+    for (int i = 0; i < SM_TH / 64; ++i) w += red[tid * (SM_TH / 64) + i];
+    if (w) atomicAdd(&a.sums[2 * row + tid], w);
+  }
   if (n == 0) return;
   // (more than CAP: the row's count goes past SM_LIST, and k_sample_pick does it without the list)
   if (tid == 0) at = atomicAdd(&a.listed[row], n > CAP ? SM_LIST + 1 : n);
@@ -562,19 +580,19 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
           if (bin >= b0 && bin <= b1) f(list[i]);
         }
       };
-      double total = s.total;
+      u64 total = a.sums[2 * row + 1];
       if (s.kb >= 0) {
         cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, 0, s.best);
         if (top_p < 1.f) {
           u64 w = 0, all;
           each(s.kb, s.kb, [&](u64 key) { w += key >= cut ? r.units(r.weight(sm_value((uint32_t)(key >> 32)))) : 0; });
           sm_block_scan<SM_T>(w, t.red, &all);
-          total = s.ahead + (double)all;
+          total += all;
         }
       }
       if (top_p < 1.f) {
-        const u64 need = (u64)__builtin_ceil((double)top_p * total);
-        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, (u64)(s.base + 0.5), cut, s.best);
+        const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
+        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, a.sums[2 * row], cut, s.best);
         cut = c > cut ? c : cut;
       }
       __syncthreads();

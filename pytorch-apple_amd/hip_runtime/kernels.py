@@ -138,10 +138,10 @@ _struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), 
                           ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
                           ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
                           ("pad", I)])
-_struct("SampleRow", [("best", LL), ("ahead", C.c_double), ("base", C.c_double), ("total", C.c_double), ("mode", I),
+_struct("SampleRow", [("best", LL), ("mode", I),
                       ("kb", I), ("kr", I), ("plo", I), ("phi", I), ("pad", I)])
 _struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
-                       ("best", P), ("cnt", P), ("wts", P), ("row", P), ("groups", P), ("listed", P), ("list", P),
+                       ("best", P), ("bins", P), ("row", P), ("groups", P), ("sums", P), ("listed", P), ("list", P),
                        ("rows", I), ("vocab", I), ("dtype", I), ("shift", I), ("parts", I), ("ngroups", I),
                        ("per", I), ("pad", I)])
 
