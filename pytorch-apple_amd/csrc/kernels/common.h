@@ -636,7 +636,7 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   int page_groups;            // page_size / 16
   unsigned group_magic;       // ceil(2^32 / page_groups); 0 where page_groups is 1
   int grid_wide;              // workgroups of the wide tiles (the first ones), the rest take narrow tiles
-  int grid_narrow;
+  int grid_narrow;            // workgroups of the narrow tiles
   int pad;
 };
 

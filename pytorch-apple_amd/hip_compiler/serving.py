@@ -175,8 +175,9 @@ def lower_sample(low, node: OpNode) -> None:
     width = 16 // ELEM_SIZE[x.dtype]
     pieces = (V + width - 2) // width + 1   # most that a row, wherever it starts, can touch
     # Pieces a thread: few, so that few rows take many workgroups, but not over 32 parts, whose bins one workgroup adds
-    # up at 0.25 us a part. One row of 151,936 in bf16 is 10 parts of 8 (15 + 10 + 15 us), 19 of 4 (TBD) or
-    # 75 of 1 (5 + 23 + 5); 256 rows take 8.
+    # up. The first three launches for one row of 151,936 in bf16: 10 + 9 + 17 us in 10 parts of 8, 6 + 9 + 10 in 19 of
+    # 4, 5 + 11 + 7 in 38 of 2 (but call after call 45 us rather than 43), 5 + 14 + 6 in 75 of 1. 256 rows of float32:
+    # 39 + 10 + 57 by 8, 41 + 17 + 63 by 2.
     def parts_of(per):
         return -(-pieces // (256 * per))
     per = next((p for p in (1, 2, 4) if parts_of(p) <= 32 and B * parts_of(p) <= 1024), 8)

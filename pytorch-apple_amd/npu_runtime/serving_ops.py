@@ -190,8 +190,8 @@ def sample(logits, temperature, top_k, top_p, min_p, u):
     less than top_p times the sum of them all; ``min_p`` those of weight >= min_p (the largest weight is 1).
     The first ranked is always kept. The token is the first, by index, at which the running sum of the kept
     weights passes u times their sum (the last of positive weight where none does). ``temperature`` <= 0 or NaN
-    takes the first ranked; ``top_p`` and ``min_p`` that are NaN keep all. A NaN logit counts as -inf; where some are +inf they alone weigh, 1 each; a row without any
-    number gives 0. Weights and sums are held in 64 bits."""
+    takes the first ranked; ``top_p`` and ``min_p`` that are NaN keep all. A NaN logit counts as -inf; where some are
+    +inf they alone weigh, 1 each; a row without any number gives 0. Weights and sums are held in 64 bits."""
     check_sample(logits, temperature, top_k, top_p, min_p, u)
     x = logits.double()
     x = torch.where(x.isnan(), -torch.inf, x)
