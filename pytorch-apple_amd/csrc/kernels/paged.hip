@@ -13,6 +13,11 @@ __device__ __forceinline__ int pg_sequence(const int* q_start, int B, int row, i
   return n;
 }
 
+// Position of row `row` of sequence b; a length far below 0 stays there.
+__device__ __forceinline__ int pg_position(const int* q_start, const int* kv_len, int b, int row) {
+  return max(kv_len[b], -(1 << 30)) - (q_start[b + 1] - row);
+}
+
 // Page of position pos of sequence b, or -1 where it has no place.
 __device__ __forceinline__ int pg_page(const int* table, int b, int M, int page_size, long long pages, int pos) {
   if (pos < 0 || pos / page_size >= M) return -1;
@@ -34,7 +39,7 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_any(const Paged
   if (tid < 64) {
     const int b = pg_sequence(a.q_start, a.B, row, tid);
     const bool real = b < a.B && row >= a.q_start[0];
-    const int pos = real ? a.kv_len[min(b, a.B - 1)] - a.q_start[b + 1] + row : 0;
+    const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : 0;
     if (tid == 0) place[0] = real ? b : -1, place[1] = pos, place[2] = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
   }
   __syncthreads();
@@ -84,7 +89,7 @@ __device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
   const bool in = row < a.N;
   const int b = in ? pg_sequence(a.q_start, a.B, row, lane) : a.B;
   const bool real = b < a.B && row >= a.q_start[0];
-  const int pos = real ? a.kv_len[b] - a.q_start[b + 1] + row : 0;
+  const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : 0;
   const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
   if (real)
     for (int j = tid; j < half; j += TH) {
@@ -146,7 +151,7 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.H / a.KVH);
   const int b = pg_sequence(a.q_start, a.B, row, lane);
   const bool real = b < a.B && row >= a.q_start[0];
-  const int pos = real ? a.kv_len[b] - a.q_start[b + 1] + row : -1;
+  const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : -1;
   for (int d = lane; d < a.D; d += 64) q[d] = ld_f(a.q, row * a.q_rs + h * a.q_hs + d, a.dtype);
   float m = -INFINITY, l = 0.f, o[PG_ANY_D / 64] = {};
   const int end = min((long long)pos + 1, (long long)a.M * a.page_size);
@@ -312,6 +317,7 @@ __device__ __forceinline__ void pt_scan3(int (&v)[3], int (&total)[3], int (&red
 __device__ __forceinline__ int pt_splits(const PtSeq& q, int share) { return max(1, (q.blocks + share - 1) / share); }
 
 // Narrow sequences' blocks (by 256 threads; ends with a barrier); returns their number, and that of rows and heads.
+// None where q_start descends: sequences then overlap, and their tiles could be more than the launch has room for.
 template <int PB>
 __device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t, int hi, int* rows) {
   int total[3] = {0, 0, 0};
@@ -319,7 +325,9 @@ __device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t
     const int b = c + threadIdx.x;
     int v[3] = {0, 0, 0};
     if (b < a.B) {
-      const PtSeq q = pt_seq<PT_NARROW, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], 0, hi);
+      const int s0 = a.q_start[b], s1 = a.q_start[b + 1];
+      const PtSeq q = pt_seq<PT_NARROW, PB>(a, b, s0, s1, a.kv_len[b], 0, hi);
+      v[2] = s1 < s0;
       v[0] = q.tiles * q.blocks * a.KVH;
       v[1] = q.n * a.H;
     }
@@ -327,8 +335,8 @@ __device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t
     if (b < a.B) t.items[b] = v[0], t.cost[b] = v[1];
   }
   __syncthreads();
-  *rows = total[1];
-  return total[0];
+  *rows = total[2] ? 0 : total[1];
+  return total[2] ? 0 : total[0];
 }
 
 // Workgroups that share `all` narrow blocks, of at most `most`, and the first block of workgroup w
@@ -344,17 +352,20 @@ __device__ __forceinline__ int pt_build_wide(const PagedAttnArgs& a, PtList& t, 
   const int tid = threadIdx.x;
   int work[3] = {0, 0, 0};
   for (int b = tid; b < a.B; b += 256) {
-    const PtSeq q = pt_seq<PT_WIDE, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], PT_NARROW, ANY);
+    const int s0 = a.q_start[b], s1 = a.q_start[b + 1];
+    const PtSeq q = pt_seq<PT_WIDE, PB>(a, b, s0, s1, a.kv_len[b], PT_NARROW, ANY);
+    work[1] |= s1 < s0;
     work[0] += q.tiles * q.blocks * a.KVH;
   }
   int total[3] = {0, 0, 0};
   pt_scan3(work, total, t.red);
   const int share = max((total[0] + PT_WIDE_ITEMS - 1) / PT_WIDE_ITEMS, PT_WIDE_LEAST);
+  const bool down = total[1] != 0;
   total[0] = total[1] = total[2] = 0;
   for (int c = 0; c < a.B; c += 256) {
     const int b = c + tid;
     int v[3] = {0, 0, 0};
-    if (b < a.B) {
+    if (b < a.B && !down) {
       const PtSeq q = pt_seq<PT_WIDE, PB>(a, b, a.q_start[b], a.q_start[b + 1], a.kv_len[b], PT_NARROW, ANY);
       const int S = pt_splits(q, share);
       v[0] = q.tiles * S * a.KVH;
@@ -1135,7 +1146,10 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
                                   [](int s) { return s; }, out(q, h, row));
         });
   }
-  const int s0 = start[0], s1 = start[a.B];
+  int down = 0;   // (no batch: every row)
+  for (int b = lane; b < a.B; b += 64) down |= start[b + 1] < start[b];
+  const bool none = __ballot(down) != 0;
+  const int s0 = none ? 0 : start[0], s1 = none ? 0 : start[a.B];
   for (int row = me; row < a.N; row += waves) {
     if (row >= s0 && row < s1) continue;
     uint4* o = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);

@@ -14,6 +14,9 @@ Three tensors say which sequence a row belongs to (all int32):
   ``q_start[b] + i`` of n sits at position ``kv_len[b] - n + i``.
 * ``block_table`` [B, M]: position p of b lies in row ``p % page_size`` of page ``block_table[b, p // page_size]``.
 
+The definitions below refuse a ``q_start`` that descends. A device takes the three as they come, since reading them
+would wait for it: attention then gives zeros, append writes what it writes within the pools.
+
 A position that has no place (before 0, past the table, in a page that is not one of the pool's) is not
 written and is closed to attention: its key and value are not read, whatever they hold. Where two rows name
 one place it holds one of them. Pools are [P, KVH, page_size, D] (page_layout "hnd") or

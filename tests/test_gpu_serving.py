@@ -299,6 +299,37 @@ def test_paged_attention_of_many_sequences(backend, seqs):
     _attention(backend, R.batch([min(int(k), 1) for k in kv], [int(k) for k in kv], 16, pad=5), 4, 1, 64, "bfloat16", 16, "hnd")
 
 
+@pytest.mark.parametrize("D,starts", [(128, [0, 5, 2, 40]), (64, [3, 1, 0, 0]), (128, [0, 40] * 30 + [0])])
+def test_paged_attention_of_starts_that_descend(backend, D, starts):
+    """No batch: nothing outside the tensors is touched, and every row is zero."""
+    from irgen.serving import build_paged_attention_ir
+
+    B, dt = len(starts) - 1, torch.bfloat16
+    t = {"q": _rand(1, 41, 4, D).to(dt), "k_pages": _rand(2, 9, 2, 16, D).to(dt), "v_pages": _rand(3, 9, 2, 16, D).to(dt),
+         "block_table": torch.arange(B * 4, dtype=torch.int32).view(B, 4) % 9, "q_start": torch.tensor(starts, dtype=torch.int32),
+         "kv_len": torch.full((B,), 60, dtype=torch.int32)}
+    out, = _run(build_paged_attention_ir(41, B, 9, 16, 4, 4, 2, D), backend, t)
+    assert out.eq(0).all()
+
+
+def test_lengths_far_out_of_range(backend):
+    """Lengths at the ends of int32: positions before 0 have no place, those past the table neither."""
+    from irgen.serving import build_paged_append_ir, build_paged_attention_ir
+
+    dt, lim = torch.bfloat16, torch.iinfo(torch.int32)
+    meta = {"block_table": torch.arange(12, dtype=torch.int32).view(3, 4), "q_start": torch.tensor([0, 2, 4, 6], dtype=torch.int32),
+            "kv_len": torch.tensor([lim.min, lim.max, 70], dtype=torch.int32)}
+    t = {"q": _rand(1, 6, 4, 128).to(dt), "k": _rand(4, 6, 2, 128).to(dt), "v": _rand(5, 6, 2, 128).to(dt),
+         "k_pages": _rand(2, 12, 2, 16, 128).to(dt), "v_pages": _rand(3, 12, 2, 16, 128).to(dt), **meta, "inv_freq": _inv(64)}
+    _, kp, vp = _run(build_paged_append_ir(6, 3, 12, 16, 4, 4, 2, 128), backend, t)
+    assert torch.equal(kp, t["k_pages"]) and torch.equal(vp, t["v_pages"])
+    a = {n: t[n] for n in ("q", "k_pages", "v_pages", *meta)}
+    out, = _run(build_paged_attention_ir(6, 3, 12, 16, 4, 4, 2, 128), backend, a)
+    full, = _run(build_paged_attention_ir(6, 3, 12, 16, 4, 4, 2, 128), backend,
+                 {**a, "kv_len": torch.tensor([-1, 1 << 30, 66], dtype=torch.int32)})
+    assert out[:2].eq(0).all() and torch.isfinite(out.float()).all() and torch.equal(out, full)
+
+
 # ---------------------------------------------------------------- together, captured, on other streams
 
 def _step_graph(N, B, P, page, M, H, KVH, D, V, dtype):
