@@ -29,7 +29,8 @@
 #define SM_MAX_PARTS 1024      // of a row
 #define SM_BINS 512            // of width T / 16
 #define SM_MAX_PER 8           // pieces of a part per thread, which stay in registers (SampleArgs.per)
-#define SM_LIST 4096           // tokens of the bins around the cuts
+#define SM_LIST 16384          // tokens of the bins around the cuts: a tenth of 150,000, as where their spread is T / 4
+#define SM_NEAR 4096           // of them in LDS, if no more
 #define SM_RANK 256            // tokens ranked against each other: n^2 reads of LDS, 4 us at 256
 #define SM_SPLIT 2048
 #define SM_GROUPS 4096         // groups of 64 pieces: vocab <= SM_GROUPS * 64 * (4 | 8)
@@ -532,7 +533,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
   constexpr int E = SmPieces<DT>::E, PER = SM_GROUPS / SM_T;
   __shared__ SmCut t;
   __shared__ u64 groups[SM_GROUPS];
-  __shared__ u64 list[SM_LIST];
+  __shared__ u64 near[SM_NEAR];
   static_assert(SM_SPLIT == 2 * SM_T && SM_RANK <= SM_T, "");
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const SmPieces<DT> x(a, row);
@@ -571,13 +572,18 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
   if (listed) {
     for (int g = tid; g < ng; g += SM_T) groups[g] = a.groups[(long long)row * a.ngroups + g];
     if (s.mode == 2) {
-      for (int i = tid; i < (int)n; i += SM_T) list[i] = a.list[(long long)row * SM_LIST + i];
+      const u64* far = a.list + (long long)row * SM_LIST;
+      const bool in = n <= SM_NEAR;
+      if (in)
+        for (int i = tid; i < (int)n; i += SM_T) near[i] = far[i];
       __syncthreads();
+      auto list = [&](int i) { return in ? near[i] : far[i]; };
       const int top = r.grid(r.max);
       auto each = [&](int b0, int b1, auto f) {   // keys of bins b0 .. b1
         for (int i = tid; i < (int)n; i += SM_T) {
-          const int bin = top - r.grid(sm_value((uint32_t)(list[i] >> 32)));
-          if (bin >= b0 && bin <= b1) f(list[i]);
+          const u64 key = list(i);
+          const int bin = top - r.grid(sm_value((uint32_t)(key >> 32)));
+          if (bin >= b0 && bin <= b1) f(key);
         }
       };
       u64 total = a.sums[2 * row + 1];
@@ -597,8 +603,9 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       }
       __syncthreads();
       for (int i = tid; i < (int)n; i += SM_T) {
-        const int idx = (int)~(uint32_t)list[i];
-        const u64 w = kept(sm_value((uint32_t)(list[i] >> 32)), idx, least);
+        const u64 key = list(i);
+        const int idx = (int)~(uint32_t)key;
+        const u64 w = kept(sm_value((uint32_t)(key >> 32)), idx, least);
         if (w) atomicAdd(&groups[(idx + x.skew) / E / 64], w);
       }
     }

@@ -16,7 +16,7 @@ PAGED_APPEND_ROW_N = 1024      # up to this many rows a workgroup per row, past 
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
 PT_GRID = 512                  # two workgroups per CU
 # sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, bins, tokens of a list
-SAMPLE_MAX_PIECES, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 512, 4096
+SAMPLE_MAX_PIECES, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 512, 16384
 SAMPLE_PICK_PIECES = 1024      # up to this many pieces k_sample_pick alone
 
 

@@ -138,3 +138,12 @@ def test_the_step_graph_is_one_program():
 
     plan = partition(build_paged_ir(40, 6, 40, 16, 12, QwenConfig(layers=2)), is_hip_op_supported)
     assert [p.target for p in plan.steps] == ["npu"]
+
+
+def test_the_program_survives_its_file(tmp_path):
+    from hip_compiler import compile_subgraph
+    from hip_compiler.program_io import load_program, save_program
+
+    prog = compile_subgraph(build_paged_ir(40, 6, 40, 16, 12, QwenConfig(layers=1)))
+    save_program(prog, tmp_path / "step.hipbin")
+    assert load_program(tmp_path / "step.hipbin") == prog
