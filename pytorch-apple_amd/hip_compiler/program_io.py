@@ -121,16 +121,16 @@ def load_program(path: str) -> HIPProgram:
 
 def compiler_fingerprint() -> str:
     """Hash of every source the lowering depends on: the compiler itself, the IR reader and
-    partitioner it imports (``npu_compiler``) and the kernel-argument layouts the launch records
-    are packed against (``hip_runtime/kernels.py``). A cached program is reused only with the
-    lowering that produced it."""
+    partitioner it imports (``npu_compiler``), the serving operators' argument checks and the
+    kernel-argument layouts the launch records are packed against (``hip_runtime/kernels.py``).
+    A cached program is reused only with the lowering that produced it."""
     h = hashlib.sha256()
     here = os.path.dirname(os.path.abspath(__file__))
     pkg = os.path.dirname(here)
     files = [os.path.join(here, n) for n in sorted(os.listdir(here)) if n.endswith(".py")]
     npu = os.path.join(pkg, "npu_compiler")
     files += [os.path.join(npu, n) for n in sorted(os.listdir(npu)) if n.endswith(".py")]
-    files.append(os.path.join(pkg, "hip_runtime", "kernels.py"))
+    files += [os.path.join(pkg, "npu_runtime", "serving_ops.py"), os.path.join(pkg, "hip_runtime", "kernels.py")]
     for path in files:
         with open(path, "rb") as f:
             h.update(os.path.relpath(path, pkg).encode() + b"\0" + f.read())

@@ -426,3 +426,28 @@ def test_a_pool_that_starts_between_pieces_is_refused(backend):
     odd.copy_(vp)
     with pytest.raises(ValueError, match="16"):
         dag.execute({**bufs, "v_pages": backend.allocate_buffer(odd)})
+
+
+def test_an_exported_module(backend):
+    """A module that calls the ops, traced and run on the device, against its own eager run. float32 sums of up to 64
+    products and 40 positions, in another order: 64 + 40 half steps of values under 10."""
+    from irgen.exporter import extract_ir
+
+    class Step(torch.nn.Module):
+        def forward(self, q, k, v, k_pages, v_pages, table, start, kv, inv, logits, t, top_k, p, m, u):
+            q, k_pages, v_pages = torch.ops.serving.paged_append(q, k, v, k_pages, v_pages, table, start, kv, inv,
+                                                                 page_layout="nhd")
+            o = torch.ops.serving.paged_attention(q, k_pages, v_pages, table, start, kv, 0.125, page_layout="nhd")
+            return o.flatten(1), k_pages, v_pages, torch.ops.serving.sample(logits, t, top_k, p, m, u)
+
+    bt = R.batch([5, 1, 0], [40, 17, 3], 8, pad=2, seed=4)
+    kp, vp = R.pools(bt, 2, 8, 64, "float32", "nhd")
+    par = _params(6, 9)
+    args = (_rand(1, bt["rows"], 4, 64), _rand(2, bt["rows"], 2, 64), _rand(3, bt["rows"], 2, 64), kp, vp, *_meta(bt).values(),
+            _inv(32), 3 * _rand(5, 6, 9000), *par.values())
+    want = Step()(*(a.clone() for a in args))
+    ir = extract_ir(Step(), args, "step")
+    got = _run(ir, backend, {i["name"]: a.clone() for i, a in zip(ir["graph_inputs"], args)})
+    for a, b in zip(got[:3], want[:3]):
+        assert (a - b).abs().max() <= 10 * 104 * 2.0 ** -24
+    assert torch.equal(got[3], want[3])
