@@ -644,8 +644,8 @@ struct SampleRow {            // sample.hip: what k_sample_merge finds out about
   unsigned long long best;    // key of the first ranked token
   int mode;                   // 0: the first ranked, 1: every token, 2: a cut within the listed bins, 3: not binned
   int kb, kr;                 // bin of the k-th token (-1: no cut) and its rank there, from 1
+  int kn;                     // tokens of bin kb
   int plo, phi;               // bins in which the last kept token lies
-  int pad;
 };
 
 struct SampleArgs {           // sample.hip: one token per row of logits [rows, vocab]

@@ -290,7 +290,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   __shared__ double f[SM_MAX_PARTS + 32];   // their largest tokens' weights
   __shared__ unsigned oddc[SM_BINS];
   __shared__ double oddw[SM_BINS];
-  __shared__ int kb, kr, plo, phi;
+  __shared__ int kb, kr, kn, plo, phi;
   __shared__ double ahead, in_kb, base;
   const int row = blockIdx.x, tid = threadIdx.x, bin = tid & (SM_BINS - 1), odd = tid / SM_BINS;
   const u64 key = tid < a.parts ? a.best[(long long)row * a.parts + tid] : 0;
@@ -301,7 +301,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
   const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
   SampleRow s;
-  s.best = best, s.kb = -1, s.kr = 0, s.plo = s.phi = -1, s.pad = 0;
+  s.best = best, s.kb = -1, s.kr = s.kn = 0, s.plo = s.phi = -1;
   s.mode = sm_greedy(r.max, T, top_k, top_p) ? 0 : !r.binned(1048576.f) ? 3 : k || p ? 2 : 1;
   if (s.mode != 2) {
     if (tid == 0) a.row[row] = s;
@@ -313,7 +313,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   off[tid] = any ? min(top - r.grid(most), SM_BINS) : SM_BINS;
   f[tid] = any ? r.weight(most) : 0.0;
   if (tid < 32) off[SM_MAX_PARTS + tid] = SM_BINS, f[SM_MAX_PARTS + tid] = 0.0;
-  if (tid == 0) kb = -1, kr = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
+  if (tid == 0) kb = -1, kr = kn = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
   __syncthreads();
   unsigned c = 0;
   double w = 0.0;
@@ -338,12 +338,12 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   const unsigned c0 = sm_block_scan<SM_T>(c, redc, &call);
   const double w0 = sm_block_scan<SM_T>(w, redw, &wall);
   if (k && c0 < (unsigned)top_k && c0 + c >= (unsigned)top_k) {
-    kb = bin, kr = top_k - (int)c0, ahead = w0;
+    kb = bin, kr = top_k - (int)c0, kn = (int)c, ahead = w0;
     // the bin's first kr tokens weigh at least their share of it, and at most all
     in_kb = w, base = w * (double)kr / (double)c;
   }
   __syncthreads();
-  s.kb = kb, s.kr = kr;
+  s.kb = kb, s.kr = kr, s.kn = kn;
   s.plo = s.phi = kb;
   if (p) {
     // (the slack is several times the error of the bins' weights)
@@ -445,32 +445,36 @@ struct SmCut {
 };
 
 // The smallest key in [lo, hi] with less than `need` before it: `before`, and the weights (1 each where `weigh` is
-// false) of the larger keys in [lo, hi]. each(f) calls f(key) for the keys of its thread; 0: none has it.
+// false) of the larger keys in [lo, hi]. `members`: how many these are, 0 where not known. each(f) calls f(key) for the keys of its thread; 0: none has it.
 template <typename F>
-__device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool weigh, u64 need, u64 before, u64 lo, u64 hi) {
+__device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool weigh, u64 need, u64 before, u64 lo, u64 hi,
+                                  u64 members) {
   const int tid = threadIdx.x;
   auto units = [&](u64 k) { return weigh ? r.units(r.weight(sm_value((uint32_t)(k >> 32)))) : 1ull; };
-  u64 least = ~0ull, most = 0, members = 0;
   __syncthreads();
-  each([&](u64 k) {
-    if (k < lo || k > hi) return;
-    least = k < least ? k : least, most = k > most ? k : most, ++members;
-  });
-  members = sm_wave_sum(members), least = ~sm_wave_max(~least), most = sm_wave_max(most);
-  if ((tid & 63) == 0) {
-    const int w = tid >> 6;
-    t.key[w] = least, t.key[SM_T / 64 + w] = most, t.w[w] = members;
-  }
-  __syncthreads();
-  members = 0;
+  if (members == 0 || members > SM_RANK) {
+    u64 least = ~0ull, most = 0;
+    members = 0;
+    each([&](u64 k) {
+      if (k < lo || k > hi) return;
+      least = k < least ? k : least, most = k > most ? k : most, ++members;
+    });
+    members = sm_wave_sum(members), least = ~sm_wave_max(~least), most = sm_wave_max(most);
+    if ((tid & 63) == 0) {
+      const int w = tid >> 6;
+      t.key[w] = least, t.key[SM_T / 64 + w] = most, t.w[w] = members;
+    }
+    __syncthreads();
+    members = 0;
 #pragma unroll
-  for (int w = 0; w < SM_T / 64; ++w) {
-    least = t.key[w] < least ? t.key[w] : least, most = t.key[SM_T / 64 + w] > most ? t.key[SM_T / 64 + w] : most;
-    members += t.w[w];
+    for (int w = 0; w < SM_T / 64; ++w) {
+      least = t.key[w] < least ? t.key[w] : least, most = t.key[SM_T / 64 + w] > most ? t.key[SM_T / 64 + w] : most;
+      members += t.w[w];
+    }
+    if (members == 0) return 0;
+    lo = least, hi = most;
+    __syncthreads();
   }
-  if (members == 0) return 0;
-  lo = least, hi = most;
-  __syncthreads();
   while (members > SM_RANK) {
     const int bits = 64 - __builtin_clzll((hi - lo) | 1), sh = max(bits - 11, 0);
     for (int i = tid; i < SM_SPLIT; i += SM_T) t.cnt[i] = 0, t.sum[i] = 0;
@@ -588,7 +592,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       };
       u64 total = a.sums[2 * row + 1];
       if (s.kb >= 0) {
-        cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, 0, s.best);
+        cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, 0, s.best, (u64)s.kn);
         if (top_p < 1.f) {
           u64 w = 0, all;
           each(s.kb, s.kb, [&](u64 key) { w += key >= cut ? r.units(r.weight(sm_value((uint32_t)(key >> 32)))) : 0; });
@@ -598,7 +602,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       }
       if (top_p < 1.f) {
         const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
-        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, a.sums[2 * row], cut, s.best);
+        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, a.sums[2 * row], cut, s.best, 0);
         cut = c > cut ? c : cut;
       }
       __syncthreads();
@@ -624,14 +628,14 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       }
       __syncthreads();
     };
-    if (k) cut = sm_cut(t, each, r, false, (u64)top_k, 0, 0, s.best);
+    if (k) cut = sm_cut(t, each, r, false, (u64)top_k, 0, 0, s.best, 0);
     if (top_p < 1.f) {
       weigh(0.0);
       u64 w = 0, total;
       for (int g = tid; g < ng; g += SM_T) w += groups[g];
       sm_block_scan<SM_T>(w, t.red, &total);
       const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
-      const u64 c = sm_cut(t, each, r, true, need, 0, cut, s.best);
+      const u64 c = sm_cut(t, each, r, true, need, 0, cut, s.best, 0);
       cut = c > cut ? c : cut;
     }
     weigh(least);

@@ -19,7 +19,7 @@ would wait for it: attention then gives zeros, append writes what it writes with
 
 A position that has no place (before 0, past the table, in a page that is not one of the pool's) is not
 written and is closed to attention: its key and value are not read, whatever they hold. Where two rows name
-one place it holds one of them. Pools are [P, KVH, page_size, D] (page_layout "hnd") or
+one place, each element of it is one of theirs. Pools are [P, KVH, page_size, D] (page_layout "hnd") or
 [P, page_size, KVH, D] ("nhd").
 """
 

@@ -330,6 +330,22 @@ def test_lengths_far_out_of_range(backend):
     assert out[:2].eq(0).all() and torch.isfinite(out.float()).all() and torch.equal(out, full)
 
 
+def test_rows_that_name_one_place(backend):
+    """Two sequences on one page: each element of the place is one of theirs, and nothing else changes."""
+    from irgen.serving import build_paged_append_ir
+
+    t = {"q": _rand(1, 2, 4, 128), "k": _rand(2, 2, 2, 128), "v": _rand(3, 2, 2, 128), "k_pages": _rand(4, 3, 2, 16, 128),
+         "v_pages": _rand(5, 3, 2, 16, 128)}
+    t = {n: x.to(torch.bfloat16) for n, x in t.items()}
+    t |= {"block_table": torch.ones(2, 1, dtype=torch.int32), "q_start": torch.arange(3, dtype=torch.int32),
+          "kv_len": torch.full((2,), 6, dtype=torch.int32), "inv_freq": _inv(64)}
+    _, _, vp = _run(build_paged_append_ir(2, 2, 3, 16, 1, 4, 2, 128), backend, t)
+    got = vp[1, :, 5].clone()
+    assert ((got == t["v"][0]) | (got == t["v"][1])).all()
+    vp[1, :, 5] = t["v_pages"][1, :, 5]
+    assert torch.equal(vp, t["v_pages"])
+
+
 # ---------------------------------------------------------------- together, captured, on other streams
 
 def _step_graph(N, B, P, page, M, H, KVH, D, V, dtype):
