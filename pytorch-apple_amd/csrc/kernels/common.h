@@ -646,6 +646,8 @@ struct SampleRow {            // sample.hip: what k_sample_merge finds out about
   int kb, kr;                 // bin of the k-th token (-1: no cut) and its rank there, from 1
   int kn;                     // tokens of bin kb
   int plo, phi;               // bins in which the last kept token lies
+  int pn;                     // tokens of these
+  int pad;
 };
 
 struct SampleArgs {           // sample.hip: one token per row of logits [rows, vocab]

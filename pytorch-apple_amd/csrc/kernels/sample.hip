@@ -290,7 +290,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   __shared__ double f[SM_MAX_PARTS + 32];   // their largest tokens' weights
   __shared__ unsigned oddc[SM_BINS];
   __shared__ double oddw[SM_BINS];
-  __shared__ int kb, kr, kn, plo, phi;
+  __shared__ int kb, kr, kn, plo, phi, pn;
   __shared__ double ahead, in_kb, base;
   const int row = blockIdx.x, tid = threadIdx.x, bin = tid & (SM_BINS - 1), odd = tid / SM_BINS;
   const u64 key = tid < a.parts ? a.best[(long long)row * a.parts + tid] : 0;
@@ -301,7 +301,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   r.init(sm_value((uint32_t)(best >> 32)), T, a.shift);
   const bool k = top_k > 0 && top_k < a.vocab, p = top_p < 1.f;
   SampleRow s;
-  s.best = best, s.kb = -1, s.kr = s.kn = 0, s.plo = s.phi = -1;
+  s.best = best, s.kb = -1, s.kr = s.kn = s.pn = s.pad = 0, s.plo = s.phi = -1;
   s.mode = sm_greedy(r.max, T, top_k, top_p) ? 0 : !r.binned(1048576.f) ? 3 : k || p ? 2 : 1;
   if (s.mode != 2) {
     if (tid == 0) a.row[row] = s;
@@ -313,7 +313,7 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
   off[tid] = any ? min(top - r.grid(most), SM_BINS) : SM_BINS;
   f[tid] = any ? r.weight(most) : 0.0;
   if (tid < 32) off[SM_MAX_PARTS + tid] = SM_BINS, f[SM_MAX_PARTS + tid] = 0.0;
-  if (tid == 0) kb = -1, kr = kn = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
+  if (tid == 0) kb = -1, kr = kn = pn = 0, ahead = in_kb = 0.0, plo = phi = SM_BINS;
   __syncthreads();
   unsigned c = 0;
   double w = 0.0;
@@ -354,6 +354,9 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
     __syncthreads();
     const int last = kb < 0 ? SM_BINS - 1 : kb;
     s.plo = min(plo, last), s.phi = min(phi, last);
+    if (c && bin >= s.plo && bin <= s.phi) atomicAdd(&pn, (int)c);
+    __syncthreads();
+    s.pn = pn;
   } else if (kb < 0) {
     s.mode = 1;   // (fewer tokens weigh anything than k)
   }
@@ -445,16 +448,16 @@ struct SmCut {
 };
 
 // The smallest key in [lo, hi] with less than `need` before it: `before`, and the weights (1 each where `weigh` is
-// false) of the larger keys in [lo, hi]. `members`: how many these are, 0 where not known. each(f) calls f(key) for the keys of its thread; 0: none has it.
+// false) of the larger keys in [lo, hi]. `members`: no less than there are (their range is then
+// [lo, hi] as given), or 0, not known. each(f) calls f(key) for the keys of its thread; 0: none has it.
 template <typename F>
 __device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool weigh, u64 need, u64 before, u64 lo, u64 hi,
                                   u64 members) {
   const int tid = threadIdx.x;
   auto units = [&](u64 k) { return weigh ? r.units(r.weight(sm_value((uint32_t)(k >> 32)))) : 1ull; };
   __syncthreads();
-  if (members == 0 || members > SM_RANK) {
+  if (members == 0) {
     u64 least = ~0ull, most = 0;
-    members = 0;
     each([&](u64 k) {
       if (k < lo || k > hi) return;
       least = k < least ? k : least, most = k > most ? k : most, ++members;
@@ -531,6 +534,10 @@ __device__ __forceinline__ u64 sm_cut(SmCut& t, F each, const SmRow& r, bool wei
   return found == ~0ull ? 0 : found;
 }
 
+// A key below those of the grid's place g, and not below those of place g - 2 (whose values are off by a 16th, and the
+// quotient by an 8th, of a place).
+__device__ __forceinline__ u64 sm_low(const SmRow& r, int g) { return (u64)sm_order(((float)g - 0.5f) / r.scale) << 32; }
+
 // grid (rows)
 template <int DT>
 __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
@@ -592,7 +599,8 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       };
       u64 total = a.sums[2 * row + 1];
       if (s.kb >= 0) {
-        cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, 0, s.best, (u64)s.kn);
+        cut = sm_cut(t, [&](auto f) { each(s.kb, s.kb, f); }, r, false, (u64)s.kr, 0, sm_low(r, top - s.kb),
+                     min(s.best, sm_low(r, top - s.kb + 2)), (u64)s.kn);
         if (top_p < 1.f) {
           u64 w = 0, all;
           each(s.kb, s.kb, [&](u64 key) { w += key >= cut ? r.units(r.weight(sm_value((uint32_t)(key >> 32)))) : 0; });
@@ -602,7 +610,8 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs& a) {
       }
       if (top_p < 1.f) {
         const u64 need = (u64)__builtin_ceil((double)top_p * (double)total);
-        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, a.sums[2 * row], cut, s.best, 0);
+        const u64 c = sm_cut(t, [&](auto f) { each(s.plo, s.phi, f); }, r, true, need, a.sums[2 * row],
+                             max(cut, sm_low(r, top - s.phi)), min(s.best, sm_low(r, top - s.plo + 2)), (u64)s.pn);
         cut = c > cut ? c : cut;
       }
       __syncthreads();

@@ -188,7 +188,7 @@ def lower_sample(low, node: OpNode) -> None:
     args = dict(logits=low.ref(xv), temperature=low.ref(low.contiguous(temperature.name)),
                 top_k=low.ref(low.contiguous(top_k.name)), top_p=low.ref(low.contiguous(top_p.name)),
                 min_p=low.ref(low.contiguous(min_p.name)), u=low.ref(low.contiguous(u.name)), out=low.ref(out),
-                best=ws("best", 8 * B * parts), bins=ws("bins", 8 * B * parts * SAMPLE_BINS), row=ws("row", 32 * B),
+                best=ws("best", 8 * B * parts), bins=ws("bins", 8 * B * parts * SAMPLE_BINS), row=ws("row", 40 * B),
                 groups=ws("groups", 8 * B * groups), sums=ws("sums", 16 * B),
                 listed=ws("listed", 4 * B), list=ws("list", 8 * B * SAMPLE_LIST), rows=B, vocab=V,
                 dtype=DTYPE_CODE[x.dtype], shift=min(44, 62 - V.bit_length()), parts=parts, ngroups=groups, per=per)

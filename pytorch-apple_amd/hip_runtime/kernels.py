@@ -139,7 +139,8 @@ _struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), 
                           ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
                           ("pad", I)])
 _struct("SampleRow", [("best", LL), ("mode", I),
-                      ("kb", I), ("kr", I), ("kn", I), ("plo", I), ("phi", I)])
+                      ("kb", I), ("kr", I), ("kn", I), ("plo", I), ("phi", I),
+                      ("pn", I), ("pad", I)])
 _struct("SampleArgs", [("logits", P), ("temperature", P), ("top_k", P), ("top_p", P), ("min_p", P), ("u", P), ("out", P),
                        ("best", P), ("bins", P), ("row", P), ("groups", P), ("sums", P), ("listed", P), ("list", P),
                        ("rows", I), ("vocab", I), ("dtype", I), ("shift", I), ("parts", I), ("ngroups", I),
