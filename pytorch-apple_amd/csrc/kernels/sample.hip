@@ -13,11 +13,11 @@
 //     512 bins of l of width T / 16, on one grid for all parts of a row and down from the part's largest (after 32 T
 //     weights round to 0, so the bins hold all that weigh), near enough to say where a cut lies; _merge adds the parts
 //     up and finds the bins in which the k-th token and the end of the top-p sum lie; _collect sums the weights before
-//     those bins, those that are kept for sure also in groups of 64 sixteen-byte
-//     pieces and lists the tokens of those bins; _pick ranks the listed ones (a few hundred to a few thousand), adds
+//     those bins, those that are kept for sure also in groups of 64 sixteen-byte pieces, and lists the tokens of
+//     those bins; _pick ranks the listed ones (a few hundred to a few thousand), adds
 //     the kept ones to their groups, finds the group by a scan and the token in it by one wave.
-//     One row of 151,936 (bf16): 6 + 9 + 10 + 21 us, all waiting on memory and barriers, _pick most (16 waves of one
-//     workgroup). 256 rows in float32: 39 + 10 + 57 + 22 us; _hist reads at 4.0 TB/s, _collect does 45 instructions a
+//     One row of 151,936 (bf16): 6 + 9 + 10 + 16 us, all waiting on memory and barriers, _pick most (16 waves of one
+//     workgroup). 256 rows in float32: 39 + 10 + 58 + 17 us; _hist reads at 4.0 TB/s, _collect does some 45 instructions a
 //     token, two thirds of them the double exponential.
 //   * _pick alone does a row of few tokens, and one that the bins do not tell apart (more than SM_LIST tokens in a
 //     bin: equal logits; infinite ones): it splits the range of keys 2048 ways a pass over the row until at most 256
@@ -31,7 +31,7 @@
 #define SM_MAX_PER 8           // pieces of a part per thread, which stay in registers (SampleArgs.per)
 #define SM_LIST 16384          // tokens of the bins around the cuts: a tenth of 150,000, as where their spread is T / 4
 #define SM_NEAR 4096           // of them in LDS, if no more
-#define SM_RANK 256            // tokens ranked against each other: n^2 reads of LDS, 4 us at 256
+#define SM_RANK 256            // tokens ranked against each other, four threads a token
 #define SM_SPLIT 2048
 #define SM_GROUPS 4096         // groups of 64 pieces: vocab <= SM_GROUPS * 64 * (4 | 8)
 

@@ -80,6 +80,7 @@ class PagedGenerator:
             self.graphs.append((dag, rows, [o["name"] for o in ir["graph_outputs"]]))
         self._bufs: dict = {}
         self._written: dict = {}
+        self._moved: dict = {}
 
     # -- buffers ---------------------------------------------------------------------------
 
@@ -181,9 +182,16 @@ class PagedGenerator:
         for name, arr in (("block_table", table), ("q_start", start), ("kv_len", kv), ("last_rows", last), ("u", u),
                           *par.items()):
             feed[name] = self._input(name, arr)
-        out = dag.execute({**feed, **self._pools()})
+        pools = self._pools()
+        out = dag.execute({**feed, **pools})
         if self.backend is None:
             self._bufs["pools"] = dict(zip(self.pool_names, (out[o] for o in outputs[1:])))
+        else:
+            if rows not in self._moved:   # (pools that the program does not update in place; a graph's are always the same)
+                self._moved[rows] = [(n, o) for n, o in zip(self.pool_names, outputs[1:])
+                                     if out[o].native_handle.data_ptr() != pools[n].native_handle.data_ptr()]
+            for n, o in self._moved[rows]:
+                pools[n].native_handle.copy_(out[o].native_handle)
         tokens = out[outputs[0]]
         tokens = tokens.to_numpy() if hasattr(tokens, "to_numpy") else np.asarray(tokens)
         for s in drawn:

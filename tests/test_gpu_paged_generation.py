@@ -30,3 +30,21 @@ def test_generation_of_a_batch(backend, dtype, D, layout, half):
     assert gen.generate(ps, 9, par) == gen.generate(ps, 9, par)
     # top_k 1 is the likeliest token whatever else
     assert gen.generate(ps, 9, SamplingParams(temperature=1.5, top_k=1, top_p=0.3)) == got
+
+
+def test_pools_that_are_not_updated_in_place(backend):
+    """A step graph that reads a pool a second time gets a copy of it written: the generator carries it over."""
+    from irgen.qwen import build_paged_ir
+    from npu_runtime.paged_generation import PagedGenerator, SamplingParams
+
+    cfg = QwenConfig(hidden=256, intermediate=512, layers=1, heads=4, kv_heads=2, head_dim=64, vocab=4096)
+    ir = build_paged_ir(24, 3, 20, 16, 6, cfg)
+    w = M.make_weights(ir, cfg)
+    ps, greedy = M.prompts(cfg, [5, 40, 1]), SamplingParams(temperature=0.0)
+    want = PagedGenerator(M.executor(ir, w, backend), ir, backend=backend).generate(ps, 6, greedy)
+    pool = next(i for i in ir["graph_inputs"] if i["name"] == "k_pages_0")
+    ir["nodes"].append({"name": "twice", "op_type": "aten.add.Tensor", "inputs": [pool, pool], "attrs": {},
+                        "outputs": [{**pool, "name": "twice", "producer_node": "twice", "producer_output_idx": 0}]})
+    ir["graph_outputs"].append({**pool, "name": "twice"})
+    gen = PagedGenerator(M.executor(ir, w, backend), ir, backend=backend)
+    assert gen.generate(ps, 6, greedy) == want and gen._moved == {24: [("k_pages_0", ir["graph_outputs"][1]["name"])]}
