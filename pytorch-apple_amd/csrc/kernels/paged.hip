@@ -79,7 +79,8 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_any(const Paged
 // aligned rows). A wave per row, or the four waves of a workgroup where rows are few (_row): one row's chain of lookups
 // (q_start, kv_len, block_table, each waiting for the one before) is what it takes then, and its heads are done in one
 // step instead of three. Cosines and sines are taken once per row, for all heads, by a lane each. Bound by the bytes: each
-// row is read once and written once (5963 rows of 32 + 8 heads, 147 MB: 25.7 us, 5.7 TB/s).
+// row is read once and written once (5963 rows of 32 + 8 heads, 147 MB: 33 us, 4.4 TB/s; 34 with one
+// step's loads in flight at a time).
 template <int DT, int WAVES>
 __device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
   constexpr int ROWS = 4 / WAVES, TH = 64 * WAVES;
@@ -103,35 +104,54 @@ __device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
   // steps: pairs of pieces, then the pieces past R, then v's
   const int pairs = half / 8, rest = (a.D - a.R) / 8, qk = a.H + a.KVH;
   const int n0 = qk * pairs, n1 = n0 + qk * rest, n2 = n1 + a.KVH * (a.D / 8);
-  for (int i = tid; i < n2; i += TH) {
-    const bool pair = i < n0, v = i >= n1;
-    const int k = pair ? i : v ? i - n1 : i - n0, per = pair ? pairs : v ? a.D / 8 : rest;
-    const int h = k / per, e = (pair ? 0 : v ? 0 : a.R) + k % per * 8;
+  struct Step {
+    uint4 x, y;
+    uint16_t* dst;   // null: nothing to write
+    int e;
+    bool pair;
+  };
+  auto get = [&](int i) {
+    Step t;
+    const bool v = i >= n1;
+    t.pair = i < n0;
+    const int k = t.pair ? i : v ? i - n1 : i - n0, per = t.pair ? pairs : v ? a.D / 8 : rest;
+    const int h = k / per;
+    t.e = (t.pair ? 0 : v ? 0 : a.R) + k % per * 8;
     const bool isq = !v && h < a.H;
-    if (!isq && page < 0) continue;
     const int hk = v ? h : h - a.H;
     const uint16_t* src = isq ? (const uint16_t*)a.q + row * a.q_rs + h * a.q_hs
                          : v  ? (const uint16_t*)a.v + row * a.v_rs + hk * a.v_hs
                               : (const uint16_t*)a.k + row * a.k_rs + hk * a.k_hs;
-    uint16_t* dst = isq ? (uint16_t*)a.q_out + ((long long)row * a.H + h) * a.D
-                        : (uint16_t*)(v ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
-    const uint4 x = *(const uint4*)(src + e);
-    if (!pair) {
-      *(uint4*)(dst + e) = real ? x : make_uint4(0, 0, 0, 0);
-      continue;
+    t.dst = isq ? (uint16_t*)a.q_out + ((long long)row * a.H + h) * a.D
+            : page < 0 ? nullptr
+                       : (uint16_t*)(v ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
+    t.x = *(const uint4*)(src + t.e);
+    t.y = *(const uint4*)(src + t.e + (t.pair ? half : 0));
+    return t;
+  };
+  auto put = [&](const Step& t) {
+    if (!t.dst) return;
+    if (!t.pair) {
+      *(uint4*)(t.dst + t.e) = real ? t.x : make_uint4(0, 0, 0, 0);
+      return;
     }
-    const uint4 y = *(const uint4*)(src + half + e);
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    const uint32_t xw[4] = {t.x.x, t.x.y, t.x.z, t.x.w}, yw[4] = {t.y.x, t.y.y, t.y.z, t.y.w};
     uint32_t lo[4], up[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 c = *(const float2*)&cs[mine][0][e + 2 * j], d = *(const float2*)&cs[mine][1][e + 2 * j];
+      const float2 c = *(const float2*)&cs[mine][0][t.e + 2 * j], d = *(const float2*)&cs[mine][1][t.e + 2 * j];
       const float x0 = gm_lo<DT>(xw[j]), x1 = gm_hi<DT>(xw[j]), y0 = gm_lo<DT>(yw[j]), y1 = gm_hi<DT>(yw[j]);
       lo[j] = real ? gm_pack2<DT>(x0 * c.x - y0 * d.x, x1 * c.y - y1 * d.y) : 0u;
       up[j] = real ? gm_pack2<DT>(y0 * c.x + x0 * d.x, y1 * c.y + x1 * d.y) : 0u;
     }
-    *(uint4*)(dst + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    *(uint4*)(dst + half + e) = make_uint4(up[0], up[1], up[2], up[3]);
+    *(uint4*)(t.dst + t.e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *(uint4*)(t.dst + half + t.e) = make_uint4(up[0], up[1], up[2], up[3]);
+  };
+  for (int i = tid; i < n2; i += 2 * TH) {   // two steps' loads in flight
+    const bool two = i + TH < n2;
+    const Step s = get(i), t = get(two ? i + TH : i);
+    put(s);
+    if (two) put(t);
   }
 }
 extern "C" __global__ void __launch_bounds__(256) k_paged_append_bf16(const PagedAppendArgs a) { append_body<HS_BF16, 1>(a); }
