@@ -79,8 +79,8 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_any(const Paged
 // aligned rows). A wave per row, or the four waves of a workgroup where rows are few (_row): one row's chain of lookups
 // (q_start, kv_len, block_table, each waiting for the one before) is what it takes then, and its heads are done in one
 // step instead of three. Cosines and sines are taken once per row, for all heads, by a lane each. Bound by the bytes: each
-// row is read once and written once (5963 rows of 32 + 8 heads, 147 MB: 33 us, 4.4 TB/s; 34 with one
-// step's loads in flight at a time).
+// row is read once and written once (5963 rows of 32 + 8 heads, 147 MB: 33 us, 4.4 TB/s; 34 with the loads of one step in
+// flight rather than two).
 template <int DT, int WAVES>
 __device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
   constexpr int ROWS = 4 / WAVES, TH = 64 * WAVES;
