@@ -13,9 +13,10 @@ __device__ __forceinline__ int pg_sequence(const int* q_start, int B, int row, i
   return n;
 }
 
-// Position of row `row` of sequence b; a length far below 0 stays there.
-__device__ __forceinline__ int pg_position(const int* q_start, const int* kv_len, int b, int row) {
-  return max(kv_len[b], -(1 << 30)) - (q_start[b + 1] - row);
+// Position of row `row` of a sequence of `kv` positions whose rows end before `end`. Both may be any number: a position
+// far below 0 stays there.
+__device__ __forceinline__ int pg_position(int kv, int end, int row) {
+  return (int)max((long long)kv - ((long long)end - row), -(1ll << 30));
 }
 
 // Page of position pos of sequence b, or -1 where it has no place.
@@ -39,7 +40,7 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_any(const Paged
   if (tid < 64) {
     const int b = pg_sequence(a.q_start, a.B, row, tid);
     const bool real = b < a.B && row >= a.q_start[0];
-    const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : 0;
+    const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
     if (tid == 0) place[0] = real ? b : -1, place[1] = pos, place[2] = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
   }
   __syncthreads();
@@ -90,7 +91,7 @@ __device__ __forceinline__ void append_body(const PagedAppendArgs& a) {
   const bool in = row < a.N;
   const int b = in ? pg_sequence(a.q_start, a.B, row, lane) : a.B;
   const bool real = b < a.B && row >= a.q_start[0];
-  const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : 0;
+  const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
   const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
   if (real)
     for (int j = tid; j < half; j += TH) {
@@ -171,7 +172,7 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.H / a.KVH);
   const int b = pg_sequence(a.q_start, a.B, row, lane);
   const bool real = b < a.B && row >= a.q_start[0];
-  const int pos = real ? pg_position(a.q_start, a.kv_len, b, row) : -1;
+  const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : -1;
   for (int d = lane; d < a.D; d += 64) q[d] = ld_f(a.q, row * a.q_rs + h * a.q_hs + d, a.dtype);
   float m = -INFINITY, l = 0.f, o[PG_ANY_D / 64] = {};
   const int end = min((long long)pos + 1, (long long)a.M * a.page_size);
@@ -274,23 +275,23 @@ __device__ __forceinline__ int pt_ldc(const int* p, long long i) {
   return ((const __attribute__((address_space(4))) int*)p)[i];
 }
 
-// A sequence's share of the work: rows, tiles of R rows, blocks of PB positions that its last tile needs. Batches that
-// name rows outside the tensor have none.
+// A sequence's share of the work: its rows that the tensor has (start, n), their positions (kv - n + i), tiles of R rows,
+// blocks of PB positions that its last tile needs.
 struct PtSeq {
   int start, n, kv, tiles, blocks;
 };
 template <int R, int PB>
 __device__ __forceinline__ PtSeq pt_seq(const PagedAttnArgs& a, int b, int s0, int s1, int kv, int lo, int hi) {
-  PtSeq q{s0, s1 - s0, max(kv, -(1 << 30)), 0, 0};
+  const int start = max(s0, 0), stop = min(s1, a.N);
+  PtSeq q{start, max(stop, start) - start, pg_position(kv, s1, stop), 0, 0};
   const int G = a.H / a.KVH;
-  const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.N;
-  const long long rows = ok ? (long long)q.n * G : 0;
+  const long long rows = (long long)q.n * G;
   if (rows <= lo || rows > hi) {
     q.n = 0;
     return q;
   }
   q.tiles = (int)((rows + R - 1) / R);
-  const long long end = min((long long)max(kv, 1), (long long)a.M * a.page_size);
+  const long long end = min((long long)max(q.kv, 1), (long long)a.M * a.page_size);
   q.blocks = (int)((end + PB - 1) / PB);   // (at least one: a tile without positions writes its zeros)
   return q;
 }

@@ -9,7 +9,7 @@ Three tensors say which sequence a row belongs to (all int32):
 
 * ``q_start`` [B + 1], non-decreasing: rows ``q_start[b] .. q_start[b + 1] - 1`` of the packed new tokens are
   sequence b's, none for an idle one. Rows of no sequence are padding: they are computed as zeros and
-  written nowhere.
+  written nowhere. Of a sequence that begins before the rows or ends behind them, those that there are count.
 * ``kv_len`` [B]: positions in b's cache with the new tokens as the last of them, so that row
   ``q_start[b] + i`` of n sits at position ``kv_len[b] - n + i``.
 * ``block_table`` [B, M]: position p of b lies in row ``p % page_size`` of page ``block_table[b, p // page_size]``.

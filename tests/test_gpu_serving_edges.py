@@ -1,0 +1,120 @@
+"""Paged operators where batches reach past the tensors, on every kernel path.
+
+Tolerances count roundings (``serving_ref``)."""
+
+import pytest
+import torch
+
+import serving_ref as R
+from conftest import gpu_available
+from test_gpu_serving import _dag, _meta, _rand, _run
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a ROCm GPU")]
+
+LIM = torch.iinfo(torch.int32)
+
+
+def _calls(backend, ir, tensors, changes):
+    """The output of one program on ``tensors``, then with each of ``changes`` made to its inputs."""
+    bufs = {k: backend.allocate_buffer(t.cuda()) for k, t in tensors.items()}
+    dag, name = _dag(ir, backend), ir["graph_outputs"][0]["name"]
+    print(f"[case] {ir['model_name']} {[(i['name'], i['shape'], i['dtype']) for i in ir['graph_inputs'][:1]]}", flush=True)
+    outs = []
+    for change in ({}, *changes):
+        for k, t in change.items():
+            bufs[k].native_handle.copy_(t)
+        outs.append(dag.execute(bufs)[name].to_torch().cpu().clone())
+    return outs
+
+
+# the paths: both tile widths of the tiled kernels, and the plain kernel
+PATHS = [(128, "bfloat16", 16), (64, "float16", 32), (80, "bfloat16", 16), (64, "float32", 16)]
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+@pytest.mark.parametrize("news,kvs,before,behind", [
+    ([4, 1, 40, 3], [30, 9, 300, 8], 2, 20),     # the first sequence begins before the rows, the third ends behind them
+    ([6], [6], 0, 2), ([6], [40], 2, 0), ([1, 1, 1], [5, 5, 900], 0, 1),
+    ([70, 0, 90], [700, 3, 91], 33, 40),         # long chunks cut at both ends
+    ([3, 5], [3, 5], 3, 4)])                     # one row of one sequence
+def test_sequences_that_reach_past_the_rows(backend, D, dtype, page, news, kvs, before, behind):
+    """The rows that there are, each at its own position; nothing of an earlier call shows. The reference has the
+    missing rows too, and is cut."""
+    from irgen.serving import build_paged_attention_ir
+
+    H, KVH = 4, 2
+    bt = R.batch(news, kvs, page, seed=D)
+    kp, vp = R.pools(bt, KVH, page, D, dtype, stale=float("nan"))
+    q = _rand(3, bt["rows"], H, D, dtype=dtype)
+    out, mag, big = R.attention64(q, kp, vp, bt, page, D ** -0.5)
+    pad = 3
+    N = bt["rows"] - before - behind + (pad if behind == 0 else 0)
+    here = torch.zeros(N, H, D, dtype=q.dtype)
+    real = bt["rows"] - before - behind
+    here[:real] = q[before:before + real]
+    start = (bt["q_start"] - before).to(torch.int32)
+    B = len(news)
+    ir = build_paged_attention_ir(N, B, bt["pages"], page, bt["block_table"].shape[1], H, KVH, D, dtype)
+    valid = {"q": 100 + here, "k_pages": kp, "v_pages": torch.full_like(vp, 100.0), **_meta(bt),
+             "q_start": torch.tensor([0] + [N] * B, dtype=torch.int32), "kv_len": torch.full((B,), N, dtype=torch.int32)}
+    _, got = _calls(backend, ir, valid, [{"q": here, "v_pages": vp, "q_start": start, "kv_len": bt["kv_len"]}])
+    sl = slice(before, before + real)
+    tol = R.attention_tol(dtype, D, max(kvs), out[sl], mag[sl], big[sl])
+    worst = ((got[:real].double() - out[sl]).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+    assert got[real:].eq(0).all()
+
+
+@pytest.mark.parametrize("D,dtype,rows", [(128, "bfloat16", 0), (128, "float16", 1100), (80, "float32", 0)])
+def test_appended_sequences_that_reach_past_the_rows(backend, D, dtype, rows):
+    """Only the rows that there are rotate and are written, each at its own position. Tolerance as in test_paged_append."""
+    from irgen.serving import build_paged_append_ir
+    from test_gpu_serving import _inv
+
+    H, KVH, page, before, behind = 4, 2, 16, 2, 20
+    bt = R.batch([4, 1, 40 + rows, 3], [30, 9, 300 + rows, 8], page, seed=D)
+    kp, vp = R.pools(bt, KVH, page, D, dtype)
+    q, k, v = (_rand(i, bt["rows"], h, D, dtype=dtype) for i, h in enumerate((H, KVH, KVH)))
+    cut = slice(before, bt["rows"] - behind)
+    N = bt["rows"] - before - behind
+    ir = build_paged_append_ir(N, 4, bt["pages"], page, bt["block_table"].shape[1], H, KVH, D, dtype)
+    got = _run(ir, backend, {"q": q[cut], "k": k[cut], "v": v[cut], "k_pages": kp, "v_pages": vp, **_meta(bt),
+                             "q_start": (bt["q_start"] - before).to(torch.int32), "inv_freq": _inv(D // 2)})
+    ref = list(R.append64(q, k, v, kp, vp, bt, _inv(D // 2), page))
+    ref[0] = ref[0][cut]
+    places = R.places(bt, page)
+    for row, b, p in places[:before] + places[bt["rows"] - behind:]:   # the missing rows' places stay as they were
+        pg, off = R.slot(bt, b, p, page)
+        for x, old in ((ref[1], kp), (ref[2], vp)):
+            x[pg, :, off] = old[pg, :, off].double().numpy()
+    for g, x in zip(got[:2], ref[:2]):
+        assert (abs(g.double().numpy() - x) <= 1.001 * R.HALF_STEP[dtype] * abs(x) + 7 * 2.0 ** -24 * 16).all()
+    assert (got[2].double().numpy() == ref[2]).all()
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+def test_starts_and_lengths_at_the_ends_of_int32(backend, D, dtype, page):
+    """A row sits at kv_len - (q_start[b + 1] - row), whatever the two are."""
+    from irgen.serving import build_paged_attention_ir
+
+    N, H, KVH = 6, 4, 2
+    bt = R.batch([N], [4 * page], page)
+    kp, vp = R.pools(bt, KVH, page, D, dtype)
+    q = _rand(3, N, H, D, dtype=dtype)
+    bt["kv_len"][0] = N
+    out, mag, big = R.attention64(q, kp, vp, bt, page, D ** -0.5)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)   # noqa: E731
+    t = {"q": q, "k_pages": kp, "v_pages": vp, **_meta(bt)}
+    ir = build_paged_attention_ir(N, 1, bt["pages"], page, bt["block_table"].shape[1], H, KVH, D, dtype)
+    far = [{"q_start": i32(0, LIM.max), "kv_len": i32(LIM.max)},      # row i at position i
+           {"q_start": i32(LIM.min, LIM.max), "kv_len": i32(LIM.max)},
+           {"q_start": i32(LIM.min, N), "kv_len": i32(N)}]
+    none = [{"q_start": i32(0, LIM.max), "kv_len": i32(k)} for k in (LIM.min, -1, 0, 5, LIM.max - N)]
+    none += [{"q_start": i32(LIM.min, k), "kv_len": i32(N)} for k in (LIM.min, -5, 0)]
+    first, *got = _calls(backend, ir, t, far + none)
+    tol = R.attention_tol(dtype, D, N, out, mag, big)
+    for g in (first, *got[:len(far)]):
+        worst = ((g.double() - out).abs() / tol).max().item()
+        assert worst <= 1.0, worst
+    for g in got[len(far):]:
+        assert g.eq(0).all()
