@@ -13,6 +13,13 @@ __device__ __forceinline__ int pg_sequence(const int* q_start, int B, int row, i
   return n;
 }
 
+// Whether q_start descends somewhere (no batch), by one wave.
+__device__ __forceinline__ bool pg_descends(const int* q_start, int B, int lane) {
+  bool down = false;
+  for (int i = lane; i < B; i += 64) down |= q_start[i + 1] < q_start[i];
+  return __ballot(down) != 0;
+}
+
 // Position of row `row` of a sequence of `kv` positions whose rows end before `end`. Both may be any number: a position
 // far below 0 stays there.
 __device__ __forceinline__ int pg_position(int kv, int end, int row) {
@@ -171,7 +178,7 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
   __shared__ int at[64];   // page of each of the step's positions, -1: closed
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.H / a.KVH);
   const int b = pg_sequence(a.q_start, a.B, row, lane);
-  const bool real = b < a.B && row >= a.q_start[0];
+  const bool real = b < a.B && row >= a.q_start[0] && !pg_descends(a.q_start, a.B, lane);
   const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : -1;
   for (int d = lane; d < a.D; d += 64) q[d] = ld_f(a.q, row * a.q_rs + h * a.q_hs + d, a.dtype);
   float m = -INFINITY, l = 0.f, o[PG_ANY_D / 64] = {};

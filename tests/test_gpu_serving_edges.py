@@ -118,3 +118,18 @@ def test_starts_and_lengths_at_the_ends_of_int32(backend, D, dtype, page):
         assert worst <= 1.0, worst
     for g in got[len(far):]:
         assert g.eq(0).all()
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+@pytest.mark.parametrize("starts", [[0, 5, 2, 40], [3, 1, 0, 0], [0, 40] * 30 + [0], [9, LIM.min, LIM.max]])
+def test_starts_that_descend_are_no_batch_on_any_path(backend, D, dtype, page, starts):
+    from irgen.serving import build_paged_attention_ir
+
+    B, N = len(starts) - 1, 41
+    t = {"q": _rand(1, N, 4, D, dtype=dtype), "k_pages": _rand(2, 9, 2, page, D, dtype=dtype),
+         "v_pages": _rand(3, 9, 2, page, D, dtype=dtype),
+         "block_table": torch.arange(B * 4, dtype=torch.int32).view(B, 4) % 9,
+         "q_start": torch.tensor([0] + [N] * B, dtype=torch.int32), "kv_len": torch.full((B,), 60, dtype=torch.int32)}
+    ir = build_paged_attention_ir(N, B, 9, page, 4, 4, 2, D, dtype)
+    before, got = _calls(backend, ir, t, [{"q_start": torch.tensor(starts, dtype=torch.int32)}])
+    assert before.ne(0).any() and got.eq(0).all()
