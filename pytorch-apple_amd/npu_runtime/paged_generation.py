@@ -50,7 +50,7 @@ def _shapes(ir: dict) -> dict:
 
 class PagedGenerator:
     """``step`` (and ``decode``, a graph of one row per slot, if given) run by ``DAGExecutor`` s on ``backend``, or by
-    all-CPU plans with ``backend=None``."""
+    all-CPU plans with ``backend=None``. A ``decode`` of as many rows as ``step`` has nothing to save and is not run."""
 
     def __init__(self, step, step_ir: dict, decode=None, decode_ir: dict | None = None, backend=None):
         shapes = _shapes(step_ir)
@@ -67,7 +67,7 @@ class PagedGenerator:
                     if n["op_type"] == "serving.paged_append.default")
         dims = shapes[self.pool_names[0]][0]
         self.pages, self.page_size = dims[0], dims[2 if pool == "hnd" else 1]
-        self.graphs = []   # (executor, rows, output names), the smallest first
+        self.graphs = []   # (executor, rows, output names) of decode, if it is run, and step: no two of the same rows
         for dag, ir in ((decode, decode_ir), (step, step_ir)):
             if dag is None and ir is None:
                 continue
@@ -78,6 +78,8 @@ class PagedGenerator:
             if rows < self.slots:
                 raise ValueError(f"a graph of {rows} rows for {self.slots} slots: every slot needs a row")
             self.graphs.append((dag, rows, [o["name"] for o in ir["graph_outputs"]]))
+        if len(self.graphs) == 2 and self.graphs[0][1] == self.graphs[1][1]:
+            del self.graphs[0]
         self._bufs: dict = {}
         self._written: dict = {}
         self._moved: dict = {}
@@ -187,7 +189,7 @@ class PagedGenerator:
         if self.backend is None:
             self._bufs["pools"] = dict(zip(self.pool_names, (out[o] for o in outputs[1:])))
         else:
-            if rows not in self._moved:   # (pools that the program does not update in place; a graph's are always the same)
+            if rows not in self._moved:   # (pools that the graph of these rows does not update in place, always the same)
                 self._moved[rows] = [(n, o) for n, o in zip(self.pool_names, outputs[1:])
                                      if out[o].native_handle.data_ptr() != pools[n].native_handle.data_ptr()]
             for n, o in self._moved[rows]:
