@@ -63,10 +63,12 @@ class PagedGenerator:
         self.slots, self.table_pages = shapes["block_table"][0]
         if not self.pool_names:
             raise ValueError("not a paged step graph: it has no page pools")
-        pool = next(n["attrs"].get("page_layout", "hnd") for n in step_ir["nodes"]
-                    if n["op_type"] == "serving.paged_append.default")
+        layouts = {n["attrs"].get("page_layout", "hnd") for ir in (step_ir, decode_ir) if ir is not None
+                   for n in ir["nodes"] if n["op_type"] in ("serving.paged_append.default", "serving.paged_attention.default")}
+        if len(layouts) != 1:
+            raise ValueError(f"not graphs of one page_layout: {sorted(layouts)}")
         dims = shapes[self.pool_names[0]][0]
-        self.pages, self.page_size = dims[0], dims[2 if pool == "hnd" else 1]
+        self.pages, self.page_size = dims[0], dims[2 if layouts == {"hnd"} else 1]
         self.graphs = []   # (executor, rows, output names) of decode, if it is run, and step: no two of the same rows
         for dag, ir in ((decode, decode_ir), (step, step_ir)):
             if dag is None and ir is None:

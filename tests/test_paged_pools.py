@@ -64,3 +64,14 @@ def test_each_graph_carries_its_own_pools_over(step_inplace, decode_inplace, row
     # the same steps, and so the same sums: keys and values of every place are equal
     for name, pool in ref._pools().items():
         assert np.array_equal(gen._pools()[name].to_numpy(), pool)
+
+
+def test_graphs_of_two_page_layouts_are_refused():
+    """Pools of as many positions a page as K/V heads have one shape in both layouts."""
+    irs = [build_paged_ir(n, 2, 6, CFG.kv_heads, 9, CFG, layout) for n, layout in ((8, "hnd"), (2, "nhd"))]
+    with pytest.raises(ValueError, match="layout"):
+        PagedGenerator(None, irs[0], object(), irs[1])
+    mixed = build_paged_ir(8, 2, 6, CFG.kv_heads, 9, CFG)
+    next(n for n in mixed["nodes"] if n["op_type"] == "serving.paged_attention.default")["attrs"]["page_layout"] = "nhd"
+    with pytest.raises(ValueError, match="layout"):
+        PagedGenerator(None, mixed)
