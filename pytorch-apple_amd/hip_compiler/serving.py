@@ -91,7 +91,7 @@ def lower_paged_append(low, node: OpNode) -> None:
     qv, kv, vv = (_rows_view(low, t.name) for t in (q, k, v))
     q_out = low.new_storage(node.outputs[0].name, q.shape, q.dtype)
     low.views[node.outputs[0].name] = q_out
-    pools = [low.inplace_or_copy(t, o) for t, o in ((kp, node.outputs[1]), (vp, node.outputs[2]))]
+    pools = [low.inplace_or_copy(node, t, o) for t, o in ((kp, node.outputs[1]), (vp, node.outputs[2]))]
     if N == 0:
         return
     kernel, grid = "k_paged_append_any", N

@@ -1555,14 +1555,33 @@ class Lowering:
                 expect = t * s
         return st if st is not None else 0
 
-    def inplace_or_copy(self, self_t, out) -> TView:
-        """Where an op that updates part of ``self_t`` writes: the tensor itself when it is a whole graph input that
-        nothing else reads (a cache), else a copy of it."""
+    def _only_reader(self, node: OpNode, name: str) -> bool:
+        """Whether ``node``, once, is all that reads the memory of its operand ``name``, under any name: that of the
+        storage and of every view of it, the views and updates that lead to ``name`` apart. None is a graph output."""
+        storage = self.views[name].storage
+        names = {n for n, v in self.views.items() if v.storage == storage}
+        if names & self.graph_output_names:
+            return False
+
+        def reads(n: OpNode) -> list[str]:   # (a getitem lists every output of its source)
+            one = n.op_type == "<built-in function getitem>"
+            return [t.name for t in (n.inputs[int(n.attrs["index"]):][:1] if one else n.inputs) if t.name in names]
+
+        path, at = [], name
+        while at is not None and at in self.producer:
+            path.append(self.producer[at])
+            at = next(iter(reads(path[-1])), None)
+        readers = {n.name: n for t in names for n in self.consumers.get(t, []) if reads(n)}
+        return reads(node) == [name] and set(readers) == {node.name, *(n.name for n in path if reads(n))} \
+            and all(len(reads(n)) == 1 for n in path if reads(n))
+
+    def inplace_or_copy(self, node: OpNode, self_t, out) -> TView:
+        """Where ``node``, which updates part of its operand ``self_t``, writes: the tensor itself when it is a whole graph
+        input that nothing else reads (a cache), else a copy of it."""
         tv = self.view(self_t.name)
         st = self.storages[tv.storage]
-        if (self.inplace_inputs and st.kind == "input" and len(self.consumers.get(self_t.name, [])) == 1
-                and tv.is_contiguous() and tv.offset == 0 and tv.numel * tv.itemsize == st.nbytes
-                and self_t.name not in self.graph_output_names):
+        if (self.inplace_inputs and st.kind == "input" and tv.is_contiguous() and tv.offset == 0
+                and tv.numel * tv.itemsize == st.nbytes and self._only_reader(node, self_t.name)):
             self.flush_chains_reading(tv.storage)
             self.mutated_inputs.add(tv.storage)
             self.views[out.name] = tv
@@ -1576,7 +1595,7 @@ class Lowering:
         self_t, idx_t, src_t = node.inputs[0], node.inputs[1], node.inputs[2]
         out = node.outputs[0]
         dim = int(node.attrs.get("dim", 0)) % len(self_t.shape)
-        dst = self.inplace_or_copy(self_t, out)
+        dst = self.inplace_or_copy(node, self_t, out)
         tv, inplace = dst, dst.storage in self.mutated_inputs
         src = self.view(src_t.name)
         shape = list(tv.shape)
