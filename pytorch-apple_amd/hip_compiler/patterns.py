@@ -671,7 +671,7 @@ def _inplace_target(low, cx: _Ctx, t_name: str):
     past, cpos = ic.inputs[0], ic.inputs[1]
     st = low.storages.get(past.name)
     if (st is None or st.kind != "input" or len(low.consumers.get(past.name, [])) != 1
-            or past.name in low.graph_output_names or not low.inplace_inputs or cpos.shape != [1]):
+            or past.name in low.graph_output_names | low.kept_inputs or not low.inplace_inputs or cpos.shape != [1]):
         return None
     return ic, past.name, cpos.name
 
@@ -814,7 +814,7 @@ def _inplace_target_t(low, cx: _Ctx, t_name: str, T: int):
     past, cpos = ic.inputs[0], ic.inputs[1]
     st = low.storages.get(past.name)
     if (st is None or st.kind != "input" or len(low.consumers.get(past.name, [])) != 1
-            or past.name in low.graph_output_names or not low.inplace_inputs or cpos.shape != [T]):
+            or past.name in low.graph_output_names | low.kept_inputs or not low.inplace_inputs or cpos.shape != [T]):
         return None
     return ic, past.name, cpos.name
 

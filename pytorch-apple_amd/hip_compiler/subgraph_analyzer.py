@@ -338,6 +338,7 @@ class Lowering:
         self.attn_info: dict[str, dict] = {}     # split decode attention output -> partials (foldable prologue)
         self.mask_extents: dict[tuple, Ref] = {}  # prefill mask view -> per-query-block open extent
         self.graph_output_names = {o.name for o in graph.graph_outputs}
+        self.kept_inputs = set(graph.kept_inputs)
         self.mutated_inputs: set[str] = set()
         self._uid = 0
         for spec in graph.graph_inputs:
@@ -1557,10 +1558,11 @@ class Lowering:
 
     def _only_reader(self, node: OpNode, name: str) -> bool:
         """Whether ``node``, once, is all that reads the memory of its operand ``name``, under any name: that of the
-        storage and of every view of it, the views and updates that lead to ``name`` apart. None is a graph output."""
+        storage and of every view of it, the views and updates that lead to ``name`` apart. None is a graph output or read
+        after the graph."""
         storage = self.views[name].storage
         names = {n for n, v in self.views.items() if v.storage == storage}
-        if names & self.graph_output_names:
+        if names & (self.graph_output_names | self.kept_inputs):
             return False
 
         def reads(n: OpNode) -> list[str]:   # (a getitem lists every output of its source)

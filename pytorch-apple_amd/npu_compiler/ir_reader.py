@@ -44,6 +44,7 @@ class IRGraph:
     weight_name_mapping: dict[str, str]
     nodes: list[OpNode]
     constants: dict = field(default_factory=dict)
+    kept_inputs: list[str] = field(default_factory=list)   # graph inputs whose contents are read after the graph has run
 
     def get_node_by_name(self, name: str) -> OpNode | None:
         return next((n for n in self.nodes if n.name == name), None)
@@ -81,6 +82,7 @@ def load_ir_from_dict(data: dict) -> IRGraph:
         weight_name_mapping=dict(data.get("weight_name_mapping", {})),
         nodes=[_node(n) for n in data["nodes"]],
         constants=dict(data.get("constants", {})),
+        kept_inputs=list(data.get("kept_inputs", [])),
     )
 
 

@@ -66,7 +66,7 @@ class DAGExecutor:
                 self._dispatch_table.append(("transfer", step, None, None))
                 continue
             if step.target == "npu":
-                program = self._compile_fn(_build_sub_ir_dict(step, plan.original_ir))
+                program = self._compile_fn(_with_kept_inputs(_build_sub_ir_dict(step, plan.original_ir), step, plan))
                 self.npu_programs[step.partition_id] = program
                 ex = backend.create_executor(program)
                 self._npu_executors[step.partition_id] = ex
@@ -188,6 +188,16 @@ class DAGExecutor:
                     pool[name] = val.to_numpy(dtype=val.dtype)
             elif isinstance(val, np.ndarray):
                 pool[name] = self.backend.allocate_buffer(val)
+
+
+def _with_kept_inputs(sub_ir: dict, part: Partition, plan: PartitionPlan) -> dict:
+    """``sub_ir`` with those of its graph inputs listed that a later partition reads or that are graph outputs of the
+    whole: the partition must leave them as they are (no update in place)."""
+    after = plan.steps[plan.steps.index(part) + 1:]
+    later = {n for s in after if isinstance(s, Partition) for n in s.input_names}
+    later |= {o["name"] for o in plan.original_ir.get("graph_outputs", [])}
+    kept = sorted(g["name"] for g in sub_ir["graph_inputs"] if g["name"] in later)
+    return {**sub_ir, "kept_inputs": kept} if kept else sub_ir
 
 
 def _build_sub_ir_dict(part: Partition, original_ir: dict) -> dict:

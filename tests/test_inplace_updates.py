@@ -122,3 +122,54 @@ def test_index_copy_of_a_view_with_another_reader():
     assert _updated(compile_subgraph(b.to_dict())) == ["past"]
     b.output(b.op("aten.mul.Tensor", [past, past]))
     assert _updated(compile_subgraph(b.to_dict())) == []
+
+
+class _Backend:
+    def create_executor(self, program):
+        return program
+
+
+def _partitions(ir, on_host):
+    """Inputs that each device partition updates in place, ``on_host`` being the ops that stay on the CPU."""
+    from hip_compiler import is_hip_op_supported
+    from npu_compiler import partition
+    from npu_runtime import DAGExecutor
+
+    plan = partition(ir, lambda op, attrs=None: op not in on_host and is_hip_op_supported(op, attrs))
+    dag = DAGExecutor(plan, _Backend(), compile_fn=compile_subgraph)
+    return [_updated(dag.npu_programs[i]) for i in sorted(dag.npu_programs)]
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_a_reader_in_another_partition(first):
+    """A partition on the host that reads a pool behind the update gets what the graph's input held; one before it is
+    done by then."""
+    s = _Step()
+    kp, vp = s.pool("k_pages"), s.pool("v_pages")
+    other = s.twice(kp) if first else None
+    q, k2, v2 = s.append(kp, vp)
+    s.b.output(q, k2, v2, other if first else s.twice(kp))
+    ir = s.b.to_dict()
+    assert _partitions(ir, {"aten.mul.Tensor"}) == [["k_pages", "v_pages"] if first else ["v_pages"]]
+    assert _partitions(ir, set()) == [["v_pages"]]
+
+
+def test_a_pool_that_two_partitions_update():
+    """What the first returned is updated by the second, unless it is a graph output."""
+    for out in (False, True):
+        s = _Step()
+        kp, vp = s.pool("k_pages"), s.pool("v_pages")
+        q, k1, v1 = s.append(kp, vp)
+        s.q = s.twice(q)   # on the host, between the two
+        q, k2, v2 = s.append(k1, v1)
+        s.b.output(q, k2, v2, *([k1] if out else []))
+        k1, v1 = k1.name, v1.name
+        assert _partitions(s.b.to_dict(), {"aten.mul.Tensor"}) == [["k_pages", "v_pages"], [v1] if out else sorted([k1, v1])]
+
+
+def test_a_graph_input_that_is_an_output_of_the_whole():
+    s = _Step()
+    kp, vp = s.pool("k_pages"), s.pool("v_pages")
+    q, k2, v2 = s.append(kp, vp)
+    s.b.output(q, k2, v2, kp)
+    assert _partitions(s.b.to_dict(), set()) == [["v_pages"]]
