@@ -477,6 +477,13 @@ __device__ __forceinline__ int pt_xv(int r) {
   return (D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
 }
 
+// Exponentials go to the second product in the pools' type, half a step of each (its operands have 16 bits; the sum takes
+// them unrounded). They are e^(s - m) 2^pt_up, so that float16 holds those far below the largest: a running maximum lags by up
+// to 8 in the exponent (softmax), so 2^15 is the most (65504 fits), and its smallest step, 2^-24, is 2^-31 of the largest.
+// Without the factor 16 nats below the largest a probability had one or two bits. bfloat16 has the range as it is.
+template <int DT>
+constexpr float pt_up = DT == HS_F16 ? 7.f : 0.f;
+
 // The state of a wave's 32 rows over the positions seen so far.
 template <int DT, int D>
 struct PtWave {
@@ -545,8 +552,8 @@ struct PtWave {
   }
 
   // Maximum and exponentials (left in s). Outputs are rescaled when a row's maximum has grown by more than 8 in
-  // the exponent, not at every new maximum: the exponentials stay below 2^8, as exact as below 1, and of 32 rows some
-  // row's maximum grows in nearly every block.
+  // the exponent, not at every new maximum: the exponentials stay below 2^8 (times 2^pt_up), as exact as below 1, and of
+  // 32 rows some row's maximum grows in nearly every block.
   template <int NB>
   __device__ __forceinline__ void softmax(pt_f32x16 (&s)[NB]) {
     float bm = -INFINITY;
@@ -569,7 +576,7 @@ struct PtWave {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
     }
-    const float mc = m == -INFINITY ? 0.f : -m * c;   // nothing open yet: every score is -inf
+    const float mc = m == -INFINITY ? 0.f : __builtin_fmaf(-m, c, pt_up<DT>);   // nothing open yet: every score is -inf
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
@@ -709,7 +716,8 @@ __device__ __forceinline__ void pt_load(const char* group, unsigned row_bytes, i
 }
 
 // One row over positions p0 .. p1 - 1 by a wave, 64 at a time, reading open positions only: the row's maximum of the raw
-// scores, sum of exponentials and the lane's outputs (dims lane * E ..). For tiles whose product is not finite.
+// scores, sum of exponentials and the lane's outputs (dims lane * E ..), times 2^pt_up as the tiles' (they may be joined
+// with them). For tiles whose product is not finite.
 template <int DT, int D>
 __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it, int row, int p0, int p1, float& m,
                                        float& l, float (&x)[D / 64]) {
@@ -730,7 +738,7 @@ __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it,
 #pragma unroll 1
       for (int d = 0; d < D; ++d) s = fmaf(gm_ld<DT>(q, d), gm_ld<DT>(a.k_pages, at + d), s);
     s = page < 0 ? -INFINITY : s * flip;
-    const float mn = fmaxf(m, wave_max(s)), mc = mn == -INFINITY ? 0.f : -mn * c;
+    const float mn = fmaxf(m, wave_max(s)), mc = mn == -INFINITY ? 0.f : __builtin_fmaf(-mn, c, pt_up<DT>);
     const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
     const float e = page < 0 ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, mc));
     m = mn;

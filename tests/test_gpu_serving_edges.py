@@ -1,4 +1,4 @@
-"""Paged operators where batches reach past the tensors, on every kernel path.
+"""Paged operators where batches reach past the tensors, and where a type's range ends, on every kernel path.
 
 Tolerances count roundings (``serving_ref``)."""
 
@@ -133,3 +133,67 @@ def test_starts_that_descend_are_no_batch_on_any_path(backend, D, dtype, page, s
     ir = build_paged_attention_ir(N, B, 9, page, 4, 4, 2, D, dtype)
     before, got = _calls(backend, ir, t, [{"q_start": torch.tensor(starts, dtype=torch.int32)}])
     assert before.ne(0).any() and got.eq(0).all()
+
+
+def _sink(news, kvs, sink, gap, D, page, H=4, KVH=2):
+    """Every score is exact: q picks out one dim of k. Place ``sink`` leads all others by ``gap`` to ``gap`` + 1.5 nats, and
+    holds the value 0, so that the output is what the others weigh."""
+    bt = R.batch(news, kvs, page, seed=7)
+    q = torch.zeros(bt["rows"], H, D, dtype=torch.float16)
+    q[:, :, 0] = 1.0
+    kp, vp = R.pools(bt, KVH, page, D, "float16")
+    kp[..., 1:] = 0
+    g = torch.Generator().manual_seed(5)
+    kp[..., 0] = (-gap - 1.5 * torch.rand(kp.shape[:-1], generator=g)).to(torch.float16)
+    for b in range(len(kvs)):
+        pg, off = R.slot(bt, b, sink, page)
+        kp[pg, :, off, 0], vp[pg, :, off] = 0.0, 0.0
+    vp *= 256   # (the outputs are then no subnormal numbers)
+    return bt, q, kp, vp
+
+
+@pytest.mark.parametrize("gap", [12.0, 14.0, 15.5])
+@pytest.mark.parametrize("D,page,news,kvs,sink", [
+    (128, 16, [1], [4000], 0), (64, 32, [1, 1], [4000, 900], 0), (128, 16, [1], [4000], 890),   # narrow tiles
+    (128, 16, [40], [3000], 0), (64, 32, [70], [2000], 1000)])                                  # wide ones
+def test_float16_probabilities_far_below_the_largest(backend, gap, D, page, news, kvs, sink):
+    """The probabilities are rounded to float16 for the second product, scaled by 2^7: half a step of each, or 2^-32 of
+    the largest where that is more (half of 2^-24, the type's smallest step). Any sequence's largest weighs 1 before
+    the division by their sum, which is at least 1."""
+    from irgen.serving import build_paged_attention_ir
+
+    bt, q, kp, vp = _sink(news, kvs, sink, gap, D, page)
+    ir = build_paged_attention_ir(bt["rows"], len(news), bt["pages"], page, bt["block_table"].shape[1], 4, 2, D, "float16",
+                                  scale=1.0)
+    got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, **_meta(bt)})
+    out, mag, big = R.attention64(q, kp, vp, bt, page, 1.0)
+    total = torch.zeros_like(out)   # sum |v| over the open places
+    for row, b, p in R.places(bt, page):
+        pg, off = zip(*(R.slot(bt, b, j, page) for j in range(p + 1)))
+        total[row] = vp[list(pg), :, list(off)].double().abs().sum(0).repeat_interleave(2, 0)
+    # the output itself may be subnormal: half of 2^-24
+    tol = R.attention_tol("float16", D, max(kvs), out, mag, big) + 2.0 ** -32 * total + 2.0 ** -25
+    worst = ((got.double() - out).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 32)])
+@pytest.mark.parametrize("new,kv,at", [(8, 9000, 8995), (40, 9000, 8980), (40, 9000, 8969)])
+def test_float16_parts_done_row_by_row_join_the_others(backend, D, page, new, kv, at):
+    """A value that is no number in the last part of a split tile, open to its later rows only: that part is done again
+    row by row, and the earlier rows' parts join as if it were not there."""
+    from irgen.serving import build_paged_attention_ir
+
+    bt = R.batch([new], [kv], page, seed=1)
+    kp, vp = R.pools(bt, 2, page, D, "float16")
+    pg, off = R.slot(bt, 0, at, page)
+    vp[pg, :, off] = float("nan")
+    q = _rand(9, new, 4, D, dtype="float16")
+    ir = build_paged_attention_ir(new, 1, bt["pages"], page, bt["block_table"].shape[1], 4, 2, D, "float16")
+    got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, **_meta(bt)})
+    out, mag, big = R.attention64(q, kp, vp, bt, page, D ** -0.5)
+    clean = at - (kv - new)
+    assert 0 <= clean < new and got[clean:].isnan().all()
+    tol = R.attention_tol("float16", D, kv, out[:clean], mag[:clean], big[:clean])
+    worst = ((got[:clean].double() - out[:clean]).abs() / tol).max().item()
+    assert worst <= 1.0, worst
