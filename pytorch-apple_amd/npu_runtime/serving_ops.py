@@ -54,9 +54,10 @@ def _check_pages(op: str, q, k_pages, v_pages, block_table, q_start, kv_len, pag
     _need(len(q.shape) == 3, f"{op}: q must be [rows, heads, head_dim], got {list(q.shape)}")
     _need(len(k_pages.shape) == 4 and tuple(k_pages.shape) == tuple(v_pages.shape),
           f"{op}: k_pages and v_pages must be pools of one 4-dimensional shape")
-    kvh = k_pages.shape[1 if page_layout == "hnd" else 2]
+    kvh, page_size = (k_pages.shape[i] for i in ((1, 2) if page_layout == "hnd" else (2, 1)))
+    _need(page_size > 0, f"{op}: pages of no position")
     _need(k_pages.shape[3] == q.shape[2], f"{op}: pools of head_dim {k_pages.shape[3]}, q of {q.shape[2]}")
-    _need(kvh > 0 and q.shape[1] % kvh == 0, f"{op}: {q.shape[1]} query heads do not divide among {kvh} K/V heads")
+    _need(kvh > 0 and q.shape[1] > 0 and q.shape[1] % kvh == 0, f"{op}: {q.shape[1]} query heads do not divide among {kvh} K/V heads")
     _need(len(kv_len.shape) == 1 and tuple(q_start.shape) == (kv_len.shape[0] + 1,)
           and len(block_table.shape) == 2 and block_table.shape[0] == kv_len.shape[0],
           f"{op}: need kv_len [B], q_start [B + 1] and block_table [B, M]")

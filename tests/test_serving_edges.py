@@ -4,6 +4,8 @@ import pytest
 import torch
 
 import serving_ref as R
+from hip_compiler import compile_subgraph
+from irgen.serving import build_paged_append_ir, build_paged_attention_ir
 from npu_runtime.serving_ops import paged_attention
 
 
@@ -17,3 +19,28 @@ def test_sequences_that_reach_past_the_rows(news, kvs, before, behind):
     out, mag, big = (t[cut] for t in R.attention64(q, kp, vp, bt, 16, 32 ** -0.5))
     got = paged_attention(q[cut], kp, vp, bt["block_table"], bt["q_start"] - before, bt["kv_len"], 32 ** -0.5)
     assert ((got.double() - out).abs() <= R.attention_tol("float32", 32, max(kvs), out, mag, big)).all()
+
+
+@pytest.mark.parametrize("heads,page,what", [(4, 0, "no position"), (0, 8, "do not divide")])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_pages_of_no_position_and_no_heads_are_refused(heads, page, what, layout):
+    """A kernel would divide by the page size, or be launched over no heads."""
+    shape = (5, 2, page, 16) if layout == "hnd" else (5, page, 2, 16)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)   # noqa: E731
+    for device in ("cpu", "meta"):
+        q, kv, pool = (torch.zeros(s, device=device) for s in ((3, heads, 16), (3, 2, 16), shape))
+        meta = [t.to(device) for t in (i32(2, 3), i32(3), i32(2))]
+        with pytest.raises(ValueError, match=what):
+            torch.ops.serving.paged_attention(q, pool, pool, *meta, 1.0, page_layout=layout)
+        with pytest.raises(ValueError, match=what):
+            torch.ops.serving.paged_append(q, kv, kv, pool, pool, *meta, torch.zeros(8, device=device), page_layout=layout)
+    # (built on a graph that is in order: the builder runs the check as well)
+    for build in (build_paged_append_ir, build_paged_attention_ir):
+        ir = build(3, 2, 5, 8, 3, 4, 2, 16, "float32", layout)
+        for t in [*ir["graph_inputs"], *(t for n in ir["nodes"] for t in [*n["inputs"], *n["outputs"]])]:
+            if t["shape"][1:] == list(((5, 2, 8, 16) if layout == "hnd" else (5, 8, 2, 16))[1:]):
+                t["shape"] = list(shape)
+            elif t["shape"] == [3, 4, 16]:
+                t["shape"] = [3, heads, 16]
+        with pytest.raises(ValueError, match=what):
+            compile_subgraph(ir)
