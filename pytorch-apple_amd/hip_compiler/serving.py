@@ -120,7 +120,9 @@ def lower_paged_attention(low, node: OpNode) -> None:
     check_paged_attention(q, kp, vp, table, q_start, kv_len, layout)
     N, H, D = (int(s) for s in q.shape)
     KVH, ps = _pool_dims(kp.shape, layout)
-    _check_i32(node.op_type, rows=N * H * D, table=int(table.shape[0]) * int(table.shape[1]), page=KVH * ps * D)
+    # (the plain kernel steps by 64 positions up to a table's last)
+    _check_i32(node.op_type, rows=N * H * D, table=int(table.shape[0]) * int(table.shape[1]), page=KVH * ps * D,
+               **{"positions of a table": int(table.shape[1]) * ps + 63})
     if D > PAGED_ANY_MAX_D:
         raise NotImplementedError(f"{node.op_type}: head_dim {D} is over {PAGED_ANY_MAX_D}")
     qv = _rows_view(low, q.name)

@@ -44,3 +44,19 @@ def test_pages_of_no_position_and_no_heads_are_refused(heads, page, what, layout
                 t["shape"] = [3, heads, 16]
         with pytest.raises(ValueError, match=what):
             compile_subgraph(ir)
+
+
+def test_tables_of_positions_past_32_bits_are_refused():
+    """The plain kernel's steps over the positions would pass 2^31 - 1, and begin again below 0."""
+    pages = lambda M: build_paged_attention_ir(1, 1, 4, 64, M, 2, 1, 16, "float32")   # noqa: E731
+    for M in (1 << 25, 1 << 26):
+        with pytest.raises(NotImplementedError, match="positions of a table"):
+            compile_subgraph(pages(M))
+    assert compile_subgraph(pages((1 << 25) - 1)).steps[-1].kernel == "k_paged_attn_any"
+    for M in (1 << 25, (1 << 25) - 1):   # (the tiled kernels' counts end before that)
+        ir = build_paged_attention_ir(1, 1, 4, 64, M, 2, 1, 64)
+        if M == 1 << 25:
+            with pytest.raises(NotImplementedError, match="positions of a table"):
+                compile_subgraph(ir)
+        else:
+            assert compile_subgraph(ir).steps[-1].kernel == "k_paged_attn_any"
