@@ -135,6 +135,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
     tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype)
     if tiled:
         qv = _aligned_rows(low, q.name, qv)
+        kv, vv = (low.aligned16(v, t.name) for t, v in ((kp, kv), (vp, vv)))
     args = dict(q=low.ref(qv), k_pages=low.ref(kv), v_pages=low.ref(vv), out=low.ref(out), part_o=None, part_ml=None,
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,

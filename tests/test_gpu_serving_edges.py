@@ -197,3 +197,19 @@ def test_float16_parts_done_row_by_row_join_the_others(backend, D, page, new, kv
     tol = R.attention_tol("float16", D, kv, out[:clean], mag[:clean], big[:clean])
     worst = ((got[:clean].double() - out[:clean]).abs() / tol).max().item()
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "bfloat16"), (128, "float16"), (80, "bfloat16")])
+@pytest.mark.parametrize("offset", [0, 8, 4, 1])
+def test_pools_that_are_ranges_of_an_input(backend, D, dtype, offset):
+    from test_serving_edges import _sliced_pools
+
+    bt = R.batch([3], [50], 16)
+    bt["block_table"], bt["pages"] = torch.tensor([[2, 0, 3, 1]], dtype=torch.int32), 4
+    kp, vp = R.pools(bt, 2, 16, D, dtype)
+    q = _rand(9, 3, 4, D, dtype=dtype)
+    flat = torch.cat([torch.full((offset,), float("nan"), dtype=kp.dtype), kp.flatten(), vp.flatten()])
+    got, = _run(_sliced_pools(offset, D, dtype), backend, {"q": q, "flat": flat, **_meta(bt)})
+    out, mag, big = R.attention64(q, kp, vp, bt, 16, D ** -0.5)
+    worst = ((got.double() - out).abs() / R.attention_tol(dtype, D, 50, out, mag, big)).max().item()
+    assert worst <= 1.0, worst

@@ -60,3 +60,26 @@ def test_tables_of_positions_past_32_bits_are_refused():
                 compile_subgraph(ir)
         else:
             assert compile_subgraph(ir).steps[-1].kernel == "k_paged_attn_any"
+
+
+def _sliced_pools(offset, D, dtype, N=3, page=16, pages=4):
+    """Attention over pools that are ranges of one flat input, beginning ``offset`` elements into it."""
+    from irgen.builder import IRBuilder
+    from irgen.serving import batch_inputs, paged_attention as attend
+
+    b = IRBuilder("Sliced")
+    size = pages * 2 * page * D
+    q, flat = b.input("q", [N, 4, D], dtype), b.input("flat", [offset + 2 * size], dtype)
+    cut = lambda at: b.op("aten.view.default", [b.op("aten.slice.Tensor", [flat], {"dim": 0, "start": at, "end": at + size})],
+                          {"size": [pages, 2, page, D]})   # noqa: E731
+    batch = batch_inputs(b, 1, pages)
+    b.output(attend(b, q, cut(offset), cut(offset + size), batch, D ** -0.5))
+    return b.to_dict()
+
+
+@pytest.mark.parametrize("offset,copies", [(0, 0), (8, 0), (4, 2), (1, 2)])
+def test_pools_that_begin_between_pieces_of_an_input_are_copied(offset, copies):
+    """The tiled kernels read pools in pieces of 16 bytes; the plain one by elements."""
+    steps = compile_subgraph(_sliced_pools(offset, 64, "bfloat16")).steps
+    assert [s.kind for s in steps].count("copy") == copies and steps[-1].kernel.startswith("k_paged_combine")
+    assert [s.kind for s in compile_subgraph(_sliced_pools(offset, 80, "bfloat16")).steps] == ["paged_attention"]
