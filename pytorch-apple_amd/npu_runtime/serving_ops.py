@@ -167,7 +167,7 @@ def paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, pa
     out = torch.zeros(N, H, D)
     for b in range(kv_len.numel()):
         rows = (seq == b).nonzero()[:, 0]
-        S = int(kv_len[b])
+        S = min(int(kv_len[b]), block_table.shape[1] * K.shape[1])   # (no places past the table)
         if rows.numel() == 0 or S <= 0:
             continue
         p = torch.arange(S)

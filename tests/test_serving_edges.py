@@ -83,3 +83,16 @@ def test_pools_that_begin_between_pieces_of_an_input_are_copied(offset, copies):
     steps = compile_subgraph(_sliced_pools(offset, 64, "bfloat16")).steps
     assert [s.kind for s in steps].count("copy") == copies and steps[-1].kernel.startswith("k_paged_combine")
     assert [s.kind for s in compile_subgraph(_sliced_pools(offset, 80, "bfloat16")).steps] == ["paged_attention"]
+
+
+def test_lengths_at_the_end_of_int32_take_no_memory():
+    """A sequence is looked at as far as its table reaches."""
+    bt = R.batch([2, 1], [40, 20], 16, extra_pages=0)
+    kp, vp = R.pools(bt, 2, 16, 32, "float32")
+    q = torch.randn(3, 4, 32, generator=torch.Generator().manual_seed(2))
+    ends = torch.full((2,), torch.iinfo(torch.int32).max, dtype=torch.int32)
+    bt["block_table"][1] = bt["block_table"][0]
+    got = paged_attention(q, kp, vp, bt["block_table"], bt["q_start"], ends, 0.2)
+    bt["kv_len"][:] = 48 + 2   # every row behind the table's 48 positions
+    out, mag, big = R.attention64(q, kp, vp, bt, 16, 0.2)
+    assert ((got.double() - out).abs() <= R.attention_tol("float32", 32, 48, out, mag, big)).all()
