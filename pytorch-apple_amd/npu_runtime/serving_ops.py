@@ -158,7 +158,7 @@ def paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_fr
 
 def paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, page_layout="hnd"):
     """softmax(scale q . k) v over the positions up to each row's own; query heads h of one K/V head h // (H / KVH)
-    share its pages. A row with no open position is zero."""
+    share its pages. A row with no open position is zero, and so is one whose open positions all score -inf."""
     check_paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, page_layout)
     N, H, D = q.shape
     K, V = _by_token(k_pages, page_layout), _by_token(v_pages, page_layout)
@@ -181,7 +181,7 @@ def paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, pa
         m = s.amax(-1, keepdim=True)
         e = torch.where(open_, (s - torch.where(m == float("-inf"), torch.zeros(()), m)).exp(), torch.zeros(()))
         z = e.sum(-1, keepdim=True)
-        o = (e @ v.unsqueeze(1)) / torch.where(open_.any(-1)[:, None], z, torch.ones(()))
+        o = (e @ v.unsqueeze(1)) / torch.where(z == 0, torch.ones(()), z)
         out[rows] = o.permute(2, 0, 1, 3).reshape(len(rows), H, D)
     return out.to(q.dtype)
 

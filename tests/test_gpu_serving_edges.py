@@ -213,3 +213,14 @@ def test_pools_that_are_ranges_of_an_input(backend, D, dtype, offset):
     out, mag, big = R.attention64(q, kp, vp, bt, 16, D ** -0.5)
     worst = ((got.double() - out).abs() / R.attention_tol(dtype, D, 50, out, mag, big)).max().item()
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+def test_rows_whose_scores_are_all_negative_infinity(backend, D, dtype, page):
+    from irgen.serving import build_paged_attention_ir
+    from test_serving_edges import all_infinite
+
+    q, kp, vp, (table, start, kv) = all_infinite(dtype, D, page)
+    ir = build_paged_attention_ir(3, 1, kp.shape[0], page, table.shape[1], 4, 2, D, dtype, scale=0.2)
+    got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, "block_table": table, "q_start": start, "kv_len": kv})
+    assert got[:2].eq(0).all() and torch.equal(got[2], vp[table[0, 0], :, 2].repeat_interleave(2, 0))

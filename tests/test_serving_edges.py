@@ -96,3 +96,20 @@ def test_lengths_at_the_end_of_int32_take_no_memory():
     bt["kv_len"][:] = 48 + 2   # every row behind the table's 48 positions
     out, mag, big = R.attention64(q, kp, vp, bt, 16, 0.2)
     assert ((got.double() - out).abs() <= R.attention_tol("float32", 32, 48, out, mag, big)).all()
+
+
+def test_rows_whose_scores_are_all_negative_infinity():
+    """They have nothing to weigh, as rows without an open position; with one finite score among them it takes all."""
+    q, kp, vp, meta = all_infinite("float32", 32, 16)
+    got = paged_attention(q, kp, vp, *meta, 0.2)
+    assert got[:2].eq(0).all() and torch.equal(got[2], vp[meta[0][0, 0], :, 2].repeat_interleave(2, 0))
+
+
+def all_infinite(dtype, D, page):
+    """Three rows at positions 0, 1 and 2; the keys of 0 and 1 score -inf, that of 2 does not."""
+    bt = R.batch([3], [3], page)
+    kp, vp = R.pools(bt, 2, page, D, dtype)
+    pg = int(bt["block_table"][0, 0])
+    kp[pg, :, :2, 0] = float("-inf")
+    q = torch.randn(3, 4, D, generator=torch.Generator().manual_seed(2)).abs().to(R.DT[dtype])
+    return q, kp, vp, [bt[n] for n in ("block_table", "q_start", "kv_len")]
