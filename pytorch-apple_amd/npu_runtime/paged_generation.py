@@ -193,9 +193,13 @@ class PagedGenerator:
         else:
             if rows not in self._moved:   # (pools that the graph of these rows does not update in place, always the same)
                 self._moved[rows] = [(n, o) for n, o in zip(self.pool_names, outputs[1:])
-                                     if out[o].native_handle.data_ptr() != pools[n].native_handle.data_ptr()]
+                                     if isinstance(out[o], np.ndarray)   # (of a part of the graph that runs on the host)
+                                     or out[o].native_handle.data_ptr() != pools[n].native_handle.data_ptr()]
             for n, o in self._moved[rows]:
-                pools[n].native_handle.copy_(out[o].native_handle)
+                if isinstance(out[o], np.ndarray):
+                    pools[n].write_from_numpy(out[o])
+                else:
+                    pools[n].native_handle.copy_(out[o].native_handle)
         tokens = out[outputs[0]]
         tokens = tokens.to_numpy() if hasattr(tokens, "to_numpy") else np.asarray(tokens)
         for s in drawn:

@@ -53,3 +53,32 @@ def test_old_contents_are_kept_for_their_readers(backend, how, on_host):
         y = got[o["name"]]
         y = torch.from_numpy(y.copy()) if not hasattr(y, "to_torch") else y.to_torch().cpu()
         assert (y - torch.from_numpy(want[o["name"]])).abs().max() <= 10 * 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_generation_with_the_append_on_the_host(backend, dtype):
+    """A plan that leaves the caches' update to the CPU: the generator takes the pools back to the device. Pools are then
+    compared place by place with those of a generator whose plan is all on the device: the same rotations, rounded once
+    (and what the layer before rounds otherwise: one layer)."""
+    import test_paged_generation as M
+    from hip_compiler import compile_subgraph, is_hip_op_supported
+    from irgen.qwen import QwenConfig, build_paged_ir
+    from npu_compiler import partition
+    from npu_runtime import DAGExecutor
+    from npu_runtime.paged_generation import PagedGenerator, SamplingParams
+
+    cfg = QwenConfig(hidden=256, intermediate=512, layers=1, heads=4, kv_heads=2, head_dim=64, vocab=4096, dtype=dtype)
+    ir = build_paged_ir(24, 3, 20, 16, 6, cfg)
+    w = M.make_weights(ir, cfg)
+    ps, greedy = M.prompts(cfg, [5, 40, 1]), SamplingParams(temperature=0.0)
+    plan = partition(ir, lambda op, attrs=None: op != "serving.paged_append.default" and is_hip_op_supported(op, attrs))
+    dag = DAGExecutor(plan, backend, compile_fn=compile_subgraph)
+    dag.load_weights(w)
+    print(f"[case] {dtype}", flush=True)
+    gens = [PagedGenerator(d, ir, backend=backend) for d in (M.executor(ir, w, backend), dag)]
+    got = [g.generate(ps, 1, greedy) for g in gens]
+    assert got[0] == got[1]
+    half = {"bfloat16": 2.0 ** -8, "float32": 2.0 ** -24}[dtype]
+    for a, b in zip(*(g._pools().values() for g in gens)):
+        a, b = a.native_handle.double(), b.native_handle.double()
+        assert a.ne(0).any() and ((a - b).abs() <= 2.01 * half * torch.maximum(a.abs(), b.abs()) + 2.0 ** -20 * a.abs().max()).all()

@@ -29,7 +29,7 @@ class _Backend:
 
 
 class _Program:
-    """A graph run on the host; pools are updated in place or returned in buffers of its own."""
+    """A graph run on the host; pools are updated in place, or returned in buffers of its own or as host arrays (None)."""
 
     def __init__(self, ir, weights, inplace):
         self.dag, self.inplace, self.calls = M.executor(ir, weights), inplace, 0
@@ -44,11 +44,11 @@ class _Program:
             new = torch.from_numpy(np.array(out[name]))
             if self.inplace:
                 feed[pool].native_handle.copy_(new)
-            got[name] = feed[pool] if self.inplace else _Buffer(new)
+            got[name] = feed[pool] if self.inplace else new.numpy() if self.inplace is None else _Buffer(new)
         return got
 
 
-@pytest.mark.parametrize("step_inplace,decode_inplace", [(False, True), (True, False), (False, False)])
+@pytest.mark.parametrize("step_inplace,decode_inplace", [(False, True), (True, False), (False, False), (None, True), (True, None)])
 @pytest.mark.parametrize("rows,decode_rows", [(6, 6), (9, 3), (4, 7)])
 def test_each_graph_carries_its_own_pools_over(step_inplace, decode_inplace, rows, decode_rows):
     """Also where both graphs have as many rows (one of them takes every step then), or the one of decode steps has more."""
