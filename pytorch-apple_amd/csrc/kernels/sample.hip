@@ -19,9 +19,10 @@
 //     One row of 151,936 (bf16): 6 + 9 + 10 + 16 us, all waiting on memory and barriers, _pick most (16 waves of one
 //     workgroup). 256 rows in float32: 39 + 10 + 58 + 17 us; _hist reads at 4.0 TB/s, _collect does some 45 instructions a
 //     token, two thirds of them the double exponential.
-//   * _pick alone does a row of few tokens, and one that the bins do not tell apart (more than SM_LIST tokens in a
-//     bin: equal logits; infinite ones): it splits the range of keys 2048 ways a pass over the row until at most 256
-//     tokens are left around the cut.
+//   * _pick alone does a row of few tokens, and one that the bins do not tell apart (more than SM_LIST tokens near the
+//     cuts, or more than SM_PART_LIST in one part: equal logits; infinite ones): it splits the range of keys 2048 ways
+//     a pass over the row until at most 256 tokens are left around the cut. 4,000 such tokens next to each other in
+//     each of 256 rows: 407 us, 136 where they lie all over the row.
 #include "common.h"
 
 #define SM_T 1024              // threads of _pick
@@ -30,7 +31,9 @@
 #define SM_BINS 512            // of width T / 16
 #define SM_MAX_PER 8           // pieces of a part per thread, which stay in registers (SampleArgs.per)
 #define SM_LIST 16384          // tokens of the bins around the cuts: a tenth of 150,000, as where their spread is T / 4
-#define SM_NEAR 4096           // of them in LDS, if no more
+#define SM_PART_LIST 1024      // of them in one part (up to 2^14 tokens): where that is of 8 pieces in 16 bits, a row of
+                               // 151,936 has 10 parts and lists 10,240 at most
+#define SM_NEAR 4096           // of a row's list in LDS, if no more
 #define SM_RANK 256            // tokens ranked against each other, four threads a token
 #define SM_SPLIT 2048
 #define SM_GROUPS 4096         // groups of 64 pieces: vocab <= SM_GROUPS * 64 * (4 | 8)
@@ -368,8 +371,8 @@ extern "C" __global__ void __launch_bounds__(SM_T) k_sample_merge(const SampleAr
 // grid (parts, rows): wave i of a part takes its groups i, i + 4, ..., all loads in flight together.
 template <int DT>
 __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
-  constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER, CAP = 1024;
-  __shared__ u64 list[CAP];
+  constexpr int E = SmPieces<DT>::E, N = SM_MAX_PER;
+  __shared__ u64 list[SM_PART_LIST];
   __shared__ unsigned n, at;
   __shared__ u64 red[2 * SM_TH / 64];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -410,7 +413,7 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
       }
       if (bin >= sure && s.mode == 2 && bin < SM_BINS && (bin <= s.phi || bin == s.kb)) {
         const unsigned k = atomicAdd(&n, 1u);
-        if (k < CAP) list[k] = sm_key(v[j], x.first(c) + j);
+        if (k < SM_PART_LIST) list[k] = sm_key(v[j], x.first(c) + j);
       }
     }
     sum = sm_wave_sum(sum);
@@ -429,10 +432,10 @@ __device__ __forceinline__ void sample_collect_body(const SampleArgs& a) {
     if (w) atomicAdd(&a.sums[2 * row + tid], w);
   }
   if (n == 0) return;
-  // (more than CAP: the row's count goes past SM_LIST, and k_sample_pick does it without the list)
-  if (tid == 0) at = atomicAdd(&a.listed[row], n > CAP ? SM_LIST + 1 : n);
+  // (more than the part lists: the row's count goes past SM_LIST, and k_sample_pick does it without the list)
+  if (tid == 0) at = atomicAdd(&a.listed[row], n > SM_PART_LIST ? SM_LIST + 1 : n);
   __syncthreads();
-  for (int i = tid; i < (int)min(n, (unsigned)CAP); i += SM_TH)
+  for (int i = tid; i < (int)min(n, (unsigned)SM_PART_LIST); i += SM_TH)
     if (at + i < SM_LIST) a.list[(long long)row * SM_LIST + at + i] = list[i];
 }
 

@@ -224,3 +224,19 @@ def test_rows_whose_scores_are_all_negative_infinity(backend, D, dtype, page):
     ir = build_paged_attention_ir(3, 1, kp.shape[0], page, table.shape[1], 4, 2, D, dtype, scale=0.2)
     got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, "block_table": table, "q_start": start, "kv_len": kv})
     assert got[:2].eq(0).all() and torch.equal(got[2], vp[table[0, 0], :, 2].repeat_interleave(2, 0))
+
+
+@pytest.mark.parametrize("n", [1000, 1025, 2500, 4000])
+@pytest.mark.parametrize("B,dtype", [(2, "float32"), (2, "bfloat16"), (90, "float16")])
+def test_sample_where_the_tokens_around_a_cut_lie_next_to_each_other(backend, B, dtype, n):
+    """All of them in one part of the row, up to the 1,024 that a part lists and past it: the ranking is then from memory."""
+    from irgen.serving import build_sample_ir
+    from test_gpu_serving import _params
+
+    V, g = 50021, torch.Generator().manual_seed(n)
+    x = -40.0 + torch.randn(B, V, generator=g)
+    x[:, 9000:9000 + n] = 4.0 + 0.01 * torch.randn(B, n, generator=g)
+    x = x.to(R.DT[dtype])
+    par = _params(B, n, T=(0.7, 1.0, 1.5), k=(0, n // 2, n - 1), p=(1.0, 0.9, 0.4), m=(0.0, 0.5))
+    got, = _run(build_sample_ir(B, V, dtype), backend, {"logits": x, **par})
+    assert torch.equal(got, R.sample64(x, **par))
