@@ -10,14 +10,20 @@ from npu_runtime.serving_ops import check_paged_append, check_paged_attention, c
 
 PAGED_ANY_MAX_D = 256          # paged.hip PG_ANY_D
 PAGED_APPEND_MAX_R = 256       # paged.hip PG_APPEND_R
-PAGED_APPEND_ROW_N = 1024      # up to this many rows a workgroup per row, past it a wave
+# Up to this many rows a workgroup per row, past it a wave. us by workgroups / by waves, in 16 bits: 16 rows of 12 + 2 heads
+# of 128 3.8 / 5.1, 1,024 5.1 / 5.7, 2,048 7.5 / 6.8, 8,192 21.9 / 14.8; 14 + 2 of 64: 3.9 / 3.9, 4.6 / 4.3, 6.5 / 5.0,
+# 18.8 / 10.2; 32 + 8 of 128, whose rows keep four waves busy: 4.1 / 7.2, 6.7 / 8.7, 10.5 / 12.9, 32.4 / 34.4.
+PAGED_APPEND_ROW_N = 1024
 # paged.hip: sequences of a list, rows of a tile, fewest blocks of a narrow workgroup and of a wide tile's split, items
 # that wide tiles are split towards
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
 PT_GRID = 512                  # two workgroups per CU
 # sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, bins, tokens of a list
 SAMPLE_MAX_PIECES, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 512, 16384
-SAMPLE_PICK_PIECES = 1024      # up to this many pieces k_sample_pick alone
+# Up to this many pieces k_sample_pick alone, past it the four launches. us alone / four, top-k 50 and top-p 0.95, bfloat16:
+# 500 pieces 30.7 / 30.4 for one row and 32.7 / 34.0 for 256, 1,000 35.3 / 29.8 and 36.8 / 36.2, 2,000 44.1 / 30.6 and
+# 47.3 / 39.9; float32: 500 27.3 / 28.7 and 28.7 / 32.3, 1,000 30.7 / 28.4 and 31.6 / 34.5, 2,000 36.8 / 29.2 and 38.3 / 36.6.
+SAMPLE_PICK_PIECES = 1024
 
 
 def _rows_view(low, name: str) -> TView:
@@ -58,7 +64,11 @@ def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_s
     pages that are no multiple of 16 positions, more sequences than the item list holds, or sizes whose item
     counts could pass 32 bits. Wide tiles are left out where the rows average at most two tokens per sequence: a
     decode step's batches then need no workgroups that look for chunks, and a longer chunk in one takes several
-    narrow tiles."""
+    narrow tiles. us with wide tiles / without, 32 heads over 8 of 128: 64 sequences over up to 4,000 positions, all but
+    one of them decoding, the chunk of 1 token 160 / 156, of 64 168 / 160, of 200 187 / 177, of 400 203 / 205; six prompts
+    of 1,000 111 / 299, 16 of 100 26 / 54; one chunk over 30,000 positions, of 16 tokens 39 / 35, of 64 59 / 61, of 256
+    146 / 188. So between two and some six tokens per sequence the rule costs up to 6% (with 12 over 2 heads, whose caches
+    are read in a third of the time, up to 29%: 46 / 35 at 2.5): a launch does not know whether its rows are one chunk or many."""
     if dtype not in ("bfloat16", "float16") or D not in (64, 128) or page_size % 16 or not 0 < B <= PT_MAXB or M < 1 or P < 1:
         return None
     G, block = H // KVH, 8192 // (2 * D)
