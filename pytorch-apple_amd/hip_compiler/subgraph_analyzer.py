@@ -1567,7 +1567,7 @@ class Lowering:
 
         def reads(n: OpNode) -> list[str]:   # (a getitem lists every output of its source)
             one = n.op_type == "<built-in function getitem>"
-            return [t.name for t in (n.inputs[int(n.attrs["index"]):][:1] if one else n.inputs) if t.name in names]
+            return [t.name for t in (n.inputs[int(n.attrs.get("index", 0)):][:1] if one else n.inputs) if t.name in names]
 
         path, at = [], name
         while at is not None and at in self.producer:

@@ -240,3 +240,58 @@ def test_sample_where_the_tokens_around_a_cut_lie_next_to_each_other(backend, B,
     par = _params(B, n, T=(0.7, 1.0, 1.5), k=(0, n // 2, n - 1), p=(1.0, 0.9, 0.4), m=(0.0, 0.5))
     got, = _run(build_sample_ir(B, V, dtype), backend, {"logits": x, **par})
     assert torch.equal(got, R.sample64(x, **par))
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+@pytest.mark.parametrize("news,kvs,lead,pad", [([1, 40, 0], [9, 300, 3], 5, 3), ([0, 0], [9, 0], 2, 2), ([0], [40], 0, 1),
+                                               ([1], [1], 1, 0), ([33] * 5, [33, 600, 40, 35, 33], 70, 70)])
+def test_rows_of_no_sequence_before_and_behind(backend, D, dtype, page, news, kvs, lead, pad):
+    from irgen.serving import build_paged_attention_ir
+
+    bt = R.batch(news, kvs, page, pad=pad, lead=lead, seed=2)
+    kp, vp = R.pools(bt, 2, page, D, dtype, stale=float("nan"))
+    q = _rand(9, bt["rows"], 4, D, dtype=dtype)
+    ir = build_paged_attention_ir(bt["rows"], len(news), bt["pages"], page, bt["block_table"].shape[1], 4, 2, D, dtype)
+    got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, **_meta(bt)})
+    out, mag, big = R.attention64(q, kp, vp, bt, page, D ** -0.5)
+    tol = R.attention_tol(dtype, D, max(kvs + [1]), out, mag, big)
+    worst = ((got.double() - out).abs() / tol).max().item()
+    assert worst <= 1.0, worst
+    s = bt["q_start"].tolist()
+    assert got[:s[0]].eq(0).all() and got[s[-1]:].eq(0).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(128, "bfloat16"), (64, "float32")])
+@pytest.mark.parametrize("B,M,P", [(0, 3, 4), (2, 0, 4), (2, 3, 0), (0, 0, 0)])
+def test_no_sequences_no_table_no_pages(backend, D, dtype, B, M, P):
+    """Nothing has a place: attention gives zeros, append rotates the rows of sequences and writes nothing."""
+    from irgen.serving import build_paged_append_ir, build_paged_attention_ir
+    from npu_runtime.serving_ops import paged_append
+    from test_gpu_serving import _inv
+
+    q, k, v = (_rand(i, 3, h, D, dtype=dtype) for i, h in ((1, 4), (2, 2), (3, 2)))
+    kp, vp = _rand(4, P, 2, 16, D, dtype=dtype), _rand(5, P, 2, 16, D, dtype=dtype)
+    meta = {"block_table": torch.zeros(B, M, dtype=torch.int32), "q_start": torch.tensor([0, 1, 3][:B + 1], dtype=torch.int32),
+            "kv_len": torch.full((B,), 20, dtype=torch.int32)}
+    got, = _run(build_paged_attention_ir(3, B, P, 16, M, 4, 2, D, dtype), backend, {"q": q, "k_pages": kp, "v_pages": vp, **meta})
+    assert got.eq(0).all()
+    t = {"q": q, "k": k, "v": v, "k_pages": kp, "v_pages": vp, **meta, "inv_freq": _inv(D // 2)}
+    got = _run(build_paged_append_ir(3, B, P, 16, M, 4, 2, D, dtype), backend, t)
+    want = paged_append(*t.values())
+    assert torch.equal(got[1], kp) and torch.equal(got[2], vp)
+    assert ((got[0].double() - want[0].double()).abs() <= 2.01 * R.HALF_STEP[dtype] * want[0].abs().double() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("D,dtype,page", PATHS)
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_negative_and_zero_scales(backend, D, dtype, page, scale):
+    from irgen.serving import build_paged_attention_ir
+
+    bt = R.batch([1, 50, 3], [900, 700, 3], page, pad=1, seed=3)
+    kp, vp = R.pools(bt, 2, page, D, dtype, stale=float("nan"))
+    q = _rand(9, bt["rows"], 4, D, dtype=dtype)
+    ir = build_paged_attention_ir(bt["rows"], 3, bt["pages"], page, bt["block_table"].shape[1], 4, 2, D, dtype, scale=scale)
+    got, = _run(ir, backend, {"q": q, "k_pages": kp, "v_pages": vp, **_meta(bt)})
+    out, mag, big = R.attention64(q, kp, vp, bt, page, scale)
+    worst = ((got.double() - out).abs() / R.attention_tol(dtype, D, 900, out, mag, big)).max().item()
+    assert worst <= 1.0, worst
