@@ -10,7 +10,7 @@ kinds:
 * ``append``     q and k rotated to their positions, k and v written into the pages. With ``norm`` each head of q and k is
                  first divided by its root mean square and multiplied by a weight. With ``cache`` 8 the pages hold e4m3 bytes
                  beside one power of two per position and K/V head (``k_scales``, ``v_scales``, its exponent + 127): the
-                 smallest one, 2^-126 at least, with which the head's largest magnitude is at most 448.
+                 smallest one, 2^-100 at least, with which the head's largest magnitude is at most 448.
 * ``attention``  causal attention of the new tokens over such pages of 8 bits.
 
 8-bit outputs are returned as tensors of the 8-bit floating types that their bytes are.
@@ -224,7 +224,7 @@ def _sequence_of(t, rows):
 
 def _plain_quantise(x):
     """(e4m3 bytes, exponent bytes) of float32 heads."""
-    m, x2 = torch.frexp(x.abs().amax(-1).clamp(min=2.0 ** -118))
+    m, x2 = torch.frexp(x.abs().amax(-1).clamp(min=2.0 ** -92))
     e = x2 - 9 + (m > 0.875)             # the largest magnitude is m 2^x2, and 448 is 0.875 2^9
     y = torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn)
     return y.view(torch.uint8), (e + 127).to(torch.uint8)
@@ -330,7 +330,7 @@ def exact(case, seed):
             heads = [turn(t["k"][at:at + new].double(), "k_weight"), t["v"][at:at + new].double()]
             for i, x in enumerate(heads):
                 if eight:
-                    s = 2.0 ** torch.ceil(torch.log2(x.abs().amax(-1) / 448)).clamp(min=-126)
+                    s = 2.0 ** torch.ceil(torch.log2(x.abs().amax(-1) / 448)).clamp(min=-100)
                     scales[i][page, off], x = s, x / s[..., None]
                 pools[i][page, off] = x
         else:
