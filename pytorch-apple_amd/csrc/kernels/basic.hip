@@ -21,6 +21,8 @@ extern "C" __global__ void __launch_bounds__(256) k_copy(const CopyArgs a) {
       ((long long*)a.dst)[dof] = ((const long long*)a.src)[so];
     } else if (a.sdtype == a.ddtype && (a.sdtype == HS_BF16 || a.sdtype == HS_F16)) {
       ((uint16_t*)a.dst)[dof] = ((const uint16_t*)a.src)[so];
+    } else if (a.sdtype == a.ddtype && a.sdtype == HS_U8) {   // (st_f would make truth values of uint8 numbers)
+      ((unsigned char*)a.dst)[dof] = ((const unsigned char*)a.src)[so];
     } else if (a.ddtype == HS_I64 || a.ddtype == HS_I32) {
       const long long v = (a.sdtype == HS_I64 || a.sdtype == HS_I32 || a.sdtype == HS_U8)
                               ? ld_i(a.src, so, a.sdtype) : (long long)ld_f(a.src, so, a.sdtype);

@@ -615,6 +615,12 @@ struct PagedAppendArgs {      // paged.hip: rotate q and k, write k and v into t
   int N, B, M, H, KVH, D, R, page_size;
   float scaling;
   int dtype;
+  const void* q_weight;       // [D] norms of q's and k's heads
+  const void* k_weight;
+  unsigned char* k_scales;    // pages of 8 bits: exponent + 127 of position r, head h, page p at (p * KVH + h) * page_size + r
+  unsigned char* v_scales;
+  float eps;
+  int pad;
 };
 
 struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over paged K and V
@@ -638,6 +644,8 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   int grid_wide;              // workgroups of the wide tiles (the first ones), the rest take narrow tiles
   int grid_narrow;            // workgroups of the narrow tiles
   int pad;
+  const unsigned char* k_scales;   // pages of 8 bits: exponent + 127 of position r, head h, page p at (p * KVH + h) * page_size + r
+  const unsigned char* v_scales;
 };
 
 struct SampleRow {            // sample.hip: what k_sample_merge finds out about a row

@@ -1,7 +1,8 @@
 // Paged K/V caches: append with rotation, and causal attention of packed rows over the pages.
 //
 // Rows of the packed new tokens belong to sequences (q_start), sequences hold kv_len positions, position p of
-// sequence b lies in row p % page_size of page table[b][p / page_size]. The metadata lies on the device and is
+// sequence b lies in row p % page_size of page table[b][p / page_size]. Pages hold the queries' type, or e4m3 bytes
+// with a power of two per position and K/V head (F8 in what follows). The metadata lies on the device and is
 // taken as it comes: whatever it holds, no kernel here reads or writes outside its tensors (a row of no
 // sequence is padding; a position before 0, past the table or in a page outside the pool has no place).
 #include "common.h"
@@ -32,6 +33,25 @@ __device__ __forceinline__ int pg_page(const int* table, int b, int M, int page_
   const int page = table[(long long)b * M + pos / page_size];
   return page >= 0 && page < pages ? page : -1;
 }
+
+// place of a position's power of two in pages of 8 bits
+__device__ __forceinline__ long long pg_scale_at(long long page, int h, int KVH, int page_size, int row) {
+  return (page * KVH + h) * page_size + row;
+}
+
+// 2^(b - 127); 255 is NaN, 0 is 0
+__device__ __forceinline__ float pg_scale(unsigned b) { return __uint_as_float(b == 255u ? 0x7fc00000u : b << 23); }
+
+// The byte of the power of two with which a head of largest finite magnitude `most` is quantised: the smallest s >= 2^-100
+// with most <= 448 s = 1.75 2^8 s. With most = 1.m 2^x it is 2^(x - 8), or twice that where 1.m > 1.75.
+__device__ __forceinline__ unsigned pg_quant_byte(float most) {
+  const unsigned u = __float_as_uint(fmaxf(most, 2.0194839e-28f));   // 2^-92
+  return (u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+}
+// its inverse (27 <= byte <= 247)
+__device__ __forceinline__ float pg_quant_inverse(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+// |x| of a finite x, else 0
+__device__ __forceinline__ float pg_finite(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 
 // ------------------------------------------------------------------ append
 
@@ -167,13 +187,246 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_append_bf16_row(const 
 extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16(const PagedAppendArgs a) { append_body<HS_F16, 1>(a); }
 extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16_row(const PagedAppendArgs a) { append_body<HS_F16, 4>(a); }
 
+// ------------------------------------------------------------------ append of normed heads, and into pages of 8 bits
+//
+// y = rotation of x / sqrt(mean(x^2) + eps) weight (NORM), of x otherwise; pages of 8 bits (F8) take k and v as e4m3
+// with pg_quant_byte's power of two. fp32 up to the one rounding of each result.
+
+// k_paged_*_append_any: one workgroup per row, a wave per head; any type, head size and strides. A head is read again for
+// each thing that is needed of the whole of it (sum of squares, largest magnitude).
+template <bool NORM, bool F8>
+__device__ __forceinline__ void append_heads_any(const PagedAppendArgs& a) {
+  __shared__ int place[3];   // sequence, position, page
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  if (tid < 64) {
+    const int b = pg_sequence(a.q_start, a.B, row, tid);
+    const bool real = b < a.B && row >= a.q_start[0];
+    const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
+    if (tid == 0) place[0] = real ? b : -1, place[1] = pos, place[2] = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
+  }
+  __syncthreads();
+  const int pos = place[1], page = place[2], half = a.R / 2, per = half + a.D - a.R;
+  const bool real = place[0] >= 0;
+  const long long slot = page < 0 ? 0 : page * a.page_stride + (pos % a.page_size) * a.row_stride;
+  for (int h = tid >> 6; h < a.H + 2 * a.KVH; h += 4) {
+    const bool isq = h < a.H, isv = h >= a.H + a.KVH;
+    const int hk = isv ? h - a.H - a.KVH : h - a.H;
+    if (!isq && page < 0) continue;
+    const void* src = isq ? a.q : isv ? a.v : a.k;
+    const long long so = isq ? row * a.q_rs + h * a.q_hs : isv ? row * a.v_rs + hk * a.v_hs : row * a.k_rs + hk * a.k_hs;
+    const void* weight = isq ? a.q_weight : a.k_weight;
+    float r = 1.f;
+    if (NORM && !isv) {
+      float ss = 0.f;
+      for (int d = lane; d < a.D; d += 64) {
+        const float x = ld_f(src, so + d, a.dtype);
+        ss = fmaf(x, x, ss);
+      }
+      r = 1.f / sqrtf(wave_sum(ss) / (float)a.D + a.eps);
+    }
+    auto get = [&](int d) {
+      const float x = ld_f(src, so + d, a.dtype);
+      return NORM && !isv ? x * r * ld_f(weight, d, a.dtype) : x;
+    };
+    // f(dim, value) for the lane's results
+    auto each = [&](auto f) {
+      for (int e = lane; e < per; e += 64) {
+        if (e < half) {
+          float s = 0.f, c = 1.f;
+          if (!isv) {
+            sincos_rot_d((double)pos * (double)a.inv_freq[e], &s, &c);
+            c *= a.scaling, s *= a.scaling;
+          }
+          const float lo = get(e), hi = get(half + e);
+          f(e, isv ? lo : lo * c - hi * s);
+          f(half + e, isv ? hi : hi * c + lo * s);
+        } else {
+          f(a.R + e - half, get(a.R + e - half));
+        }
+      }
+    };
+    if (isq || !F8) {
+      void* dst = isq ? a.q_out : isv ? a.v_pages : a.k_pages;
+      const long long to = isq ? ((long long)row * a.H + h) * a.D : slot + hk * a.head_stride;
+      each([&](int d, float y) { st_f(dst, to + d, a.dtype, real ? y : 0.f); });
+      continue;
+    }
+    float most = 0.f;
+    each([&](int, float y) { most = fmaxf(most, pg_finite(y)); });
+    const unsigned byte = pg_quant_byte(wave_max(most));
+    const float inv = pg_quant_inverse(byte);
+    unsigned char* dst = (unsigned char*)(isv ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
+    each([&](int d, float y) { dst[d] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(y * inv, 0.f, 0, false); });
+    if (lane == 0) (isv ? a.v_scales : a.k_scales)[pg_scale_at(page, hk, a.KVH, a.page_size, pos % a.page_size)] = (unsigned char)byte;
+  }
+}
+extern "C" __global__ void __launch_bounds__(256) k_paged_norm_append_any(const PagedAppendArgs a) { append_heads_any<true, false>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_quant_append_any(const PagedAppendArgs a) { append_heads_any<false, true>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_norm_quant_append_any(const PagedAppendArgs a) { append_heads_any<true, true>(a); }
+
+// k_paged_*_append_*: 16-bit types, D and R multiples of 16, D <= 256, 16-byte aligned rows. A head lies in LP lanes of a row
+// of 16 (the power of two from D / 16, at least 4), 16 dims each in two pieces of 8: those that rotate together, or past R
+// two neighbours. So what is needed of a whole head (sum of squares, largest magnitude) takes two to four steps across
+// lanes, and a lane's cosines, sines and weights are the same for all heads of its row and stay in registers. A wave
+// per row, or the four waves of a workgroup where rows are few (_row).
+template <bool MAX>
+__device__ __forceinline__ float pg_heads(float v, int LP) {
+  auto join = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
+  v = join(v, HS_DPP(v, HS_QUAD_XOR1));
+  v = join(v, HS_DPP(v, HS_QUAD_XOR2));
+  if (LP > 4) v = join(v, HS_DPP(v, HS_ROW_HALF_MIRROR));
+  if (LP > 8) v = join(v, HS_DPP(v, HS_ROW_MIRROR));
+  return v;
+}
+
+// four values times inv as e4m3, the first in the lowest byte; NaN where they are not finite
+__device__ __forceinline__ uint32_t pg_e4m3(const float* v, float inv) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+}
+
+template <int DT, int WAVES, bool NORM, bool F8>
+__device__ __forceinline__ void append_heads(const PagedAppendArgs& a) {
+  constexpr int ROWS = 4 / WAVES, TH = 64 * WAVES;
+  __shared__ __attribute__((aligned(16))) float cs[ROWS][2][PG_APPEND_R / 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = wave / WAVES, tid = (wave % WAVES) * 64 + lane;
+  const int row = blockIdx.x * ROWS + mine, half = a.R / 2;
+  const bool in = row < a.N;
+  const int b = in ? pg_sequence(a.q_start, a.B, row, lane) : a.B;
+  const bool real = b < a.B && row >= a.q_start[0];
+  const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
+  const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
+  if (real)
+    for (int j = tid; j < half; j += TH) {
+      float s, c;
+      sincos_rot_d((double)pos * (double)a.inv_freq[j], &s, &c);
+      cs[mine][0][j] = c * a.scaling, cs[mine][1][j] = s * a.scaling;
+    }
+  __syncthreads();
+  if (!in) return;
+  const int need = a.D / 16, LP = need <= 4 ? 4 : need <= 8 ? 8 : 16, sub = tid & (LP - 1);
+  const bool has = sub < need, turns = has && sub < a.R / 16;
+  const int e0 = !has ? 0 : turns ? sub * 8 : a.R + (sub - a.R / 16) * 16, e1 = !has ? 0 : turns ? half + sub * 8 : e0 + 8;
+  float c[8], s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
+  if (turns && real) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = cs[mine][0][e0 + j], s[j] = cs[mine][1][e0 + j];
+  }
+  uint4 wq0, wq1, wk0, wk1;
+  if constexpr (NORM) {
+    const uint16_t *wq = (const uint16_t*)a.q_weight, *wk = (const uint16_t*)a.k_weight;
+    wq0 = *(const uint4*)(wq + e0), wq1 = *(const uint4*)(wq + e1);
+    wk0 = *(const uint4*)(wk + e0), wk1 = *(const uint4*)(wk + e1);
+  }
+  const int off = page < 0 ? 0 : pos % a.page_size, heads = a.H + 2 * a.KVH;
+  const long long slot = page < 0 ? 0 : page * a.page_stride + off * a.row_stride;
+  struct Step {
+    uint4 x, y;
+    int h;
+  };
+  auto get = [&](int h) {
+    Step t;
+    t.h = h;
+    const bool isq = h < a.H, isv = h >= a.H + a.KVH;
+    const int hk = isv ? h - a.H - a.KVH : h - a.H;
+    const uint16_t* src = isq ? (const uint16_t*)a.q + row * a.q_rs + h * a.q_hs
+                        : isv ? (const uint16_t*)a.v + row * a.v_rs + hk * a.v_hs
+                              : (const uint16_t*)a.k + row * a.k_rs + hk * a.k_hs;
+    t.x = *(const uint4*)(src + e0);
+    t.y = *(const uint4*)(src + e1);
+    return t;
+  };
+  auto put = [&](const Step& t) {
+    const bool isq = t.h < a.H, isv = t.h >= a.H + a.KVH;
+    const int hk = isv ? t.h - a.H - a.KVH : t.h - a.H;
+    const uint32_t xw[4] = {t.x.x, t.x.y, t.x.z, t.x.w}, yw[4] = {t.y.x, t.y.y, t.y.z, t.y.w};
+    float x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[2 * j] = gm_lo<DT>(xw[j]), x[2 * j + 1] = gm_hi<DT>(xw[j]), y[2 * j] = gm_lo<DT>(yw[j]), y[2 * j + 1] = gm_hi<DT>(yw[j]);
+    if constexpr (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], fmaf(y[j], y[j], ss));
+      ss = pg_heads<false>(has ? ss : 0.f, LP);
+      if (!isv) {
+        const float r = 1.f / sqrtf(ss / (float)a.D + a.eps);
+        const uint4 w0 = isq ? wq0 : wk0, w1 = isq ? wq1 : wk1;
+        const uint32_t uw[4] = {w0.x, w0.y, w0.z, w0.w}, vw[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[2 * j] *= r * gm_lo<DT>(uw[j]), x[2 * j + 1] *= r * gm_hi<DT>(uw[j]);
+          y[2 * j] *= r * gm_lo<DT>(vw[j]), y[2 * j + 1] *= r * gm_hi<DT>(vw[j]);
+        }
+      }
+    }
+    if (!isv && turns) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float lo = x[j] * c[j] - y[j] * s[j], up = y[j] * c[j] + x[j] * s[j];
+        x[j] = lo, y[j] = up;
+      }
+    }
+    if (F8 && !isq) {
+      if (page < 0) return;
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(pg_finite(x[j]), pg_finite(y[j])));
+      const unsigned byte = pg_quant_byte(pg_heads<true>(has ? most : 0.f, LP));
+      const float inv = pg_quant_inverse(byte);
+      if (!has) return;
+      unsigned char* dst = (unsigned char*)(isv ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
+      *(uint2*)(dst + e0) = make_uint2(pg_e4m3(x, inv), pg_e4m3(x + 4, inv));
+      *(uint2*)(dst + e1) = make_uint2(pg_e4m3(y, inv), pg_e4m3(y + 4, inv));
+      if (sub == 0) (isv ? a.v_scales : a.k_scales)[pg_scale_at(page, hk, a.KVH, a.page_size, off)] = (unsigned char)byte;
+      return;
+    }
+    uint16_t* dst = isq ? (uint16_t*)a.q_out + ((long long)row * a.H + t.h) * a.D
+                        : (uint16_t*)(isv ? a.v_pages : a.k_pages) + slot + hk * a.head_stride;
+    if (!has || (!isq && page < 0)) return;
+    uint32_t lo[4], up[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo[j] = real ? gm_pack2<DT>(x[2 * j], x[2 * j + 1]) : 0u;
+      up[j] = real ? gm_pack2<DT>(y[2 * j], y[2 * j + 1]) : 0u;
+    }
+    *(uint4*)(dst + e0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *(uint4*)(dst + e1) = make_uint4(up[0], up[1], up[2], up[3]);
+  };
+  const int step = TH / LP;
+  for (int h = tid / LP; h < heads; h += 2 * step) {   // two steps' loads in flight
+    const bool two = h + step < heads;
+    const Step u = get(h), t = get(two ? h + step : h);
+    put(u);
+    if (two) put(t);
+  }
+}
+
+#define PG_APPENDS(NAME, NORM, F8)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_bf16(const PagedAppendArgs a) { append_heads<HS_BF16, 1, NORM, F8>(a); }     \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_bf16_row(const PagedAppendArgs a) { append_heads<HS_BF16, 4, NORM, F8>(a); } \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_f16(const PagedAppendArgs a) { append_heads<HS_F16, 1, NORM, F8>(a); }       \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_f16_row(const PagedAppendArgs a) { append_heads<HS_F16, 4, NORM, F8>(a); }
+PG_APPENDS(norm, true, false)
+PG_APPENDS(quant, false, true)
+PG_APPENDS(norm_quant, true, true)
+
 // ------------------------------------------------------------------ attention
 //
 // k_paged_attn_any: one wave per (row, query head), 64 positions a step: a lane scores one position (its key's row
 // against q in LDS), the wave takes maximum and sum, then every lane adds its dims of 64 values. Any type, page size
 // and head size up to 256; fp32 throughout. Closed positions are never loaded, so what lies there (NaN) does not enter.
 #define PG_ANY_D 256
-extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAttnArgs a) {
+// element i of a pool, without its power of two
+template <bool F8>
+__device__ __forceinline__ float pg_cached(const void* p, long long i, int dt) {
+  if constexpr (F8) return __builtin_amdgcn_cvt_f32_fp8(((const unsigned char*)p)[i], 0);
+  else return ld_f(p, i, dt);
+}
+template <bool F8>
+__device__ __forceinline__ void attn_any_body(const PagedAttnArgs& a) {
   __shared__ float q[PG_ANY_D], p[64];
   __shared__ int at[64];   // page of each of the step's positions, -1: closed
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.H / a.KVH);
@@ -191,7 +444,8 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
     if (page >= 0) {
       const long long ko = page * a.page_stride + kvh * a.head_stride + (mine % a.page_size) * a.row_stride;
       s = 0.f;
-      for (int d = 0; d < a.D; ++d) s = fmaf(q[d], ld_f(a.k_pages, ko + d, a.dtype), s);
+      for (int d = 0; d < a.D; ++d) s = fmaf(q[d], pg_cached<F8>(a.k_pages, ko + d, a.dtype), s);
+      if constexpr (F8) s *= pg_scale(a.k_scales[pg_scale_at(page, kvh, a.KVH, a.page_size, mine % a.page_size)]);
       s *= a.scale;
     }
     // (wave_max's fmaxf drops a NaN score: its exponential below keeps it)
@@ -209,7 +463,9 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
       for (int j = 0; j < min(64, end - p0); ++j) {
         if (at[j] < 0) continue;
         const long long vo = at[j] * a.page_stride + kvh * a.head_stride + ((p0 + j) % a.page_size) * a.row_stride;
-        x = fmaf(p[j], ld_f(a.v_pages, vo + i * 64 + lane, a.dtype), x);
+        float v = pg_cached<F8>(a.v_pages, vo + i * 64 + lane, a.dtype);
+        if constexpr (F8) v *= pg_scale(a.v_scales[pg_scale_at(at[j], kvh, a.KVH, a.page_size, (p0 + j) % a.page_size)]);
+        x = fmaf(p[j], v, x);
       }
       o[i] = x;
     }
@@ -219,6 +475,8 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAtt
     if (i * 64 + lane < a.D)
       st_f(a.out, ((long long)row * a.H + h) * a.D + i * 64 + lane, a.dtype, l == 0.f ? 0.f : o[i] / l);
 }
+extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAttnArgs a) { attn_any_body<false>(a); }
+extern "C" __global__ void __launch_bounds__(64) k_paged_quant_attn_any(const PagedAttnArgs a) { attn_any_body<true>(a); }
 
 // ------------------------------------------------------------------ attention on matrix cores
 //
@@ -496,6 +754,8 @@ struct PtWave {
   int pos;                                 // position of row fr, -1: none open
   int lane, fr, hi;
 
+  // F8: the queries in the order in which a narrow tile reads K, 16 dims of a position at a time
+  template <bool F8 = false>
   __device__ __forceinline__ void init(const PagedAttnArgs& a, const PtItem& it, int row0) {
     lane = threadIdx.x & 63, fr = lane & 31, hi = lane >> 5;
     const int G = a.H / a.KVH, rows = it.q.n * G, r = min(row0 + fr, rows - 1), t = r / G;
@@ -506,7 +766,7 @@ struct PtWave {
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // a negative scale: of -q
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      uint4 v = *(const uint4*)(p + ks * 16 + hi * 8);
+      uint4 v = *(const uint4*)(p + (F8 ? ks / 2 * 32 + hi * 16 + ks % 2 * 8 : ks * 16 + hi * 8));
       qf[ks] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
     }
 #pragma unroll
@@ -595,7 +855,9 @@ struct PtWave {
 
   // P in the B operand's layout: lane half 0 needs positions 0-7 / 16-23 of 32, half 1 8-15 / 24-31
   template <int NB>
-  __device__ __forceinline__ void pack(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) const {
+  __device__ __forceinline__ void pack(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) const { pack_of<NB>(s, p); }
+  template <int NB>
+  __device__ __forceinline__ static void pack_of(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) {
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
       uint32_t g[4][2];
@@ -611,6 +873,15 @@ struct PtWave {
         p[2 * sb + i / 2] = make_uint4(g[i][0], g[i][1], g[i + 1][0], g[i + 1][1]);
       }
     }
+  }
+
+  // what packing rounds away
+  template <int NB>
+  __device__ __forceinline__ static void rest_of(pt_f32x16 (&s)[NB]) {
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[sb][e] -= gm_round<DT>(s[sb][e]);
   }
 
   // Outputs, and the sums of the exponentials s. The operands are read four ahead, in an order that the compiler keeps:
@@ -672,26 +943,32 @@ struct PtWave {
 // 0 where there is no page), and which have a page. Looked up once for 16 (or 32) blocks: a scalar load per block left its
 // latency, 700 cycles, in every block's way. The next window's page ids are on their way to the wave's slot of LDS
 // meanwhile (to registers, the compiler's wait for them would cover the K and V loads in flight).
-struct PtWindow {
+template <bool F8>
+struct PtWindowT {
   uint32_t lo, hi;
   unsigned long long ok;
+  unsigned long long scale;   // 8 bits: place of the group's powers of two
 };
+typedef PtWindowT<false> PtWindow;
 __device__ __forceinline__ unsigned pt_page_of(const PagedAttnArgs& a, int group) {   // may lie past the table
   const unsigned grp = (unsigned)group + (threadIdx.x & 63);
   return a.group_magic ? __umulhi(grp, a.group_magic) : grp;
 }
-__device__ __forceinline__ PtWindow pt_window(const PagedAttnArgs& a, const PtItem& it, int group, int id) {
-  PtWindow w;
+template <bool F8 = false>
+__device__ __forceinline__ PtWindowT<F8> pt_window(const PagedAttnArgs& a, const PtItem& it, int group, int id) {
+  PtWindowT<F8> w;
   const unsigned grp = (unsigned)group + (threadIdx.x & 63), at = pt_page_of(a, group);
   const bool ok = at < (unsigned)a.M && (unsigned long long)(long long)id < (unsigned long long)a.pages;
-  const unsigned long long off = 2ull * ((ok ? id : 0) * a.page_stride + it.h * a.head_stride +
+  const unsigned long long off = (F8 ? 1ull : 2ull) * ((ok ? id : 0) * a.page_stride + it.h * a.head_stride +
                                          (ok ? (long long)((grp - at * a.page_groups) * 16) * a.row_stride : 0));
   w.lo = (uint32_t)off, w.hi = (uint32_t)(off >> 32);
   w.ok = __ballot(ok);
+  if constexpr (F8) w.scale = pg_scale_at(ok ? id : 0, it.h, a.KVH, a.page_size, ok ? (int)((grp - at * a.page_groups) * 16) : 0);
   return w;
 }
-__device__ __forceinline__ PtWindow pt_window(const PagedAttnArgs& a, const PtItem& it, int group) {
-  return pt_window(a, it, group, a.table[(long long)it.b * a.M + min(pt_page_of(a, group), (unsigned)a.M - 1)]);
+template <bool F8 = false>
+__device__ __forceinline__ PtWindowT<F8> pt_window(const PagedAttnArgs& a, const PtItem& it, int group) {
+  return pt_window<F8>(a, it, group, a.table[(long long)it.b * a.M + min(pt_page_of(a, group), (unsigned)a.M - 1)]);
 }
 // page ids of a window to slot[64]
 __device__ __forceinline__ void pt_fetch(const PagedAttnArgs& a, const PtItem& it, int group, int* slot) {
@@ -703,7 +980,8 @@ __device__ __forceinline__ void pt_fetch(const PagedAttnArgs& a, const PtItem& i
 }
 
 // offset of group i of the window (uniform)
-__device__ __forceinline__ unsigned long long pt_place(const PtWindow& w, int i) {
+template <bool F8>
+__device__ __forceinline__ unsigned long long pt_place(const PtWindowT<F8>& w, int i) {
   return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(w.hi, i) << 32) | (uint32_t)__builtin_amdgcn_readlane(w.lo, i);
 }
 
@@ -715,10 +993,17 @@ __device__ __forceinline__ void pt_load(const char* group, unsigned row_bytes, i
   gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
 }
 
+// element i of a pool, without its power of two
+template <int DT, bool F8>
+__device__ __forceinline__ float pt_cached(const void* p, long long i) {
+  if constexpr (F8) return __builtin_amdgcn_cvt_f32_fp8(((const unsigned char*)p)[i], 0);
+  else return gm_ld<DT>(p, i);
+}
+
 // One row over positions p0 .. p1 - 1 by a wave, 64 at a time, reading open positions only: the row's maximum of the raw
 // scores, sum of exponentials and the lane's outputs (dims lane * E ..), times 2^pt_up as the tiles' (they may be joined
 // with them). For tiles whose product is not finite.
-template <int DT, int D>
+template <int DT, int D, bool F8>
 __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it, int row, int p0, int p1, float& m,
                                        float& l, float (&x)[D / 64]) {
   constexpr int E = D / 64;
@@ -733,10 +1018,15 @@ __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it,
   for (; p0 < end; p0 += 64) {
     const int pos = p0 + lane, page = pos < end ? pg_page(a.table, it.b, a.M, a.page_size, a.pages, pos) : -1;
     const long long at = page < 0 ? 0 : page * a.page_stride + it.h * a.head_stride + (pos % a.page_size) * a.row_stride;
-    float s = 0.f;
-    if (page >= 0)
+    float s = 0.f, vs = 1.f;
+    if (page >= 0) {
 #pragma unroll 1
-      for (int d = 0; d < D; ++d) s = fmaf(gm_ld<DT>(q, d), gm_ld<DT>(a.k_pages, at + d), s);
+      for (int d = 0; d < D; ++d) s = fmaf(gm_ld<DT>(q, d), pt_cached<DT, F8>(a.k_pages, at + d), s);
+      if constexpr (F8) {
+        const long long i = pg_scale_at(page, it.h, a.KVH, a.page_size, pos % a.page_size);
+        s *= pg_scale(a.k_scales[i]), vs = pg_scale(a.v_scales[i]);
+      }
+    }
     s = page < 0 ? -INFINITY : s * flip;
     const float mn = fmaxf(m, wave_max(s)), mc = mn == -INFINITY ? 0.f : __builtin_fmaf(-mn, c, pt_up<DT>);
     const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
@@ -748,16 +1038,19 @@ __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it,
 #pragma unroll 1
     for (int j = 0; j < min(64, end - p0); ++j) {
       const long long aj = __shfl(at, j, 64);
-      const float ej = __shfl(e, j, 64);
+      const float ej = __shfl(e, j, 64), vj = F8 ? __shfl(vs, j, 64) : 1.f;
       if (__shfl(page, j, 64) < 0) continue;
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = fmaf(ej, gm_ld<DT>(a.v_pages, aj + lane * E + i), x[i]);
+      for (int i = 0; i < E; ++i) {
+        const float v = pt_cached<DT, F8>(a.v_pages, aj + lane * E + i);
+        x[i] = fmaf(ej, F8 ? v * vj : v, x[i]);
+      }
     }
   }
 }
 
 // rows r0, r0 + step, ... of a tile one by one, written as the tile's rows are (part: index of its first partial row)
-template <int DT, int D>
+template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_rows(const PagedAttnArgs& a, const PtItem& it, int tile0, int r0, int r1, int step, int p0,
                                      int p1, long long part) {
   constexpr int E = D / 64;
@@ -765,7 +1058,7 @@ __device__ __forceinline__ void pt_rows(const PagedAttnArgs& a, const PtItem& it
 #pragma unroll 1
   for (int row = r0; row < r1; row += step) {
     float m, l, x[E];
-    pt_row<DT, D>(a, it, row, p0, p1, m, l, x);
+    pt_row<DT, D, F8>(a, it, row, p0, p1, m, l, x);
     if (it.slot >= 0) {
       const long long at = part + row - tile0;
       if (lane == 0) *(float2*)(a.part_ml + at * 2) = make_float2(m, l);
@@ -790,19 +1083,87 @@ struct PtV {
   static constexpr bool value = true;
 };
 
-template <int DT, int D>
+template <int DT, int D, bool F8 = false>
 struct PtNarrow {
-  static constexpr int PB = 8192 / (2 * D), NB = PB / 32, NG = PB / 16;   // positions of a block: 8 KiB of K, 8 of V
-  static constexpr int LPG = 2 * D * 16 / 1024;                             // loads per group
+  static constexpr int PB = F8 ? 64 : 8192 / (2 * D), NB = PB / 32, NG = PB / 16;   // positions of a block: 8 KiB of K, 8 of V
+  static constexpr int LPG = (F8 ? 1 : 2) * D * 16 / 1024;                          // loads per group
   static constexpr int OLD = 64 + 4;                                        // output row in LDS (floats)
 };
+
+// Ends a narrow tile: joins its four waves, writes its rows. `odd`: the wave's outputs are not to be used, as where they are
+// not finite.
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void pt_join_waves(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, char* lds,
+                                              float (*ml)[2][32], bool odd) {
+  constexpr int PB = PtNarrow<DT, D, F8>::PB, OLD = PtNarrow<DT, D, F8>::OLD;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.H / a.KVH, rows = it.q.n * G, row0 = it.tile * 32;
+  // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
+  const float l = w.row_sum();
+  if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
+  if (__syncthreads_or(odd || w.bad_output())) {
+    pt_rows<DT, D, F8>(a, it, row0, row0 + wave, min(row0 + 32, rows), 4, it.b0 * PB, it.b1 * PB, (long long)it.slot * 32);
+    __syncthreads();
+    return;
+  }
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
+  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - M) * w.c);
+  float* ob = (float*)lds;
+  const int valid = min(32, rows - row0);
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half) {   // dims 64 half .. + 64
+    if (half) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const pt_f32x16& o = w.o[2 * half + t];
+        float4 v;
+        v.x = o[4 * i] * f, v.y = o[4 * i + 1] * f, v.z = o[4 * i + 2] * f, v.w = o[4 * i + 3] * f;
+        *(float4*)&ob[(wave * 32 + w.fr) * OLD + t * 32 + 8 * i + 4 * w.hi] = v;
+      }
+    __syncthreads();
+    for (int idx = tid; idx < valid * 8; idx += 256) {   // (row, 8 dims)
+      const int ch = idx & 7, r = idx >> 3;
+      float Mr = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Mr = fmaxf(Mr, ml[i][0][r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        L += ml[i][0][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i][0][r] - Mr) * w.c) * ml[i][1][r];
+      float x[8] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4* p = (const float4*)&ob[(i * 32 + r) * OLD + 8 * ch];
+        const float4 u = p[0], v = p[1];
+        x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w;
+        x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
+      }
+      if (it.slot >= 0) {
+        float* po = a.part_o + ((long long)it.slot * 32 + r) * D + 64 * half + 8 * ch;
+        *(float4*)po = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(po + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        if (half == 0 && ch == 0) *(float2*)(a.part_ml + ((long long)it.slot * 32 + r) * 2) = make_float2(Mr, L);
+      } else {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int row = row0 + r, t = row / G;
+        uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + 64 * half + 8 * ch;
+        *(uint4*)out = make_uint4(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv),
+                                  gm_pack2<DT>(x[4] * inv, x[5] * inv), gm_pack2<DT>(x[6] * inv, x[7] * inv));
+      }
+    }
+  }
+  __syncthreads();   // the next item's loads go to the same LDS
+}
 
 template <int DT, int D>
 __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32], int (*slots)[64]) {
   using C = PtNarrow<DT, D>;
-  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, OLD = C::OLD;
+  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.H / a.KVH, rows = it.q.n * G, row0 = it.tile * 32;
+  const int row0 = it.tile * 32;
   PtWave<DT, D> w;
   const unsigned row_bytes = (unsigned)(2 * a.row_stride);
   char* Kt = lds + wave * 16384;
@@ -871,67 +1232,46 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
     if (more) load(PtV{}, blk + 4);
     bad = bad_next;
   }
-  // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
+  pt_join_waves<DT, D, false>(a, it, w, lds, ml, false);
+}
+
+// ------------------------------------------------------------------ wide tiles
+
+// Writes a wide tile's rows. `odd`: its outputs are not to be used, as where they are not finite.
+template <int DT, int D, bool F8>
+__device__ __forceinline__ void pt_end_wide(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, bool odd) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.H / a.KVH, rows = it.q.n * G;
+  const int tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
   const float l = w.row_sum();
-  if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
-  if (__syncthreads_or(w.bad_output())) {
-    pt_rows<DT, D>(a, it, row0, row0 + wave, min(row0 + 32, rows), 4, b0 * PB, b1 * PB, (long long)it.slot * 32);
-    __syncthreads();
-    return;
-  }
-  float M = -INFINITY;
+  const int row = row0 + w.fr;
+  const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
+  if (row0 < rows && (odd || w.bad_output())) {
+    pt_rows<DT, D, F8>(a, it, tile0, row0, min(row0 + 32, rows), 1, it.b0 * 64, it.b1 * 64, part);
+  } else if (row < rows) {
+    if (it.slot >= 0) {
+      const long long at = part + row - tile0;
+      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
-  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - M) * w.c);
-  float* ob = (float*)lds;
-  const int valid = min(32, rows - row0);
+      for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-  for (int half = 0; half < D / 64; ++half) {   // dims 64 half .. + 64
-    if (half) __syncthreads();
+        for (int i = 0; i < 4; ++i)
+          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
+              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t0 = row / G;
+      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const pt_f32x16& o = w.o[2 * half + t];
-        float4 v;
-        v.x = o[4 * i] * f, v.y = o[4 * i + 1] * f, v.z = o[4 * i + 2] * f, v.w = o[4 * i + 3] * f;
-        *(float4*)&ob[(wave * 32 + w.fr) * OLD + t * 32 + 8 * i + 4 * w.hi] = v;
-      }
-    __syncthreads();
-    for (int idx = tid; idx < valid * 8; idx += 256) {   // (row, 8 dims)
-      const int ch = idx & 7, r = idx >> 3;
-      float Mr = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Mr = fmaxf(Mr, ml[i][0][r]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        L += ml[i][0][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i][0][r] - Mr) * w.c) * ml[i][1][r];
-      float x[8] = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4* p = (const float4*)&ob[(i * 32 + r) * OLD + 8 * ch];
-        const float4 u = p[0], v = p[1];
-        x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w;
-        x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
-      }
-      if (it.slot >= 0) {
-        float* po = a.part_o + ((long long)it.slot * 32 + r) * D + 64 * half + 8 * ch;
-        *(float4*)po = make_float4(x[0], x[1], x[2], x[3]);
-        *(float4*)(po + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        if (half == 0 && ch == 0) *(float2*)(a.part_ml + ((long long)it.slot * 32 + r) * 2) = make_float2(Mr, L);
-      } else {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const int row = row0 + r, t = row / G;
-        uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + 64 * half + 8 * ch;
-        *(uint4*)out = make_uint4(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv),
-                                  gm_pack2<DT>(x[4] * inv, x[5] * inv), gm_pack2<DT>(x[6] * inv, x[7] * inv));
-      }
+        for (int i = 0; i < 4; ++i)
+          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
+              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
+                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
     }
   }
   __syncthreads();   // the next item's loads go to the same LDS
 }
-
-// ------------------------------------------------------------------ wide tiles
 
 template <int DT, int D>
 __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
@@ -997,47 +1337,354 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
     w.template outputs<NB>(Vt, p, s);
   }
-  const float l = w.row_sum();
-  const int row = row0 + w.fr;
-  const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
-  if (row0 < rows && w.bad_output()) {
-    pt_rows<DT, D>(a, it, tile0, row0, min(row0 + 32, rows), 1, b0 * PB, b1 * PB, part);
-  } else if (row < rows) {
-    if (it.slot >= 0) {
-      const long long at = part + row - tile0;
-      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
-              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
-    } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int t0 = row / G;
-      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
-              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
-                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
-    }
+  pt_end_wide<DT, D, false>(a, it, w, false);
+}
+
+// ------------------------------------------------------------------ pages of 8 bits
+//
+// The same tiles over e4m3 numbers K_jd 2^ke_j and V_jd 2^ve_j. The products stay in 16 bits: e4m3 queries or probabilities
+// would carry 3 bits of mantissa into every output. Numbers of 4 bits are exact in both 16-bit types, so what a tile
+// computes is the 16-bit tile's result on the dequantised pages.
+//   * Narrow: half the bytes come to LDS, and become 16 bits on the way from there to the matrix instructions. A lane of
+//     K's operand holds one position, so 2^ke_j comes with the conversion. A lane of V's holds eight positions of one dim:
+//     2^ve_j goes to the probabilities, which are therefore taken in bfloat16 (whose range holds any power of two) whatever the
+//     queries' type, for float16 in two parts, the second the first's rounding error, each with its product: float16's
+//     own 11 bits at least. Bound by memory, beside which the second product costs nothing.
+//   * Wide: bound by the matrix cores, so each block is converted once for all four waves, powers of two included, by way of
+//     registers one block ahead, into the LDS layout of 16-bit pages; the rest is the 16-bit tile.
+// K in float16 can overflow where 2^ke is 2^8 or more (keys above 57,344), bfloat16 where a power is 2^120; probabilities times
+// powers below 2^-100 reach the end of bfloat16; byte 255 is NaN: tiles that see such a byte in an open place are done row
+// by row, like those with outputs that are not finite. (0, what was never written, is none of them: it counts as 2^-127 or 0.
+// float16 below 2^-14 takes steps of 2^-24, of keys as of any float16 key.)
+
+template <int DT>
+constexpr unsigned pt_least_odd = DT == HS_F16 ? 135u : 247u;   // odd power bytes: 1 .. 26, and from here on
+__device__ __forceinline__ bool pt_odd(unsigned byte, unsigned least) { return byte - 1u < 26u || byte >= least; }
+
+// whether one of four bytes is odd: bit 7 of a byte's sum says whether it is at least the number that takes 128 to it
+__device__ __forceinline__ bool pt_any_odd(uint32_t w, unsigned least) {
+  constexpr uint32_t ONES = 0x01010101u;
+  const uint32_t low = w & (0x7f * ONES), top = w & (0x80 * ONES);
+  const uint32_t from_least = (low + (256u - least) * ONES) & top, from_1 = low + 0x7f * ONES, from_27 = low + (128u - 27u) * ONES;
+  return (from_least | (from_1 & ~from_27 & ~w & (0x80 * ONES))) != 0;
+}
+
+// eight e4m3 numbers times 2^(power - 127) as DT
+template <int DT>
+__device__ __forceinline__ uint4 pt_widen(uint32_t a, uint32_t b, float power) {
+  uint4 r;
+  if constexpr (DT == HS_BF16) {
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, true));
+  } else {
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, power, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, power, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, power, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, power, true));
   }
-  __syncthreads();   // the next item's loads go to the same LDS
+  return r;
+}
+
+// Transposing LDS read of bytes: lanes 2r + c of each 16-lane group address row r, columns 8c .. 8c + 7; lane i gets column i
+// of rows 0 .. 7.
+__device__ __forceinline__ uint2 pt_read_tr8(const char* p) {
+  typedef __attribute__((ext_vector_type(2))) int i32x2;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       (__attribute__((address_space(3))) i32x2*)(__attribute__((address_space(3))) char*)p));
+}
+
+// Rows' swizzles, as pt_xk and pt_xv, for rows of D bytes: the 32 rows of K's 16-byte reads, and the 8 rows x 2 chunks of V's
+// transposing reads by 32 lanes, hit every bank.
+template <int D>
+__device__ __forceinline__ int pt_xk8(int r) {
+  return D == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+template <int D>
+__device__ __forceinline__ int pt_xv8(int r) {
+  return D == 128 ? ((r >> 1) & 3) << 1 : ((r >> 2) & 1) << 1;
+}
+template <int D, bool V>
+__device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, int i, unsigned lds, int lane) {
+  constexpr int PER = 1024 / D, SL = D / 16;   // rows per load, slots of a row
+  const int r = i * PER + lane / SL, ch = (lane % SL) ^ (V ? pt_xv8<D>(r) : pt_xk8<D>(r));
+  gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32], int (*slots)[64],
+                                           uint32_t (*powers)[64]) {
+  using C = PtNarrow<DT, D, true>;
+  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, TD = D / 32;
+  constexpr int LD = NG * LPG;   // loads of a block's K, and of its V
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row0 = it.tile * 32;
+  PtWave<DT, D> w;
+  const unsigned row_bytes = (unsigned)a.row_stride;
+  char* Kt = lds + wave * 16384;
+  char* Vt = Kt + 8192;
+  const unsigned k0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)Kt, v0 = k0 + 8192;
+  uint32_t* pw = powers[wave];   // the block's powers of two: K's 64 bytes, then V's
+  const unsigned pw0 = (unsigned)(size_t)(__attribute__((address_space(3))) uint32_t*)pw;
+  const int b0 = it.b0, b1 = it.b1;
+  constexpr int WB = 64 / NG;   // blocks of a window
+  PtWindowT<true> cur;
+  int* ids = slots[wave];
+  int wi;                       // window of cur
+  unsigned bad = 0, bad_next;   // groups of the present and the next block without a page
+  bool odd = false;
+  auto seek = [&](int blk) {    // cur: the block's window
+    if (blk / WB != wi) {
+      ++wi;
+      cur = pt_window<true>(a, it, wi * 64, ids[lane]);
+      pt_fetch(a, it, (wi + 1) * 64, ids);
+    }
+    return ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
+  };
+  auto load = [&](auto v, int blk) {
+    constexpr bool V = decltype(v)::value;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const char* p = (const char*)(V ? a.v_pages : a.k_pages) + pt_place(cur, blk % WB * NG + g);
+#pragma unroll
+      for (int i = 0; i < LPG; ++i) pt_load8<D, V>(p, row_bytes, i, (V ? v0 : k0) + (g * LPG + i) * 1024, lane);
+    }
+  };
+  auto load_powers = [&](int blk) {   // lane i of 32: four bytes of K's (i < 16) or V's; the upper half repeats them
+    const int g = blk % WB * NG + ((lane & 15) >> 2);
+    const unsigned long long at = ((unsigned long long)(uint32_t)__shfl((int)(cur.scale >> 32), g, 64) << 32) |
+                                  (uint32_t)__shfl((int)(uint32_t)cur.scale, g, 64);
+    const unsigned char* p = ((lane & 16) ? a.v_scales : a.k_scales) + at + (lane & 3) * 4;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(pw0) : "memory", "m0");
+  };
+  int blk = b0 + wave;
+  if (blk < b1) {
+    wi = blk / WB;
+    cur = pt_window<true>(a, it, wi * 64);
+    pt_fetch(a, it, (wi + 1) * 64, ids);
+    bad = seek(blk);
+    load_powers(blk);
+    load(PtK{}, blk);
+    load(PtV{}, blk);
+  }
+  w.template init<true>(a, it, row0);
+  // the queries are waited for here: at their first use the wait would cover the loads in flight of every block
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
+  // positions that the tile's first row has open, and its last
+  const int pmin = __builtin_amdgcn_readfirstlane(w.pos), pend = __builtin_amdgcn_readlane(w.pos, 31);
+  for (; blk < b1; blk += 4) {
+    const bool more = blk + 4 < b1;
+    const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
+    gm_vmcnt<LD>();   // powers and K have landed; V's loads may be on their way
+    asm volatile("" ::: "memory");
+    if (blk * PB + PB - 1 > pend || bad) {   // the powers of places closed to every row: anything (0 x NaN)
+      if (lane < 32) {
+        const int j = (lane & 15) * 4;
+        uint32_t p = pw[lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (blk * PB + j + i > pend || ((bad >> (j >> 4)) & 1)) p = (p & ~(255u << (8 * i))) | (127u << (8 * i));
+        pw[lane] = p;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    odd = odd || pt_any_odd(pw[lane & 31], pt_least_odd<DT>);
+    uint32_t vp[NB][4];   // V's powers, at the places of the lane's scores
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vp[sb][i] = pw[16 + sb * 8 + 2 * i + w.hi];
+    // S^T = K Q^T
+    pt_f32x16 s[NB];
+    {
+      constexpr int KS = D / 32;   // 16-byte reads of a position
+      uint4 k[KS];
+      auto read = [&](int sb, int ks) { return *(const uint4*)(Kt + (sb * 32 + w.fr) * D + (((2 * ks + w.hi) ^ pt_xk8<D>(w.fr)) * 16)); };
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[ks] = read(0, ks);
+#pragma unroll
+      for (int sb = 0; sb < NB; ++sb) {
+        const float power = __uint_as_float((uint32_t)((const unsigned char*)pw)[sb * 32 + w.fr] << 23);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[sb][e] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s[sb] = pt_mfma<DT>(pt_widen<DT>(k[ks].x, k[ks].y, power), w.qf[2 * ks], s[sb]);
+          s[sb] = pt_mfma<DT>(pt_widen<DT>(k[ks].z, k[ks].w, power), w.qf[2 * ks + 1], s[sb]);
+          if (sb + 1 < NB) k[ks] = read(sb + 1, ks);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's rows and the powers are in registers
+    if (more) {
+      bad_next = seek(blk + 4);
+      load_powers(blk + 4);
+      load(PtK{}, blk + 4);
+    }
+    if (!open) w.template mask<NB>(s, blk * PB, bad);
+    w.template softmax<NB>(s);
+    if (more) gm_vmcnt<LD + 1>();   // V has landed; the next powers' and K's loads may be on their way
+    else gm_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    if (blk * PB + PB - 1 > pend || bad) {
+      constexpr int SL = D / 16;
+#pragma unroll 1
+      for (int i = lane; i < PB * SL; i += 64) {
+        const int j = i / SL;
+        if (blk * PB + j > pend || ((bad >> (j >> 4)) & 1)) *(uint4*)(Vt + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    // O^T += V^T P^T, 32 positions at a time, the operands read four ahead
+    float sum[2] = {w.l, 0.f};
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb) {
+      constexpr int N = 2 * TD;
+      auto read = [&](int i) {   // rows 8 hi + r of half block i / TD, dims 32 t + 16 g + 8 c
+        const int r = sb * 32 + (i / TD) * 16 + 8 * w.hi + ((lane & 15) >> 1), ch = 2 * (i % TD) + ((lane >> 4) & 1);
+        return pt_read_tr8(Vt + r * D + ((ch ^ pt_xv8<D>(r)) * 16) + (lane & 1) * 8);
+      };
+      uint2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = read(i);
+      pt_f32x16 e[1] = {s[sb]};
+      uint4 p[2], p2[2];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        sum[k & 1] += e[0][k];
+        const uint32_t u = vp[sb][k >> 2];
+        const uint32_t f = (k & 3) == 0 ? u << 23 : (k & 3) == 1 ? u << 15 : (k & 3) == 2 ? u << 7 : u >> 1;
+        e[0][k] *= __uint_as_float(f & 0x7f800000u);
+      }
+      PtWave<HS_BF16, D>::template pack_of<1>(e, p);
+      if constexpr (DT == HS_F16) {   // the rounding errors, in turn
+        PtWave<HS_BF16, D>::template rest_of<1>(e);
+        PtWave<HS_BF16, D>::template pack_of<1>(e, p2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint4 vf = pt_widen<HS_BF16>(v[i % 4].x, v[i % 4].y, 1.f);
+        w.o[i % TD] = pt_mfma<HS_BF16>(vf, p[i / TD], w.o[i % TD]);
+        if constexpr (DT == HS_F16) w.o[i % TD] = pt_mfma<HS_BF16>(vf, p2[i / TD], w.o[i % TD]);
+        if (i + 4 < N) v[i % 4] = read(i + 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    w.l = sum[0] + sum[1];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) load(PtV{}, blk + 4);
+    bad = bad_next;
+  }
+  pt_join_waves<DT, D, true>(a, it, w, lds, ml, odd);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
+  constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V, in 16 bits
+  constexpr int PCS = D / 64;                                           // 16-byte pieces of a row that a thread takes, of K and of V
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.H / a.KVH, rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
+  const int first = it.q.kv - it.q.n;   // position of token 0
+  const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
+  const int b0 = it.b0, b1 = it.b1;
+  constexpr int WB = 64 / NG;   // blocks of a window
+  PtWindowT<true> cur;
+  int* ids = slots[wave];
+  int wi = b0 / WB;             // window of cur
+  unsigned bad = 0, bad_next = 0;   // groups of the present and the next block without a page
+  const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's position
+  // a wave converts its group of 16 positions, four lanes a position
+  const int gr = lane >> 2, part = lane & 3;
+  uint4 kr[PCS], vr[PCS];
+  unsigned kb = 127, vb = 127;
+  bool odd = false;
+  auto issue = [&](int blk) {
+    if (blk / WB != wi) {
+      ++wi;
+      cur = pt_window<true>(a, it, wi * 64, ids[lane]);
+      pt_fetch(a, it, (wi + 1) * 64, ids);
+    }
+    bad_next = ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
+    const int g = blk % WB * NG + wave;
+    const unsigned long long at = pt_place(cur, g) + (unsigned long long)((unsigned)gr * (unsigned)a.row_stride + part * (D / 4));
+    const unsigned long long sc = (((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(cur.scale >> 32), g) << 32) |
+                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)cur.scale, g)) + gr;
+#pragma unroll
+    for (int i = 0; i < PCS; ++i) {
+      kr[i] = *(const uint4*)((const char*)a.k_pages + at + i * 16);
+      vr[i] = *(const uint4*)((const char*)a.v_pages + at + i * 16);
+    }
+    kb = a.k_scales[sc], vb = a.v_scales[sc];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto stage = [&](int blk) {   // what issue(blk) loaded, as 16 bits; zeros in the places that are closed to every row
+    char* K = lds + (blk & 1) * 2 * BYTES;
+    const int r = wave * 16 + gr;
+    const bool closed = blk * PB + r > pend || ((bad_next >> wave) & 1);
+    odd = odd || (!closed && (pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>)));
+    const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
+#pragma unroll
+    for (int i = 0; i < PCS; ++i) {
+      uint4 k = kr[i], v = vr[i];
+      if (closed) k = v = make_uint4(0, 0, 0, 0);
+      const int c = 2 * (part * PCS + i);   // chunks of 8 dims
+      char *kd = K + r * RB, *vd = K + BYTES + r * RB;
+      *(uint4*)(kd + ((c ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.x, k.y, closed ? 1.f : kp);
+      *(uint4*)(kd + (((c + 1) ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.z, k.w, closed ? 1.f : kp);
+      *(uint4*)(vd + ((c ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(v.x, v.y, closed ? 1.f : vp);
+      *(uint4*)(vd + (((c + 1) ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(v.z, v.w, closed ? 1.f : vp);
+    }
+  };
+  if (b0 < b1) {
+    cur = pt_window<true>(a, it, wi * 64);
+    pt_fetch(a, it, (wi + 1) * 64, ids);
+    issue(b0);
+  }
+  PtWave<DT, D> w;
+  w.init(a, it, row0);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
+  if (b0 < b1) stage(b0);
+  // positions that every row of the wave has open, and that any has
+  const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
+  const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
+  for (int blk = b0; blk < b1; ++blk) {
+    bad = bad_next;
+    __syncthreads();   // the block is in LDS, and every wave is done with the other stage
+    if (blk + 1 < b1) issue(blk + 1);
+    if (blk * PB <= pmax) {   // wave-uniform
+      const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
+      const char* Kt = lds + (blk & 1) * 2 * BYTES;
+      pt_f32x16 s[NB];
+      w.template scores<NB>(Kt, s);
+      if (!open) w.template mask<NB>(s, blk * PB, bad);
+      __builtin_amdgcn_s_setprio(1);   // vector instructions first: the other workgroup's matrix instructions run on beside them
+      w.template softmax<NB>(s);
+      uint4 p[2 * NB];
+      w.template pack<NB>(s, p);
+      __builtin_amdgcn_s_setprio(0);
+      w.template outputs<NB>(Kt + BYTES, p, s);
+    }
+    if (blk + 1 < b1) stage(blk + 1);
+  }
+  pt_end_wide<DT, D, true>(a, it, w, __syncthreads_or(odd));
 }
 
 // ------------------------------------------------------------------ kernels
 
 // grid_wide = 0: sequences of any number of rows on narrow tiles (batches that are nearly all single tokens)
-template <int DT, int D>
+template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
-  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
   __shared__ float ml[4][2][32];
   __shared__ int ids[4][64];
   __shared__ PtList t;
+  __shared__ uint32_t powers[F8 ? 4 : 1][64];
   const int nw = a.grid_wide;
   int x;
   if ((int)blockIdx.x >= nw) {
@@ -1048,7 +1695,8 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     for (int at = pt_first(all, workers, w); at < end;) {
       PtItem it;
       at = pt_item_narrow<NPB>(a, t, w, at, end, hi, it);
-      pt_narrow<DT, D>(a, it, lds, ml, ids);
+      if constexpr (F8) pt_narrow8<DT, D>(a, it, lds, ml, ids, powers);
+      else pt_narrow<DT, D>(a, it, lds, ml, ids);
     }
     return;
   }
@@ -1063,7 +1711,10 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
   };
   const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
-  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) {
+    if constexpr (F8) pt_wide8<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+    else pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+  }
 }
 
 // Joins S parts of one row (by a wave): part s lies `rel(s)` slots of R rows after row `first` of the parts.
@@ -1118,9 +1769,9 @@ __device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first,
 
 // k_paged_combine: joins the parts of split tiles, a wave per row and head, and zeroes the rows of no sequence.
 // (A part without open positions has maximum -inf and outputs of zero.)
-template <int DT, int D>
+template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
-  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
   __shared__ PtList t;
   __shared__ int start[PT_MAXB + 1], kv[PT_MAXB];   // (a row looks its sequence up in LDS: from memory it is 1 us)
   for (int b = threadIdx.x; b <= a.B; b += 256) {
@@ -1193,10 +1844,13 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
   }
 }
 
-#define PT_KERNELS(NAME, DT, D)                                                                                                  \
-  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_##NAME(const PagedAttnArgs a) { pt_attn_body<DT, D>(a); }     \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_combine_##NAME(const PagedAttnArgs a) { pt_combine_body<DT, D>(a); }
-PT_KERNELS(bf16_d128, HS_BF16, 128)
-PT_KERNELS(bf16_d64, HS_BF16, 64)
-PT_KERNELS(f16_d128, HS_F16, 128)
-PT_KERNELS(f16_d64, HS_F16, 64)
+#define PT_KERNELS(NAME, DT, D, F8)                                                                                               \
+  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_##NAME##_d##D(const PagedAttnArgs a) { pt_attn_body<DT, D, F8>(a); }
+#define PT_COMBINES(NAME, DT, D, F8)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_d##D(const PagedAttnArgs a) { pt_combine_body<DT, D, F8>(a); }
+#define PT_ALL(M, NAME)                                                                                                           \
+  M(NAME##_bf16, HS_BF16, 128, false) M(NAME##_bf16, HS_BF16, 64, false) M(NAME##_f16, HS_F16, 128, false) M(NAME##_f16, HS_F16, 64, false) \
+  M(quant_##NAME##_bf16, HS_BF16, 128, true) M(quant_##NAME##_bf16, HS_BF16, 64, true) M(quant_##NAME##_f16, HS_F16, 128, true)   \
+  M(quant_##NAME##_f16, HS_F16, 64, true)
+PT_ALL(PT_KERNELS, attn)
+PT_ALL(PT_COMBINES, combine)

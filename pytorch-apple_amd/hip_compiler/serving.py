@@ -6,10 +6,11 @@ from __future__ import annotations
 
 from hip_compiler.program import DTYPE_CODE, ELEM_SIZE, LaunchStep, TView
 from npu_compiler.ir_reader import OpNode
-from npu_runtime.serving_ops import check_paged_append, check_paged_attention, check_sample
+from npu_runtime.serving_ops import check_paged_append, check_paged_attention, check_paged_quant_attention, check_sample
 
 PAGED_ANY_MAX_D = 256          # paged.hip PG_ANY_D
 PAGED_APPEND_MAX_R = 256       # paged.hip PG_APPEND_R
+PAGED_HEADS_MAX_D = 256        # paged.hip append_heads: a head in 16 lanes
 # Up to this many rows a workgroup per row, past it a wave. us by workgroups / by waves, in 16 bits: 16 rows of 12 + 2 heads
 # of 128 3.8 / 5.1, 1,024 5.1 / 5.7, 2,048 7.5 / 6.8, 8,192 21.9 / 14.8; 14 + 2 of 64: 3.9 / 3.9, 4.6 / 4.3, 6.5 / 5.0,
 # 18.8 / 10.2; 32 + 8 of 128, whose rows keep four waves busy: 4.1 / 7.2, 6.7 / 8.7, 10.5 / 12.9, 32.4 / 34.4.
@@ -59,7 +60,8 @@ def _aligned_rows(low, name: str, v: TView) -> TView:
     return out
 
 
-def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_size: int, dtype: str) -> dict | None:
+def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_size: int, dtype: str,
+                block: int | None = None) -> dict | None:
     """Launch of the tiled attention kernels (paged.hip), None where they do not apply: other types or head sizes,
     pages that are no multiple of 16 positions, more sequences than the item list holds, or sizes whose item
     counts could pass 32 bits. Wide tiles are left out where the rows average at most two tokens per sequence: a
@@ -71,7 +73,7 @@ def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_s
     are read in a third of the time, up to 29%: 46 / 35 at 2.5): a launch does not know whether its rows are one chunk or many."""
     if dtype not in ("bfloat16", "float16") or D not in (64, 128) or page_size % 16 or not 0 < B <= PT_MAXB or M < 1 or P < 1:
         return None
-    G, block = H // KVH, 8192 // (2 * D)
+    G, block = H // KVH, block or 8192 // (2 * D)   # positions of a narrow tile's block
     blocks = -(-M * page_size // block)
     tiles = lambda R: KVH * (N * G // R + min(N, B))
     if (tiles(PT_NARROW) + 2 * PT_GRID) * (2 * blocks + 3) >= 2 ** 31 or M * page_size * page_size >= 2 ** 40 \
@@ -91,43 +93,64 @@ def _batch(low, table, q_start, kv_len) -> dict:
                 kv_len=low.ref(low.contiguous(kv_len.name)), B=int(kv_len.shape[0]), M=int(table.shape[1]))
 
 
+def _append_kernel(dtype: str, N: int, D: int, R: int, heads: bool) -> tuple[str, int]:
+    """(suffix, grid) of an append kernel; ``heads``: one of those that need whole heads."""
+    piece = 16 if heads else 8
+    if dtype not in ("bfloat16", "float16") or D % piece or R % 16 or R > PAGED_APPEND_MAX_R or (heads and D > PAGED_HEADS_MAX_D):
+        return "any", N
+    few = N <= PAGED_APPEND_ROW_N
+    return ("bf16" if dtype == "bfloat16" else "f16") + ("_row" if few else ""), N if few else -(-N // 4)
+
+
 def lower_paged_append(low, node: OpNode) -> None:
-    q, k, v, kp, vp, table, q_start, kv_len, inv = node.inputs
+    name = node.op_type.split(".")[1]
+    norm, quant = "norm_" in name, "quant_" in name
+    rest = list(node.inputs)
+    q, k, v = (rest.pop(0) for _ in range(3))
+    weights = tuple(rest.pop(0) for _ in range(2)) if norm else None
+    pools = [rest.pop(0) for _ in range(4 if quant else 2)]
+    table, q_start, kv_len, inv = rest
     layout = node.attrs.get("page_layout", "hnd")
-    check_paged_append(q, k, v, kp, vp, table, q_start, kv_len, inv, layout)
+    eps = float(node.attrs["eps"]) if norm else 0.0
+    kp, scales = pools[0], tuple(pools[2:]) or None
+    check_paged_append(q, k, v, *pools[:2], table, q_start, kv_len, inv, layout, weights, scales, eps)
     N, H, D = (int(s) for s in q.shape)
     KVH, ps = _pool_dims(kp.shape, layout)
     _check_i32(node.op_type, rows=N * H * D, table=int(table.shape[0]) * int(table.shape[1]), page=KVH * ps * D)
     qv, kv, vv = (_rows_view(low, t.name) for t in (q, k, v))
+    wv = tuple(low.contiguous(t.name) for t in weights or ())
     q_out = low.new_storage(node.outputs[0].name, q.shape, q.dtype)
     low.views[node.outputs[0].name] = q_out
-    pools = [low.inplace_or_copy(node, t, o) for t, o in ((kp, node.outputs[1]), (vp, node.outputs[2]))]
+    written = [low.ref(low.inplace_or_copy(node, t, o)) for t, o in zip(pools, node.outputs[1:])]
     if N == 0:
         return
-    kernel, grid = "k_paged_append_any", N
     R = 2 * int(inv.shape[0])
-    if q.dtype in ("bfloat16", "float16") and D % 8 == 0 and R % 16 == 0 and R <= PAGED_APPEND_MAX_R:
+    suffix, grid = _append_kernel(q.dtype, N, D, R, norm or quant)
+    pieces = []
+    if suffix != "any":
         qv, kv, vv = (_aligned_rows(low, t.name, v) for t, v in ((q, qv), (k, kv), (v, vv)))
-        few = N <= PAGED_APPEND_ROW_N
-        kernel = f"k_paged_append_{'bf16' if q.dtype == 'bfloat16' else 'f16'}" + ("_row" if few else "")
-        grid = N if few else -(-N // 4)
+        wv = tuple(low.aligned16(v, t.name) for t, v in zip(weights or (), wv))
+        pieces = ["q", "k", "v", "k_pages", "v_pages"] + (["q_weight", "k_weight"] if norm else [])
+    wq, wk = (low.ref(v) for v in wv) if norm else (None, None)
+    ks, vs = written[2:] if quant else (None, None)
     low.emit(LaunchStep(
-        kind="paged_append", kernel=kernel, module="paged", arg_struct="PagedAppendArgs",
-        args=dict(q=low.ref(qv), k=low.ref(kv), v=low.ref(vv), k_pages=low.ref(pools[0]), v_pages=low.ref(pools[1]),
+        kind="paged_append", kernel=f"k_{name}_{suffix}", module="paged", arg_struct="PagedAppendArgs",
+        args=dict(q=low.ref(qv), k=low.ref(kv), v=low.ref(vv), k_pages=written[0], v_pages=written[1],
                   q_out=low.ref(q_out), **_batch(low, table, q_start, kv_len),
                   inv_freq=low.ref(low.contiguous(inv.name)), q_rs=qv.strides[0], q_hs=qv.strides[1], k_rs=kv.strides[0],
                   k_hs=kv.strides[1], v_rs=vv.strides[0], v_hs=vv.strides[1], **_pool_strides(kp.shape, layout),
                   pages=int(kp.shape[0]), N=N, H=H, KVH=KVH, D=D, R=R, page_size=ps,
-                  scaling=float(node.attrs.get("attention_scaling", 1.0)), dtype=DTYPE_CODE[q.dtype]),
+                  scaling=float(node.attrs.get("attention_scaling", 1.0)), dtype=DTYPE_CODE[q.dtype], q_weight=wq, k_weight=wk,
+                  k_scales=ks, v_scales=vs, eps=eps, pad=0),
         grid=(grid, 1, 1), inputs=[t.name for t in node.inputs], outputs=[o.name for o in node.outputs],
-        params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D,
-                "pieces16": [] if kernel == "k_paged_append_any" else ["q", "k", "v", "k_pages", "v_pages"]}))
+        params={"rows": N, "seqs": int(kv_len.shape[0]), "heads": H, "kv_heads": KVH, "head_dim": D, "pieces16": pieces}))
 
 
 def lower_paged_attention(low, node: OpNode) -> None:
-    q, kp, vp, table, q_start, kv_len = node.inputs
+    quant = node.op_type == "serving.paged_quant_attention.default"
+    q, kp, vp, *scales, table, q_start, kv_len = node.inputs
     layout = node.attrs.get("page_layout", "hnd")
-    check_paged_attention(q, kp, vp, table, q_start, kv_len, layout)
+    (check_paged_quant_attention if quant else check_paged_attention)(q, kp, vp, *scales, table, q_start, kv_len, layout)
     N, H, D = (int(s) for s in q.shape)
     KVH, ps = _pool_dims(kp.shape, layout)
     # (the plain kernel steps by 64 positions up to a table's last)
@@ -136,28 +159,30 @@ def lower_paged_attention(low, node: OpNode) -> None:
     if D > PAGED_ANY_MAX_D:
         raise NotImplementedError(f"{node.op_type}: head_dim {D} is over {PAGED_ANY_MAX_D}")
     qv = _rows_view(low, q.name)
-    kv, vv = (low.contiguous(t.name) for t in (kp, vp))
+    caches = [low.contiguous(t.name) for t in (kp, vp, *scales)]
     out = low.new_storage(node.outputs[0].name, q.shape, q.dtype)
     low.views[node.outputs[0].name] = out
     if N == 0:
         return
     B, M, P = int(kv_len.shape[0]), int(table.shape[1]), int(kp.shape[0])
-    tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype)
+    tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype, 64 if quant else None)
     if tiled:
         qv = _aligned_rows(low, q.name, qv)
-        kv, vv = (low.aligned16(v, t.name) for t, v in ((kp, kv), (vp, vv)))
-    args = dict(q=low.ref(qv), k_pages=low.ref(kv), v_pages=low.ref(vv), out=low.ref(out), part_o=None, part_ml=None,
+        caches = [low.aligned16(v, t.name) for t, v in zip((kp, vp, *scales), caches)]
+    kv, vv, ks, vs = [low.ref(v) for v in caches] + ([] if quant else [None, None])
+    args = dict(q=low.ref(qv), k_pages=kv, v_pages=vv, out=low.ref(out), part_o=None, part_ml=None,
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
                 scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
-                grid_narrow=0, pad=0)
+                grid_narrow=0, pad=0, k_scales=ks, v_scales=vs)
     params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
     ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
+    prefix = "k_paged_quant_" if quant else "k_paged_"
     if tiled is None:
-        low.emit(LaunchStep(kind="paged_attention", kernel="k_paged_attn_any", module="paged", arg_struct="PagedAttnArgs",
+        low.emit(LaunchStep(kind="paged_attention", kernel=prefix + "attn_any", module="paged", arg_struct="PagedAttnArgs",
                             args=args, grid=(N, H, 1), block=(64, 1, 1), inputs=ins, outputs=outs, params=params))
         return
-    params["pieces16"] = ["q", "k_pages", "v_pages"]
+    params["pieces16"] = ["q", "k_pages", "v_pages"] + (["k_scales", "v_scales"] if quant else [])
     groups = ps // 16
     part_rows = 2 * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
@@ -166,10 +191,10 @@ def lower_paged_attention(low, node: OpNode) -> None:
                 grid_narrow=tiled["grid_narrow"])
     name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
-        kind="paged_attention", kernel="k_paged_attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
+        kind="paged_attention", kernel=prefix + "attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
         grid=(tiled["grid_wide"] + tiled["grid_narrow"], 1, 1), inputs=ins, outputs=outs, params={**params, "mfma": True}))
     low.emit(LaunchStep(
-        kind="paged_attention", kernel="k_paged_combine_" + name, module="paged", arg_struct="PagedAttnArgs",
+        kind="paged_attention", kernel=prefix + "combine_" + name, module="paged", arg_struct="PagedAttnArgs",
         args=dict(args), grid=(min(1024, -(-N * H // 4)), 1, 1), inputs=ins, outputs=outs, params=params))
 
 
@@ -216,5 +241,6 @@ def lower_sample(low, node: OpNode) -> None:
                             params={"rows": B, "vocab": V}))
 
 
-LOWERINGS = {"serving.paged_append.default": lower_paged_append,
-             "serving.paged_attention.default": lower_paged_attention, "serving.sample.default": lower_sample}
+LOWERINGS = {**{f"serving.paged_{form}append.default": lower_paged_append for form in ("", "norm_", "quant_", "norm_quant_")},
+             **{f"serving.paged_{form}attention.default": lower_paged_attention for form in ("", "quant_")},
+             "serving.sample.default": lower_sample}

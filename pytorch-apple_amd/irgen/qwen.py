@@ -26,7 +26,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from irgen.builder import IRBuilder, T
-from irgen.serving import batch_inputs, paged_append, paged_attention, pool_shape, sampling_inputs
+from irgen.serving import append, attention, batch_inputs, cache_inputs, sampling_inputs
 
 INT64_MAX = 9223372036854775807
 
@@ -216,7 +216,8 @@ def build_decode_ir(max_cache_len: int, cfg: QwenConfig = QWEN2_5_1_5B, argmax: 
 
 
 def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pages: int,
-                   cfg: QwenConfig = QWEN2_5_1_5B, layout: str = "hnd") -> dict:
+                   cfg: QwenConfig = QWEN2_5_1_5B, layout: str = "hnd", cache: str | None = None,
+                   qk_norm: bool = False) -> dict:
     """One step of a server: ``tokens`` rows (decoded tokens and prompt chunks of up to ``seqs`` sequences, packed, rows
     of no sequence behind them) over paged caches, one sampled token per sequence. No counterpart in the reference,
     whose graphs hold one sequence each.
@@ -224,21 +225,22 @@ def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pag
     Inputs: ``input_ids`` int64 [tokens]; ``block_table`` [seqs, table_pages], ``q_start`` [seqs + 1] and ``kv_len``
     [seqs] int32 as ``npu_runtime.serving_ops`` defines them; ``last_rows`` int64 [seqs], the row from which a
     sequence's next token is drawn (any row where none is); ``temperature``, ``top_k``, ``top_p``, ``min_p`` and ``u``
-    [seqs]; per layer ``k_pages_{i}`` and ``v_pages_{i}``. Outputs: ``next_token`` int64 [seqs], then the pools, which
-    a device updates in place. The weights are those of ``build_decode_ir``."""
+    [seqs]; per layer ``k_pages_{i}`` and ``v_pages_{i}``, and with ``cache`` "float8_e4m3fn", whose pages are of 8 bits,
+    ``k_scales_{i}`` and ``v_scales_{i}``. Outputs: ``next_token`` int64 [seqs], then the pools, which a device updates
+    in place. The weights are those of ``build_decode_ir``; with ``qk_norm`` each head of q and k is normed before the
+    rotation, by ``self_attn.q_norm.weight`` and ``self_attn.k_norm.weight`` [head_dim]."""
     b = IRBuilder("Qwen2.5_Paged")
     H, KVH, D, Hd, dt = cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.hidden, cfg.dtype
     ids = b.input("input_ids", [tokens], "int64")
     batch = batch_inputs(b, seqs, table_pages)
     last_rows = b.input("last_rows", [seqs], "int64")
     params = sampling_inputs(b, seqs)
-    shape = pool_shape(pages, page_size, KVH, D, layout)
-    pools = [(b.input(f"k_pages_{li}", shape, dt), b.input(f"v_pages_{li}", shape, dt)) for li in range(cfg.layers)]
+    pools = [cache_inputs(b, pages, page_size, KVH, D, layout, dt, cache, f"_{li}") for li in range(cfg.layers)]
     emb = b.weight("model.embed_tokens.weight", [cfg.vocab, Hd], dt)
     inv = b.weight("model.rotary_emb.inv_freq", [D // 2], "float32", buffer=True)
     x = b.op("aten.embedding.default", [emb, ids])
     written = []
-    for li, (kp, vp) in enumerate(pools):
+    for li, kv in enumerate(pools):
         pre = f"model.layers.{li}."
 
         def heads(name: str, n: int) -> T:
@@ -248,13 +250,14 @@ def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pag
 
         h = rmsnorm(b, x, b.weight(pre + "input_layernorm.weight", [Hd], dt), cfg.eps)
         q, k, v = heads("q", H), heads("k", KVH), heads("v", KVH)
-        q, kp, vp = paged_append(b, q, k, v, kp, vp, batch, inv, layout)
-        o = paged_attention(b, q, kp, vp, batch, D ** -0.5, layout)
+        norms = tuple(b.weight(f"{pre}self_attn.{n}_norm.weight", [D], dt) for n in "qk") if qk_norm else None
+        q, *kv = append(b, q, k, v, kv, batch, inv, layout, weights=norms, eps=cfg.eps)
+        o = attention(b, q, kv, batch, D ** -0.5, layout)
         o = b.op("aten.reshape.default", [o], {"shape": [tokens, H * D]})
         a = linear(b, o, b.weight(pre + "self_attn.o_proj.weight", [Hd, H * D], dt))
         x = b.op("aten.add.Tensor", [x, a])
         x = mlp_block(b, cfg, pre + "mlp.", x, pre + "post_attention_layernorm.weight")
-        written += [kp, vp]
+        written += kv
     x = b.op("aten.embedding.default", [x, last_rows])   # the rows that a token is drawn from
     h = rmsnorm(b, x, b.weight("model.norm.weight", [Hd], dt), cfg.eps)
     lm = emb if cfg.tie_embeddings else b.weight("lm_head.weight", [cfg.vocab, Hd], dt)

@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-_TORCH = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}
+_TORCH = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32, "uint8": torch.uint8}
 _BATCH = ("block_table", "q_start", "kv_len", "last_rows", "temperature", "top_k", "top_p", "min_p", "u")
 
 
@@ -58,13 +58,13 @@ class PagedGenerator:
         if missing:
             raise ValueError(f"not a paged step graph: it has no input {missing}")
         self.backend = backend
-        self.pool_names = [n for n in shapes if n not in ("input_ids", *_BATCH)]
+        self.pool_names = [n for n in shapes if n not in ("input_ids", *_BATCH)]   # (pages first, then their scales if any)
         self.shapes = shapes
         self.slots, self.table_pages = shapes["block_table"][0]
         if not self.pool_names:
             raise ValueError("not a paged step graph: it has no page pools")
         layouts = {n["attrs"].get("page_layout", "hnd") for ir in (step_ir, decode_ir) if ir is not None
-                   for n in ir["nodes"] if n["op_type"] in ("serving.paged_append.default", "serving.paged_attention.default")}
+                   for n in ir["nodes"] if n["op_type"].startswith("serving.paged_")}
         if len(layouts) != 1:
             raise ValueError(f"not graphs of one page_layout: {sorted(layouts)}")
         dims = shapes[self.pool_names[0]][0]

@@ -21,6 +21,14 @@ A position that has no place (before 0, past the table, in a page that is not on
 written and is closed to attention: its key and value are not read, whatever they hold. Where two rows name
 one place, each element of it is one of theirs. Pools are [P, KVH, page_size, D] (page_layout "hnd") or
 [P, page_size, KVH, D] ("nhd").
+
+Pools of 8 bits (the ``quant`` operators) are uint8 of the same shapes: bytes of e4m3 numbers (``torch.float8_e4m3fn``),
+beside ``k_scales`` and ``v_scales``, uint8 [P, KVH, page_size] in either layout: a byte s per position and head stands
+for the power of two 2^(s - 127) that its numbers are multiplied by (``torch.float8_e8m0fnu``, 255 is NaN; but 0, as places
+that nothing was written to may hold, stands for 0). A power of two costs e4m3 no precision, since its steps are
+relative, and is exact to divide and multiply by.
+
+``norm`` operators divide each head of q and k by its root mean square first, as models do that norm their heads.
 """
 
 from __future__ import annotations
@@ -35,6 +43,16 @@ _LIB.define("paged_append(Tensor q, Tensor k, Tensor v, Tensor k_pages, Tensor v
             "-> (Tensor, Tensor, Tensor)")
 _LIB.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor q_start, "
             "Tensor kv_len, float scale, str page_layout=\"hnd\") -> Tensor")
+_CACHE8 = "Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor q_start, Tensor kv_len, "
+_LIB.define("paged_norm_append(Tensor q, Tensor k, Tensor v, Tensor q_weight, Tensor k_weight, Tensor k_pages, Tensor v_pages, "
+            "Tensor block_table, Tensor q_start, Tensor kv_len, Tensor inv_freq, float eps, float attention_scaling=1.0, "
+            "str page_layout=\"hnd\") -> (Tensor, Tensor, Tensor)")
+_LIB.define("paged_quant_append(Tensor q, Tensor k, Tensor v, " + _CACHE8 + "Tensor inv_freq, float attention_scaling=1.0, "
+            "str page_layout=\"hnd\") -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+_LIB.define("paged_norm_quant_append(Tensor q, Tensor k, Tensor v, Tensor q_weight, Tensor k_weight, " + _CACHE8 +
+            "Tensor inv_freq, float eps, float attention_scaling=1.0, str page_layout=\"hnd\") "
+            "-> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+_LIB.define("paged_quant_attention(Tensor q, " + _CACHE8 + "float scale, str page_layout=\"hnd\") -> Tensor")
 _LIB.define("sample(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, Tensor min_p, Tensor u) -> Tensor")
 
 
@@ -49,7 +67,7 @@ def _is(t, name: str) -> bool:
     return str(t.dtype).replace("torch.", "") == name
 
 
-def _check_pages(op: str, q, k_pages, v_pages, block_table, q_start, kv_len, page_layout: str) -> None:
+def _check_pages(op: str, q, k_pages, v_pages, block_table, q_start, kv_len, page_layout: str, scales=None) -> None:
     _need(page_layout in LAYOUTS, f"{op}: page_layout {page_layout!r} is not one of {LAYOUTS}")
     _need(len(q.shape) == 3, f"{op}: q must be [rows, heads, head_dim], got {list(q.shape)}")
     _need(len(k_pages.shape) == 4 and tuple(k_pages.shape) == tuple(v_pages.shape),
@@ -63,16 +81,29 @@ def _check_pages(op: str, q, k_pages, v_pages, block_table, q_start, kv_len, pag
           f"{op}: need kv_len [B], q_start [B + 1] and block_table [B, M]")
     for name, t in (("block_table", block_table), ("q_start", q_start), ("kv_len", kv_len)):
         _need(_is(t, "int32"), f"{op}: {name} must be int32, got {t.dtype}")
-    _need(str(q.dtype) == str(k_pages.dtype) == str(v_pages.dtype) and
-          any(_is(q, d) for d in ("bfloat16", "float16", "float32")),
-          f"{op}: q and the pools must share one floating type")
+    floating = any(_is(q, d) for d in ("bfloat16", "float16", "float32"))
+    if scales is None:
+        _need(str(q.dtype) == str(k_pages.dtype) == str(v_pages.dtype) and floating,
+              f"{op}: q and the pools must share one floating type")
+        return
+    _need(floating, f"{op}: q must be bfloat16, float16 or float32, got {q.dtype}")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("k_scales", scales[0]), ("v_scales", scales[1])):
+        _need(_is(t, "uint8"), f"{op}: {name} must be uint8, got {t.dtype}")
+    for name, t in (("k_scales", scales[0]), ("v_scales", scales[1])):
+        _need(tuple(t.shape) == (k_pages.shape[0], kvh, page_size), f"{op}: {name} must be [{k_pages.shape[0]}, {kvh}, {page_size}]")
 
 
-def check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout: str) -> None:
-    """Raise ``ValueError`` unless the operands (tensors, specs or views: shape and dtype are read) fit."""
-    op = "serving.paged_append"
-    _check_pages(op, q, k_pages, v_pages, block_table, q_start, kv_len, page_layout)
+def check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout: str, weights=None,
+                       scales=None, eps=None) -> None:
+    """Raise ``ValueError`` unless the operands (tensors, specs or views: shape and dtype are read) fit. ``weights``: (q_weight,
+    k_weight) of the forms that norm, with their ``eps``; ``scales``: (k_scales, v_scales) of those that quantise."""
+    op = "serving.paged_" + ("norm_" if weights else "") + ("quant_" if scales else "") + "append"
+    _check_pages(op, q, k_pages, v_pages, block_table, q_start, kv_len, page_layout, scales)
     kvh = k_pages.shape[1 if page_layout == "hnd" else 2]
+    if weights:
+        for name, t in zip(("q_weight", "k_weight"), weights):
+            _need(tuple(t.shape) == (q.shape[2],) and str(t.dtype) == str(q.dtype), f"{op}: {name} must be [{q.shape[2]}] of q's type")
+        _need(eps >= 0, f"{op}: eps must not be negative, got {eps}")
     for name, t in (("k", k), ("v", v)):
         _need(tuple(t.shape) == (q.shape[0], kvh, q.shape[2]) and str(t.dtype) == str(q.dtype),
               f"{op}: {name} must be [{q.shape[0]}, {kvh}, {q.shape[2]}] of q's type")
@@ -82,6 +113,11 @@ def check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, 
 
 def check_paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, page_layout: str) -> None:
     _check_pages("serving.paged_attention", q, k_pages, v_pages, block_table, q_start, kv_len, page_layout)
+
+
+def check_paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, page_layout: str) -> None:
+    _check_pages("serving.paged_quant_attention", q, k_pages, v_pages, block_table, q_start, kv_len, page_layout,
+                 (k_scales, v_scales))
 
 
 def check_sample(logits, temperature, top_k, top_p, min_p, u) -> None:
@@ -135,31 +171,100 @@ def paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_fr
     x'[j + r] = x[j + r] c + x[j] d for j < r, the dimensions from 2 r on as they are, one rounding at the
     end. Returns (rotated q, k_pages, v_pages)."""
     check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout)
+    return _append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling, page_layout)
+
+
+def paged_norm_append(q, k, v, q_weight, k_weight, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, eps,
+                      attention_scaling=1.0, page_layout="hnd"):
+    """``paged_append`` of heads that are normed first: x / sqrt(mean(x^2) + eps) * weight over a head's dimensions, in 32
+    bits, not rounded before the rotation."""
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, (q_weight, k_weight), eps=eps)
+    return _append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling, page_layout,
+                   (q_weight, k_weight), eps)
+
+
+def paged_quant_append(q, k, v, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, inv_freq,
+                       attention_scaling=1.0, page_layout="hnd"):
+    """``paged_append`` into pools of 8 bits. Of each head's k (rotated, unrounded) and v: s = 2^e with the smallest e >= -100
+    for which its largest finite magnitude is at most 448 s, then x / s rounded to e4m3 once; NaN and infinities become
+    NaN. Returns (rotated q, k_pages, v_pages, k_scales, v_scales). Where two rows name one place, its numbers and its power
+    may be of different rows."""
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, scales=(k_scales, v_scales))
+    return _append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling, page_layout,
+                   scales=(k_scales, v_scales))
+
+
+def paged_norm_quant_append(q, k, v, q_weight, k_weight, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len,
+                            inv_freq, eps, attention_scaling=1.0, page_layout="hnd"):
+    """``paged_quant_append`` of heads normed as by ``paged_norm_append``."""
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, (q_weight, k_weight),
+                       (k_scales, v_scales), eps)
+    return _append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling, page_layout,
+                   (q_weight, k_weight), eps, (k_scales, v_scales))
+
+
+def quantise(x):
+    """(bytes of e4m3 numbers, byte of the power of two) of heads [..., D], as ``paged_quant_append`` defines them."""
+    x = x.float()
+    m, two = torch.frexp(torch.where(x.isfinite(), x.abs(), torch.zeros(())).amax(-1).clamp(min=2.0 ** -92))
+    e = two - 9 + (m > 0.875)   # m 2^two <= 448 2^e = 0.875 2^(9 + e)
+    return torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn).view(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def dequantise(pages, scales, page_layout="hnd"):
+    """float32 pools of the numbers that pools of 8 bits hold."""
+    s = torch.where(scales == 0, torch.zeros(()), scales.view(torch.float8_e8m0fnu).float())
+    s = (s if page_layout == "hnd" else s.transpose(1, 2))[..., None]
+    return pages.view(torch.float8_e4m3fn).float() * s
+
+
+def _append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling, page_layout, weights=None,
+            eps=0.0, scales=None):
     b, pos = row_places(q.shape[0], q_start, kv_len)
     r = inv_freq.shape[0]
     f = pos[:, None].double() * inv_freq.double()
     c = (f.cos() * attention_scaling).float()[:, None]
     d = (f.sin() * attention_scaling).float()[:, None]
 
-    def rotate(x):
-        lo, hi, rest = x[..., :r].float(), x[..., r:2 * r].float(), x[..., 2 * r:]
-        return torch.cat([(lo * c - hi * d).to(x.dtype), (hi * c + lo * d).to(x.dtype), rest], -1)
+    def normed(x, i):
+        x = x.float()
+        return x if weights is None else x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weights[i].float()
 
-    q_out = torch.where((b >= 0)[:, None, None], rotate(q), torch.zeros((), dtype=q.dtype))
+    def rotated(x):
+        lo, hi, rest = x[..., :r], x[..., r:2 * r], x[..., 2 * r:]
+        return torch.cat([lo * c - hi * d, hi * c + lo * d, rest], -1)
+
+    q_out = torch.where((b >= 0)[:, None, None], rotated(normed(q, 0)), torch.zeros(())).to(q.dtype)
     ps = k_pages.shape[2 if page_layout == "hnd" else 1]
     page, off, ok = _slots(b, pos, block_table, k_pages.shape[0], ps)
-    out = []
-    for pool, new in ((k_pages, rotate(k)), (v_pages, v)):
+    pools, powers = [], []
+    for i, (pool, new) in enumerate(((k_pages, rotated(normed(k, 1))), (v_pages, v))):
         pool = pool.clone()
-        _by_token(pool, page_layout)[page[ok], off[ok]] = new[ok]
-        out.append(pool)
-    return q_out, out[0], out[1]
+        if scales is not None:
+            new, s = quantise(new)
+            powers.append(scales[i].clone())
+            powers[i].transpose(1, 2)[page[ok], off[ok]] = s[ok]
+        _by_token(pool, page_layout)[page[ok], off[ok]] = new[ok].to(pool.dtype)
+        pools.append(pool)
+    return (q_out, *pools, *powers)
 
 
 def paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, page_layout="hnd"):
     """softmax(scale q . k) v over the positions up to each row's own; query heads h of one K/V head h // (H / KVH)
     share its pages. A row with no open position is zero, and so is one whose open positions all score -inf."""
     check_paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, page_layout)
+    return _attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, page_layout)
+
+
+def paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, scale, page_layout="hnd"):
+    """``paged_attention`` over the numbers that pools of 8 bits hold. A power byte of 255 makes them NaN. They, and their
+    products with q before the scale, are held in 32 bits."""
+    check_paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, page_layout)
+    return _attention(q, dequantise(k_pages, k_scales, page_layout), dequantise(v_pages, v_scales, page_layout), block_table,
+                      q_start, kv_len, scale, page_layout)
+
+
+def _attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, page_layout):
     N, H, D = q.shape
     K, V = _by_token(k_pages, page_layout), _by_token(v_pages, page_layout)
     G = H // K.shape[2]
@@ -231,7 +336,35 @@ def sample(logits, temperature, top_k, top_p, min_p, u):
 def _paged_append_meta(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, attention_scaling=1.0,
                        page_layout="hnd"):
     check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout)
-    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k_pages, v_pages))
+    return _like(q, k_pages, v_pages)
+
+
+def _like(*ts):
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts)
+
+
+def _paged_norm_append_meta(q, k, v, q_weight, k_weight, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, eps,
+                            attention_scaling=1.0, page_layout="hnd"):
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, (q_weight, k_weight), eps=eps)
+    return _like(q, k_pages, v_pages)
+
+
+def _paged_quant_append_meta(q, k, v, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, inv_freq,
+                             attention_scaling=1.0, page_layout="hnd"):
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, scales=(k_scales, v_scales))
+    return _like(q, k_pages, v_pages, k_scales, v_scales)
+
+
+def _paged_norm_quant_append_meta(q, k, v, q_weight, k_weight, k_pages, v_pages, k_scales, v_scales, block_table, q_start,
+                                  kv_len, inv_freq, eps, attention_scaling=1.0, page_layout="hnd"):
+    check_paged_append(q, k, v, k_pages, v_pages, block_table, q_start, kv_len, inv_freq, page_layout, (q_weight, k_weight),
+                       (k_scales, v_scales), eps)
+    return _like(q, k_pages, v_pages, k_scales, v_scales)
+
+
+def _paged_quant_attention_meta(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, scale, page_layout="hnd"):
+    check_paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, page_layout)
+    return _like(q)[0]
 
 
 def _paged_attention_meta(q, k_pages, v_pages, block_table, q_start, kv_len, scale, page_layout="hnd"):
@@ -245,7 +378,11 @@ def _sample_meta(logits, temperature, top_k, top_p, min_p, u):
 
 
 for _name, _cpu, _meta in (("paged_append", paged_append, _paged_append_meta),
+                           ("paged_norm_append", paged_norm_append, _paged_norm_append_meta),
+                           ("paged_quant_append", paged_quant_append, _paged_quant_append_meta),
+                           ("paged_norm_quant_append", paged_norm_quant_append, _paged_norm_quant_append_meta),
                            ("paged_attention", paged_attention, _paged_attention_meta),
+                           ("paged_quant_attention", paged_quant_attention, _paged_quant_attention_meta),
                            ("sample", sample, _sample_meta)):
     _LIB.impl(_name, _cpu, "CPU")
     _LIB.impl(_name, _meta, "Meta")
