@@ -855,9 +855,7 @@ struct PtWave {
 
   // P in the B operand's layout: lane half 0 needs positions 0-7 / 16-23 of 32, half 1 8-15 / 24-31
   template <int NB>
-  __device__ __forceinline__ void pack(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) const { pack_of<NB>(s, p); }
-  template <int NB>
-  __device__ __forceinline__ static void pack_of(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) {
+  __device__ __forceinline__ void pack(const pt_f32x16 (&s)[NB], uint4 (&p)[2 * NB]) const {
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
       uint32_t g[4][2];
@@ -873,15 +871,6 @@ struct PtWave {
         p[2 * sb + i / 2] = make_uint4(g[i][0], g[i][1], g[i + 1][0], g[i + 1][1]);
       }
     }
-  }
-
-  // what packing rounds away
-  template <int NB>
-  __device__ __forceinline__ static void rest_of(pt_f32x16 (&s)[NB]) {
-#pragma unroll
-    for (int sb = 0; sb < NB; ++sb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[sb][e] -= gm_round<DT>(s[sb][e]);
   }
 
   // Outputs, and the sums of the exponentials s. The operands are read four ahead, in an order that the compiler keeps:
@@ -1387,6 +1376,17 @@ __device__ __forceinline__ uint4 pt_widen(uint32_t a, uint32_t b, float power) {
   return r;
 }
 
+// pack for 16 positions: the lane's eight values in the B operand's layout
+template <int DT>
+__device__ __forceinline__ uint4 pt_pack16(const float (&e)[8]) {
+  uint32_t g[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g[i] = gm_pack2<DT>(e[2 * i], e[2 * i + 1]);
+  pt_swap32(g[0], g[2]);
+  pt_swap32(g[1], g[3]);
+  return make_uint4(g[0], g[1], g[2], g[3]);
+}
+
 // Transposing LDS read of bytes: lanes 2r + c of each 16-lane group address row r, columns 8c .. 8c + 7; lane i gets column i
 // of rows 0 .. 7.
 __device__ __forceinline__ uint2 pt_read_tr8(const char* p) {
@@ -1550,28 +1550,33 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
       uint2 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = read(i);
-      pt_f32x16 e[1] = {s[sb]};
-      uint4 p[2], p2[2];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        sum[k & 1] += e[0][k];
-        const uint32_t u = vp[sb][k >> 2];
-        const uint32_t f = (k & 3) == 0 ? u << 23 : (k & 3) == 1 ? u << 15 : (k & 3) == 2 ? u << 7 : u >> 1;
-        e[0][k] *= __uint_as_float(f & 0x7f800000u);
-      }
-      PtWave<HS_BF16, D>::template pack_of<1>(e, p);
-      if constexpr (DT == HS_F16) {   // the rounding errors, in turn
-        PtWave<HS_BF16, D>::template rest_of<1>(e);
-        PtWave<HS_BF16, D>::template pack_of<1>(e, p2);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      for (int h = 0; h < 2; ++h) {   // 16 positions
+        float e[8];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint4 vf = pt_widen<HS_BF16>(v[i % 4].x, v[i % 4].y, 1.f);
-        w.o[i % TD] = pt_mfma<HS_BF16>(vf, p[i / TD], w.o[i % TD]);
-        if constexpr (DT == HS_F16) w.o[i % TD] = pt_mfma<HS_BF16>(vf, p2[i / TD], w.o[i % TD]);
-        if (i + 4 < N) v[i % 4] = read(i + 4);
+        for (int k = 0; k < 8; ++k) {
+          const float x = s[sb][8 * h + k];
+          sum[k & 1] += x;
+          const uint32_t u = vp[sb][2 * h + (k >> 2)];
+          const uint32_t f = (k & 3) == 0 ? u << 23 : (k & 3) == 1 ? u << 15 : (k & 3) == 2 ? u << 7 : u >> 1;
+          e[k] = x * __uint_as_float(f & 0x7f800000u);
+        }
+        const uint4 p = pt_pack16<HS_BF16>(e);
+        uint4 p2;
+        if constexpr (DT == HS_F16) {   // the rounding errors, in turn
+#pragma unroll
+          for (int k = 0; k < 8; ++k) e[k] -= gm_round<HS_BF16>(e[k]);
+          p2 = pt_pack16<HS_BF16>(e);
+        }
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = h * TD; i < h * TD + TD; ++i) {
+          const uint4 vf = pt_widen<HS_BF16>(v[i % 4].x, v[i % 4].y, 1.f);
+          w.o[i % TD] = pt_mfma<HS_BF16>(vf, p, w.o[i % TD]);
+          if constexpr (DT == HS_F16) w.o[i % TD] = pt_mfma<HS_BF16>(vf, p2, w.o[i % TD]);
+          if (i + 4 < N) v[i % 4] = read(i + 4);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     w.l = sum[0] + sum[1];
@@ -1597,8 +1602,12 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& i
   int wi = b0 / WB;             // window of cur
   unsigned bad = 0, bad_next = 0;   // groups of the present and the next block without a page
   const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's position
-  // a wave converts its group of 16 positions, four lanes a position
-  const int gr = lane >> 2, part = lane & 3;
+  // A wave converts its group of 16 positions, four lanes a position. LDS takes the writes of 8 lanes at a time, two positions'
+  // here: K's swizzle sends those to different banks (D = 64: of positions 0 and 2), for V every other position writes its
+  // odd chunk first.
+  const int gr = D == 128 ? lane >> 2 : (lane >> 4) << 2 | ((lane >> 2) & 1) << 1 | ((lane >> 3) & 1), part = lane & 3;
+  const bool turn = (lane >> 2) & 1;
+  const unsigned ko = (unsigned)gr * (unsigned)a.row_stride + part * 16;   // 16-byte pieces part + 4 i of a row
   uint4 kr[PCS], vr[PCS];
   unsigned kb = 127, vb = 127;
   bool odd = false;
@@ -1610,33 +1619,39 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& i
     }
     bad_next = ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
     const int g = blk % WB * NG + wave;
-    const unsigned long long at = pt_place(cur, g) + (unsigned long long)((unsigned)gr * (unsigned)a.row_stride + part * (D / 4));
-    const unsigned long long sc = (((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(cur.scale >> 32), g) << 32) |
-                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)cur.scale, g)) + gr;
+    const unsigned long long at = pt_place(cur, g);
+    const unsigned long long sc = ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(cur.scale >> 32), g) << 32) |
+                                  (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)cur.scale, g);
+    const char *k = (const char*)a.k_pages + at, *v = (const char*)a.v_pages + at;
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
-      kr[i] = *(const uint4*)((const char*)a.k_pages + at + i * 16);
-      vr[i] = *(const uint4*)((const char*)a.v_pages + at + i * 16);
+      kr[i] = *(const uint4*)(k + (ko + i * 64));
+      vr[i] = *(const uint4*)(v + (ko + i * 64));
     }
-    kb = a.k_scales[sc], vb = a.v_scales[sc];
+    kb = (a.k_scales + sc)[gr], vb = (a.v_scales + sc)[gr];
     __builtin_amdgcn_sched_barrier(0);
   };
   auto stage = [&](int blk) {   // what issue(blk) loaded, as 16 bits; zeros in the places that are closed to every row
     char* K = lds + (blk & 1) * 2 * BYTES;
     const int r = wave * 16 + gr;
-    const bool closed = blk * PB + r > pend || ((bad_next >> wave) & 1);
-    odd = odd || (!closed && (pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>)));
+    if (blk * PB + PB - 1 > pend || bad_next) {
+      if (blk * PB + r > pend || ((bad_next >> wave) & 1)) {
+        kb = vb = 127;
+#pragma unroll
+        for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    odd = odd || pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>);
     const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
+    char *kd = K + r * RB, *vd = K + BYTES + r * RB;
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
-      uint4 k = kr[i], v = vr[i];
-      if (closed) k = v = make_uint4(0, 0, 0, 0);
-      const int c = 2 * (part * PCS + i);   // chunks of 8 dims
-      char *kd = K + r * RB, *vd = K + BYTES + r * RB;
-      *(uint4*)(kd + ((c ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.x, k.y, closed ? 1.f : kp);
-      *(uint4*)(kd + (((c + 1) ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.z, k.w, closed ? 1.f : kp);
-      *(uint4*)(vd + ((c ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(v.x, v.y, closed ? 1.f : vp);
-      *(uint4*)(vd + (((c + 1) ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(v.z, v.w, closed ? 1.f : vp);
+      const int c = 2 * (part + 4 * i), d = c + turn;   // chunks of 8 dims
+      const uint4 k = kr[i], v = vr[i];
+      *(uint4*)(kd + ((c ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.x, k.y, kp);
+      *(uint4*)(kd + (((c + 1) ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.z, k.w, kp);
+      *(uint4*)(vd + ((d ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(turn ? v.z : v.x, turn ? v.w : v.y, vp);
+      *(uint4*)(vd + (((d ^ 1) ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
     }
   };
   if (b0 < b1) {
