@@ -504,6 +504,7 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_quant_attn_any(const Pa
 #define PT_NARROW 32             // rows
 #define PT_WIDE 128
 #define PT_NARROW_LEAST 4        // fewest blocks of a narrow workgroup: one per wave
+#define PT_WAVE_LEAST 1          // and of a wave over pages of 8 bits
 #define PT_WIDE_ITEMS 480        // items that wide tiles are split towards: one round of two workgroups per CU
 #define PT_WIDE_LEAST 8          // fewest blocks of a split
 
@@ -625,9 +626,11 @@ __device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t
   return total[2] ? 0 : total[0];
 }
 
-// Workgroups that share `all` narrow blocks, of at most `most`, and the first block of workgroup w
+// Workgroups (8 bits: waves) that share `all` narrow blocks, of at most `most`, and the first block of number w
+template <bool F8>
 __device__ __forceinline__ int pt_workers(int all, int most) {
-  return max(1, min(most, (all + PT_NARROW_LEAST - 1) / PT_NARROW_LEAST));
+  constexpr int LEAST = F8 ? PT_WAVE_LEAST : PT_NARROW_LEAST;
+  return max(1, min(most, (all + LEAST - 1) / LEAST));
 }
 __device__ __forceinline__ int pt_first(int all, int workers, int w) { return (int)((long long)all * w / workers); }
 
@@ -1079,80 +1082,12 @@ struct PtNarrow {
   static constexpr int OLD = 64 + 4;                                        // output row in LDS (floats)
 };
 
-// Ends a narrow tile: joins its four waves, writes its rows. `odd`: the wave's outputs are not to be used, as where they are
-// not finite.
-template <int DT, int D, bool F8>
-__device__ __forceinline__ void pt_join_waves(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, char* lds,
-                                              float (*ml)[2][32], bool odd) {
-  constexpr int PB = PtNarrow<DT, D, F8>::PB, OLD = PtNarrow<DT, D, F8>::OLD;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.H / a.KVH, rows = it.q.n * G, row0 = it.tile * 32;
-  // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
-  const float l = w.row_sum();
-  if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
-  if (__syncthreads_or(odd || w.bad_output())) {
-    pt_rows<DT, D, F8>(a, it, row0, row0 + wave, min(row0 + 32, rows), 4, it.b0 * PB, it.b1 * PB, (long long)it.slot * 32);
-    __syncthreads();
-    return;
-  }
-  float M = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
-  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - M) * w.c);
-  float* ob = (float*)lds;
-  const int valid = min(32, rows - row0);
-#pragma unroll
-  for (int half = 0; half < D / 64; ++half) {   // dims 64 half .. + 64
-    if (half) __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const pt_f32x16& o = w.o[2 * half + t];
-        float4 v;
-        v.x = o[4 * i] * f, v.y = o[4 * i + 1] * f, v.z = o[4 * i + 2] * f, v.w = o[4 * i + 3] * f;
-        *(float4*)&ob[(wave * 32 + w.fr) * OLD + t * 32 + 8 * i + 4 * w.hi] = v;
-      }
-    __syncthreads();
-    for (int idx = tid; idx < valid * 8; idx += 256) {   // (row, 8 dims)
-      const int ch = idx & 7, r = idx >> 3;
-      float Mr = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Mr = fmaxf(Mr, ml[i][0][r]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        L += ml[i][0][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i][0][r] - Mr) * w.c) * ml[i][1][r];
-      float x[8] = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4* p = (const float4*)&ob[(i * 32 + r) * OLD + 8 * ch];
-        const float4 u = p[0], v = p[1];
-        x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w;
-        x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
-      }
-      if (it.slot >= 0) {
-        float* po = a.part_o + ((long long)it.slot * 32 + r) * D + 64 * half + 8 * ch;
-        *(float4*)po = make_float4(x[0], x[1], x[2], x[3]);
-        *(float4*)(po + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        if (half == 0 && ch == 0) *(float2*)(a.part_ml + ((long long)it.slot * 32 + r) * 2) = make_float2(Mr, L);
-      } else {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const int row = row0 + r, t = row / G;
-        uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + 64 * half + 8 * ch;
-        *(uint4*)out = make_uint4(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv),
-                                  gm_pack2<DT>(x[4] * inv, x[5] * inv), gm_pack2<DT>(x[6] * inv, x[7] * inv));
-      }
-    }
-  }
-  __syncthreads();   // the next item's loads go to the same LDS
-}
-
 template <int DT, int D>
 __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32], int (*slots)[64]) {
   using C = PtNarrow<DT, D>;
-  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG;
+  constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, OLD = C::OLD;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row0 = it.tile * 32;
+  const int G = a.H / a.KVH, rows = it.q.n * G, row0 = it.tile * 32;
   PtWave<DT, D> w;
   const unsigned row_bytes = (unsigned)(2 * a.row_stride);
   char* Kt = lds + wave * 16384;
@@ -1221,21 +1156,78 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
     if (more) load(PtV{}, blk + 4);
     bad = bad_next;
   }
-  pt_join_waves<DT, D, false>(a, it, w, lds, ml, false);
+  // join the four waves: sum over waves of e^(m_w - M) o_w, e^(m_w - M) l_w
+  const float l = w.row_sum();
+  if (w.hi == 0) ml[wave][0][w.fr] = w.m, ml[wave][1][w.fr] = l;
+  if (__syncthreads_or(w.bad_output())) {
+    pt_rows<DT, D>(a, it, row0, row0 + wave, min(row0 + 32, rows), 4, b0 * PB, b1 * PB, (long long)it.slot * 32);
+    __syncthreads();
+    return;
+  }
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, ml[i][0][w.fr]);
+  const float f = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - M) * w.c);
+  float* ob = (float*)lds;
+  const int valid = min(32, rows - row0);
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half) {   // dims 64 half .. + 64
+    if (half) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const pt_f32x16& o = w.o[2 * half + t];
+        float4 v;
+        v.x = o[4 * i] * f, v.y = o[4 * i + 1] * f, v.z = o[4 * i + 2] * f, v.w = o[4 * i + 3] * f;
+        *(float4*)&ob[(wave * 32 + w.fr) * OLD + t * 32 + 8 * i + 4 * w.hi] = v;
+      }
+    __syncthreads();
+    for (int idx = tid; idx < valid * 8; idx += 256) {   // (row, 8 dims)
+      const int ch = idx & 7, r = idx >> 3;
+      float Mr = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Mr = fmaxf(Mr, ml[i][0][r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        L += ml[i][0][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i][0][r] - Mr) * w.c) * ml[i][1][r];
+      float x[8] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4* p = (const float4*)&ob[(i * 32 + r) * OLD + 8 * ch];
+        const float4 u = p[0], v = p[1];
+        x[0] += u.x, x[1] += u.y, x[2] += u.z, x[3] += u.w;
+        x[4] += v.x, x[5] += v.y, x[6] += v.z, x[7] += v.w;
+      }
+      if (it.slot >= 0) {
+        float* po = a.part_o + ((long long)it.slot * 32 + r) * D + 64 * half + 8 * ch;
+        *(float4*)po = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(po + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        if (half == 0 && ch == 0) *(float2*)(a.part_ml + ((long long)it.slot * 32 + r) * 2) = make_float2(Mr, L);
+      } else {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int row = row0 + r, t = row / G;
+        uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t) * a.H + it.h * G + row - t * G) * D + 64 * half + 8 * ch;
+        *(uint4*)out = make_uint4(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv),
+                                  gm_pack2<DT>(x[4] * inv, x[5] * inv), gm_pack2<DT>(x[6] * inv, x[7] * inv));
+      }
+    }
+  }
+  __syncthreads();   // the next item's loads go to the same LDS
 }
 
 // ------------------------------------------------------------------ wide tiles
 
-// Writes a wide tile's rows. `odd`: its outputs are not to be used, as where they are not finite.
+// Writes the rows row0 .. of one wave, of a tile that begins at row tile0: as outputs, or as a part (whose first row is
+// `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite.
 template <int DT, int D, bool F8>
-__device__ __forceinline__ void pt_end_wide(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, bool odd) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.H / a.KVH, rows = it.q.n * G;
-  const int tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
+__device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
+                                       int rows, int p0, int p1, long long part, bool odd) {
+  const int G = a.H / a.KVH;
   const float l = w.row_sum();
   const int row = row0 + w.fr;
-  const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
   if (row0 < rows && (odd || w.bad_output())) {
-    pt_rows<DT, D, F8>(a, it, tile0, row0, min(row0 + 32, rows), 1, it.b0 * 64, it.b1 * 64, part);
+    pt_rows<DT, D, F8>(a, it, tile0, row0, min(row0 + 32, rows), 1, p0, p1, part);
   } else if (row < rows) {
     if (it.slot >= 0) {
       const long long at = part + row - tile0;
@@ -1259,8 +1251,11 @@ __device__ __forceinline__ void pt_end_wide(const PagedAttnArgs& a, const PtItem
                          gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
     }
   }
-  __syncthreads();   // the next item's loads go to the same LDS
 }
+
+// the first row of the wide tiles' parts, behind those of the narrow ones: two per workgroup, or with 8 bits per wave
+template <bool F8>
+__device__ __forceinline__ long long pt_wide_parts(const PagedAttnArgs& a) { return (long long)(F8 ? 8 : 2) * a.grid_narrow * PT_NARROW; }
 
 template <int DT, int D>
 __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
@@ -1326,7 +1321,8 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
     w.template outputs<NB>(Vt, p, s);
   }
-  pt_end_wide<DT, D, false>(a, it, w, false);
+  pt_end<DT, D, false>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<false>(a) + (long long)it.slot * PT_WIDE, false);
+  __syncthreads();   // the next item's loads go to the same LDS
 }
 
 // ------------------------------------------------------------------ pages of 8 bits
@@ -1413,8 +1409,7 @@ __device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, 
 }
 
 template <int DT, int D>
-__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem& it, char* lds, float (*ml)[2][32], int (*slots)[64],
-                                           uint32_t (*powers)[64]) {
+__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64], uint32_t (*powers)[64]) {
   using C = PtNarrow<DT, D, true>;
   constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, TD = D / 32;
   constexpr int LD = NG * LPG;   // loads of a block's K, and of its V
@@ -1458,7 +1453,7 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
     const unsigned char* p = ((lane & 16) ? a.v_scales : a.k_scales) + at + (lane & 3) * 4;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(pw0) : "memory", "m0");
   };
-  int blk = b0 + wave;
+  int blk = b0;
   if (blk < b1) {
     wi = blk / WB;
     cur = pt_window<true>(a, it, wi * 64);
@@ -1474,8 +1469,8 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
   for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
   // positions that the tile's first row has open, and its last
   const int pmin = __builtin_amdgcn_readfirstlane(w.pos), pend = __builtin_amdgcn_readlane(w.pos, 31);
-  for (; blk < b1; blk += 4) {
-    const bool more = blk + 4 < b1;
+  for (; blk < b1; ++blk) {
+    const bool more = blk + 1 < b1;
     const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
     gm_vmcnt<LD>();   // powers and K have landed; V's loads may be on their way
     asm volatile("" ::: "memory");
@@ -1521,9 +1516,9 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's rows and the powers are in registers
     if (more) {
-      bad_next = seek(blk + 4);
-      load_powers(blk + 4);
-      load(PtK{}, blk + 4);
+      bad_next = seek(blk + 1);
+      load_powers(blk + 1);
+      load(PtK{}, blk + 1);
     }
     if (!open) w.template mask<NB>(s, blk * PB, bad);
     w.template softmax<NB>(s);
@@ -1581,10 +1576,11 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
     }
     w.l = sum[0] + sum[1];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) load(PtV{}, blk + 4);
+    if (more) load(PtV{}, blk + 1);
     bad = bad_next;
   }
-  pt_join_waves<DT, D, true>(a, it, w, lds, ml, odd);
+  const int rows = it.q.n * (a.H / a.KVH);
+  pt_end<DT, D, true>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, (long long)it.slot * PT_NARROW, __ballot(odd) != 0ull);
 }
 
 template <int DT, int D>
@@ -1686,7 +1682,8 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& i
     }
     if (blk + 1 < b1) stage(blk + 1);
   }
-  pt_end_wide<DT, D, true>(a, it, w, __syncthreads_or(odd));
+  odd = __syncthreads_or(odd);   // (and the next item's blocks go to the same LDS)
+  pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<true>(a) + (long long)it.slot * PT_WIDE, odd);
 }
 
 // ------------------------------------------------------------------ kernels
@@ -1696,21 +1693,22 @@ template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
   constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
-  __shared__ float ml[4][2][32];
+  __shared__ float ml[F8 ? 1 : 4][2][32];
   __shared__ int ids[4][64];
   __shared__ PtList t;
   __shared__ uint32_t powers[F8 ? 4 : 1][64];
   const int nw = a.grid_wide;
   int x;
   if ((int)blockIdx.x >= nw) {
-    const int hi = nw ? PT_NARROW : ANY, w = blockIdx.x - nw;
-    const int all = pt_build_narrow<NPB>(a, t, hi, &x), workers = pt_workers(all, gridDim.x - nw);
+    const int hi = nw ? PT_NARROW : ANY, per = F8 ? 4 : 1;
+    const int w = (blockIdx.x - nw) * per + (F8 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    const int all = pt_build_narrow<NPB>(a, t, hi, &x), workers = pt_workers<F8>(all, (gridDim.x - nw) * per);
     if (w >= workers) return;
     const int end = pt_first(all, workers, w + 1);
     for (int at = pt_first(all, workers, w); at < end;) {
       PtItem it;
       at = pt_item_narrow<NPB>(a, t, w, at, end, hi, it);
-      if constexpr (F8) pt_narrow8<DT, D>(a, it, lds, ml, ids, powers);
+      if constexpr (F8) pt_narrow8<DT, D>(a, it, lds, ids, powers);
       else pt_narrow<DT, D>(a, it, lds, ml, ids);
     }
     return;
@@ -1732,18 +1730,19 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
   }
 }
 
-// Joins S parts of one row (by a wave): part s lies `rel(s)` slots of R rows after row `first` of the parts.
-template <int DT, int D, int R, typename F>
-__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out) {
+// Adds parts s0 .. s1 - 1 of one row to its maximum, sum and the lane's 4 dims (by a wave): part s lies `rel(s)` slots of R
+// rows after row `first` of the parts. L and x are then the lane's own, to be summed over lanes (pt_gathered).
+template <int D, int R, typename F>
+__device__ __forceinline__ void pt_gather(const PagedAttnArgs& a, long long first, int s0, int s1, F rel, float& M, float& L,
+                                          float (&x)[4]) {
   // a load covers PER parts: lane (part, 4 dims); a batch is eight of them
   constexpr int LN = D / 4, PER = 64 / LN;
   const int lane = threadIdx.x & 63;
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
   const float* mls = a.part_ml + first * 2;
   const float* os = a.part_o + first * D;
-  float M = -INFINITY, L = 0.f, x[4] = {};
-  for (int s0 = 0; s0 < S; s0 += 64) {
-    const int n = min(64, S - s0);
+  for (; s0 < s1; s0 += 64) {
+    const int n = min(64, s1 - s0);
     const float2 ml = *(const float2*)(mls + rel(s0 + min(lane, n - 1)) * R * 2);
     float4 v[8];
     auto fetch = [&](int j) {   // (past the last part: it again, weighed 0)
@@ -1773,13 +1772,60 @@ __device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first,
       }
     }
   }
+}
+// sums over the lanes of a wave: L, and x of the lanes that hold the same dims
+template <int D>
+__device__ __forceinline__ void pt_gathered(float& L, float (&x)[4]) {
   L = wave_sum(L);
 #pragma unroll
-  for (int o = LN; o < 64; o <<= 1)
+  for (int o = D / 4; o < 64; o <<= 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o, 64);
+}
+template <int DT, int D>
+__device__ __forceinline__ void pt_put(uint16_t* out, float L, const float (&x)[4]) {
+  const int lane = threadIdx.x & 63;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  if (lane < LN) *(uint2*)(out + lane * 4) = make_uint2(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv));
+  if (lane < D / 4) *(uint2*)(out + lane * 4) = make_uint2(gm_pack2<DT>(x[0] * inv, x[1] * inv), gm_pack2<DT>(x[2] * inv, x[3] * inv));
+}
+// Joins S parts of one row (by a wave).
+template <int DT, int D, int R, typename F>
+__device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out) {
+  float M = -INFINITY, L = 0.f, x[4] = {};
+  pt_gather<D, R>(a, first, 0, S, rel, M, L, x);
+  pt_gathered<D>(L, x);
+  pt_put<DT, D>(out, L, x);
+}
+// The same by a workgroup, a quarter of the parts a wave. (Ends with a barrier.)
+template <int DT, int D, int R, typename F>
+__device__ __forceinline__ void pt_join4(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out, float (*sh)[4][D / 4 + 2]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
+  float M = -INFINITY, L = 0.f, x[4] = {};
+  pt_gather<D, R>(a, first, S * wave / 4, S * (wave + 1) / 4, rel, M, L, x);
+  pt_gathered<D>(L, x);
+  if (lane < D / 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[wave][e][lane] = x[e];
+  if (lane == 0) sh[wave][0][D / 4] = M, sh[wave][0][D / 4 + 1] = L;
+  __syncthreads();
+  if (wave == 0) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = fmaxf(most, sh[i][0][D / 4]);
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = sh[i][0][D / 4], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
+      L += f * sh[i][0][D / 4 + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += f * sh[i][e][min(lane, D / 4 - 1)];
+    }
+    pt_put<DT, D>(out, L, x);
+  }
+  __syncthreads();
 }
 
 // k_paged_combine: joins the parts of split tiles, a wave per row and head, and zeroes the rows of no sequence.
@@ -1788,13 +1834,16 @@ template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
   constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
   __shared__ PtList t;
+  __shared__ float quarters[F8 ? 4 : 1][4][D / 4 + 2];
   __shared__ int start[PT_MAXB + 1], kv[PT_MAXB];   // (a row looks its sequence up in LDS: from memory it is 1 us)
   for (int b = threadIdx.x; b <= a.B; b += 256) {
     start[b] = a.q_start[b];
     if (b < a.B) kv[b] = a.kv_len[b];
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.H / a.KVH, waves = gridDim.x * 4, me = blockIdx.x * 4 + wave, hi = a.grid_wide ? PT_NARROW : ANY;
+  const int G = a.H / a.KVH, hi = a.grid_wide ? PT_NARROW : ANY;
+  const bool four = F8 && a.join4;   // a workgroup's four waves take the same rows
+  const int waves = four ? gridDim.x : gridDim.x * 4, me = four ? blockIdx.x : blockIdx.x * 4 + wave;
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   // Each wave takes a run of rows and looks up where they lie only where a sequence, head or tile begins: looked up
   // row by row (binary search, divisions) a batch of 7,100 rows takes 18 us rather than 15.
@@ -1820,8 +1869,8 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
     return (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D;
   };
   int rows;
-  const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers(all, a.grid_narrow);
-  int w0 = 0, w1 = 0;   // workgroups that hold the tile's first and last block
+  const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers<F8>(all, (F8 ? 4 : 1) * a.grid_narrow);
+  int w0 = 0, w1 = 0;   // workgroups (8 bits: waves) that hold the tile's first and last block
   runs(
       uniform(rows), [&](int b, int s0, int s1, int kv) { return pt_seq<PT_NARROW, NPB>(a, b, s0, s1, kv, 0, hi); },
       [](int row) { return row % PT_NARROW == 0; },
@@ -1831,9 +1880,13 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
           w0 = uniform((int)((((long long)g0 + 1) * workers - 1) / all));
           w1 = uniform((int)((((long long)g0 + q.blocks) * workers - 1) / all));
         }
-        if (w0 != w1)
-          pt_join<DT, D, PT_NARROW>(a, (long long)2 * w0 * PT_NARROW + row % PT_NARROW, w1 - w0 + 1,
-                                    [](int s) { return 2 * s + (s == 0); }, out(q, h, row));
+        if (w0 == w1) return;
+        const long long first = (long long)2 * w0 * PT_NARROW + row % PT_NARROW;
+        auto rel = [](int s) { return 2 * s + (s == 0); };
+        if constexpr (F8) {
+          if (four) return pt_join4<DT, D, PT_NARROW>(a, first, w1 - w0 + 1, rel, out(q, h, row), quarters);
+        }
+        pt_join<DT, D, PT_NARROW>(a, first, w1 - w0 + 1, rel, out(q, h, row));
       });
   if (a.grid_wide) {
     __syncthreads();
@@ -1844,7 +1897,7 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
         [](int) { return false; },
         [&](int b, const PtSeq& q, int h, int row, bool) {
           const int S = pt_splits(q, share), slot = (b ? uniform(t.slots[b - 1]) : 0) + (h * q.tiles + row / PT_WIDE) * S;
-          pt_join<DT, D, PT_WIDE>(a, (long long)(2 * a.grid_narrow * PT_NARROW) + (long long)slot * PT_WIDE + row % PT_WIDE, S,
+          pt_join<DT, D, PT_WIDE>(a, pt_wide_parts<F8>(a) + (long long)slot * PT_WIDE + row % PT_WIDE, S,
                                   [](int s) { return s; }, out(q, h, row));
         });
   }
@@ -1855,7 +1908,7 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
   for (int row = me; row < a.N; row += waves) {
     if (row >= s0 && row < s1) continue;
     uint4* o = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
-    for (int i = lane; i < a.H * D / 8; i += 64) o[i] = make_uint4(0, 0, 0, 0);
+    for (int i = four ? threadIdx.x : lane; i < a.H * D / 8; i += four ? 256 : 64) o[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
