@@ -783,9 +783,12 @@ struct PtWave {
   // scores of 32 NB positions from Kt; the operands are read eight (D = 64: four) ahead
   template <int NB>
   __device__ __forceinline__ void scores(const char* Kt, pt_f32x16 (&s)[NB]) const {
+    scores_of<NB>([&](int sb, int ks) { return *(const uint4*)(Kt + (sb * 32 + fr) * RB + (((2 * ks + hi) ^ pt_xk<D>(fr)) * 16)); }, s);
+  }
+  template <int NB, typename F>
+  __device__ __forceinline__ void scores_of(F read, pt_f32x16 (&s)[NB]) const {
     constexpr int KS = D / 16;
     uint4 k[KS];
-    auto read = [&](int sb, int ks) { return *(const uint4*)(Kt + (sb * 32 + fr) * RB + (((2 * ks + hi) ^ pt_xk<D>(fr)) * 16)); };
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) k[ks] = read(0, ks);
     __builtin_amdgcn_sched_barrier(0);
@@ -881,8 +884,11 @@ struct PtWave {
   // not, depending on code elsewhere.
   template <int NB>
   __device__ __forceinline__ void outputs(const char* Vt, const uint4 (&p)[2 * NB], const pt_f32x16 (&s)[NB]) {
+    outputs_of<NB>([&](int i) { return vfrag(Vt, i / TD / 2, i / TD % 2, i % TD); }, p, s);
+  }
+  template <int NB, typename F>   // (operand i: of 16 positions i / TD, 32 dims i % TD)
+  __device__ __forceinline__ void outputs_of(F read, const uint4 (&p)[2 * NB], const pt_f32x16 (&s)[NB]) {
     constexpr int N = 2 * NB * TD, EL = NB * 16 / N;
-    auto read = [&](int i) { return vfrag(Vt, i / TD / 2, i / TD % 2, i % TD); };
     uint4 v[4];
     float sum[2] = {l, 0.f};
 #pragma unroll
@@ -1583,36 +1589,35 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
   pt_end<DT, D, true>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, (long long)it.slot * PT_NARROW, __ballot(odd) != 0ull);
 }
 
+// Items item, item + step, ... below `items`. The next item's first block is on its way while the last of the present one is
+// computed, its pages' ids before that.
 template <int DT, int D>
-__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
+__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtList& t, int item, int items, int step, char* lds, int (*slots)[64]) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V, in 16 bits
   constexpr int PCS = D / 64;                                           // 16-byte pieces of a row that a thread takes, of K and of V
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.H / a.KVH, rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
-  const int first = it.q.kv - it.q.n;   // position of token 0
-  const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
-  const int b0 = it.b0, b1 = it.b1;
-  constexpr int WB = 64 / NG;   // blocks of a window
-  PtWindowT<true> cur;
+  constexpr int WB = 64 / NG, TD = D / 32;                              // blocks of a window; output tiles
+  if (item >= items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.H / a.KVH;
   int* ids = slots[wave];
-  int wi = b0 / WB;             // window of cur
+  PtWindowT<true> cur;
+  int wi = 0;                       // window of cur
   unsigned bad = 0, bad_next = 0;   // groups of the present and the next block without a page
-  const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's position
   // A wave converts its group of 16 positions, four lanes a position. LDS takes the writes of 8 lanes at a time, two positions'
   // here: K's swizzle sends those to different banks (D = 64: of positions 0 and 2), for V every other position writes its
   // odd chunk first.
   const int gr = D == 128 ? lane >> 2 : (lane >> 4) << 2 | ((lane >> 2) & 1) << 1 | ((lane >> 3) & 1), part = lane & 3;
   const bool turn = (lane >> 2) & 1;
   const unsigned ko = (unsigned)gr * (unsigned)a.row_stride + part * 16;   // 16-byte pieces part + 4 i of a row
+  // Places in LDS. A swizzle is an exclusive or, so a fragment's place is another's with a constant: one instruction each from
+  // a place that changes with the block, where the compiler would keep thirty in registers (and spill: a reload waits
+  // for the loads in flight). Fragments as PtWave's: chunk 2 ks + hi of K's row fr; of V's, two times four rows, 4 apart.
+  const int fr = lane & 31, hi = lane >> 5, vrow = (lane & 15) >> 2, sr = wave * 16 + gr;
+  const unsigned krd = fr * RB + ((hi ^ pt_xk<D>(fr)) * 16);
+  const unsigned vrd = BYTES + (8 * hi + vrow) * RB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ pt_xv<D>(vrow)) * 16) + (lane & 1) * 8;
+  const unsigned kwr = sr * RB + (((2 * part) ^ pt_xk<D>(sr & 31)) * 16), vwr = BYTES + sr * RB + (((2 * part + turn) ^ pt_xv<D>(sr)) * 16);
   uint4 kr[PCS], vr[PCS];
   unsigned kb = 127, vb = 127;
-  bool odd = false;
-  auto issue = [&](int blk) {
-    if (blk / WB != wi) {
-      ++wi;
-      cur = pt_window<true>(a, it, wi * 64, ids[lane]);
-      pt_fetch(a, it, (wi + 1) * 64, ids);
-    }
+  auto issue = [&](int blk) {   // (a block of the window cur)
     bad_next = ~(unsigned)(cur.ok >> (blk % WB * NG)) & ((1u << NG) - 1);
     const int g = blk % WB * NG + wave;
     const unsigned long long at = pt_place(cur, g);
@@ -1627,63 +1632,99 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtItem& i
     kb = (a.k_scales + sc)[gr], vb = (a.v_scales + sc)[gr];
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto stage = [&](int blk) {   // what issue(blk) loaded, as 16 bits; zeros in the places that are closed to every row
-    char* K = lds + (blk & 1) * 2 * BYTES;
-    const int r = wave * 16 + gr;
-    if (blk * PB + PB - 1 > pend || bad_next) {
-      if (blk * PB + r > pend || ((bad_next >> wave) & 1)) {
-        kb = vb = 127;
-#pragma unroll
-        for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    odd = odd || pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>);
-    const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
-    char *kd = K + r * RB, *vd = K + BYTES + r * RB;
-#pragma unroll
-    for (int i = 0; i < PCS; ++i) {
-      const int c = 2 * (part + 4 * i), d = c + turn;   // chunks of 8 dims
-      const uint4 k = kr[i], v = vr[i];
-      *(uint4*)(kd + ((c ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.x, k.y, kp);
-      *(uint4*)(kd + (((c + 1) ^ pt_xk<D>(r & 31)) * 16)) = pt_widen<DT>(k.z, k.w, kp);
-      *(uint4*)(vd + ((d ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(turn ? v.z : v.x, turn ? v.w : v.y, vp);
-      *(uint4*)(vd + (((d ^ 1) ^ pt_xv<D>(r)) * 16)) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
-    }
+  // page id of the lane's group in the window of an item's first block, and that block's loads
+  auto first_id = [&](const PtItem& x) {
+    return a.table[(long long)x.b * a.M + min(pt_page_of(a, x.b0 / WB * 64), (unsigned)a.M - 1)];
   };
-  if (b0 < b1) {
-    cur = pt_window<true>(a, it, wi * 64);
-    pt_fetch(a, it, (wi + 1) * 64, ids);
-    issue(b0);
-  }
-  PtWave<DT, D> w;
-  w.init(a, it, row0);
+  auto begin = [&](const PtItem& x, int id) {
+    if (x.b0 >= x.b1) return;
+    wi = x.b0 / WB;
+    cur = pt_window<true>(a, x, wi * 64, id);
+    pt_fetch(a, x, (wi + 1) * 64, ids);
+    issue(x.b0);
+  };
+  PtItem it = pt_item_wide(a, t, item);
+  begin(it, first_id(it));
+  for (;;) {
+    const int rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
+    const int first = it.q.kv - it.q.n;   // position of token 0
+    const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
+    const int b0 = it.b0, b1 = it.b1;
+    const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's position
+    bool odd = false;
+    auto stage = [&](int blk) {   // what was loaded, as 16 bits; zeros in the places that are closed to every row
+      if (blk * PB + PB - 1 > pend || bad_next) {
+        if (blk * PB + sr > pend || ((bad_next >> wave) & 1)) {
+          kb = vb = 127;
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
-  if (b0 < b1) stage(b0);
-  // positions that every row of the wave has open, and that any has
-  const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
-  const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
-  for (int blk = b0; blk < b1; ++blk) {
-    bad = bad_next;
-    __syncthreads();   // the block is in LDS, and every wave is done with the other stage
-    if (blk + 1 < b1) issue(blk + 1);
-    if (blk * PB <= pmax) {   // wave-uniform
-      const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
-      const char* Kt = lds + (blk & 1) * 2 * BYTES;
-      pt_f32x16 s[NB];
-      w.template scores<NB>(Kt, s);
-      if (!open) w.template mask<NB>(s, blk * PB, bad);
-      __builtin_amdgcn_s_setprio(1);   // vector instructions first: the other workgroup's matrix instructions run on beside them
-      w.template softmax<NB>(s);
-      uint4 p[2 * NB];
-      w.template pack<NB>(s, p);
-      __builtin_amdgcn_s_setprio(0);
-      w.template outputs<NB>(Kt + BYTES, p, s);
+          for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      odd = odd || pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>);
+      const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
+      const unsigned kat = kwr + (blk & 1) * 2 * BYTES, vat = vwr + (blk & 1) * 2 * BYTES;
+#pragma unroll
+      for (int i = 0; i < PCS; ++i) {
+        const uint4 k = kr[i], v = vr[i];
+        *(uint4*)(lds + (kat ^ (i * 128))) = pt_widen<DT>(k.x, k.y, kp);
+        *(uint4*)(lds + (kat ^ (i * 128 + 16))) = pt_widen<DT>(k.z, k.w, kp);
+        *(uint4*)(lds + (vat ^ (i * 128))) = pt_widen<DT>(turn ? v.z : v.x, turn ? v.w : v.y, vp);
+        *(uint4*)(lds + (vat ^ (i * 128 + 16))) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
+      }
+    };
+    const bool last = item + step >= items;
+    PtItem nx = it;
+    int id = 0;
+    if (!last) {
+      nx = pt_item_wide(a, t, item + step);
+      id = first_id(nx);
     }
-    if (blk + 1 < b1) stage(blk + 1);
+    PtWave<DT, D> w;
+    w.init(a, it, row0);
+    if (b0 < b1) stage(b0);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
+    // positions that every row of the wave has open, and that any has
+    const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
+    const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
+    for (int blk = b0; blk < b1; ++blk) {
+      bad = bad_next;
+      __syncthreads();   // the block is in LDS, and every wave is done with the other stage
+      if (blk + 1 < b1) {
+        if ((blk + 1) / WB != wi) {
+          ++wi;
+          cur = pt_window<true>(a, it, wi * 64, ids[lane]);
+          pt_fetch(a, it, (wi + 1) * 64, ids);
+        }
+        issue(blk + 1);
+      } else if (!last) {
+        begin(nx, id);
+      }
+      if (blk * PB <= pmax) {   // wave-uniform
+        const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
+        const unsigned stage_at = (blk & 1) * 2 * BYTES, kat = krd + stage_at, vat = vrd + stage_at;
+        pt_f32x16 s[NB];
+        w.template scores_of<NB>([&](int sb, int ks) { return *(const uint4*)(lds + (kat ^ (ks * 32)) + sb * 32 * RB); }, s);
+        if (!open) w.template mask<NB>(s, blk * PB, bad);
+        __builtin_amdgcn_s_setprio(1);   // vector instructions first: the other workgroup's matrix instructions run on beside them
+        w.template softmax<NB>(s);
+        uint4 p[2 * NB];
+        w.template pack<NB>(s, p);
+        __builtin_amdgcn_s_setprio(0);
+        w.template outputs_of<NB>([&](int i) {
+          const char* q = lds + i / TD * 16 * RB;
+          const uint2 lo = pt_read_tr(q + (vat ^ (i % TD * 64))), up = pt_read_tr(q + 4 * RB + (vat ^ (i % TD * 64 + 32)));
+          return make_uint4(lo.x, lo.y, up.x, up.y);
+        }, p, s);
+      }
+      if (blk + 1 < b1) stage(blk + 1);
+    }
+    if (b0 >= b1 && !last) begin(nx, id);
+    odd = __syncthreads_or(odd);   // (and the next item's blocks go to the same LDS)
+    pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<true>(a) + (long long)it.slot * PT_WIDE, odd);
+    if (last) return;
+    it = nx, item += step;
   }
-  odd = __syncthreads_or(odd);   // (and the next item's blocks go to the same LDS)
-  pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<true>(a) + (long long)it.slot * PT_WIDE, odd);
 }
 
 // ------------------------------------------------------------------ kernels
@@ -1724,9 +1765,11 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
   };
   const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
-  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) {
-    if constexpr (F8) pt_wide8<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
-    else pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+  const int me = i0 + (blockIdx.x >> 3), step = nw >> 3;
+  if constexpr (F8) {
+    pt_wide8<DT, D>(a, t, me, i1, step, lds, ids);
+  } else {
+    for (int item = me; item < i1; item += step) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
   }
 }
 
