@@ -646,6 +646,7 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   int join4;                  // pages of 8 bits: the combine kernel takes a row by the four waves of a workgroup
   const unsigned char* k_scales;   // pages of 8 bits: exponent + 127 of position r, head h, page p at (p * KVH + h) * page_size + r
   const unsigned char* v_scales;
+  int* joins;                      // [N, H, 2] where the row's parts are: the first one's row, 2 parts + (1: of a wide tile)
 };
 
 struct SampleRow {            // sample.hip: what k_sample_merge finds out about a row

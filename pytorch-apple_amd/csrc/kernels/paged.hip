@@ -626,10 +626,9 @@ __device__ __forceinline__ int pt_build_narrow(const PagedAttnArgs& a, PtList& t
   return total[2] ? 0 : total[0];
 }
 
-// Workgroups (8 bits: waves) that share `all` narrow blocks, of at most `most`, and the first block of number w
-template <bool F8>
+// Workgroups that share `all` narrow blocks, of at most `most`, and the first block of workgroup w
+template <int LEAST = PT_NARROW_LEAST>
 __device__ __forceinline__ int pt_workers(int all, int most) {
-  constexpr int LEAST = F8 ? PT_WAVE_LEAST : PT_NARROW_LEAST;
   return max(1, min(most, (all + LEAST - 1) / LEAST));
 }
 __device__ __forceinline__ int pt_first(int all, int workers, int w) { return (int)((long long)all * w / workers); }
@@ -1226,7 +1225,7 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
 
 // Writes the rows row0 .. of one wave, of a tile that begins at row tile0: as outputs, or as a part (whose first row is
 // `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite.
-template <int DT, int D, bool F8>
+template <int DT, int D, bool F8 = false>
 __device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
                                        int rows, int p0, int p1, long long part, bool odd) {
   const int G = a.H / a.KVH;
@@ -1258,10 +1257,6 @@ __device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it,
     }
   }
 }
-
-// the first row of the wide tiles' parts, behind those of the narrow ones: two per workgroup, or with 8 bits per wave
-template <bool F8>
-__device__ __forceinline__ long long pt_wide_parts(const PagedAttnArgs& a) { return (long long)(F8 ? 8 : 2) * a.grid_narrow * PT_NARROW; }
 
 template <int DT, int D>
 __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
@@ -1327,7 +1322,8 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
     w.template outputs<NB>(Vt, p, s);
   }
-  pt_end<DT, D, false>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<false>(a) + (long long)it.slot * PT_WIDE, false);
+  const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
+  pt_end<DT, D>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, false);
   __syncthreads();   // the next item's loads go to the same LDS
 }
 
@@ -1414,8 +1410,202 @@ __device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, 
   gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
 }
 
+// Work, dealt out in equal ranges to the last block: narrow tiles' blocks to waves, wide tiles' to workgroups. A range begins
+// and ends inside tiles, whose parts its slots 2 w (a part behind another) and 2 w + 1 (a tile's first part) take.
+struct PtItem8 : PtItem {
+  int parts;   // a tile's first part: how many there are. 0: a later one
+};
+
+// A tile's first part tells k_paged_quant_combine where each of its rows' parts are: [first part's row, 2 parts + kind].
+__device__ __forceinline__ void pt_tell(const PagedAttnArgs& a, const PtItem8& it, int row, int rows, long long part, int wide) {
+  const int G = a.H / a.KVH, t = row / G;
+  if (it.parts && row < rows && (threadIdx.x & 63) < 32)
+    ((int2*)a.joins)[(long long)(it.q.start + t) * a.H + it.h * G + row - t * G] = make_int2((int)part, 2 * it.parts + wide);
+}
+
+struct PtList8 {
+  union {
+    int items[PT_MAXB];                  // narrow: running sums of blocks
+    unsigned long long cost[PT_MAXB];    // wide: of costs (pt_cost)
+  };
+  int red[3][4];
+  unsigned long long red64[4];
+};
+
+// Narrow sequences' blocks, as pt_build_narrow.
+__device__ __forceinline__ int pt_build_narrow8(const PagedAttnArgs& a, PtList8& t, int hi) {
+  int total[3] = {0, 0, 0};
+  for (int c = 0; c < a.B; c += 256) {
+    const int b = c + threadIdx.x;
+    int v[3] = {0, 0, 0};
+    if (b < a.B) {
+      const int s0 = a.q_start[b], s1 = a.q_start[b + 1];
+      const PtSeq q = pt_seq<PT_NARROW, 64>(a, b, s0, s1, a.kv_len[b], 0, hi);
+      v[0] = q.tiles * q.blocks * a.KVH;
+      v[1] = s1 < s0;
+    }
+    pt_scan3(v, total, t.red);
+    if (b < a.B) t.items[b] = v[0];
+  }
+  __syncthreads();
+  return total[1] ? 0 : total[0];
+}
+
+// The item of wave w that starts at block `at` of all narrow blocks; `end`: of its range. Returns the next start.
+__device__ __forceinline__ int pt_item_narrow8(const PagedAttnArgs& a, const PtList8& t, int w, int at, int end, int hi, int all,
+                                               int workers, PtItem8& it) {
+  it.b = __builtin_amdgcn_readfirstlane(pt_find(t.items, a.B, at));
+  it.q = pt_seq<PT_NARROW, 64>(a, it.b, pt_ldc(a.q_start, it.b), pt_ldc(a.q_start, it.b + 1), pt_ldc(a.kv_len, it.b), 0, hi);
+  const int i = at - (it.b ? __builtin_amdgcn_readfirstlane(t.items[it.b - 1]) : 0), tl = i / it.q.blocks;
+  it.tile = tl % it.q.tiles, it.h = tl / it.q.tiles;
+  it.b0 = i % it.q.blocks, it.b1 = min(it.q.blocks, it.b0 + end - at);
+  const int next = at + it.b1 - it.b0;
+  const bool split = it.b1 < it.q.blocks;
+  it.slot = it.b0 > 0 ? 2 * w : split ? 2 * w + 1 : -1;
+  // (the wave that holds the tile's last block)
+  it.parts = it.b0 > 0 ? 0 : split ? (int)((((long long)at + it.q.blocks) * workers - 1) / all) - w + 1 : 1;
+  const int seen = pt_seen<PT_NARROW, 64>(a, it.q, it.tile);
+  it.b0 = min(it.b0, seen), it.b1 = min(it.b1, seen);
+  return next;
+}
+
+// What wide tiles cost, in positions times G: tile i of a sequence sees about the positions before its first token and
+// those of (i + 1/2) 128 / G tokens, and begins and ends in the time of two blocks.
+struct PtCost {
+  long long c0, head;   // of tile 0 (tile i: c0 + 128 i), and of all tiles of a K/V head
+  __device__ __forceinline__ PtCost(const PagedAttnArgs& a, const PtSeq& q) {
+    const int G = a.H / a.KVH;
+    c0 = (min((long long)max(q.kv - q.n, 0), (long long)a.M * a.page_size) + 128) * G + 64;
+    head = before(q.tiles);
+  }
+  __device__ __forceinline__ long long before(int i) const { return i * c0 + 64ll * i * (i - 1); }
+};
+
+__device__ __forceinline__ PtSeq pt_wide_seq(const PagedAttnArgs& a, int b) {
+  return pt_seq<PT_WIDE, 64>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), PT_NARROW, 0x7fffffff);
+}
+
+// Wide sequences' costs (by 256 threads; ends with a barrier); returns their sum, 0 where q_start descends.
+__device__ __forceinline__ unsigned long long pt_build_wide8(const PagedAttnArgs& a, PtList8& t) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned long long total = 0;
+  bool down = false;
+  for (int c = 0; c < a.B; c += 256) {
+    const int b = c + tid;
+    unsigned long long v = 0;
+    if (b < a.B) {
+      const int s0 = a.q_start[b], s1 = a.q_start[b + 1];
+      const PtSeq q = pt_seq<PT_WIDE, 64>(a, b, s0, s1, a.kv_len[b], PT_NARROW, 0x7fffffff);
+      down |= s1 < s0;
+      if (q.n) v = (unsigned long long)PtCost(a, q).head * a.KVH;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned long long w = __shfl_up(v, o, 64);
+      if (lane >= o) v += w;
+    }
+    __syncthreads();
+    if (lane == 63) t.red64[wave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v += w < wave ? t.red64[w] : 0;
+    v += total;
+    if (b < a.B) t.cost[b] = v;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) total += t.red64[w];
+  }
+  return __syncthreads_or(down) ? 0 : total;
+}
+
+// A place in the wide tiles' list: block blk of a tile of a K/V head of sequence b (B: the end).
+struct PtCut {
+  int b, h, tile, blk;
+  __device__ __forceinline__ bool in(const PtCut& o) const { return b == o.b && h == o.h && tile == o.tile; }
+};
+struct PtRanges {
+  unsigned long long total;
+  unsigned long long range;   // of a workgroup
+  int workers;
+};
+
+__device__ __forceinline__ unsigned long long pt_cost_at(const PtList8& t, int b) {   // of the sequences up to b
+  if (b < 0) return 0;
+  const unsigned long long v = t.cost[b];
+  return ((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+}
+// the tile behind c's, at its first block
+__device__ __forceinline__ PtCut pt_behind(const PagedAttnArgs& a, const PtList8& t, const PtSeq& q, PtCut c) {
+  c.blk = 0;
+  if (++c.tile < q.tiles) return c;
+  c.tile = 0;
+  if (++c.h < a.KVH) return c;
+  c.h = 0;
+  const unsigned long long here = pt_cost_at(t, c.b);
+  while (++c.b < a.B && pt_cost_at(t, c.b) == here) {
+  }
+  return c;
+}
+// Where workgroup w's range begins. Ranges are of equal cost, but where tiles are short against them one that would begin
+// within an eighth of a range from a tile's border begins there: six prompts of 1,500 tokens have 120 tiles cut in two
+// rather than 480, whose parts would be written and read, for ranges that differ by up to a quarter.
+__device__ __forceinline__ PtCut pt_cut(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w) {
+  if (w >= r.workers) return PtCut{a.B, 0, 0, 0};
+  const unsigned long long x = r.range * w + r.total % r.workers * w / r.workers;
+  int lo = 0, hi = a.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (pt_cost_at(t, mid) > x) hi = mid;
+    else lo = mid + 1;
+  }
+  PtCut c{lo, 0, 0, 0};
+  const PtSeq q = pt_wide_seq(a, c.b);
+  const PtCost k(a, q);
+  long long z = (long long)(x - pt_cost_at(t, c.b - 1));
+  c.h = __builtin_amdgcn_readfirstlane(min((int)((double)z / (double)k.head), a.KVH - 1));
+  while (z < c.h * k.head) --c.h;
+  while (c.h + 1 < a.KVH && z >= (c.h + 1) * k.head) ++c.h;
+  z -= c.h * k.head;
+  const double p = (double)(k.c0 - 64);
+  c.tile = __builtin_amdgcn_readfirstlane(max(0, min((int)((sqrt(p * p + 256.0 * (double)z) - p) * (1.0 / 128.0)), q.tiles - 1)));
+  while (c.tile > 0 && z < k.before(c.tile)) --c.tile;
+  while (c.tile + 1 < q.tiles && z >= k.before(c.tile + 1)) ++c.tile;
+  z -= k.before(c.tile);
+  const int nb = pt_seen<PT_WIDE, 64>(a, q, c.tile), per = 64 * (a.H / a.KVH);
+  const long long range = (long long)r.range / per;   // in blocks
+  c.blk = __builtin_amdgcn_readfirstlane(min((int)((double)nb * (double)z / (double)(k.c0 + 128ll * c.tile)), nb));
+  const int near = nb <= range ? max(1, (int)(range / 8)) : 1;
+  if (c.blk <= near) c.blk = 0;
+  else if (nb - c.blk <= near) c = pt_behind(a, t, q, c);
+  return c;
+}
+
+// The item of workgroup w at c, up to `end` at most; c moves on.
+__device__ __forceinline__ PtItem8 pt_item_wide8(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w, PtCut& c, const PtCut& end) {
+  PtItem8 it;
+  it.b = c.b, it.h = c.h, it.tile = c.tile;
+  it.q = pt_wide_seq(a, c.b);
+  const int nb = pt_seen<PT_WIDE, 64>(a, it.q, it.tile);
+  const bool split = c.in(end) && end.blk < nb;
+  it.b0 = c.blk, it.b1 = split ? end.blk : nb;
+  it.slot = it.b0 > 0 ? 2 * w : split ? 2 * w + 1 : -1;
+  it.parts = it.b0 > 0 ? 0 : 1;
+  if (split && it.b0 == 0) {   // the last workgroup whose range begins inside the tile
+    const PtCost k(a, it.q);
+    const unsigned long long stop = pt_cost_at(t, c.b - 1) + c.h * k.head + k.before(c.tile + 1);
+    int last = (int)min((unsigned long long)r.workers - 1, stop / r.range + 1);
+    for (; last > w + 1; --last) {
+      const PtCut x = pt_cut(a, t, r, last);
+      if (x.in(c) && x.blk > 0) break;
+    }
+    it.parts = last - w + 1;
+  }
+  c = split ? end : pt_behind(a, t, it.q, c);
+  return it;
+}
+
 template <int DT, int D>
-__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64], uint32_t (*powers)[64]) {
+__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8& it, char* lds, int (*slots)[64], uint32_t (*powers)[64]) {
   using C = PtNarrow<DT, D, true>;
   constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, TD = D / 32;
   constexpr int LD = NG * LPG;   // loads of a block's K, and of its V
@@ -1586,18 +1776,29 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem&
     bad = bad_next;
   }
   const int rows = it.q.n * (a.H / a.KVH);
-  pt_end<DT, D, true>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, (long long)it.slot * PT_NARROW, __ballot(odd) != 0ull);
+  const long long part = (long long)it.slot * PT_NARROW;
+  pt_tell(a, it, row0 + w.fr, rows, part + w.fr, 0);
+  pt_end<DT, D, true>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, part, __ballot(odd) != 0ull);
 }
 
-// Items item, item + step, ... below `items`. The next item's first block is on its way while the last of the present one is
-// computed, its pages' ids before that.
+// A workgroup's range of the wide tiles. The next item's first block is on its way while the last of the present one is
+// computed, its pages' ids before that. XCD i (workgroups i, i + 8, ...) takes neighbouring ranges: they read the same blocks.
 template <int DT, int D>
-__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtList& t, int item, int items, int step, char* lds, int (*slots)[64]) {
+__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, char* lds, int (*slots)[64]) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V, in 16 bits
   constexpr int PCS = D / 64;                                           // 16-byte pieces of a row that a thread takes, of K and of V
   constexpr int WB = 64 / NG, TD = D / 32;                              // blocks of a window; output tiles
-  if (item >= items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.H / a.KVH;
+  PtRanges r;
+  r.total = pt_build_wide8(a, t);
+  r.workers = (int)max(1ull, min((unsigned long long)a.grid_wide, r.total / (PT_WIDE_LEAST * PB * G)));
+  r.range = r.total / r.workers;
+  const int each = (r.workers + 7) >> 3, me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if (r.total == 0 || (int)(blockIdx.x >> 3) >= each || me >= r.workers) return;
+  PtCut at = pt_cut(a, t, r, me);
+  const PtCut end = pt_cut(a, t, r, me + 1);
+  auto done = [&]() { return at.in(end) && at.blk == end.blk; };
+  if (done() && at.blk == 0) return;   // (inside a tile: an empty part, since the others count it)
   int* ids = slots[wave];
   PtWindowT<true> cur;
   int wi = 0;                       // window of cur
@@ -1643,7 +1844,7 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtList& t
     pt_fetch(a, x, (wi + 1) * 64, ids);
     issue(x.b0);
   };
-  PtItem it = pt_item_wide(a, t, item);
+  PtItem8 it = pt_item_wide8(a, t, r, me, at, end);
   begin(it, first_id(it));
   for (;;) {
     const int rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
@@ -1672,11 +1873,11 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtList& t
         *(uint4*)(lds + (vat ^ (i * 128 + 16))) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
       }
     };
-    const bool last = item + step >= items;
-    PtItem nx = it;
+    const bool last = done();
+    PtItem8 nx = it;
     int id = 0;
     if (!last) {
-      nx = pt_item_wide(a, t, item + step);
+      nx = pt_item_wide8(a, t, r, me, at, end);
       id = first_id(nx);
     }
     PtWave<DT, D> w;
@@ -1721,36 +1922,35 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, const PtList& t
     }
     if (b0 >= b1 && !last) begin(nx, id);
     odd = __syncthreads_or(odd);   // (and the next item's blocks go to the same LDS)
-    pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, pt_wide_parts<true>(a) + (long long)it.slot * PT_WIDE, odd);
+    const long long part = (long long)8 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;   // (behind the narrow tiles')
+    pt_tell(a, it, row0 + w.fr, rows, part + row0 + w.fr - tile0, 1);
+    pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, odd);
     if (last) return;
-    it = nx, item += step;
+    it = nx;
   }
 }
 
 // ------------------------------------------------------------------ kernels
 
 // grid_wide = 0: sequences of any number of rows on narrow tiles (batches that are nearly all single tokens)
-template <int DT, int D, bool F8 = false>
+template <int DT, int D>
 __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
-  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
-  __shared__ float ml[F8 ? 1 : 4][2][32];
+  __shared__ float ml[4][2][32];
   __shared__ int ids[4][64];
   __shared__ PtList t;
-  __shared__ uint32_t powers[F8 ? 4 : 1][64];
   const int nw = a.grid_wide;
   int x;
   if ((int)blockIdx.x >= nw) {
-    const int hi = nw ? PT_NARROW : ANY, per = F8 ? 4 : 1;
-    const int w = (blockIdx.x - nw) * per + (F8 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-    const int all = pt_build_narrow<NPB>(a, t, hi, &x), workers = pt_workers<F8>(all, (gridDim.x - nw) * per);
+    const int hi = nw ? PT_NARROW : ANY, w = blockIdx.x - nw;
+    const int all = pt_build_narrow<NPB>(a, t, hi, &x), workers = pt_workers(all, gridDim.x - nw);
     if (w >= workers) return;
     const int end = pt_first(all, workers, w + 1);
     for (int at = pt_first(all, workers, w); at < end;) {
       PtItem it;
       at = pt_item_narrow<NPB>(a, t, w, at, end, hi, it);
-      if constexpr (F8) pt_narrow8<DT, D>(a, it, lds, ids, powers);
-      else pt_narrow<DT, D>(a, it, lds, ml, ids);
+      pt_narrow<DT, D>(a, it, lds, ml, ids);
     }
     return;
   }
@@ -1765,11 +1965,30 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
     return ci ? i0 + (int)((long long)(at - c0) * ii / ci) : i0;
   };
   const int xcd = blockIdx.x & 7, i0 = bound(xcd), i1 = bound(xcd + 1);
-  const int me = i0 + (blockIdx.x >> 3), step = nw >> 3;
-  if constexpr (F8) {
-    pt_wide8<DT, D>(a, t, me, i1, step, lds, ids);
-  } else {
-    for (int item = me; item < i1; item += step) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+  for (int item = i0 + (blockIdx.x >> 3); item < i1; item += nw >> 3) pt_wide<DT, D>(a, pt_item_wide(a, t, item), lds, ids);
+}
+
+// Over pages of 8 bits: wide tiles' workgroups first, then the narrow ones', each wave of which takes blocks of its own.
+template <int DT, int D>
+__device__ __forceinline__ void pt_attn8_body(const PagedAttnArgs& a) {
+  constexpr int ANY = 0x7fffffff;
+  __shared__ __attribute__((aligned(1024))) char lds[65536];
+  __shared__ int ids[4][64];
+  __shared__ uint32_t powers[4][64];
+  __shared__ PtList8 t;
+  const int nw = a.grid_wide;
+  if ((int)blockIdx.x < nw) {
+    pt_wide8<DT, D>(a, t, lds, ids);
+    return;
+  }
+  const int hi = nw ? PT_NARROW : ANY, w = (blockIdx.x - nw) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all = pt_build_narrow8(a, t, hi), workers = pt_workers<PT_WAVE_LEAST>(all, (gridDim.x - nw) * 4);
+  if (w >= workers) return;
+  const int end = pt_first(all, workers, w + 1);
+  for (int at = pt_first(all, workers, w); at < end;) {
+    PtItem8 it;
+    at = pt_item_narrow8(a, t, w, at, end, hi, all, workers, it);
+    pt_narrow8<DT, D>(a, it, lds, ids, powers);
   }
 }
 
@@ -1839,54 +2058,19 @@ __device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first,
   pt_gathered<D>(L, x);
   pt_put<DT, D>(out, L, x);
 }
-// The same by a workgroup, a quarter of the parts a wave. (Ends with a barrier.)
-template <int DT, int D, int R, typename F>
-__device__ __forceinline__ void pt_join4(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out, float (*sh)[4][D / 4 + 2]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
-  float M = -INFINITY, L = 0.f, x[4] = {};
-  pt_gather<D, R>(a, first, S * wave / 4, S * (wave + 1) / 4, rel, M, L, x);
-  pt_gathered<D>(L, x);
-  if (lane < D / 4)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sh[wave][e][lane] = x[e];
-  if (lane == 0) sh[wave][0][D / 4] = M, sh[wave][0][D / 4 + 1] = L;
-  __syncthreads();
-  if (wave == 0) {
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) most = fmaxf(most, sh[i][0][D / 4]);
-    L = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float m = sh[i][0][D / 4], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
-      L += f * sh[i][0][D / 4 + 1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += f * sh[i][e][min(lane, D / 4 - 1)];
-    }
-    pt_put<DT, D>(out, L, x);
-  }
-  __syncthreads();
-}
-
 // k_paged_combine: joins the parts of split tiles, a wave per row and head, and zeroes the rows of no sequence.
 // (A part without open positions has maximum -inf and outputs of zero.)
-template <int DT, int D, bool F8 = false>
+template <int DT, int D>
 __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
-  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D, F8>::PB;
+  constexpr int ANY = 0x7fffffff, NPB = PtNarrow<DT, D>::PB;
   __shared__ PtList t;
-  __shared__ float quarters[F8 ? 4 : 1][4][D / 4 + 2];
   __shared__ int start[PT_MAXB + 1], kv[PT_MAXB];   // (a row looks its sequence up in LDS: from memory it is 1 us)
   for (int b = threadIdx.x; b <= a.B; b += 256) {
     start[b] = a.q_start[b];
     if (b < a.B) kv[b] = a.kv_len[b];
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.H / a.KVH, hi = a.grid_wide ? PT_NARROW : ANY;
-  const bool four = F8 && a.join4;   // a workgroup's four waves take the same rows
-  const int waves = four ? gridDim.x : gridDim.x * 4, me = four ? blockIdx.x : blockIdx.x * 4 + wave;
+  const int G = a.H / a.KVH, waves = gridDim.x * 4, me = blockIdx.x * 4 + wave, hi = a.grid_wide ? PT_NARROW : ANY;
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   // Each wave takes a run of rows and looks up where they lie only where a sequence, head or tile begins: looked up
   // row by row (binary search, divisions) a batch of 7,100 rows takes 18 us rather than 15.
@@ -1912,8 +2096,8 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
     return (uint16_t*)a.out + ((long long)(q.start + tk) * a.H + h * G + row - tk * G) * D;
   };
   int rows;
-  const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers<F8>(all, (F8 ? 4 : 1) * a.grid_narrow);
-  int w0 = 0, w1 = 0;   // workgroups (8 bits: waves) that hold the tile's first and last block
+  const int all = pt_build_narrow<NPB>(a, t, hi, &rows), workers = pt_workers(all, a.grid_narrow);
+  int w0 = 0, w1 = 0;   // workgroups that hold the tile's first and last block
   runs(
       uniform(rows), [&](int b, int s0, int s1, int kv) { return pt_seq<PT_NARROW, NPB>(a, b, s0, s1, kv, 0, hi); },
       [](int row) { return row % PT_NARROW == 0; },
@@ -1923,13 +2107,9 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
           w0 = uniform((int)((((long long)g0 + 1) * workers - 1) / all));
           w1 = uniform((int)((((long long)g0 + q.blocks) * workers - 1) / all));
         }
-        if (w0 == w1) return;
-        const long long first = (long long)2 * w0 * PT_NARROW + row % PT_NARROW;
-        auto rel = [](int s) { return 2 * s + (s == 0); };
-        if constexpr (F8) {
-          if (four) return pt_join4<DT, D, PT_NARROW>(a, first, w1 - w0 + 1, rel, out(q, h, row), quarters);
-        }
-        pt_join<DT, D, PT_NARROW>(a, first, w1 - w0 + 1, rel, out(q, h, row));
+        if (w0 != w1)
+          pt_join<DT, D, PT_NARROW>(a, (long long)2 * w0 * PT_NARROW + row % PT_NARROW, w1 - w0 + 1,
+                                    [](int s) { return 2 * s + (s == 0); }, out(q, h, row));
       });
   if (a.grid_wide) {
     __syncthreads();
@@ -1940,7 +2120,7 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
         [](int) { return false; },
         [&](int b, const PtSeq& q, int h, int row, bool) {
           const int S = pt_splits(q, share), slot = (b ? uniform(t.slots[b - 1]) : 0) + (h * q.tiles + row / PT_WIDE) * S;
-          pt_join<DT, D, PT_WIDE>(a, pt_wide_parts<F8>(a) + (long long)slot * PT_WIDE + row % PT_WIDE, S,
+          pt_join<DT, D, PT_WIDE>(a, (long long)(2 * a.grid_narrow * PT_NARROW) + (long long)slot * PT_WIDE + row % PT_WIDE, S,
                                   [](int s) { return s; }, out(q, h, row));
         });
   }
@@ -1951,17 +2131,116 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
   for (int row = me; row < a.N; row += waves) {
     if (row >= s0 && row < s1) continue;
     uint4* o = (uint4*)((uint16_t*)a.out + (long long)row * a.H * D);
-    for (int i = four ? threadIdx.x : lane; i < a.H * D / 8; i += four ? 256 : 64) o[i] = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < a.H * D / 8; i += 64) o[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-#define PT_KERNELS(NAME, DT, D, F8)                                                                                               \
-  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_##NAME##_d##D(const PagedAttnArgs a) { pt_attn_body<DT, D, F8>(a); }
-#define PT_COMBINES(NAME, DT, D, F8)                                                                                              \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_d##D(const PagedAttnArgs a) { pt_combine_body<DT, D, F8>(a); }
-#define PT_ALL(M, NAME)                                                                                                           \
-  M(NAME##_bf16, HS_BF16, 128, false) M(NAME##_bf16, HS_BF16, 64, false) M(NAME##_f16, HS_F16, 128, false) M(NAME##_f16, HS_F16, 64, false) \
-  M(quant_##NAME##_bf16, HS_BF16, 128, true) M(quant_##NAME##_bf16, HS_BF16, 64, true) M(quant_##NAME##_f16, HS_F16, 128, true)   \
-  M(quant_##NAME##_f16, HS_F16, 64, true)
-PT_ALL(PT_KERNELS, attn)
-PT_ALL(PT_COMBINES, combine)
+// k_paged_quant_combine: the same over pages of 8 bits. What a row is joined of stands in a.joins, where the wave (workgroup)
+// that began its tile has put it: nothing is looked up, where doing so again took 2 to 3 of 6 us. Rows are D / 4 lanes each,
+// so a wave has the loads of several rows in flight at once; with a.join4 a workgroup's waves take a quarter of a row's
+// parts each (few rows over long caches: 256 parts a row took 9.3 us by one wave a row).
+template <int DT, int D>
+__device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
+  constexpr int LN = D / 4, PER = 64 / LN;
+  __shared__ float quarters[4][4][LN + 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LN;
+  const int s0 = a.q_start[0], s1 = a.q_start[a.B], rows = a.N * a.H;
+  const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
+  const bool none = pg_descends(a.q_start, a.B, lane);   // no batch: every row is zero
+  auto far = [&](const int2 j, int s) { return s ? (2 * s - 1) * (j.y & 1 ? PT_WIDE : PT_NARROW) : 0; };   // rows from the first part's
+  auto zero = [&](int u) {
+    const int row = u / a.H;
+    return none || row < s0 || row >= s1;
+  };
+  uint16_t* out = (uint16_t*)a.out;
+  if (a.join4) {
+    for (int u = blockIdx.x; u < rows; u += gridDim.x) {
+      if (zero(u)) {
+        if (threadIdx.x < D / 4) *(uint2*)(out + (long long)u * D + threadIdx.x * 4) = make_uint2(0, 0);
+        continue;
+      }
+      const int2 j = ((const int2*)a.joins)[u];
+      const int S = j.y >> 1;
+      if (S < 2) continue;
+      float M = -INFINITY, L = 0.f, x[4] = {};
+      pt_gather<D, 1>(a, j.x, S * wave / 4, S * (wave + 1) / 4, [&](int s) { return far(j, s); }, M, L, x);
+      pt_gathered<D>(L, x);
+      if (lane < LN)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) quarters[wave][e][lane] = x[e];
+      if (lane == 0) quarters[wave][0][LN] = M, quarters[wave][0][LN + 1] = L;
+      __syncthreads();
+      if (wave == 0) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, quarters[i][0][LN]);
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float m = quarters[i][0][LN], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
+          L += f * quarters[i][0][LN + 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] += f * quarters[i][e][sub];
+        }
+        pt_put<DT, D>(out + (long long)u * D, L, x);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  const int step = gridDim.x * 4 * PER;
+  for (int u0 = (blockIdx.x * 4 + wave) * PER; u0 < rows; u0 += step) {
+    const int u = u0 + lane / LN;
+    if (u >= rows) continue;
+    uint2* to = (uint2*)(out + (long long)u * D) + sub;
+    if (zero(u)) {
+      *to = make_uint2(0, 0);
+      continue;
+    }
+    const int2 j = ((const int2*)a.joins)[u];
+    const int S = j.y >> 1;
+    if (S < 2) continue;
+    const float2* mls = (const float2*)a.part_ml + j.x;
+    const float4* os = (const float4*)(a.part_o + (long long)j.x * D) + sub;
+    float M = -INFINITY, L = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < S; p += 8) {
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p + i < S) {
+          const long long at = far(j, p + i);
+          ml[i] = mls[at];
+          v[i] = os[at * LN];
+        }
+      float most = M;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p + i < S) most = fmaxf(most, ml[i].x);
+      const float old = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - most) * c);
+      M = most, L *= old, x.x *= old, x.y *= old, x.z *= old, x.w *= old;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p + i < S) {
+          const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - most) * c);
+          L = fmaf(f, ml[i].y, L);
+          x.x = fmaf(f, v[i].x, x.x), x.y = fmaf(f, v[i].y, x.y), x.z = fmaf(f, v[i].z, x.z), x.w = fmaf(f, v[i].w, x.w);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *to = make_uint2(gm_pack2<DT>(x.x * inv, x.y * inv), gm_pack2<DT>(x.z * inv, x.w * inv));
+  }
+}
+
+#define PT_KERNELS(NAME, DT, D)                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_##NAME(const PagedAttnArgs a) { pt_attn_body<DT, D>(a); }     \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_combine_##NAME(const PagedAttnArgs a) { pt_combine_body<DT, D>(a); }  \
+  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_quant_attn_##NAME(const PagedAttnArgs a) { pt_attn8_body<DT, D>(a); } \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_quant_combine_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D>(a); }
+PT_KERNELS(bf16_d128, HS_BF16, 128)
+PT_KERNELS(bf16_d64, HS_BF16, 64)
+PT_KERNELS(f16_d128, HS_F16, 128)
+PT_KERNELS(f16_d64, HS_F16, 64)

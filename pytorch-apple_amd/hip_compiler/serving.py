@@ -175,7 +175,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
                 scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
-                grid_narrow=0, join4=0, k_scales=ks, v_scales=vs)
+                grid_narrow=0, join4=0, k_scales=ks, v_scales=vs, joins=None)
     params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
     ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
     prefix = "k_paged_quant_" if quant else "k_paged_"
@@ -185,19 +185,23 @@ def lower_paged_attention(low, node: OpNode) -> None:
         return
     params["pieces16"] = ["q", "k_pages", "v_pages"] + (["k_scales", "v_scales"] if quant else [])
     groups = ps // 16
-    part_rows = (8 if quant else 2) * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
-    join4 = int(quant and not tiled["grid_wide"] and N * H <= PT_JOIN4_ROWS)
+    # (8 bits: two parts a wave and a wide tile's workgroup, else two a workgroup and wide_slots)
+    part_rows = 2 * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
+    if quant:
+        part_rows = 8 * tiled["grid_narrow"] * PT_NARROW + 2 * tiled["grid_wide"] * PT_WIDE
+    join4 = int(quant and N * H <= PT_JOIN4_ROWS)
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
                 part_ml=low.scratch(outs[0] + ".part_ml", 8 * part_rows), page_groups=groups,
                 group_magic=0 if groups == 1 else -(-2 ** 32 // groups), grid_wide=tiled["grid_wide"],
-                grid_narrow=tiled["grid_narrow"], join4=join4)
+                grid_narrow=tiled["grid_narrow"], join4=join4, joins=low.scratch(outs[0] + ".joins", 8 * N * H) if quant else None)
     name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
         kind="paged_attention", kernel=prefix + "attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
         grid=(tiled["grid_wide"] + tiled["grid_narrow"], 1, 1), inputs=ins, outputs=outs, params={**params, "mfma": True}))
+    rows_each = 1 if join4 else 4 * 64 // (D // 4) if quant else 4   # of a workgroup
     low.emit(LaunchStep(
         kind="paged_attention", kernel=prefix + "combine_" + name, module="paged", arg_struct="PagedAttnArgs",
-        args=dict(args), grid=(min(1024, N * H if join4 else -(-N * H // 4)), 1, 1), inputs=ins, outputs=outs, params=params))
+        args=dict(args), grid=(min(2048 if quant else 1024, -(-N * H // rows_each)), 1, 1), inputs=ins, outputs=outs, params=params))
 
 
 def lower_sample(low, node: OpNode) -> None:
