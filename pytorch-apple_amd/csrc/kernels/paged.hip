@@ -759,18 +759,26 @@ struct PtWave {
   // F8: the queries in the order in which a narrow tile reads K, 16 dims of a position at a time
   template <bool F8 = false>
   __device__ __forceinline__ void init(const PagedAttnArgs& a, const PtItem& it, int row0) {
+    queries<F8>(a, it, row0);
+    begin(a, it, row0);
+  }
+  template <bool F8 = false>
+  __device__ __forceinline__ void queries(const PagedAttnArgs& a, const PtItem& it, int row0) {
+    const int ln = threadIdx.x & 63, half = ln >> 5;
+    const int G = a.H / a.KVH, rows = it.q.n * G, r = min(row0 + (ln & 31), rows - 1), t = r / G;
+    const uint16_t* p = (const uint16_t*)a.q + (long long)(it.q.start + t) * a.q_rs + (long long)(it.h * G + r - t * G) * a.q_hs;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const uint4*)(p + (F8 ? ks / 2 * 32 + half * 16 + ks % 2 * 8 : ks * 16 + half * 8));
+  }
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PtItem& it, int row0) {
     lane = threadIdx.x & 63, fr = lane & 31, hi = lane >> 5;
     const int G = a.H / a.KVH, rows = it.q.n * G, r = min(row0 + fr, rows - 1), t = r / G;
     pos = it.q.kv - it.q.n + t;
     const long long last = (long long)a.M * a.page_size - 1;
     pos = pos > last ? (int)last : pos;
-    const uint16_t* p = (const uint16_t*)a.q + (long long)(it.q.start + t) * a.q_rs + (long long)(it.h * G + r - t * G) * a.q_hs;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;   // a negative scale: of -q
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      uint4 v = *(const uint4*)(p + (F8 ? ks / 2 * 32 + hi * 16 + ks % 2 * 8 : ks * 16 + hi * 8));
-      qf[ks] = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-    }
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = make_uint4(qf[ks].x ^ flip, qf[ks].y ^ flip, qf[ks].z ^ flip, qf[ks].w ^ flip);
 #pragma unroll
     for (int t2 = 0; t2 < TD; ++t2)
 #pragma unroll
@@ -1481,10 +1489,6 @@ struct PtCost {
   __device__ __forceinline__ long long before(int i) const { return i * c0 + 64ll * i * (i - 1); }
 };
 
-__device__ __forceinline__ PtSeq pt_wide_seq(const PagedAttnArgs& a, int b) {
-  return pt_seq<PT_WIDE, 64>(a, b, pt_ldc(a.q_start, b), pt_ldc(a.q_start, b + 1), pt_ldc(a.kv_len, b), PT_NARROW, 0x7fffffff);
-}
-
 // Wide sequences' costs (by 256 threads; ends with a barrier); returns their sum, 0 where q_start descends.
 __device__ __forceinline__ unsigned long long pt_build_wide8(const PagedAttnArgs& a, PtList8& t) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1528,16 +1532,11 @@ struct PtRanges {
   int workers;
 };
 
-__device__ __forceinline__ unsigned long long pt_cost_at(const PtList8& t, int b) {   // of the sequences up to b
-  if (b < 0) return 0;
-  const unsigned long long v = t.cost[b];
-  return ((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-}
+__device__ __forceinline__ unsigned long long pt_cost_at(const PtList8& t, int b) { return b < 0 ? 0 : t.cost[b]; }   // of the sequences up to b
 // the tile behind c's, at its first block
-__device__ __forceinline__ PtCut pt_behind(const PagedAttnArgs& a, const PtList8& t, const PtSeq& q, PtCut c) {
+__device__ __forceinline__ PtCut pt_behind(const PagedAttnArgs& a, const PtList8& t, int tiles, PtCut c) {
   c.blk = 0;
-  if (++c.tile < q.tiles) return c;
+  if (++c.tile < tiles) return c;
   c.tile = 0;
   if (++c.h < a.KVH) return c;
   c.h = 0;
@@ -1546,9 +1545,9 @@ __device__ __forceinline__ PtCut pt_behind(const PagedAttnArgs& a, const PtList8
   }
   return c;
 }
-// Where workgroup w's range begins. Ranges are of equal cost, but where tiles are short against them one that would begin
-// within an eighth of a range from a tile's border begins there: six prompts of 1,500 tokens have 120 tiles cut in two
-// rather than 480, whose parts would be written and read, for ranges that differ by up to a quarter.
+// Where workgroup w's range begins; a lane each may ask for another w. Ranges are of equal cost, but where tiles are short
+// against them one that would begin within an eighth of a range from a tile's border begins there: six prompts of 1,500
+// tokens so have 120 tiles cut in two rather than 480, whose parts would be written and read again.
 __device__ __forceinline__ PtCut pt_cut(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w) {
   if (w >= r.workers) return PtCut{a.B, 0, 0, 0};
   const unsigned long long x = r.range * w + r.total % r.workers * w / r.workers;
@@ -1559,48 +1558,66 @@ __device__ __forceinline__ PtCut pt_cut(const PagedAttnArgs& a, const PtList8& t
     else lo = mid + 1;
   }
   PtCut c{lo, 0, 0, 0};
-  const PtSeq q = pt_wide_seq(a, c.b);
+  const PtSeq q = pt_seq<PT_WIDE, 64>(a, lo, a.q_start[lo], a.q_start[lo + 1], a.kv_len[lo], PT_NARROW, 0x7fffffff);
   const PtCost k(a, q);
-  long long z = (long long)(x - pt_cost_at(t, c.b - 1));
-  c.h = __builtin_amdgcn_readfirstlane(min((int)((double)z / (double)k.head), a.KVH - 1));
+  long long z = (long long)(x - pt_cost_at(t, lo - 1));
+  c.h = min((int)((double)z / (double)k.head), a.KVH - 1);
   while (z < c.h * k.head) --c.h;
   while (c.h + 1 < a.KVH && z >= (c.h + 1) * k.head) ++c.h;
   z -= c.h * k.head;
   const double p = (double)(k.c0 - 64);
-  c.tile = __builtin_amdgcn_readfirstlane(max(0, min((int)((sqrt(p * p + 256.0 * (double)z) - p) * (1.0 / 128.0)), q.tiles - 1)));
+  c.tile = max(0, min((int)((sqrt(p * p + 256.0 * (double)z) - p) * (1.0 / 128.0)), q.tiles - 1));
   while (c.tile > 0 && z < k.before(c.tile)) --c.tile;
   while (c.tile + 1 < q.tiles && z >= k.before(c.tile + 1)) ++c.tile;
   z -= k.before(c.tile);
   const int nb = pt_seen<PT_WIDE, 64>(a, q, c.tile), per = 64 * (a.H / a.KVH);
-  const long long range = (long long)r.range / per;   // in blocks
-  c.blk = __builtin_amdgcn_readfirstlane(min((int)((double)nb * (double)z / (double)(k.c0 + 128ll * c.tile)), nb));
-  const int near = nb <= range ? max(1, (int)(range / 8)) : 1;
+  const int range = (int)min(r.range / per, 1ull << 30);   // in blocks
+  c.blk = min((int)((double)nb * (double)z / (double)(k.c0 + 128ll * c.tile)), nb);
+  const int near = nb <= range ? max(1, range / 8) : 1;
   if (c.blk <= near) c.blk = 0;
-  else if (nb - c.blk <= near) c = pt_behind(a, t, q, c);
+  else if (nb - c.blk <= near) c = pt_behind(a, t, q.tiles, c);
   return c;
 }
+__device__ __forceinline__ PtCut pt_cut_of(const PtCut& c, int lane) {
+  return PtCut{__builtin_amdgcn_readlane(c.b, lane), __builtin_amdgcn_readlane(c.h, lane), __builtin_amdgcn_readlane(c.tile, lane),
+               __builtin_amdgcn_readlane(c.blk, lane)};
+}
 
-// The item of workgroup w at c, up to `end` at most; c moves on.
-__device__ __forceinline__ PtItem8 pt_item_wide8(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w, PtCut& c, const PtCut& end) {
-  PtItem8 it;
-  it.b = c.b, it.h = c.h, it.tile = c.tile;
-  it.q = pt_wide_seq(a, c.b);
-  const int nb = pt_seen<PT_WIDE, 64>(a, it.q, it.tile);
-  const bool split = c.in(end) && end.blk < nb;
-  it.b0 = c.blk, it.b1 = split ? end.blk : nb;
-  it.slot = it.b0 > 0 ? 2 * w : split ? 2 * w + 1 : -1;
-  it.parts = it.b0 > 0 ? 0 : 1;
-  if (split && it.b0 == 0) {   // the last workgroup whose range begins inside the tile
-    const PtCost k(a, it.q);
-    const unsigned long long stop = pt_cost_at(t, c.b - 1) + c.h * k.head + k.before(c.tile + 1);
-    int last = (int)min((unsigned long long)r.workers - 1, stop / r.range + 1);
-    for (; last > w + 1; --last) {
-      const PtCut x = pt_cut(a, t, r, last);
-      if (x.in(c) && x.blk > 0) break;
-    }
-    it.parts = last - w + 1;
+// Workgroup w's range, and how many begin inside the tile inside which it ends.
+struct PtRange {
+  PtCut at, end;
+  int inside;
+  __device__ __forceinline__ bool done() const { return at.in(end) && at.blk == end.blk; }
+};
+__device__ __forceinline__ PtRange pt_range(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w) {
+  const int lane = threadIdx.x & 63;
+  PtCut c = pt_cut(a, t, r, w + lane);
+  PtRange g{pt_cut_of(c, 0), pt_cut_of(c, 1), 0};
+  if (g.end.blk == 0) return g;
+  for (int base = w;; base += 64) {   // (they follow each other)
+    const int n = __popcll(__ballot(c.in(g.end) && c.blk > 0 && base + lane > w));
+    g.inside += n;
+    if (__builtin_amdgcn_readlane(c.in(g.end) ? 1 : 0, 63) == 0) return g;
+    c = pt_cut(a, t, r, base + 64 + lane);
   }
-  c = split ? end : pt_behind(a, t, it.q, c);
+}
+
+// The item of workgroup w at its range's place, which moves on.
+__device__ __forceinline__ PtItem8 pt_item_wide8(const PagedAttnArgs& a, const PtList8& t, int w, PtRange& g) {
+  PtItem8 it;
+  it.b = g.at.b, it.h = g.at.h, it.tile = g.at.tile;
+  it.q = pt_seq<PT_WIDE, 64>(a, it.b, pt_ldc(a.q_start, it.b), pt_ldc(a.q_start, it.b + 1), pt_ldc(a.kv_len, it.b), PT_NARROW, 0x7fffffff);
+  const int nb = pt_seen<PT_WIDE, 64>(a, it.q, it.tile);
+  const bool split = g.at.in(g.end);   // (the end of a range is its tile's first block, or one inside)
+  it.b0 = g.at.blk, it.b1 = split ? g.end.blk : nb;
+  it.slot = it.b0 > 0 ? 2 * w : split ? 2 * w + 1 : -1;
+  it.parts = it.b0 > 0 ? 0 : split ? g.inside + 1 : 1;
+  if (split) {
+    g.at = g.end;
+  } else {
+    const PtCut c = pt_behind(a, t, it.q.tiles, g.at);
+    g.at = PtCut{__builtin_amdgcn_readfirstlane(c.b), c.h, c.tile, 0};
+  }
   return it;
 }
 
@@ -1795,10 +1812,8 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
   r.range = r.total / r.workers;
   const int each = (r.workers + 7) >> 3, me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
   if (r.total == 0 || (int)(blockIdx.x >> 3) >= each || me >= r.workers) return;
-  PtCut at = pt_cut(a, t, r, me);
-  const PtCut end = pt_cut(a, t, r, me + 1);
-  auto done = [&]() { return at.in(end) && at.blk == end.blk; };
-  if (done() && at.blk == 0) return;   // (inside a tile: an empty part, since the others count it)
+  PtRange range = pt_range(a, t, r, me);
+  if (range.done() && range.at.blk == 0) return;   // (inside a tile: an empty part, since the others count it)
   int* ids = slots[wave];
   PtWindowT<true> cur;
   int wi = 0;                       // window of cur
@@ -1844,54 +1859,63 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
     pt_fetch(a, x, (wi + 1) * 64, ids);
     issue(x.b0);
   };
-  PtItem8 it = pt_item_wide8(a, t, r, me, at, end);
+  int st = 0;   // LDS stage of the present block
+  // what was loaded, as 16 bits, to the other stage; zeros in the places that are closed to every row of the tile
+  auto stage = [&](int blk, int pend) {   // returns whether a power is odd
+    if (blk * PB + PB - 1 > pend || bad_next) {
+      if (blk * PB + sr > pend || ((bad_next >> wave) & 1)) {
+        kb = vb = 127;
+#pragma unroll
+        for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    const int odd = pt_odd(kb, pt_least_odd<DT>) | pt_odd(vb, pt_least_odd<DT>);
+    const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
+    const unsigned kat = kwr + (st ^ 1) * 2 * BYTES, vat = vwr + (st ^ 1) * 2 * BYTES;
+#pragma unroll
+    for (int i = 0; i < PCS; ++i) {
+      const uint4 k = kr[i], v = vr[i];
+      *(uint4*)(lds + (kat ^ (i * 128))) = pt_widen<DT>(k.x, k.y, kp);
+      *(uint4*)(lds + (kat ^ (i * 128 + 16))) = pt_widen<DT>(k.z, k.w, kp);
+      *(uint4*)(lds + (vat ^ (i * 128))) = pt_widen<DT>(turn ? v.z : v.x, turn ? v.w : v.y, vp);
+      *(uint4*)(lds + (vat ^ (i * 128 + 16))) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
+    }
+    return odd;
+  };
+  auto last_pos = [&](const PtItem& x) {   // the tile's last row's position
+    const int tlast = min(x.tile * PT_WIDE + PT_WIDE - 1, x.q.n * G - 1) / G;
+    return (int)min((long long)x.q.kv - x.q.n + tlast, (long long)a.M * a.page_size - 1);
+  };
+  PtItem8 it = pt_item_wide8(a, t, me, range);
+  PtWave<DT, D> w;
+  int odd = 0;
   begin(it, first_id(it));
+  w.queries(a, it, it.tile * PT_WIDE + wave * 32);
+  if (it.b0 < it.b1) odd = stage(it.b0, last_pos(it));
   for (;;) {
     const int rows = it.q.n * G, tile0 = it.tile * PT_WIDE, row0 = tile0 + wave * 32;
-    const int first = it.q.kv - it.q.n;   // position of token 0
-    const int tlast = min(tile0 + PT_WIDE - 1, rows - 1) / G;
-    const int b0 = it.b0, b1 = it.b1;
-    const int pend = (int)min((long long)first + tlast, (long long)a.M * a.page_size - 1);   // the tile's last row's position
-    bool odd = false;
-    auto stage = [&](int blk) {   // what was loaded, as 16 bits; zeros in the places that are closed to every row
-      if (blk * PB + PB - 1 > pend || bad_next) {
-        if (blk * PB + sr > pend || ((bad_next >> wave) & 1)) {
-          kb = vb = 127;
-#pragma unroll
-          for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      odd = odd || pt_odd(kb, pt_least_odd<DT>) || pt_odd(vb, pt_least_odd<DT>);
-      const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
-      const unsigned kat = kwr + (blk & 1) * 2 * BYTES, vat = vwr + (blk & 1) * 2 * BYTES;
-#pragma unroll
-      for (int i = 0; i < PCS; ++i) {
-        const uint4 k = kr[i], v = vr[i];
-        *(uint4*)(lds + (kat ^ (i * 128))) = pt_widen<DT>(k.x, k.y, kp);
-        *(uint4*)(lds + (kat ^ (i * 128 + 16))) = pt_widen<DT>(k.z, k.w, kp);
-        *(uint4*)(lds + (vat ^ (i * 128))) = pt_widen<DT>(turn ? v.z : v.x, turn ? v.w : v.y, vp);
-        *(uint4*)(lds + (vat ^ (i * 128 + 16))) = pt_widen<DT>(turn ? v.x : v.z, turn ? v.y : v.w, vp);
-      }
-    };
-    const bool last = done();
+    const int b0 = it.b0, b1 = it.b1, pend = last_pos(it);
+    const bool last = range.done();
+    int odd_next = 0;
     PtItem8 nx = it;
     int id = 0;
     if (!last) {
-      nx = pt_item_wide8(a, t, r, me, at, end);
+      nx = pt_item_wide8(a, t, me, range);
       id = first_id(nx);
     }
-    PtWave<DT, D> w;
-    w.init(a, it, row0);
-    if (b0 < b1) stage(b0);
+    const int pend_next = last_pos(nx);
+    w.begin(a, it, row0);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) asm volatile("" ::"v"(w.qf[ks].x), "v"(w.qf[ks].y), "v"(w.qf[ks].z), "v"(w.qf[ks].w));
     // positions that every row of the wave has open, and that any has
     const int pmin = __builtin_amdgcn_readfirstlane(w.pos);
     const int pmax = row0 < rows ? __builtin_amdgcn_readlane(w.pos, 31) : -1;
     for (int blk = b0; blk < b1; ++blk) {
+      const bool here = blk + 1 < b1;   // whether the next block is this item's
       bad = bad_next;
       __syncthreads();   // the block is in LDS, and every wave is done with the other stage
-      if (blk + 1 < b1) {
+      st ^= 1;
+      if (here) {
         if ((blk + 1) / WB != wi) {
           ++wi;
           cur = pt_window<true>(a, it, wi * 64, ids[lane]);
@@ -1901,32 +1925,38 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
       } else if (!last) {
         begin(nx, id);
       }
-      if (blk * PB <= pmax) {   // wave-uniform
-        const bool open = blk * PB + PB - 1 <= pmin && bad == 0;
-        const unsigned stage_at = (blk & 1) * 2 * BYTES, kat = krd + stage_at, vat = vrd + stage_at;
-        pt_f32x16 s[NB];
-        w.template scores_of<NB>([&](int sb, int ks) { return *(const uint4*)(lds + (kat ^ (ks * 32)) + sb * 32 * RB); }, s);
-        if (!open) w.template mask<NB>(s, blk * PB, bad);
-        __builtin_amdgcn_s_setprio(1);   // vector instructions first: the other workgroup's matrix instructions run on beside them
+      const bool some = blk * PB <= pmax;   // wave-uniform
+      const unsigned kat = krd + st * 2 * BYTES, vat = vrd + st * 2 * BYTES;
+      pt_f32x16 s[NB];
+      if (some) w.template scores_of<NB>([&](int sb, int ks) { return *(const uint4*)(lds + (kat ^ (ks * 32)) + sb * 32 * RB); }, s);
+      if (!here && !last) w.queries(a, nx, nx.tile * PT_WIDE + wave * 32);   // (this item's are done with)
+      if (some) {
+        if (!(blk * PB + PB - 1 <= pmin && bad == 0)) w.template mask<NB>(s, blk * PB, bad);
         w.template softmax<NB>(s);
         uint4 p[2 * NB];
         w.template pack<NB>(s, p);
-        __builtin_amdgcn_s_setprio(0);
         w.template outputs_of<NB>([&](int i) {
           const char* q = lds + i / TD * 16 * RB;
           const uint2 lo = pt_read_tr(q + (vat ^ (i % TD * 64))), up = pt_read_tr(q + 4 * RB + (vat ^ (i % TD * 64 + 32)));
           return make_uint4(lo.x, lo.y, up.x, up.y);
         }, p, s);
       }
-      if (blk + 1 < b1) stage(blk + 1);
+      if (here || (!last && nx.b0 < nx.b1)) {
+        const int more = stage(here ? blk + 1 : nx.b0, here ? pend : pend_next);
+        odd |= here ? more : 0, odd_next |= here ? 0 : more;
+      }
     }
-    if (b0 >= b1 && !last) begin(nx, id);
-    odd = __syncthreads_or(odd);   // (and the next item's blocks go to the same LDS)
+    if (b0 >= b1 && !last) {   // (an item without blocks)
+      begin(nx, id);
+      w.queries(a, nx, nx.tile * PT_WIDE + wave * 32);
+      if (nx.b0 < nx.b1) odd_next = stage(nx.b0, pend_next);
+    }
+    odd = __syncthreads_or(odd);
     const long long part = (long long)8 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;   // (behind the narrow tiles')
     pt_tell(a, it, row0 + w.fr, rows, part + row0 + w.fr - tile0, 1);
     pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, odd);
     if (last) return;
-    it = nx;
+    it = nx, odd = odd_next;
   }
 }
 
@@ -2190,48 +2220,66 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
     }
     return;
   }
-  const int step = gridDim.x * 4 * PER;
-  for (int u0 = (blockIdx.x * 4 + wave) * PER; u0 < rows; u0 += step) {
-    const int u = u0 + lane / LN;
-    if (u >= rows) continue;
-    uint2* to = (uint2*)(out + (long long)u * D) + sub;
-    if (zero(u)) {
-      *to = make_uint2(0, 0);
-      continue;
+  // a wave's run of rows, 64 at a time: a lane each looks whether there is something to do
+  const int waves = gridDim.x * 4, each = (rows + waves - 1) / waves, me = blockIdx.x * 4 + wave, stop = min(rows, (me + 1) * each);
+  for (int u0 = me * each; u0 < stop; u0 += 64) {
+    const int mine = u0 + lane;
+    int2 jm = make_int2(0, 0);
+    bool blank = false;
+    if (mine < stop) {
+      jm = ((const int2*)a.joins)[mine];
+      blank = zero(mine);
     }
-    const int2 j = ((const int2*)a.joins)[u];
-    const int S = j.y >> 1;
-    if (S < 2) continue;
-    const float2* mls = (const float2*)a.part_ml + j.x;
-    const float4* os = (const float4*)(a.part_o + (long long)j.x * D) + sub;
-    float M = -INFINITY, L = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < S; p += 8) {
-      float2 ml[8];
-      float4 v[8];
+    unsigned long long todo = __ballot(mine < stop && (blank || jm.y >= 4));
+    while (todo) {
+      // the wave's lane groups take the next PER of them
+      int k = -1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (p + i < S) {
-          const long long at = far(j, p + i);
-          ml[i] = mls[at];
-          v[i] = os[at * LN];
-        }
-      float most = M;
+      for (int g = 0; g < PER; ++g) {
+        const int first = todo ? __ffsll(todo) - 1 : -1;
+        if (first >= 0) todo &= todo - 1;
+        if (lane / LN == g) k = first;
+      }
+      const int2 j = make_int2(__shfl(jm.x, max(k, 0), 64), __shfl(jm.y, max(k, 0), 64));
+      const bool empty = __shfl((int)blank, max(k, 0), 64);
+      if (k < 0) continue;
+      uint2* to = (uint2*)(out + (long long)(u0 + k) * D) + sub;
+      if (empty) {
+        *to = make_uint2(0, 0);
+        continue;
+      }
+      const int S = j.y >> 1;
+      const float2* mls = (const float2*)a.part_ml + j.x;
+      const float4* os = (const float4*)(a.part_o + (long long)j.x * D) + sub;
+      float M = -INFINITY, L = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p = 0; p < S; p += 8) {
+        float2 ml[8];
+        float4 v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (p + i < S) most = fmaxf(most, ml[i].x);
-      const float old = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - most) * c);
-      M = most, L *= old, x.x *= old, x.y *= old, x.z *= old, x.w *= old;
+        for (int i = 0; i < 8; ++i)
+          if (p + i < S) {
+            const long long at = far(j, p + i);
+            ml[i] = mls[at];
+            v[i] = os[at * LN];
+          }
+        float most = M;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (p + i < S) {
-          const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - most) * c);
-          L = fmaf(f, ml[i].y, L);
-          x.x = fmaf(f, v[i].x, x.x), x.y = fmaf(f, v[i].y, x.y), x.z = fmaf(f, v[i].z, x.z), x.w = fmaf(f, v[i].w, x.w);
-        }
+        for (int i = 0; i < 8; ++i)
+          if (p + i < S) most = fmaxf(most, ml[i].x);
+        const float old = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - most) * c);
+        M = most, L *= old, x.x *= old, x.y *= old, x.z *= old, x.w *= old;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (p + i < S) {
+            const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - most) * c);
+            L = fmaf(f, ml[i].y, L);
+            x.x = fmaf(f, v[i].x, x.x), x.y = fmaf(f, v[i].y, x.y), x.z = fmaf(f, v[i].z, x.z), x.w = fmaf(f, v[i].w, x.w);
+          }
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      *to = make_uint2(gm_pack2<DT>(x.x * inv, x.y * inv), gm_pack2<DT>(x.z * inv, x.w * inv));
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    *to = make_uint2(gm_pack2<DT>(x.x * inv, x.y * inv), gm_pack2<DT>(x.z * inv, x.w * inv));
   }
 }
 
