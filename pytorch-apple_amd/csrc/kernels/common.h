@@ -643,7 +643,7 @@ struct PagedAttnArgs {        // paged.hip: causal attention of packed rows over
   unsigned group_magic;       // ceil(2^32 / page_groups); 0 where page_groups is 1
   int grid_wide;              // workgroups of the wide tiles (the first ones), the rest take narrow tiles
   int grid_narrow;            // workgroups of the narrow tiles
-  int join4;                  // pages of 8 bits: the combine kernel takes a row by the four waves of a workgroup
+  int pad;
   const unsigned char* k_scales;   // pages of 8 bits: exponent + 127 of position r, head h, page p at (p * KVH + h) * page_size + r
   const unsigned char* v_scales;
   int* joins;                      // [N, H, 2] where the row's parts are: the first one's row, 2 parts + (1: of a wide tile)

@@ -2167,12 +2167,12 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
 
 // k_paged_quant_combine: the same over pages of 8 bits. What a row is joined of stands in a.joins, where the wave (workgroup)
 // that began its tile has put it: nothing is looked up, where doing so again took 2 to 3 of 6 us. Rows are D / 4 lanes each,
-// so a wave has the loads of several rows in flight at once; with a.join4 a workgroup's waves take a quarter of a row's
-// parts each (few rows over long caches: 256 parts a row took 9.3 us by one wave a row).
-template <int DT, int D>
+// so a wave has the loads of several rows in flight at once. _join, for few rows: a workgroup of 16 waves joins a row, which
+// over long caches may have 256 parts (4 requests over up to 131,071 positions: 9.3 us by a wave a row, 8.9 by 4 waves).
+template <int DT, int D, bool JOIN>
 __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
-  constexpr int LN = D / 4, PER = 64 / LN;
-  __shared__ float quarters[4][4][LN + 2];
+  constexpr int LN = D / 4, PER = 64 / LN, W = JOIN ? 16 : 1;
+  __shared__ float shares[W][4][LN + 2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LN;
   const int s0 = a.q_start[0], s1 = a.q_start[a.B], rows = a.N * a.H;
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
@@ -2183,7 +2183,7 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
     return none || row < s0 || row >= s1;
   };
   uint16_t* out = (uint16_t*)a.out;
-  if (a.join4) {
+  if constexpr (JOIN) {
     for (int u = blockIdx.x; u < rows; u += gridDim.x) {
       if (zero(u)) {
         if (threadIdx.x < D / 4) *(uint2*)(out + (long long)u * D + threadIdx.x * 4) = make_uint2(0, 0);
@@ -2193,26 +2193,26 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
       const int S = j.y >> 1;
       if (S < 2) continue;
       float M = -INFINITY, L = 0.f, x[4] = {};
-      pt_gather<D, 1>(a, j.x, S * wave / 4, S * (wave + 1) / 4, [&](int s) { return far(j, s); }, M, L, x);
+      pt_gather<D, 1>(a, j.x, S * wave / W, S * (wave + 1) / W, [&](int s) { return far(j, s); }, M, L, x);
       pt_gathered<D>(L, x);
       if (lane < LN)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) quarters[wave][e][lane] = x[e];
-      if (lane == 0) quarters[wave][0][LN] = M, quarters[wave][0][LN + 1] = L;
+        for (int e = 0; e < 4; ++e) shares[wave][e][lane] = x[e];
+      if (lane == 0) shares[wave][0][LN] = M, shares[wave][0][LN + 1] = L;
       __syncthreads();
       if (wave == 0) {
         float most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most = fmaxf(most, quarters[i][0][LN]);
+        for (int i = 0; i < W; ++i) most = fmaxf(most, shares[i][0][LN]);
         L = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float m = quarters[i][0][LN], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
-          L += f * quarters[i][0][LN + 1];
+        for (int i = 0; i < W; ++i) {
+          const float m = shares[i][0][LN], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - most) * c);
+          L += f * shares[i][0][LN + 1];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] += f * quarters[i][e][sub];
+          for (int e = 0; e < 4; ++e) x[e] += f * shares[i][e][sub];
         }
         pt_put<DT, D>(out + (long long)u * D, L, x);
       }
@@ -2287,7 +2287,8 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
   extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_##NAME(const PagedAttnArgs a) { pt_attn_body<DT, D>(a); }     \
   extern "C" __global__ void __launch_bounds__(256) k_paged_combine_##NAME(const PagedAttnArgs a) { pt_combine_body<DT, D>(a); }  \
   extern "C" __global__ void __launch_bounds__(256, 2) k_paged_quant_attn_##NAME(const PagedAttnArgs a) { pt_attn8_body<DT, D>(a); } \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_quant_combine_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D>(a); }
+  extern "C" __global__ void __launch_bounds__(256) k_paged_quant_combine_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D, false>(a); } \
+  extern "C" __global__ void __launch_bounds__(1024) k_paged_quant_join_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D, true>(a); }
 PT_KERNELS(bf16_d128, HS_BF16, 128)
 PT_KERNELS(bf16_d64, HS_BF16, 64)
 PT_KERNELS(f16_d128, HS_F16, 128)

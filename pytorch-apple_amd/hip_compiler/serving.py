@@ -19,7 +19,10 @@ PAGED_APPEND_ROW_N = 1024
 # that wide tiles are split towards
 PT_MAXB, PT_NARROW, PT_WIDE, PT_NARROW_LEAST, PT_WIDE_LEAST, PT_WIDE_ITEMS = 1024, 32, 128, 4, 8, 480
 PT_GRID = 512                  # two workgroups per CU
-PT_JOIN4_ROWS = 1024           # up to so many rows and heads a workgroup joins a row's parts, past it a wave
+# Pages of 8 bits: up to so many rows times heads a workgroup joins a row's parts, past it a wave does. us of the attention by
+# a wave / by a workgroup: 12 rows over 2,048 positions 15.5 / 13.3, over 30,000 73.3 / 19.1, 48 over up to 131,072 94.5 / 56.3,
+# 256 over 30,000 87.0 / 83.7; 512 over 4,096 37.0 / 38.2, 896 over 4,096 37.7 / 43.7
+PT_JOIN_ROWS = 256
 # sample.hip: SM_GROUPS groups of 64 pieces of 16 bytes, bins, tokens of a list
 SAMPLE_MAX_PIECES, SAMPLE_BINS, SAMPLE_LIST = 4096 * 64, 512, 16384
 # Up to this many pieces k_sample_pick alone, past it the four launches. us alone / four, top-k 50 and top-p 0.95, bfloat16:
@@ -175,7 +178,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
                 scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
-                grid_narrow=0, join4=0, k_scales=ks, v_scales=vs, joins=None)
+                grid_narrow=0, pad=0, k_scales=ks, v_scales=vs, joins=None)
     params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
     ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
     prefix = "k_paged_quant_" if quant else "k_paged_"
@@ -189,19 +192,22 @@ def lower_paged_attention(low, node: OpNode) -> None:
     part_rows = 2 * tiled["grid_narrow"] * PT_NARROW + tiled["wide_slots"] * PT_WIDE
     if quant:
         part_rows = 8 * tiled["grid_narrow"] * PT_NARROW + 2 * tiled["grid_wide"] * PT_WIDE
-    join4 = int(quant and N * H <= PT_JOIN4_ROWS)
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
                 part_ml=low.scratch(outs[0] + ".part_ml", 8 * part_rows), page_groups=groups,
                 group_magic=0 if groups == 1 else -(-2 ** 32 // groups), grid_wide=tiled["grid_wide"],
-                grid_narrow=tiled["grid_narrow"], join4=join4, joins=low.scratch(outs[0] + ".joins", 8 * N * H) if quant else None)
+                grid_narrow=tiled["grid_narrow"], joins=low.scratch(outs[0] + ".joins", 8 * N * H) if quant else None)
     name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
         kind="paged_attention", kernel=prefix + "attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
         grid=(tiled["grid_wide"] + tiled["grid_narrow"], 1, 1), inputs=ins, outputs=outs, params={**params, "mfma": True}))
-    rows_each = 1 if join4 else 4 * 64 // (D // 4) if quant else 4   # of a workgroup
+    kernel, grid, threads = "combine_", min(1024, -(-N * H // 4)), 256
+    if quant and N * H <= PT_JOIN_ROWS:
+        kernel, grid, threads = "join_", N * H, 1024
+    elif quant:
+        grid = min(2048, -(-N * H // (4 * (256 // D))))
     low.emit(LaunchStep(
-        kind="paged_attention", kernel=prefix + "combine_" + name, module="paged", arg_struct="PagedAttnArgs",
-        args=dict(args), grid=(min(2048 if quant else 1024, -(-N * H // rows_each)), 1, 1), inputs=ins, outputs=outs, params=params))
+        kind="paged_attention", kernel=prefix + kernel + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
+        grid=(grid, 1, 1), block=(threads, 1, 1), inputs=ins, outputs=outs, params=params))
 
 
 def lower_sample(low, node: OpNode) -> None:

@@ -138,7 +138,7 @@ _struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), 
                           ("row_stride", LL), ("pages", LL), ("part_o", P), ("part_ml", P), ("N", I), ("B", I), ("M", I),
                           ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
                           ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
-                          ("join4", I), ("k_scales", P), ("v_scales", P), ("joins", P)])
+                          ("pad", I), ("k_scales", P), ("v_scales", P), ("joins", P)])
 _struct("SampleRow", [("best", LL), ("mode", I),
                       ("kb", I), ("kr", I), ("kn", I), ("plo", I), ("phi", I),
                       ("pn", I), ("pad", I)])
