@@ -267,8 +267,11 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_norm_quant_append_any(
 // k_paged_*_append_*: 16-bit types, D and R multiples of 16, D <= 256, 16-byte aligned rows. A head lies in LP lanes of a row
 // of 16 (the power of two from D / 16, at least 4), 16 dims each in two pieces of 8: those that rotate together, or past R
 // two neighbours. So what is needed of a whole head (sum of squares, largest magnitude) takes two to four steps across
-// lanes, and a lane's cosines, sines and weights are the same for all heads of its row and stay in registers. A wave
-// per row, or the four waves of a workgroup where rows are few (_row).
+// lanes, and a lane's cosines, sines and weights are the same for all heads of its row and stay in registers. Two waves
+// per row, or the four of a workgroup where rows are few (_row). Few rows are bound by the chain of loads to a row's place, so
+// its first heads are loaded beside that; many by memory: 9,000 rows of 32 + 8 heads of 128, normed and in 8 bits, 32 us for
+// 134 MB (4.2 TB/s; 36 with a wave's number in a vector register, 34 with two heads at a time, whose registers leave room
+// for fewer waves).
 template <bool MAX>
 __device__ __forceinline__ float pg_heads(float v, int LP) {
   auto join = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
@@ -289,39 +292,12 @@ template <int DT, int WAVES, bool NORM, bool F8>
 __device__ __forceinline__ void append_heads(const PagedAppendArgs& a) {
   constexpr int ROWS = 4 / WAVES, TH = 64 * WAVES;
   __shared__ __attribute__((aligned(16))) float cs[ROWS][2][PG_APPEND_R / 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = wave / WAVES, tid = (wave % WAVES) * 64 + lane;
-  const int row = blockIdx.x * ROWS + mine, half = a.R / 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave / WAVES, tid = (wave % WAVES) * 64 + lane;
+  const int row = blockIdx.x * ROWS + mine, half = a.R / 2, heads = a.H + 2 * a.KVH;
   const bool in = row < a.N;
-  const int b = in ? pg_sequence(a.q_start, a.B, row, lane) : a.B;
-  const bool real = b < a.B && row >= a.q_start[0];
-  const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
-  const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
-  if (real)
-    for (int j = tid; j < half; j += TH) {
-      float s, c;
-      sincos_rot_d((double)pos * (double)a.inv_freq[j], &s, &c);
-      cs[mine][0][j] = c * a.scaling, cs[mine][1][j] = s * a.scaling;
-    }
-  __syncthreads();
-  if (!in) return;
-  const int need = a.D / 16, LP = need <= 4 ? 4 : need <= 8 ? 8 : 16, sub = tid & (LP - 1);
+  const int need = a.D / 16, shift = need <= 4 ? 2 : need <= 8 ? 3 : 4, LP = 1 << shift, sub = tid & (LP - 1), step = TH >> shift;
   const bool has = sub < need, turns = has && sub < a.R / 16;
   const int e0 = !has ? 0 : turns ? sub * 8 : a.R + (sub - a.R / 16) * 16, e1 = !has ? 0 : turns ? half + sub * 8 : e0 + 8;
-  float c[8], s[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
-  if (turns && real) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = cs[mine][0][e0 + j], s[j] = cs[mine][1][e0 + j];
-  }
-  uint4 wq0, wq1, wk0, wk1;
-  if constexpr (NORM) {
-    const uint16_t *wq = (const uint16_t*)a.q_weight, *wk = (const uint16_t*)a.k_weight;
-    wq0 = *(const uint4*)(wq + e0), wq1 = *(const uint4*)(wq + e1);
-    wk0 = *(const uint4*)(wk + e0), wk1 = *(const uint4*)(wk + e1);
-  }
-  const int off = page < 0 ? 0 : pos % a.page_size, heads = a.H + 2 * a.KVH;
-  const long long slot = page < 0 ? 0 : page * a.page_stride + off * a.row_stride;
   struct Step {
     uint4 x, y;
     int h;
@@ -338,6 +314,38 @@ __device__ __forceinline__ void append_heads(const PagedAppendArgs& a) {
     t.y = *(const uint4*)(src + e1);
     return t;
   };
+  // the first two heads and the weights are on their way while the row's place and angles are found
+  const int h0 = tid >> shift;
+  Step t0{}, t1{};
+  if (in && h0 < heads) t0 = get(h0);
+  if (in && h0 + step < heads) t1 = get(h0 + step);
+  uint4 wq0, wq1, wk0, wk1;
+  if constexpr (NORM) {
+    const uint16_t *wq = (const uint16_t*)a.q_weight, *wk = (const uint16_t*)a.k_weight;
+    wq0 = *(const uint4*)(wq + e0), wq1 = *(const uint4*)(wq + e1);
+    wk0 = *(const uint4*)(wk + e0), wk1 = *(const uint4*)(wk + e1);
+  }
+  const int b = __builtin_amdgcn_readfirstlane(in ? pg_sequence(a.q_start, a.B, row, lane) : a.B);
+  const bool real = b < a.B && row >= a.q_start[0];
+  const int pos = real ? pg_position(a.kv_len[b], a.q_start[b + 1], row) : 0;
+  const int page = real ? pg_page(a.table, b, a.M, a.page_size, a.pages, pos) : -1;
+  if (real)
+    for (int j = tid; j < half; j += TH) {
+      float s, c;
+      sincos_rot_d((double)pos * (double)a.inv_freq[j], &s, &c);
+      cs[mine][0][j] = c * a.scaling, cs[mine][1][j] = s * a.scaling;
+    }
+  __syncthreads();
+  if (!in) return;
+  float c[8], s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
+  if (turns && real) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = cs[mine][0][e0 + j], s[j] = cs[mine][1][e0 + j];
+  }
+  const int off = page < 0 ? 0 : pos % a.page_size;
+  const long long slot = page < 0 ? 0 : page * a.page_stride + off * a.row_stride;
   auto put = [&](const Step& t) {
     const bool isq = t.h < a.H, isv = t.h >= a.H + a.KVH;
     const int hk = isv ? t.h - a.H - a.KVH : t.h - a.H;
@@ -395,19 +403,17 @@ __device__ __forceinline__ void append_heads(const PagedAppendArgs& a) {
     *(uint4*)(dst + e0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     *(uint4*)(dst + e1) = make_uint4(up[0], up[1], up[2], up[3]);
   };
-  const int step = TH / LP;
-  for (int h = tid / LP; h < heads; h += 2 * step) {   // two steps' loads in flight
-    const bool two = h + step < heads;
-    const Step u = get(h), t = get(two ? h + step : h);
-    put(u);
-    if (two) put(t);
+  for (int h = h0; h < heads; h += step) {   // two heads' loads are in flight while one is written
+    put(t0);
+    t0 = t1;
+    if (h + 2 * step < heads) t1 = get(h + 2 * step);
   }
 }
 
 #define PG_APPENDS(NAME, NORM, F8)                                                                                              \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_bf16(const PagedAppendArgs a) { append_heads<HS_BF16, 1, NORM, F8>(a); }     \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_bf16(const PagedAppendArgs a) { append_heads<HS_BF16, 2, NORM, F8>(a); }     \
   extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_bf16_row(const PagedAppendArgs a) { append_heads<HS_BF16, 4, NORM, F8>(a); } \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_f16(const PagedAppendArgs a) { append_heads<HS_F16, 1, NORM, F8>(a); }       \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_f16(const PagedAppendArgs a) { append_heads<HS_F16, 2, NORM, F8>(a); }       \
   extern "C" __global__ void __launch_bounds__(256) k_paged_##NAME##_append_f16_row(const PagedAppendArgs a) { append_heads<HS_F16, 4, NORM, F8>(a); }
 PG_APPENDS(norm, true, false)
 PG_APPENDS(quant, false, true)

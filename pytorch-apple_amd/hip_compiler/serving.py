@@ -14,6 +14,10 @@ PAGED_HEADS_MAX_D = 256        # paged.hip append_heads: a head in 16 lanes
 # Up to this many rows a workgroup per row, past it a wave. us by workgroups / by waves, in 16 bits: 16 rows of 12 + 2 heads
 # of 128 3.8 / 5.1, 1,024 5.1 / 5.7, 2,048 7.5 / 6.8, 8,192 21.9 / 14.8; 14 + 2 of 64: 3.9 / 3.9, 4.6 / 4.3, 6.5 / 5.0,
 # 18.8 / 10.2; 32 + 8 of 128, whose rows keep four waves busy: 4.1 / 7.2, 6.7 / 8.7, 10.5 / 12.9, 32.4 / 34.4.
+# The forms that need whole heads take two waves a row past it. us by four / two / one, 8 bits: 16 rows of 12 + 2 heads of 128
+# 4.0 / 4.1 / 4.5, 1,024 4.6 / 4.8 / 5.1, 2,048 6.2 / 5.6 / 5.9, 8,192 14.8 / 12.5 / 12.5; 14 + 2 of 64: 4.1 / 4.6 / 5.6,
+# 4.6 / 4.6 / 6.1, 6.0 / 5.3 / 6.6, 14.0 / 11.4 / 11.5; 32 + 8 of 128: 4.4 / 5.1 / 6.8, 6.5 / 7.1 / 8.7, 9.9 / 9.4 / 10.6,
+# 29.1 / 27.9 / 28.6; normed too: 5.0 / 5.8 / 8.1, 6.7 / 7.4 / 9.6, 10.3 / 10.6 / 12.2, 27.1 / 26.1 / 25.7.
 PAGED_APPEND_ROW_N = 1024
 # paged.hip: sequences of a list, rows of a tile, fewest blocks of a narrow workgroup and of a wide tile's split, items
 # that wide tiles are split towards
@@ -103,7 +107,7 @@ def _append_kernel(dtype: str, N: int, D: int, R: int, heads: bool) -> tuple[str
     if dtype not in ("bfloat16", "float16") or D % piece or R % 16 or R > PAGED_APPEND_MAX_R or (heads and D > PAGED_HEADS_MAX_D):
         return "any", N
     few = N <= PAGED_APPEND_ROW_N
-    return ("bf16" if dtype == "bfloat16" else "f16") + ("_row" if few else ""), N if few else -(-N // 4)
+    return ("bf16" if dtype == "bfloat16" else "f16") + ("_row" if few else ""), N if few else -(-N // (2 if heads else 4))
 
 
 def lower_paged_append(low, node: OpNode) -> None:
