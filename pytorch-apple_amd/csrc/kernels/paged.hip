@@ -269,7 +269,7 @@ extern "C" __global__ void __launch_bounds__(256) k_paged_norm_quant_append_any(
 // two neighbours. So what is needed of a whole head (sum of squares, largest magnitude) takes two to four steps across
 // lanes, and a lane's cosines, sines and weights are the same for all heads of its row and stay in registers. Two waves
 // per row, or the four of a workgroup where rows are few (_row). Few rows are bound by the chain of loads to a row's place, so
-// its first heads are loaded beside that; many by memory: 9,000 rows of 32 + 8 heads of 128, normed and in 8 bits, 32 us for
+// its first heads are loaded beside that; many by memory: 5,963 rows of 32 + 8 heads of 128, normed and in 8 bits, 32 us for
 // 134 MB (4.2 TB/s; 36 with a wave's number in a vector register, 34 with two heads at a time, whose registers leave room
 // for fewer waves).
 template <bool MAX>
@@ -1532,6 +1532,9 @@ struct PtCut {
   int b, h, tile, blk;
   __device__ __forceinline__ bool in(const PtCut& o) const { return b == o.b && h == o.h && tile == o.tile; }
 };
+// Fewest blocks that a range is worth, about those of a tile of one: us of 16 prompts of 16 tokens (32 + 8 heads of 128) at 8 / 4 /
+// 2 / 1 31 / 20 / 16 / 17, of 64 tokens 36 / 24 / 20 / 21, one of 256 35 / 26 / 20 / 20; 64 tokens behind 2,000 33 / 28 / 28 / 29.
+#define PT_RANGE_LEAST 2
 struct PtRanges {
   unsigned long long total;
   unsigned long long range;   // of a workgroup
@@ -1814,7 +1817,7 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.H / a.KVH;
   PtRanges r;
   r.total = pt_build_wide8(a, t);
-  r.workers = (int)max(1ull, min((unsigned long long)a.grid_wide, r.total / (PT_WIDE_LEAST * PB * G)));
+  r.workers = (int)max(1ull, min((unsigned long long)a.grid_wide, r.total / (PT_RANGE_LEAST * PB * G)));
   r.range = r.total / r.workers;
   const int each = (r.workers + 7) >> 3, me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
   if (r.total == 0 || (int)(blockIdx.x >> 3) >= each || me >= r.workers) return;
