@@ -1350,9 +1350,14 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 //     K's operand holds one position, so 2^ke_j comes with the conversion. A lane of V's holds eight positions of one dim:
 //     2^ve_j goes to the probabilities, which are therefore taken in bfloat16 (whose range holds any power of two) whatever the
 //     queries' type, for float16 in two parts, the second the first's rounding error, each with its product: float16's
-//     own 11 bits at least. Bound by memory, beside which the second product costs nothing.
+//     own 11 bits at least. Bound by memory, beside which the second product costs nothing: 64 decodes of up to 4,096 positions
+//     (32 + 8 heads of 128, 412 MB) take 88 us, 4.7 TB/s (153 from 16-bit pages), four of up to 131,071 (12 + 2) 42 (76).
 //   * Wide: bound by the matrix cores, so each block is converted once for all four waves, powers of two included, by way of
-//     registers one block ahead, into the LDS layout of 16-bit pages; the rest is the 16-bit tile.
+//     registers one block ahead, into the LDS layout of 16-bit pages; the rest is the 16-bit tile. The conversion's vector
+//     instructions and LDS writes come on top of the softmax's: 409 tokens over 30,409 positions (12 + 2 heads) take 106 us, 0.72
+//     PFLOP/s, rather than 93. (Softmax of one block between the products of another within a wave: 4.4 us a block rather than
+//     2.3 at head size 128, since its registers spill; three workgroups a CU at head size 64 spill too: 78 us rather than 70 for a
+//     mixed step.)
 // K in float16 can overflow where 2^ke is 2^8 or more (keys above 57,344), bfloat16 where a power is 2^120; probabilities times
 // powers below 2^-100 reach the end of bfloat16; byte 255 is NaN: tiles that see such a byte in an open place are done row
 // by row, like those with outputs that are not finite. (0, what was never written, is none of them: it counts as 2^-127 or 0.
@@ -1555,8 +1560,8 @@ __device__ __forceinline__ PtCut pt_behind(const PagedAttnArgs& a, const PtList8
   return c;
 }
 // Where workgroup w's range begins; a lane each may ask for another w. Ranges are of equal cost, but where tiles are short
-// against them one that would begin within an eighth of a range from a tile's border begins there: six prompts of 1,500
-// tokens so have 120 tiles cut in two rather than 480, whose parts would be written and read again.
+// against them one that would begin within an eighth of a range from a tile's border begins there, so that fewer tiles have
+// parts to be written and read again (of many prompts, else, nearly every range would begin inside a tile).
 __device__ __forceinline__ PtCut pt_cut(const PagedAttnArgs& a, const PtList8& t, const PtRanges& r, int w) {
   if (w >= r.workers) return PtCut{a.B, 0, 0, 0};
   const unsigned long long x = r.range * w + r.total % r.workers * w / r.workers;
@@ -2175,9 +2180,10 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
 }
 
 // k_paged_quant_combine: the same over pages of 8 bits. What a row is joined of stands in a.joins, where the wave (workgroup)
-// that began its tile has put it: nothing is looked up, where doing so again took 2 to 3 of 6 us. Rows are D / 4 lanes each,
-// so a wave has the loads of several rows in flight at once. _join, for few rows: a workgroup of 16 waves joins a row, which
-// over long caches may have 256 parts (4 requests over up to 131,071 positions: 9.3 us by a wave a row, 8.9 by 4 waves).
+// that began its tile has put it, so nothing is looked up here. Rows are D / 4 lanes each, so a wave has the loads of several
+// rows in flight at once. _join, for few rows: a workgroup of 16 waves joins a row, which over long caches has hundreds of
+// parts (4 requests over up to 131,071 positions: 6.6 us, 8.9 by 4 waves). Bound by the latency of dependent loads: 4 to 5 us
+// for decodes, 9 for 1,553 rows of 14 heads of 64, 11 for 5,963 rows of 32 heads of 128.
 template <int DT, int D, bool JOIN>
 __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
   constexpr int LN = D / 4, PER = 64 / LN, W = JOIN ? 16 : 1;
