@@ -83,3 +83,45 @@ def test_pools_of_more_bytes_than_32_bits_count(backend, news):
     theirs, by = step(small, table, near)
     assert all(torch.equal(a, b) for a, b in zip(ours, theirs))
     assert all(torch.equal(a[P - near:], b) and not a[:P - near].any() for a, b in zip(far, by))
+
+
+@pytest.mark.parametrize("D,dtype,page", [(128, "bfloat16", 16), (64, "float16", 32), (80, "bfloat16", 16)])
+@pytest.mark.parametrize("news,kvs", [([1, 3, 2], [300, 200, 9]), ([70, 1], [300, 5])])
+def test_queries_that_are_no_numbers(backend, D, dtype, page, news, kvs):
+    """A NaN or an infinity in a query makes its own row and head NaN (an infinity among scores of both signs); the others are
+    right as ever. (Not to the bit: 32 rows of a tile with such an output are done again row by row, whose probabilities keep
+    32 bits where a tile's are rounded to 16.)"""
+    bt = R.batch(news, kvs, page, seed=6)
+    q = _rand(9, bt["rows"], 4, D, dtype=dtype)
+    q[0, 1, 3], q[2, 2, 7] = torch.nan, torch.inf
+    if bt["rows"] > 60:
+        q[50, 0, 5], q[69, 3, 0] = -torch.inf, torch.nan
+    clean = q.isfinite().all(-1)
+    pools = Q.pools8(bt, 2, page, D)
+    got, _ = _attention(backend, bt, 4, 2, D, dtype, page, pools=pools, q=q, rows=clean)
+    assert got[~clean].isnan().all()
+
+
+def test_two_executors_on_two_streams(backend):
+    """Each with its own workspaces: calls that overlap give what calls one by one give."""
+    from irgen.serving import build_paged_attention_ir
+
+    D, page, H, KVH = 128, 16, 12, 2
+    runs = []
+    for seed, (news, kvs) in enumerate((([1] * 8, [3000] * 8), ([300, 1], [4000, 900]))):
+        bt = R.batch(news, kvs, page, seed=seed)
+        t = {"q": _rand(seed, bt["rows"], H, D, dtype="bfloat16"), **dict(zip(NAMES, Q.pools8(bt, KVH, page, D))), **_meta(bt)}
+        ir = build_paged_attention_ir(bt["rows"], len(news), bt["pages"], page, bt["block_table"].shape[1], H, KVH, D, cache=E4M3FN)
+        bufs = {k: backend.allocate_buffer(x.cuda()) for k, x in t.items()}
+        name = ir["graph_outputs"][0]["name"]
+        dags = [_dag(ir, backend) for _ in range(2)]
+        want = dags[0].execute(bufs)[name].to_torch().clone()
+        torch.cuda.synchronize()
+        runs += [(d, bufs, name, want, torch.cuda.Stream()) for d in dags]
+    for _ in range(5):
+        outs = []
+        for d, bufs, name, _, stream in runs:
+            with torch.cuda.stream(stream):
+                outs.append(d.execute(bufs)[name])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o.to_torch(), w) for o, (*_, w, _) in zip(outs, runs))

@@ -245,3 +245,12 @@ def test_the_step_graph_is_one_program_that_survives_its_file(tmp_path):
     assert sorted(prog.stats["mutated_inputs"]) == ["k_pages_0", "k_scales_0", "v_pages_0", "v_scales_0"]
     save_program(prog, tmp_path / "step.hipbin")
     assert load_program(tmp_path / "step.hipbin") == prog
+
+
+def test_graphs_of_different_caches_are_refused():
+    from npu_runtime.paged_generation import PagedGenerator
+
+    shape = dict(seqs=2, pages=4, page_size=8, table_pages=2, cfg=M.CFG)
+    step, decode = build_paged_ir(6, cache="float8_e4m3fn", **shape), build_paged_ir(2, **shape)
+    with pytest.raises(ValueError, match="slots and pools"):
+        PagedGenerator(object(), step, object(), decode)
