@@ -69,7 +69,7 @@ def _aligned_rows(low, name: str, v: TView) -> TView:
 
 
 def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_size: int, dtype: str,
-                block: int | None = None) -> dict | None:
+                quant: bool = False) -> dict | None:
     """Launch of the tiled attention kernels (paged.hip), None where they do not apply: other types or head sizes,
     pages that are no multiple of 16 positions, more sequences than the item list holds, or sizes whose item
     counts could pass 32 bits. Wide tiles are left out where the rows average at most two tokens per sequence: a
@@ -78,16 +78,21 @@ def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_s
     one of them decoding, the chunk of 1 token 160 / 156, of 64 168 / 160, of 200 187 / 177, of 400 203 / 205; six prompts
     of 1,000 111 / 299, 16 of 100 26 / 54; one chunk over 30,000 positions, of 16 tokens 39 / 35, of 64 59 / 61, of 256
     146 / 188. So between two and some six tokens per sequence the rule costs up to 6% (with 12 over 2 heads, whose caches
-    are read in a third of the time, up to 29%: 46 / 35 at 2.5): a launch does not know whether its rows are one chunk or many."""
+    are read in a third of the time, up to 29%: 46 / 35 at 2.5): a launch does not know whether its rows are one chunk or many.
+    Over pages of 8 bits (``quant``) the narrow tiles, whose waves stream by themselves, stay ahead longer: wide tiles from 16
+    tokens per sequence. The same, with / without: 63 decodes and a chunk of 64 124 / 101, 200 132 / 108, 1,000 170 / 150, 1,800
+    207 / 216; six prompts of 1,000 89 / 129, 16 of 100 23 / 34, 64 of up to 20 behind 4,000 159 / 179, of up to 14 154 / 149, of
+    up to 10 134 / 121; with 12 over 2 heads 63 and 1,000 79 / 62, 64 of up to 14 behind 4,000 59 / 66; one of 64 slots with a
+    chunk of 500 behind 4,000 55 / 63."""
     if dtype not in ("bfloat16", "float16") or D not in (64, 128) or page_size % 16 or not 0 < B <= PT_MAXB or M < 1 or P < 1:
         return None
-    G, block = H // KVH, block or 8192 // (2 * D)   # positions of a narrow tile's block
+    G, block = H // KVH, 64 if quant else 8192 // (2 * D)   # positions of a narrow tile's block
     blocks = -(-M * page_size // block)
     tiles = lambda R: KVH * (N * G // R + min(N, B))
     if (tiles(PT_NARROW) + 2 * PT_GRID) * (2 * blocks + 3) >= 2 ** 31 or M * page_size * page_size >= 2 ** 40 \
             or KVH * page_size * D >= 2 ** 30:
         return None
-    wide = N > 2 * B and N * G > PT_NARROW
+    wide = N > (16 if quant else 2) * B and N * G > PT_NARROW
     # a split tile has ceil(blocks / share) < 2 blocks / share parts, all together under twice the items aimed at;
     # nor can a tile have more than its blocks allow
     slots = min(2 * PT_WIDE_ITEMS, tiles(PT_WIDE) * -(-blocks // PT_WIDE_LEAST))
@@ -173,7 +178,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
     if N == 0:
         return
     B, M, P = int(kv_len.shape[0]), int(table.shape[1]), int(kp.shape[0])
-    tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype, 64 if quant else None)
+    tiled = paged_tiles(N, B, M, P, H, KVH, D, ps, q.dtype, quant)
     if tiled:
         qv = _aligned_rows(low, q.name, qv)
         caches = [low.aligned16(v, t.name) for t, v in zip((kp, vp, *scales), caches)]

@@ -43,6 +43,40 @@ def test_many_short_tiles(backend, D, dtype, page, seqs):
     _attention(backend, R.batch(news, kvs, page, pad=9, seed=1), 8, 2, D, dtype, page)
 
 
+@pytest.mark.parametrize("D,dtype,page", [(128, "bfloat16", 16), (64, "float16", 32)])
+@pytest.mark.parametrize("seqs", [40, 150, 400])
+def test_many_short_wide_tiles(backend, D, dtype, page, seqs):
+    """As above with chunks long enough that all but a few take wide tiles, of one to a few blocks."""
+    g = torch.Generator().manual_seed(seqs)
+    news = torch.randint(1, 50, (seqs,), generator=g).tolist()
+    kvs = [n + k for n, k in zip(news, torch.randint(0, 300, (seqs,), generator=g).tolist())]
+    _attention(backend, R.batch(news, kvs, page, pad=9, seed=1), 8, 2, D, dtype, page)
+
+
+@pytest.mark.parametrize("D,dtype,page", [(128, "bfloat16", 16), (64, "float16", 32)])
+def test_wide_tiles_over_places_that_do_not_exist(backend, D, dtype, page):
+    bt = R.batch([100, 60, 20], [300, 90, 20], page, pad=4)
+    bt["block_table"][0, 1], bt["block_table"][0, 5], bt["block_table"][1, 0] = 99999, -7, -1
+    bt["kv_len"][2] = 7                              # its first 13 tokens sit before position 0
+    got, _ = _attention(backend, bt, 4, 2, D, dtype, page)
+    assert (got[160:173] == 0).all() and (got[180:] == 0).all()
+
+
+@pytest.mark.parametrize("D,dtype,page", [(128, "bfloat16", 16), (64, "float16", 32)])
+@pytest.mark.parametrize("starts", [[0, 50, 20, 100], [0, 100, 0, 100]])
+def test_many_rows_of_starts_that_descend_give_zeros(backend, D, dtype, page, starts):
+    from irgen.serving import build_paged_attention_ir
+
+    bt = R.batch([1, 1, 1], [60, 60, 60], page)
+    t = {"q": _rand(1, 101, 4, D, dtype=dtype), **dict(zip(NAMES, Q.pools8(bt, 2, page, D))), **_meta(bt),
+         "q_start": torch.tensor(starts, dtype=torch.int32)}
+    ir = build_paged_attention_ir(101, 3, bt["pages"], page, bt["block_table"].shape[1], 4, 2, D, dtype, cache=E4M3FN)
+    bufs = {k: backend.allocate_buffer(x.cuda()) for k, x in t.items()}
+    out = _dag(ir, backend).execute(bufs)[ir["graph_outputs"][0]["name"]].to_torch()
+    torch.cuda.synchronize()
+    assert out.eq(0).all()
+
+
 @pytest.mark.parametrize("D,dtype", [(128, "bfloat16"), (64, "float16")])
 @pytest.mark.parametrize("N", [63, 64, 65])
 def test_joined_by_workgroups_and_by_waves(backend, D, dtype, N):
