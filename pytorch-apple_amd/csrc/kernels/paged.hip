@@ -510,7 +510,9 @@ extern "C" __global__ void __launch_bounds__(64) k_paged_quant_attn_any(const Pa
 #define PT_NARROW 32             // rows
 #define PT_WIDE 128
 #define PT_NARROW_LEAST 4        // fewest blocks of a narrow workgroup: one per wave
-#define PT_WAVE_LEAST 1          // and of a wave over pages of 8 bits
+// Fewest blocks of a wave over pages of 8 bits. us at 1 / 2 / 4: one token over 2,048 positions (12 + 2 heads of 128) 13.5 / 15.0 /
+// 18.7, over 8,000 14.6 / 15.8 / 21.9, 16 over 2,000 (32 + 8) 28.8 / 27.5 / 27.2, 64 over 500 (12 + 2) 16.5 / 19.7 / 23.6.
+#define PT_WAVE_LEAST 1
 #define PT_WIDE_ITEMS 480        // items that wide tiles are split towards: one round of two workgroups per CU
 #define PT_WIDE_LEAST 8          // fewest blocks of a split
 
