@@ -1239,41 +1239,6 @@ __device__ __forceinline__ void pt_narrow(const PagedAttnArgs& a, const PtItem& 
 
 // ------------------------------------------------------------------ wide tiles
 
-// Writes the rows row0 .. of one wave, of a tile that begins at row tile0: as outputs, or as a part (whose first row is
-// `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite.
-template <int DT, int D, bool F8 = false>
-__device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
-                                       int rows, int p0, int p1, long long part, bool odd) {
-  const int G = a.H / a.KVH;
-  const float l = w.row_sum();
-  const int row = row0 + w.fr;
-  if (row0 < rows && (odd || w.bad_output())) {
-    pt_rows<DT, D, F8>(a, it, tile0, row0, min(row0 + 32, rows), 1, p0, p1, part);
-  } else if (row < rows) {
-    if (it.slot >= 0) {
-      const long long at = part + row - tile0;
-      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
-              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
-    } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int t0 = row / G;
-      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
-              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
-                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
-    }
-  }
-}
-
 template <int DT, int D>
 __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it, char* lds, int (*slots)[64]) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V
@@ -1338,8 +1303,34 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
     if (blk * PB + PB - 1 > pend || bad) w.template clear_closed<NB>(Vt, blk * PB, pend, bad);
     w.template outputs<NB>(Vt, p, s);
   }
+  const float l = w.row_sum();
+  const int row = row0 + w.fr;
   const long long part = (long long)2 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;
-  pt_end<DT, D>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, false);
+  if (row0 < rows && w.bad_output()) {
+    pt_rows<DT, D>(a, it, tile0, row0, min(row0 + 32, rows), 1, b0 * PB, b1 * PB, part);
+  } else if (row < rows) {
+    if (it.slot >= 0) {
+      const long long at = part + row - tile0;
+      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
+              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t0 = row / G;
+      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
+              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
+                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
+    }
+  }
   __syncthreads();   // the next item's loads go to the same LDS
 }
 
@@ -1429,6 +1420,42 @@ __device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, 
   constexpr int PER = 1024 / D, SL = D / 16;   // rows per load, slots of a row
   const int r = i * PER + lane / SL, ch = (lane % SL) ^ (V ? pt_xv8<D>(r) : pt_xk8<D>(r));
   gm_dma16s(group, (unsigned)r * row_bytes + ch * 16, lds);
+}
+
+// Writes the rows row0 .. of one wave, of a tile that begins at row tile0: as outputs, or as a part (whose first row is
+// `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite. (For these pages: with pt_wide's
+// end as this function the 16-bit kernel takes other registers, and one token 14.1 us rather than 13.7.)
+template <int DT, int D>
+__device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
+                                       int rows, int p0, int p1, long long part, bool odd) {
+  const int G = a.H / a.KVH;
+  const float l = w.row_sum();
+  const int row = row0 + w.fr;
+  if (row0 < rows && (odd || w.bad_output())) {
+    pt_rows<DT, D, true>(a, it, tile0, row0, min(row0 + 32, rows), 1, p0, p1, part);
+  } else if (row < rows) {
+    if (it.slot >= 0) {
+      const long long at = part + row - tile0;
+      if (w.hi == 0) *(float2*)(a.part_ml + at * 2) = make_float2(w.m, l);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(float4*)(a.part_o + at * D + 32 * t + 8 * i + 4 * w.hi) =
+              make_float4(w.o[t][4 * i], w.o[t][4 * i + 1], w.o[t][4 * i + 2], w.o[t][4 * i + 3]);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t0 = row / G;
+      uint16_t* out = (uint16_t*)a.out + ((long long)(it.q.start + t0) * a.H + it.h * G + row - t0 * G) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(uint2*)(out + 32 * t + 8 * i + 4 * w.hi) =
+              make_uint2(gm_pack2<DT>(w.o[t][4 * i] * inv, w.o[t][4 * i + 1] * inv),
+                         gm_pack2<DT>(w.o[t][4 * i + 2] * inv, w.o[t][4 * i + 3] * inv));
+    }
+  }
 }
 
 // Work, dealt out in equal ranges to the last block: narrow tiles' blocks to waves, wide tiles' to workgroups. A range begins
@@ -1811,7 +1838,7 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
   const int rows = it.q.n * (a.H / a.KVH);
   const long long part = (long long)it.slot * PT_NARROW;
   pt_tell(a, it, row0 + w.fr, rows, part + w.fr, 0);
-  pt_end<DT, D, true>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, part, __ballot(odd) != 0ull);
+  pt_end<DT, D>(a, it, w, row0, row0, rows, b0 * PB, b1 * PB, part, __ballot(odd) != 0ull);
 }
 
 // A workgroup's range of the wide tiles. The next item's first block is on its way while the last of the present one is
@@ -1970,7 +1997,7 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
     odd = __syncthreads_or(odd);
     const long long part = (long long)8 * a.grid_narrow * PT_NARROW + (long long)it.slot * PT_WIDE;   // (behind the narrow tiles')
     pt_tell(a, it, row0 + w.fr, rows, part + row0 + w.fr - tile0, 1);
-    pt_end<DT, D, true>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, odd);
+    pt_end<DT, D>(a, it, w, tile0, row0, rows, b0 * PB, b1 * PB, part, odd);
     if (last) return;
     it = nx, odd = odd_next;
   }
@@ -2038,10 +2065,10 @@ __device__ __forceinline__ void pt_attn8_body(const PagedAttnArgs& a) {
   }
 }
 
-// Adds parts s0 .. s1 - 1 of one row to its maximum, sum and the lane's 4 dims (by a wave): part s lies `rel(s)` slots of R
+// Adds S parts of one row to its maximum, sum and the lane's 4 dims (by a wave): part s lies `rel(s)` slots of R
 // rows after row `first` of the parts. L and x are then the lane's own, to be summed over lanes (pt_gathered).
 template <int D, int R, typename F>
-__device__ __forceinline__ void pt_gather(const PagedAttnArgs& a, long long first, int s0, int s1, F rel, float& M, float& L,
+__device__ __forceinline__ void pt_gather(const PagedAttnArgs& a, long long first, int S, F rel, float& M, float& L,
                                           float (&x)[4]) {
   // a load covers PER parts: lane (part, 4 dims); a batch is eight of them
   constexpr int LN = D / 4, PER = 64 / LN;
@@ -2049,8 +2076,8 @@ __device__ __forceinline__ void pt_gather(const PagedAttnArgs& a, long long firs
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1e-37f);
   const float* mls = a.part_ml + first * 2;
   const float* os = a.part_o + first * D;
-  for (; s0 < s1; s0 += 64) {
-    const int n = min(64, s1 - s0);
+  for (int s0 = 0; s0 < S; s0 += 64) {
+    const int n = min(64, S - s0);
     const float2 ml = *(const float2*)(mls + rel(s0 + min(lane, n - 1)) * R * 2);
     float4 v[8];
     auto fetch = [&](int j) {   // (past the last part: it again, weighed 0)
@@ -2100,7 +2127,7 @@ __device__ __forceinline__ void pt_put(uint16_t* out, float L, const float (&x)[
 template <int DT, int D, int R, typename F>
 __device__ __forceinline__ void pt_join(const PagedAttnArgs& a, long long first, int S, F rel, uint16_t* out) {
   float M = -INFINITY, L = 0.f, x[4] = {};
-  pt_gather<D, R>(a, first, 0, S, rel, M, L, x);
+  pt_gather<D, R>(a, first, S, rel, M, L, x);
   pt_gathered<D>(L, x);
   pt_put<DT, D>(out, L, x);
 }
@@ -2210,7 +2237,8 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
       const int S = j.y >> 1;
       if (S < 2) continue;
       float M = -INFINITY, L = 0.f, x[4] = {};
-      pt_gather<D, 1>(a, j.x, S * wave / W, S * (wave + 1) / W, [&](int s) { return far(j, s); }, M, L, x);
+      const int from = S * wave / W;
+      pt_gather<D, 1>(a, j.x, S * (wave + 1) / W - from, [&](int s) { return far(j, from + s); }, M, L, x);
       pt_gathered<D>(L, x);
       if (lane < LN)
 #pragma unroll
