@@ -190,7 +190,8 @@ extern "C" __global__ void __launch_bounds__(256) k_index_copy(const IndexCopyAr
     if (idx < 0 || idx >= a.dim_size) continue;
     const long long so = o * a.src_so + j * a.src_sj + i * a.src_si;
     const long long dof = (o * a.dim_size + idx) * a.inner + i;
-    if (a.elem_bytes == 2) ((uint16_t*)a.dst)[dof] = ((const uint16_t*)a.src)[so];
+    if (a.elem_bytes == 1) ((unsigned char*)a.dst)[dof] = ((const unsigned char*)a.src)[so];
+    else if (a.elem_bytes == 2) ((uint16_t*)a.dst)[dof] = ((const uint16_t*)a.src)[so];
     else if (a.elem_bytes == 4) ((uint32_t*)a.dst)[dof] = ((const uint32_t*)a.src)[so];
     else ((uint64_t*)a.dst)[dof] = ((const uint64_t*)a.src)[so];
   }
