@@ -184,6 +184,10 @@ def generate_chain(ops: list[ChainOp], ext: list[TView], out_shape: tuple[int, .
             expr = table[op.op_type].format(a=operand(op.operands[0], fl))
         if fl and op.out_dtype in ("bfloat16", "float16"):
             expr = f"round_to({expr}, {DTYPE_CODE[op.out_dtype]})"
+        elif op.out_dtype == "uint8":   # a byte, modulo 256; truth values share its code, not its values
+            expr = f"(long long)(unsigned char)(long long)({expr})"
+        elif op.out_dtype == "bool":
+            expr = f"(({expr}) != 0)"
         body.append(f"    const {ctype} t{j} = {expr};")
         vals.append((f"t{j}", op.out_dtype))
     last, ldt = vals[-1]
@@ -198,8 +202,8 @@ def generate_chain(ops: list[ChainOp], ext: list[TView], out_shape: tuple[int, .
         body.append(f"    ((long long*)a.out)[i] = (long long)({last});")
     elif out_dtype == "int32":
         body.append(f"    ((int*)a.out)[i] = (int)({last});")
-    else:
-        body.append(f"    ((unsigned char*)a.out)[i] = (unsigned char)(({last}) != 0);")
+    else:   # uint8, or bool as 0 and 1
+        body.append(f"    ((unsigned char*)a.out)[i] = (unsigned char)({last});")
     text = "\n".join(body)
     h = hashlib.sha1(text.encode()).hexdigest()[:16]
     name = f"fused_ew_{h}"
