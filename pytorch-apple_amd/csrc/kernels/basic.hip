@@ -59,6 +59,8 @@ extern "C" __global__ void __launch_bounds__(256) k_fill(const FillArgs a) {
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n; i += stride) {
     if (a.dtype == HS_I64) ((long long*)a.out)[i] = (long long)a.value;
     else if (a.dtype == HS_F64) ((double*)a.out)[i] = a.value;
+    else if (a.dtype == HS_I32) ((int*)a.out)[i] = (int)a.value;
+    else if (a.dtype == HS_U8) ((unsigned char*)a.out)[i] = (unsigned char)(int)a.value;   // (truth values come as 0 or 1)
     else st_f(a.out, i, a.dtype, (float)a.value);
   }
 }

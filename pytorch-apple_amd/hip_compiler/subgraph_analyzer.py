@@ -1627,10 +1627,12 @@ class Lowering:
         out = node.outputs[0]
         o = self.new_storage(out.name, out.shape, out.dtype)
         n = o.numel
+        value = float(node.attrs.get("fill_value", 0.0))
+        if out.dtype == "bool":
+            value = float(value != 0)
         self.emit(LaunchStep(
             kind="special", kernel="k_fill", module="basic", arg_struct="FillArgs",
-            args=dict(out=self.ref(o), n=n, value=float(node.attrs.get("fill_value", 0.0)),
-                      dtype=DTYPE_CODE[out.dtype]),
+            args=dict(out=self.ref(o), n=n, value=value, dtype=DTYPE_CODE[out.dtype]),
             grid=grid1d(n), inputs=[], outputs=[out.name], params={"total": n}))
         self.views[out.name] = o
 

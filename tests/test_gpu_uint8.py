@@ -3,8 +3,10 @@
 import pytest
 import torch
 
+import quant_ref as Q
+import serving_ref as R
 from conftest import gpu_available
-from test_gpu_serving import _run
+from test_gpu_serving import _meta, _rand, _run
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a ROCm GPU")]
 
@@ -77,3 +79,40 @@ def test_truth_values_add_to_truth_values(backend):
     for op, want in (("aten.add.Tensor", x + y), ("aten.mul.Tensor", x * y)):
         got, = _run(_graph([(op, ["x", "y"], {}, "z")], {"x": x, "y": y}), backend, {"x": x, "y": y})
         assert got.dtype == torch.bool and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,value", [("uint8", 127), ("uint8", 255), ("uint8", 0), ("bool", True), ("bool", False), ("bool", 0.5),
+                                         ("int32", 16777217), ("int32", -5), ("int64", 16777217), ("float32", 1.5)])
+def test_tensors_of_one_number(backend, dtype, value):
+    from irgen.builder import IRBuilder
+
+    b = IRBuilder("Full")
+    x = b.input("x", [1], "float32")
+    b.output(b.op("aten.full.default", [], {"size": [5, 7], "fill_value": value, "dtype": dtype}), b.op("aten.neg.default", [x]))
+    got, _ = _run(b.to_dict(), backend, {"x": torch.ones(1)})
+    want = torch.full((5, 7), value, dtype=DT[dtype])
+    assert got.dtype == want.dtype and torch.equal(got, want)
+
+
+def test_attention_over_a_clone_and_powers_of_one_number(backend):
+    """A module that clones its k pages and makes its values' powers with torch.full, exported as one device program."""
+    from hip_compiler import is_hip_op_supported
+    from irgen.exporter import extract_ir
+    from npu_compiler import partition
+
+    class Step(torch.nn.Module):
+        def forward(self, q, kp, vp, ks, table, start, kv):
+            vs = torch.full((9, 2, 16), 121, dtype=torch.uint8)
+            return torch.ops.serving.paged_quant_attention(q, kp.clone(), vp, ks, vs, table, start, kv, 0.125)
+
+    bt = R.batch([5, 1, 0], [60, 17, 3], 16, pad=2, seed=4, spare=2)
+    assert bt["pages"] == 9
+    kp, vp, ks, vs = Q.pools8(bt, 2, 16, 64, stale=False)
+    vs = torch.full_like(vs, 121)
+    q = _rand(9, bt["rows"], 4, 64, dtype="bfloat16")
+    args = (q, kp, vp, ks, *_meta(bt).values())
+    ir = extract_ir(Step(), args, "step")
+    assert [s.target for s in partition(ir, is_hip_op_supported).steps] == ["npu"]
+    got, = _run(ir, backend, {i["name"]: a for i, a in zip(ir["graph_inputs"], args)})
+    out, mag, big = Q.attention64(q, (kp, vp, ks, vs), bt, 16, 0.125)
+    assert ((got.double() - out).abs() <= R.attention_tol("bfloat16", 64, 60, out, mag, big)).all()
