@@ -291,8 +291,8 @@ extern "C" __global__ void __launch_bounds__(256) k_argmax(const ReduceLastArgs 
 
 // ---------------------------------------------------------------- generic batched matmul
 
-// One output element per thread, fp32 accumulation, one rounding. For shapes that
-// no fused kernel claims (e.g. unpatterned attention); not a performance path.
+// One output element per thread, fp32 accumulation, one rounding (integers: 64 bits, modulo the type).
+// For shapes that no fused kernel claims (e.g. unpatterned attention); not a performance path.
 extern "C" __global__ void __launch_bounds__(256) k_bmm(const BmmArgs a) {
   long long nb = 1;
   for (int d = 0; d < a.nbatch; ++d) nb *= a.batch_shape[d];
@@ -307,6 +307,15 @@ extern "C" __global__ void __launch_bounds__(256) k_bmm(const BmmArgs a) {
       b /= a.batch_shape[d];
       ao += c * a.a_bstride[d];
       bo += c * a.b_bstride[d];
+    }
+    if (a.c_dtype == HS_I64 || a.c_dtype == HS_I32 || a.c_dtype == HS_U8) {
+      long long sum = 0;
+      for (long long k = 0; k < a.K; ++k)
+        sum += ld_i(a.a, ao + m * a.a_sm + k * a.a_sk, a.a_dtype) * ld_i(a.b, bo + k * a.b_sk + n * a.b_sn, a.b_dtype);
+      if (a.c_dtype == HS_I64) ((long long*)a.c)[t] = sum;
+      else if (a.c_dtype == HS_I32) ((int*)a.c)[t] = (int)sum;
+      else ((unsigned char*)a.c)[t] = (unsigned char)sum;
+      continue;
     }
     float acc = 0.f;
     for (long long k = 0; k < a.K; ++k)
