@@ -1337,14 +1337,17 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 // ------------------------------------------------------------------ pages of 8 bits
 //
 // The same tiles over e4m3 numbers K_jd 2^ke_j and V_jd 2^ve_j. The products stay in 16 bits: e4m3 queries or probabilities
-// would carry 3 bits of mantissa into every output. Numbers of 4 bits are exact in both 16-bit types, so what a tile
-// computes is the 16-bit tile's result on the dequantised pages.
+// would carry 3 bits of mantissa into every output. Numbers of 4 bits are exact in bfloat16, and in float16 while they are
+// multiples of 2^-24, which e4m3 numbers times 2^-15 (byte 112) are. Keys of smaller powers enter float16 products without
+// them, and their scores are multiplied by them in 32 bits: whether a block (wide: a group of 16 positions) has such is one
+// test of its bytes (a wide tile's waves tell each other in LDS: a mixed step in float16 67.8 -> 69.5 us).
 //   * Narrow: half the bytes come to LDS, and become 16 bits on the way from there to the matrix instructions. A lane of
 //     K's operand holds one position, so 2^ke_j comes with the conversion. A lane of V's holds eight positions of one dim:
 //     2^ve_j goes to the probabilities, which are therefore taken in bfloat16 (whose range holds any power of two) whatever the
-//     queries' type, for float16 in two parts, the second the first's rounding error, each with its product: float16's
-//     own 11 bits at least. Bound by memory, beside which the second product costs nothing: 64 decodes of up to 4,096 positions
-//     (32 + 8 heads of 128, 412 MB) take 88 us, 4.7 TB/s (153 from 16-bit pages), four of up to 131,071 (12 + 2) 42 (76).
+//     queries' type, for float16 in two parts, the second the first's rounding error, each with its product: float16's own
+//     11 bits at least, where bfloat16's outputs have 8 bits as its probabilities do. Bound by memory, which hides the second
+//     product: 64 decodes of up to 4,096 positions (32 + 8 heads of 128, 412 MB) take 88 us, 4.7 TB/s (153 from 16-bit pages),
+//     four of up to 131,071 (12 + 2) 42 (76).
 //   * Wide: bound by the matrix cores, so each block is converted once for all four waves, powers of two included, by way of
 //     registers one block ahead, into the LDS layout of 16-bit pages; the rest is the 16-bit tile. The conversion's vector
 //     instructions and LDS writes come on top of the softmax's: 409 tokens over 30,409 positions (12 + 2 heads) take 106 us, 0.72
@@ -1354,7 +1357,8 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 // K in float16 can overflow where 2^ke is 2^8 or more (keys above 57,344), bfloat16 where a power is 2^120; probabilities times
 // powers below 2^-100 reach the end of bfloat16; byte 255 is NaN: tiles that see such a byte in an open place are done row
 // by row, like those with outputs that are not finite. (0, what was never written, is none of them: it counts as 2^-127 or 0.
-// float16 below 2^-14 takes steps of 2^-24, of keys as of any float16 key.)
+// A wide tile holds V in float16, in steps of 2^-24 below 2^-14: half a step, 2^-25, is as much as the rounding of outputs so
+// small is off.)
 
 template <int DT>
 constexpr unsigned pt_least_odd = DT == HS_F16 ? 135u : 247u;   // odd power bytes: 1 .. 26, and from here on
@@ -1366,6 +1370,24 @@ __device__ __forceinline__ bool pt_any_odd(uint32_t w, unsigned least) {
   const uint32_t low = w & (0x7f * ONES), top = w & (0x80 * ONES);
   const uint32_t from_least = (low + (256u - least) * ONES) & top, from_1 = low + 0x7f * ONES, from_27 = low + (128u - 27u) * ONES;
   return (from_least | (from_1 & ~from_27 & ~w & (0x80 * ONES))) != 0;
+}
+
+// The first power byte from which the conversion to DT is exact for every number, which are multiples of 2^-9 (bfloat16: for all
+// that are not odd).
+template <int DT>
+constexpr unsigned pt_exact_from = DT == HS_F16 ? 112u : 0u;
+// whether one of four bytes is below `from` (0 .. 128)
+__device__ __forceinline__ bool pt_any_below(uint32_t w, unsigned from) {
+  constexpr uint32_t ONES = 0x01010101u;
+  return ((((w & (0x7f * ONES)) + (128u - from) * ONES) | w) & (0x80 * ONES)) != 0x80 * ONES;
+}
+
+// four scores, s[at ..], times the powers of four bytes
+__device__ __forceinline__ void pt_times_powers(pt_f32x16& s, int at, uint32_t u) {
+  s[at] *= __uint_as_float((u << 23) & 0x7f800000u);
+  s[at + 1] *= __uint_as_float((u << 15) & 0x7f800000u);
+  s[at + 2] *= __uint_as_float((u << 7) & 0x7f800000u);
+  s[at + 3] *= __uint_as_float((u >> 1) & 0x7f800000u);
 }
 
 // eight e4m3 numbers times 2^(power - 127) as DT
@@ -1470,6 +1492,12 @@ __device__ __forceinline__ void pt_tell(const PagedAttnArgs& a, const PtItem8& i
   if (it.parts && row < rows && (threadIdx.x & 63) < 32)
     ((int2*)a.joins)[(long long)(it.q.start + t) * a.H + it.h * G + row - t * G] = make_int2((int)part, 2 * it.parts + wide);
 }
+
+// Of a block of a wide tile in float16: whether the keys' powers of its groups of 16 positions enter by the scores (a byte
+// each), and those powers
+struct PtPowers {
+  uint32_t after, k[16];
+};
 
 struct PtList8 {
   union {
@@ -1741,7 +1769,10 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    odd = odd || pt_any_odd(pw[lane & 31], pt_least_odd<DT>);
+    const uint32_t four = pw[lane & 31];
+    odd = odd || pt_any_odd(four, pt_least_odd<DT>);
+    // K's powers enter with the conversion where it is exact, else by the scores (uniform)
+    const bool after = (__ballot(pt_any_below(four, pt_exact_from<DT>)) & 0xffffull) != 0;
     uint32_t vp[NB][4];   // V's powers, at the places of the lane's scores
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
@@ -1757,7 +1788,7 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
       for (int ks = 0; ks < KS; ++ks) k[ks] = read(0, ks);
 #pragma unroll
       for (int sb = 0; sb < NB; ++sb) {
-        const float power = __uint_as_float((uint32_t)((const unsigned char*)pw)[sb * 32 + w.fr] << 23);
+        const float power = after ? 1.f : __uint_as_float((uint32_t)((const unsigned char*)pw)[sb * 32 + w.fr] << 23);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[sb][e] = 0.f;
         __builtin_amdgcn_sched_barrier(0);
@@ -1770,6 +1801,11 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
         }
       }
     }
+    if (after)
+#pragma unroll
+      for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pt_times_powers(s[sb], 4 * i, pw[sb * 8 + 2 * i + w.hi]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's rows and the powers are in registers
     if (more) {
       bad_next = seek(blk + 1);
@@ -1844,13 +1880,14 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
 // A workgroup's range of the wide tiles. The next item's first block is on its way while the last of the present one is
 // computed, its pages' ids before that. XCD i (workgroups i, i + 8, ...) takes neighbouring ranges: they read the same blocks.
 template <int DT, int D>
-__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, char* lds, int (*slots)[64]) {
+__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, char* lds, int (*slots)[64], PtPowers* kpw) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V, in 16 bits
   constexpr int PCS = D / 64;                                           // 16-byte pieces of a row that a thread takes, of K and of V
   constexpr int WB = 64 / NG, TD = D / 32;                              // blocks of a window; output tiles
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.H / a.KVH;
+  if (DT == HS_F16 && tid < 2) kpw[tid].after = 0;
   PtRanges r;
-  r.total = pt_build_wide8(a, t);
+  r.total = pt_build_wide8(a, t);   // (a barrier)
   r.workers = (int)max(1ull, min((unsigned long long)a.grid_wide, r.total / (PT_RANGE_LEAST * PB * G)));
   r.range = r.total / r.workers;
   const int each = (r.workers + 7) >> 3, me = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
@@ -1903,6 +1940,7 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
     issue(x.b0);
   };
   int st = 0;   // LDS stage of the present block
+  unsigned told = 0;
   // what was loaded, as 16 bits, to the other stage; zeros in the places that are closed to every row of the tile
   auto stage = [&](int blk, int pend) {   // returns whether a power is odd
     if (blk * PB + PB - 1 > pend || bad_next) {
@@ -1913,7 +1951,18 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
       }
     }
     const int odd = pt_odd(kb, pt_least_odd<DT>) | pt_odd(vb, pt_least_odd<DT>);
-    const float kp = __uint_as_float(kb << 23), vp = __uint_as_float(vb << 23);
+    float kp = __uint_as_float(kb << 23);
+    const float vp = __uint_as_float(vb << 23);
+    if constexpr (DT == HS_F16) {   // a group whose keys float16 does not hold exactly: its powers enter by the scores
+      const bool after = __ballot(kb < pt_exact_from<DT>) != 0;
+      if (after || (told >> st & 1)) {   // (told: of the stages that say so, bit 0 is of stage 1)
+        PtPowers& to = kpw[st ^ 1];
+        if (lane == 0) ((unsigned char*)&to.after)[wave] = after;
+        if (after) kp = 1.f;
+        if (part == 0) ((unsigned char*)to.k)[sr] = (unsigned char)kb;
+        told = (told & (2u >> st)) | (unsigned)after << st;
+      }
+    }
     const unsigned kat = kwr + (st ^ 1) * 2 * BYTES, vat = vwr + (st ^ 1) * 2 * BYTES;
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
@@ -1969,9 +2018,19 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
         begin(nx, id);
       }
       const bool some = blk * PB <= pmax;   // wave-uniform
+      const uint32_t groups = DT == HS_F16 ? kpw[st].after : 0;
       const unsigned kat = krd + st * 2 * BYTES, vat = vrd + st * 2 * BYTES;
       pt_f32x16 s[NB];
       if (some) w.template scores_of<NB>([&](int sb, int ks) { return *(const uint4*)(lds + (kat ^ (ks * 32)) + sb * 32 * RB); }, s);
+      if constexpr (DT == HS_F16) {
+        const unsigned after = __builtin_amdgcn_readfirstlane(groups);
+        if (some && after)
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            if ((after >> (8 * g)) & 1)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) pt_times_powers(s[g / 2], 8 * (g % 2) + 4 * i, kpw[st].k[g * 4 + 2 * i + hi]);
+      }
       if (!here && !last) w.queries(a, nx, nx.tile * PT_WIDE + wave * 32);   // (this item's are done with)
       if (some) {
         if (!(blk * PB + PB - 1 <= pmin && bad == 0)) w.template mask<NB>(s, blk * PB, bad);
@@ -2049,9 +2108,10 @@ __device__ __forceinline__ void pt_attn8_body(const PagedAttnArgs& a) {
   __shared__ int ids[4][64];
   __shared__ uint32_t powers[4][64];
   __shared__ PtList8 t;
+  __shared__ PtPowers kpw[2];
   const int nw = a.grid_wide;
   if ((int)blockIdx.x < nw) {
-    pt_wide8<DT, D>(a, t, lds, ids);
+    pt_wide8<DT, D>(a, t, lds, ids, kpw);
     return;
   }
   const int hi = nw ? PT_NARROW : ANY, w = (blockIdx.x - nw) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -258,7 +258,8 @@ def paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, pa
 
 def paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, scale, page_layout="hnd"):
     """``paged_attention`` over the numbers that pools of 8 bits hold. A power byte of 255 makes them NaN. They, and their
-    products with q before the scale, are held in 32 bits."""
+    products with q before the scale, are held in 32 bits; where q is float16, a device may round values below 2^-14 to
+    multiples of 2^-24, as such outputs are."""
     check_paged_quant_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, kv_len, page_layout)
     return _attention(q, dequantise(k_pages, k_scales, page_layout), dequantise(v_pages, v_scales, page_layout), block_table,
                       q_start, kv_len, scale, page_layout)
