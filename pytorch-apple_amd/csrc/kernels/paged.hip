@@ -1356,7 +1356,7 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 //     mixed step.)
 // K in float16 can overflow where 2^ke is 2^8 or more (keys above 57,344), bfloat16 where a power is 2^120; probabilities times
 // powers below 2^-100 reach the end of bfloat16; byte 255 is NaN: tiles that see such a byte in an open place are done row
-// by row, like those with outputs that are not finite. (0, what was never written, is none of them: it counts as 2^-127 or 0.
+// by row, like those with outputs that are not finite. (0, what was never written, is none of them: it counts as 0.
 // A wide tile holds V in float16, in steps of 2^-24 below 2^-14: half a step, 2^-25, is as much as the rounding of outputs so
 // small is off.)
 
@@ -1373,13 +1373,19 @@ __device__ __forceinline__ bool pt_any_odd(uint32_t w, unsigned least) {
 }
 
 // The first power byte from which the conversion to DT is exact for every number, which are multiples of 2^-9 (bfloat16: for all
-// that are not odd).
+// that are not odd, but 0, which the conversion would take as 2^-127).
 template <int DT>
-constexpr unsigned pt_exact_from = DT == HS_F16 ? 112u : 0u;
-// whether one of four bytes is below `from` (0 .. 128)
+constexpr unsigned pt_exact_from = DT == HS_F16 ? 112u : 1u;
+// whether one of four bytes is below `from` (1 .. 128)
 __device__ __forceinline__ bool pt_any_below(uint32_t w, unsigned from) {
   constexpr uint32_t ONES = 0x01010101u;
   return ((((w & (0x7f * ONES)) + (128u - from) * ONES) | w) & (0x80 * ONES)) != 0x80 * ONES;
+}
+
+// four e4m3 numbers times 0: NaN (0x7f, 0xff) or 0
+__device__ __forceinline__ uint32_t pt_times_0(uint32_t w) {
+  constexpr uint32_t ONES = 0x01010101u;
+  return ((((w & (0x7f * ONES)) + ONES) >> 7) & ONES) * 0x7f;
 }
 
 // four scores, s[at ..], times the powers of four bytes
@@ -1948,6 +1954,13 @@ __device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, cha
         kb = vb = 127;
 #pragma unroll
         for (int i = 0; i < PCS; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (__ballot(kb == 0 || vb == 0)) {   // (the conversion takes a byte of 0 as 2^-127)
+#pragma unroll
+      for (int i = 0; i < PCS; ++i) {
+        if (kb == 0) kr[i] = make_uint4(pt_times_0(kr[i].x), pt_times_0(kr[i].y), pt_times_0(kr[i].z), pt_times_0(kr[i].w));
+        if (vb == 0) vr[i] = make_uint4(pt_times_0(vr[i].x), pt_times_0(vr[i].y), pt_times_0(vr[i].z), pt_times_0(vr[i].w));
       }
     }
     const int odd = pt_odd(kb, pt_least_odd<DT>) | pt_odd(vb, pt_least_odd<DT>);
