@@ -365,8 +365,9 @@ __device__ __forceinline__ void append_heads(const PagedAppendArgs& a) {
         const uint32_t uw[4] = {w0.x, w0.y, w0.z, w0.w}, vw[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[2 * j] *= r * gm_lo<DT>(uw[j]), x[2 * j + 1] *= r * gm_hi<DT>(uw[j]);
-          y[2 * j] *= r * gm_lo<DT>(vw[j]), y[2 * j + 1] *= r * gm_hi<DT>(vw[j]);
+          // (x r first: r times a weight may pass 32 bits where the result does not)
+          x[2 * j] = x[2 * j] * r * gm_lo<DT>(uw[j]), x[2 * j + 1] = x[2 * j + 1] * r * gm_hi<DT>(uw[j]);
+          y[2 * j] = y[2 * j] * r * gm_lo<DT>(vw[j]), y[2 * j + 1] = y[2 * j + 1] * r * gm_hi<DT>(vw[j]);
         }
       }
     }
