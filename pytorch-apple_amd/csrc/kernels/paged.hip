@@ -433,7 +433,18 @@ __device__ __forceinline__ float pg_cached(const void* p, long long i, int dt) {
   else return ld_f(p, i, dt);
 }
 template <bool F8>
-__device__ __forceinline__ void attn_any_body(const PagedAttnArgs& a) {
+struct PtArgsOf {
+  typedef PagedAttnArgs type;
+};
+template <>
+struct PtArgsOf<true> {
+  typedef PagedQuantAttnArgs type;
+};
+template <bool F8>
+using PtArgs = typename PtArgsOf<F8>::type;
+
+template <bool F8>
+__device__ __forceinline__ void attn_any_body(const PtArgs<F8>& a) {
   __shared__ float q[PG_ANY_D], p[64];
   __shared__ int at[64];   // page of each of the step's positions, -1: closed
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.H / a.KVH);
@@ -483,7 +494,7 @@ __device__ __forceinline__ void attn_any_body(const PagedAttnArgs& a) {
       st_f(a.out, ((long long)row * a.H + h) * a.D + i * 64 + lane, a.dtype, l == 0.f ? 0.f : o[i] / l);
 }
 extern "C" __global__ void __launch_bounds__(64) k_paged_attn_any(const PagedAttnArgs a) { attn_any_body<false>(a); }
-extern "C" __global__ void __launch_bounds__(64) k_paged_quant_attn_any(const PagedAttnArgs a) { attn_any_body<true>(a); }
+extern "C" __global__ void __launch_bounds__(64) k_paged_quant_attn_any(const PagedQuantAttnArgs a) { attn_any_body<true>(a); }
 
 // ------------------------------------------------------------------ attention on matrix cores
 //
@@ -1018,7 +1029,7 @@ __device__ __forceinline__ float pt_cached(const void* p, long long i) {
 // scores, sum of exponentials and the lane's outputs (dims lane * E ..), times 2^pt_up as the tiles' (they may be joined
 // with them). For tiles whose product is not finite.
 template <int DT, int D, bool F8>
-__device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it, int row, int p0, int p1, float& m,
+__device__ __forceinline__ void pt_row(const PtArgs<F8>& a, const PtItem& it, int row, int p0, int p1, float& m,
                                        float& l, float (&x)[D / 64]) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63, G = a.H / a.KVH, t = row / G;
@@ -1065,7 +1076,7 @@ __device__ __forceinline__ void pt_row(const PagedAttnArgs& a, const PtItem& it,
 
 // rows r0, r0 + step, ... of a tile one by one, written as the tile's rows are (part: index of its first partial row)
 template <int DT, int D, bool F8 = false>
-__device__ __forceinline__ void pt_rows(const PagedAttnArgs& a, const PtItem& it, int tile0, int r0, int r1, int step, int p0,
+__device__ __forceinline__ void pt_rows(const PtArgs<F8>& a, const PtItem& it, int tile0, int r0, int r1, int step, int p0,
                                      int p1, long long part) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63, G = a.H / a.KVH;
@@ -1455,7 +1466,7 @@ __device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, 
 // `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite. (For these pages: with pt_wide's
 // end as this function the 16-bit kernel takes other registers, and one token 14.1 us rather than 13.7.)
 template <int DT, int D>
-__device__ __forceinline__ void pt_end(const PagedAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
+__device__ __forceinline__ void pt_end(const PagedQuantAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
                                        int rows, int p0, int p1, long long part, bool odd) {
   const int G = a.H / a.KVH;
   const float l = w.row_sum();
@@ -1494,7 +1505,7 @@ struct PtItem8 : PtItem {
 };
 
 // A tile's first part tells k_paged_quant_combine where each of its rows' parts are: [first part's row, 2 parts + kind].
-__device__ __forceinline__ void pt_tell(const PagedAttnArgs& a, const PtItem8& it, int row, int rows, long long part, int wide) {
+__device__ __forceinline__ void pt_tell(const PagedQuantAttnArgs& a, const PtItem8& it, int row, int rows, long long part, int wide) {
   const int G = a.H / a.KVH, t = row / G;
   if (it.parts && row < rows && (threadIdx.x & 63) < 32)
     ((int2*)a.joins)[(long long)(it.q.start + t) * a.H + it.h * G + row - t * G] = make_int2((int)part, 2 * it.parts + wide);
@@ -1700,7 +1711,7 @@ __device__ __forceinline__ PtItem8 pt_item_wide8(const PagedAttnArgs& a, const P
 }
 
 template <int DT, int D>
-__device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8& it, char* lds, int (*slots)[64], uint32_t (*powers)[64]) {
+__device__ __forceinline__ void pt_narrow8(const PagedQuantAttnArgs& a, const PtItem8& it, char* lds, int (*slots)[64], uint32_t (*powers)[64]) {
   using C = PtNarrow<DT, D, true>;
   constexpr int PB = C::PB, NB = C::NB, NG = C::NG, LPG = C::LPG, TD = D / 32;
   constexpr int LD = NG * LPG;   // loads of a block's K, and of its V
@@ -1887,7 +1898,7 @@ __device__ __forceinline__ void pt_narrow8(const PagedAttnArgs& a, const PtItem8
 // A workgroup's range of the wide tiles. The next item's first block is on its way while the last of the present one is
 // computed, its pages' ids before that. XCD i (workgroups i, i + 8, ...) takes neighbouring ranges: they read the same blocks.
 template <int DT, int D>
-__device__ __forceinline__ void pt_wide8(const PagedAttnArgs& a, PtList8& t, char* lds, int (*slots)[64], PtPowers* kpw) {
+__device__ __forceinline__ void pt_wide8(const PagedQuantAttnArgs& a, PtList8& t, char* lds, int (*slots)[64], PtPowers* kpw) {
   constexpr int PB = 64, NB = 2, NG = 4, RB = 2 * D, BYTES = PB * RB;   // bytes of a block's K, and of its V, in 16 bits
   constexpr int PCS = D / 64;                                           // 16-byte pieces of a row that a thread takes, of K and of V
   constexpr int WB = 64 / NG, TD = D / 32;                              // blocks of a window; output tiles
@@ -2116,7 +2127,7 @@ __device__ __forceinline__ void pt_attn_body(const PagedAttnArgs& a) {
 
 // Over pages of 8 bits: wide tiles' workgroups first, then the narrow ones', each wave of which takes blocks of its own.
 template <int DT, int D>
-__device__ __forceinline__ void pt_attn8_body(const PagedAttnArgs& a) {
+__device__ __forceinline__ void pt_attn8_body(const PagedQuantAttnArgs& a) {
   constexpr int ANY = 0x7fffffff;
   __shared__ __attribute__((aligned(1024))) char lds[65536];
   __shared__ int ids[4][64];
@@ -2288,7 +2299,7 @@ __device__ __forceinline__ void pt_combine_body(const PagedAttnArgs& a) {
 // parts (4 requests over up to 131,071 positions: 6.6 us, 8.9 by 4 waves). Bound by the latency of dependent loads: 4 to 5 us
 // for decodes, 9 for 1,553 rows of 14 heads of 64, 11 for 5,963 rows of 32 heads of 128.
 template <int DT, int D, bool JOIN>
-__device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
+__device__ __forceinline__ void pt_combine8_body(const PagedQuantAttnArgs& a) {
   constexpr int LN = D / 4, PER = 64 / LN, W = JOIN ? 16 : 1;
   __shared__ float shares[W][4][LN + 2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LN;
@@ -2405,9 +2416,9 @@ __device__ __forceinline__ void pt_combine8_body(const PagedAttnArgs& a) {
 #define PT_KERNELS(NAME, DT, D)                                                                                                  \
   extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_##NAME(const PagedAttnArgs a) { pt_attn_body<DT, D>(a); }     \
   extern "C" __global__ void __launch_bounds__(256) k_paged_combine_##NAME(const PagedAttnArgs a) { pt_combine_body<DT, D>(a); }  \
-  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_quant_attn_##NAME(const PagedAttnArgs a) { pt_attn8_body<DT, D>(a); } \
-  extern "C" __global__ void __launch_bounds__(256) k_paged_quant_combine_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D, false>(a); } \
-  extern "C" __global__ void __launch_bounds__(1024) k_paged_quant_join_##NAME(const PagedAttnArgs a) { pt_combine8_body<DT, D, true>(a); }
+  extern "C" __global__ void __launch_bounds__(256, 2) k_paged_quant_attn_##NAME(const PagedQuantAttnArgs a) { pt_attn8_body<DT, D>(a); } \
+  extern "C" __global__ void __launch_bounds__(256) k_paged_quant_combine_##NAME(const PagedQuantAttnArgs a) { pt_combine8_body<DT, D, false>(a); } \
+  extern "C" __global__ void __launch_bounds__(1024) k_paged_quant_join_##NAME(const PagedQuantAttnArgs a) { pt_combine8_body<DT, D, true>(a); }
 PT_KERNELS(bf16_d128, HS_BF16, 128)
 PT_KERNELS(bf16_d64, HS_BF16, 64)
 PT_KERNELS(f16_d128, HS_F16, 128)

@@ -402,6 +402,7 @@ size_t hs_argsize(const char* s) {
   HS_SZ(DecodeLayerPtrs)
   HS_SZ(PagedAppendArgs)
   HS_SZ(PagedAttnArgs)
+  HS_SZ(PagedQuantAttnArgs)
   HS_SZ(SampleArgs)
   HS_SZ(SampleRow)
 #undef HS_SZ

@@ -182,17 +182,21 @@ def lower_paged_attention(low, node: OpNode) -> None:
     if tiled:
         qv = _aligned_rows(low, q.name, qv)
         caches = [low.aligned16(v, t.name) for t, v in zip((kp, vp, *scales), caches)]
-    kv, vv, ks, vs = [low.ref(v) for v in caches] + ([] if quant else [None, None])
+    kv, vv, *powers = (low.ref(v) for v in caches)
     args = dict(q=low.ref(qv), k_pages=kv, v_pages=vv, out=low.ref(out), part_o=None, part_ml=None,
                 **_batch(low, table, q_start, kv_len), q_rs=qv.strides[0], q_hs=qv.strides[1],
                 **_pool_strides(kp.shape, layout), pages=P, N=N, H=H, KVH=KVH, D=D, page_size=ps,
                 scale=float(node.attrs["scale"]), dtype=DTYPE_CODE[q.dtype], page_groups=0, group_magic=0, grid_wide=0,
-                grid_narrow=0, pad=0, k_scales=ks, v_scales=vs, joins=None)
+                grid_narrow=0, pad=0)
+    record = "PagedAttnArgs"
+    if quant:
+        record = "PagedQuantAttnArgs"
+        args |= dict(k_scales=powers[0], v_scales=powers[1], joins=None)
     params = {"rows": N, "seqs": B, "heads": H, "kv_heads": KVH, "head_dim": D}
     ins, outs = [t.name for t in node.inputs], [node.outputs[0].name]
     prefix = "k_paged_quant_" if quant else "k_paged_"
     if tiled is None:
-        low.emit(LaunchStep(kind="paged_attention", kernel=prefix + "attn_any", module="paged", arg_struct="PagedAttnArgs",
+        low.emit(LaunchStep(kind="paged_attention", kernel=prefix + "attn_any", module="paged", arg_struct=record,
                             args=args, grid=(N, H, 1), block=(64, 1, 1), inputs=ins, outputs=outs, params=params))
         return
     params["pieces16"] = ["q", "k_pages", "v_pages"] + (["k_scales", "v_scales"] if quant else [])
@@ -204,10 +208,12 @@ def lower_paged_attention(low, node: OpNode) -> None:
     args.update(part_o=low.scratch(outs[0] + ".part_o", 4 * part_rows * D),
                 part_ml=low.scratch(outs[0] + ".part_ml", 8 * part_rows), page_groups=groups,
                 group_magic=0 if groups == 1 else -(-2 ** 32 // groups), grid_wide=tiled["grid_wide"],
-                grid_narrow=tiled["grid_narrow"], joins=low.scratch(outs[0] + ".joins", 8 * N * H) if quant else None)
+                grid_narrow=tiled["grid_narrow"])
+    if quant:
+        args["joins"] = low.scratch(outs[0] + ".joins", 8 * N * H)
     name = f"{'bf16' if q.dtype == 'bfloat16' else 'f16'}_d{D}"
     low.emit(LaunchStep(
-        kind="paged_attention", kernel=prefix + "attn_" + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
+        kind="paged_attention", kernel=prefix + "attn_" + name, module="paged", arg_struct=record, args=dict(args),
         grid=(tiled["grid_wide"] + tiled["grid_narrow"], 1, 1), inputs=ins, outputs=outs, params={**params, "mfma": True}))
     kernel, grid, threads = "combine_", min(1024, -(-N * H // 4)), 256
     if quant and N * H <= PT_JOIN_ROWS:
@@ -215,7 +221,7 @@ def lower_paged_attention(low, node: OpNode) -> None:
     elif quant:
         grid = min(2048, -(-N * H // (4 * (256 // D))))
     low.emit(LaunchStep(
-        kind="paged_attention", kernel=prefix + kernel + name, module="paged", arg_struct="PagedAttnArgs", args=dict(args),
+        kind="paged_attention", kernel=prefix + kernel + name, module="paged", arg_struct=record, args=dict(args),
         grid=(grid, 1, 1), block=(threads, 1, 1), inputs=ins, outputs=outs, params=params))
 
 

@@ -133,12 +133,14 @@ _struct("PagedAppendArgs", [("q", P), ("k", P), ("v", P), ("k_pages", P), ("v_pa
                             ("row_stride", LL), ("pages", LL), ("N", I), ("B", I), ("M", I), ("H", I), ("KVH", I),
                             ("D", I), ("R", I), ("page_size", I), ("scaling", F), ("dtype", I), ("q_weight", P),
                             ("k_weight", P), ("k_scales", P), ("v_scales", P), ("eps", F), ("pad", I)])
-_struct("PagedAttnArgs", [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), ("table", P), ("q_start", P),
-                          ("kv_len", P), ("q_rs", LL), ("q_hs", LL), ("page_stride", LL), ("head_stride", LL),
-                          ("row_stride", LL), ("pages", LL), ("part_o", P), ("part_ml", P), ("N", I), ("B", I), ("M", I),
-                          ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
-                          ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
-                          ("pad", I), ("k_scales", P), ("v_scales", P), ("joins", P)])
+_PAGED_ATTN = [("q", P), ("k_pages", P), ("v_pages", P), ("out", P), ("table", P), ("q_start", P),
+               ("kv_len", P), ("q_rs", LL), ("q_hs", LL), ("page_stride", LL), ("head_stride", LL),
+               ("row_stride", LL), ("pages", LL), ("part_o", P), ("part_ml", P), ("N", I), ("B", I), ("M", I),
+               ("H", I), ("KVH", I), ("D", I), ("page_size", I), ("scale", F), ("dtype", I),
+               ("page_groups", I), ("group_magic", C.c_uint), ("grid_wide", I), ("grid_narrow", I),
+               ("pad", I)]
+_struct("PagedAttnArgs", _PAGED_ATTN)
+_struct("PagedQuantAttnArgs", _PAGED_ATTN + [("k_scales", P), ("v_scales", P), ("joins", P)])
 _struct("SampleRow", [("best", LL), ("mode", I),
                       ("kb", I), ("kr", I), ("kn", I), ("plo", I), ("phi", I),
                       ("pn", I), ("pad", I)])
