@@ -58,7 +58,7 @@ class PagedGenerator:
         if missing:
             raise ValueError(f"not a paged step graph: it has no input {missing}")
         self.backend = backend
-        self.pool_names = [n for n in shapes if n not in ("input_ids", *_BATCH)]   # (pages first, then their scales if any)
+        self.pool_names = [n for n in shapes if n not in ("input_ids", *_BATCH)]
         self.shapes = shapes
         self.slots, self.table_pages = shapes["block_table"][0]
         if not self.pool_names:
@@ -67,7 +67,9 @@ class PagedGenerator:
                    for n in ir["nodes"] if n["op_type"].startswith("serving.paged_")}
         if len(layouts) != 1:
             raise ValueError(f"not graphs of one page_layout: {sorted(layouts)}")
-        dims = shapes[self.pool_names[0]][0]
+        dims = next((shapes[n][0] for n in self.pool_names if len(shapes[n][0]) == 4), None)   # (powers of pages have three)
+        if dims is None:
+            raise ValueError("not a paged step graph: none of its pools has pages")
         self.pages, self.page_size = dims[0], dims[2 if layouts == {"hnd"} else 1]
         self.graphs = []   # (executor, rows, output names) of decode, if it is run, and step: no two of the same rows
         for dag, ir in ((decode, decode_ir), (step, step_ir)):
