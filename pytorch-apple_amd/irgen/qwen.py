@@ -217,7 +217,7 @@ def build_decode_ir(max_cache_len: int, cfg: QwenConfig = QWEN2_5_1_5B, argmax: 
 
 def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pages: int,
                    cfg: QwenConfig = QWEN2_5_1_5B, layout: str = "hnd", cache: str | None = None,
-                   qk_norm: bool = False) -> dict:
+                   qk_norm: bool = False, qkv_bias: bool = True) -> dict:
     """One step of a server: ``tokens`` rows (decoded tokens and prompt chunks of up to ``seqs`` sequences, packed, rows
     of no sequence behind them) over paged caches, one sampled token per sequence. No counterpart in the reference,
     whose graphs hold one sequence each.
@@ -228,7 +228,8 @@ def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pag
     [seqs]; per layer ``k_pages_{i}`` and ``v_pages_{i}``, and with ``cache`` "float8_e4m3fn", whose pages are of 8 bits,
     ``k_scales_{i}`` and ``v_scales_{i}``. Outputs: ``next_token`` int64 [seqs], then the pools, which a device updates
     in place. The weights are those of ``build_decode_ir``; with ``qk_norm`` each head of q and k is normed before the
-    rotation, by ``self_attn.q_norm.weight`` and ``self_attn.k_norm.weight`` [head_dim]."""
+    rotation, by ``self_attn.q_norm.weight`` and ``self_attn.k_norm.weight`` [head_dim]. ``qkv_bias`` False: of a model whose q, k
+    and v have no biases, as most that norm their heads."""
     b = IRBuilder("Qwen2.5_Paged")
     H, KVH, D, Hd, dt = cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.hidden, cfg.dtype
     ids = b.input("input_ids", [tokens], "int64")
@@ -245,7 +246,7 @@ def build_paged_ir(tokens: int, seqs: int, pages: int, page_size: int, table_pag
 
         def heads(name: str, n: int) -> T:
             w = b.weight(f"{pre}self_attn.{name}_proj.weight", [n * D, Hd], dt)
-            y = linear(b, h, w, b.weight(f"{pre}self_attn.{name}_proj.bias", [n * D], dt))
+            y = linear(b, h, w, b.weight(f"{pre}self_attn.{name}_proj.bias", [n * D], dt) if qkv_bias else None)
             return b.op("aten.view.default", [y], {"size": [tokens, n, D]})
 
         h = rmsnorm(b, x, b.weight(pre + "input_layernorm.weight", [Hd], dt), cfg.eps)
