@@ -77,7 +77,7 @@ def program_to_dict(prog: HIPProgram) -> dict:
 
 
 def program_from_dict(data: dict) -> HIPProgram:
-    from hip_runtime.kernels import builtin_kernels
+    from hip_runtime.kernels import STRUCTS, builtin_kernels
 
     if data.get("format") != FORMAT or data.get("version") != VERSION:
         raise ValueError(f"not a {FORMAT} v{VERSION} file")
@@ -93,6 +93,21 @@ def program_from_dict(data: dict) -> HIPProgram:
         if names is not None and step.kernel not in names:
             raise ValueError(f"module {step.module!r} holds no kernel {step.kernel!r}: the program was compiled for "
                              "other kernels, compile it again")
+    # kernels read their argument records as they are laid out now: a value that a record has no field for would be lost, and the
+    # kernel read past it. Attention over pages of 8 bits was once written with the record of 16-bit pages, which had its fields.
+    for step in prog.steps:
+        if step.module in generated:
+            continue
+        if step.arg_struct == "PagedAttnArgs" and step.kernel.startswith("k_paged_quant_"):
+            step.arg_struct = "PagedQuantAttnArgs"
+        if step.arg_struct not in STRUCTS:
+            raise ValueError(f"no argument record {step.arg_struct!r}: the program was compiled for other kernels, compile it again")
+        fields = {f[0] for f in STRUCTS[step.arg_struct]._fields_}
+        lost = sorted(k for k, v in step.args.items() if k not in fields and v is not None)
+        if lost:
+            raise ValueError(f"{step.arg_struct} of kernel {step.kernel!r} has no fields {lost}: the program was compiled for other "
+                             "kernels, compile it again")
+        step.args = {k: v for k, v in step.args.items() if k in fields}
     # k_mask_extent writes two ints per 32-query block; files written when it wrote one hold half the bytes
     for step in prog.steps:
         if step.kernel == "k_mask_extent":
