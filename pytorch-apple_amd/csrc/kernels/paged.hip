@@ -1361,7 +1361,7 @@ __device__ __forceinline__ void pt_wide(const PagedAttnArgs& a, const PtItem& it
 //     queries' type, for float16 in two parts, the second the first's rounding error, each with its product: float16's own
 //     11 bits at least, where bfloat16's outputs have 8 bits as its probabilities do. Bound by memory, which hides the second
 //     product: 64 decodes of up to 4,096 positions (32 + 8 heads of 128, 412 MB) take 88 us, 4.7 TB/s (153 from 16-bit pages),
-//     four of up to 131,071 (12 + 2) 42 (76).
+//     four of up to 131,071 (12 + 2) 40 (76).
 //   * Wide: bound by the matrix cores, so each block is converted once for all four waves, powers of two included, by way of
 //     registers one block ahead, into the LDS layout of 16-bit pages; the rest is the 16-bit tile. The conversion's vector
 //     instructions and LDS writes come on top of the softmax's: 409 tokens over 30,409 positions (12 + 2 heads) take 106 us, 0.72
@@ -1466,7 +1466,7 @@ __device__ __forceinline__ void pt_load8(const char* group, unsigned row_bytes, 
 
 // Writes the rows row0 .. of one wave, of a tile that begins at row tile0: as outputs, or as a part (whose first row is
 // `part`). `odd` (uniform): the wave's outputs are not to be used, as where they are not finite. (For these pages: with pt_wide's
-// end as this function the 16-bit kernel takes other registers, and one token 14.1 us rather than 13.7.)
+// end as this function the 16-bit kernel takes other registers, and one token 13.9 us rather than 13.6.)
 template <int DT, int D>
 __device__ __forceinline__ void pt_end(const PagedQuantAttnArgs& a, const PtItem& it, const PtWave<DT, D>& w, int tile0, int row0,
                                        int rows, int p0, int p1, long long part, bool odd) {

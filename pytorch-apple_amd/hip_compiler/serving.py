@@ -82,8 +82,10 @@ def paged_tiles(N: int, B: int, M: int, P: int, H: int, KVH: int, D: int, page_s
     Over pages of 8 bits (``quant``) the narrow tiles, whose waves stream by themselves, stay ahead longer: wide tiles from 16
     tokens per sequence. The same, with / without: 63 decodes and a chunk of 64 124 / 101, 200 132 / 108, 1,000 170 / 150, 1,800
     207 / 216; six prompts of 1,000 89 / 129, 16 of 100 23 / 34, 64 of up to 20 behind 4,000 159 / 179, of up to 14 154 / 149, of
-    up to 10 134 / 121; with 12 over 2 heads 63 and 1,000 79 / 62, 64 of up to 14 behind 4,000 59 / 66; one of 64 slots with a
-    chunk of 500 behind 4,000 55 / 63."""
+    up to 10 134 / 121; with 12 over 2 heads 63 and 1,000 79 / 62, 64 of up to 14 behind 4,000 59 / 66. A graph of many slots of
+    which one holds a long document pays for not knowing it, since every narrow tile reads and converts the whole cache again: one
+    of 64 with a chunk of 500 behind 4,000 77 / 82, behind 30,000 301 / 436, behind 100,000 922 / 1,826, of 1,000 behind 4,000 114 /
+    139, behind 30,000 576 / 1,072; with 12 over 2 heads 47 / 43, 134 / 149, 374 / 470, 61 / 63, 234 / 281."""
     if dtype not in ("bfloat16", "float16") or D not in (64, 128) or page_size % 16 or not 0 < B <= PT_MAXB or M < 1 or P < 1:
         return None
     G, block = H // KVH, 64 if quant else 8192 // (2 * D)   # positions of a narrow tile's block
