@@ -911,7 +911,7 @@ class Lowering:
         bb = V.broadcast_to(b.with_(shape=b.shape[:-2], strides=b.strides[:-2]), batch) if batch else None
         pad = 4 - len(batch)
         self.emit(LaunchStep(
-            kind="gemm_batched", kernel="k_bmm", module="basic", arg_struct="BmmArgs",
+            kind="gemm_batched", kernel="k_bmm" if c.dtype in FLOAT_DTYPES else "k_bmm_int", module="basic", arg_struct="BmmArgs",
             args=dict(a=self.ref(a), b=self.ref(b), c=self.ref(c),
                       batch_shape=list(batch) + [1] * pad,
                       a_bstride=(list(ab.strides) if ab else []) + [0] * pad,
