@@ -388,7 +388,8 @@ extern "C" __global__ void __launch_bounds__(256) k_maxpool2d(const PoolArgs a) 
       }
     }
     if (nan) best = NAN;
-    st_f(a.out, i, a.dtype, best);   // a max of stored values: exact in the input dtype
+    if (a.dtype == HS_U8) ((unsigned char*)a.out)[i] = (unsigned char)(int)best;   // (st_f would store a truth value)
+    else st_f(a.out, i, a.dtype, best);   // a max of stored values: exact in the input dtype
   }
 }
 
