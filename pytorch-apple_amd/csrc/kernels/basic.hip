@@ -21,8 +21,6 @@ extern "C" __global__ void __launch_bounds__(256) k_copy(const CopyArgs a) {
       ((long long*)a.dst)[dof] = ((const long long*)a.src)[so];
     } else if (a.sdtype == a.ddtype && (a.sdtype == HS_BF16 || a.sdtype == HS_F16)) {
       ((uint16_t*)a.dst)[dof] = ((const uint16_t*)a.src)[so];
-    } else if (a.sdtype == a.ddtype && a.sdtype == HS_U8) {   // (st_f would make truth values of uint8 numbers)
-      ((unsigned char*)a.dst)[dof] = ((const unsigned char*)a.src)[so];
     } else if (a.ddtype == HS_I64 || a.ddtype == HS_I32) {
       const long long v = (a.sdtype == HS_I64 || a.sdtype == HS_I32 || a.sdtype == HS_U8)
                               ? ld_i(a.src, so, a.sdtype) : (long long)ld_f(a.src, so, a.sdtype);
@@ -30,6 +28,22 @@ extern "C" __global__ void __launch_bounds__(256) k_copy(const CopyArgs a) {
     } else {
       st_f(a.dst, dof, a.ddtype, ld_f(a.src, so, a.sdtype));
     }
+  }
+}
+
+// The same of uint8 to uint8 and of bool to bool, which st_f would make truth values of. (As one more case of k_copy it takes
+// strided copies of 64 x 128 x 300 fp32 elements from 12.6 to 12.9 us; with one body for both, 13.2.)
+extern "C" __global__ void __launch_bounds__(256) k_copy_bytes(const CopyArgs a) {
+  const long long stride = (long long)gridDim.x * blockDim.x;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.n; i += stride) {
+    long long rem = i, so = 0, dof = 0;
+    for (int d = a.ndim - 1; d >= 0; --d) {
+      const long long c = rem % a.shape[d];
+      rem /= a.shape[d];
+      so += c * a.sstride[d];
+      dof += c * a.dstride[d];
+    }
+    ((unsigned char*)a.dst)[dof] = ((const unsigned char*)a.src)[so];
   }
 }
 

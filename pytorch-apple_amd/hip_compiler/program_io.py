@@ -27,7 +27,7 @@ import json
 import os
 import tempfile
 
-from hip_compiler.program import BufferAllocation, HIPProgram, KernelSource, LaunchStep, Ref, Storage, TView
+from hip_compiler.program import DTYPE_CODE, BufferAllocation, HIPProgram, KernelSource, LaunchStep, Ref, Storage, TView
 from npu_compiler.ir_reader import TensorSpec
 
 FORMAT, VERSION = "hipbin", 1
@@ -108,6 +108,10 @@ def program_from_dict(data: dict) -> HIPProgram:
             raise ValueError(f"{step.arg_struct} of kernel {step.kernel!r} has no fields {lost}: the program was compiled for other "
                              "kernels, compile it again")
         step.args = {k: v for k, v in step.args.items() if k in fields}
+    # bytes are copied by a kernel of their own, which k_copy once did too
+    for step in prog.steps:
+        if step.kernel == "k_copy" and step.args["sdtype"] == step.args["ddtype"] == DTYPE_CODE["uint8"]:
+            step.kernel = "k_copy_bytes"
     # k_mask_extent writes two ints per 32-query block; files written when it wrote one hold half the bytes
     for step in prog.steps:
         if step.kernel == "k_mask_extent":

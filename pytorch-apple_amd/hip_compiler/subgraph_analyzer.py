@@ -432,8 +432,9 @@ class Lowering:
                           dstride=[0] * 6, ndim=1, sdtype=DTYPE_CODE[src.dtype], ddtype=DTYPE_CODE[dst.dtype]),
                 grid=grid1d(-(-chunks // 8), cap=8192), inputs=ins, outputs=outs, params={"total": n}))
             return
+        kernel = "k_copy_bytes" if DTYPE_CODE[src.dtype] == DTYPE_CODE[dst.dtype] == DTYPE_CODE["uint8"] else "k_copy"
         self.emit(LaunchStep(
-            kind="copy", kernel="k_copy", module="basic", arg_struct="CopyArgs",
+            kind="copy", kernel=kernel, module="basic", arg_struct="CopyArgs",
             args=dict(dst=self.ref(dst), src=self.ref(src), n=n, shape=shape, sstride=ss, dstride=ds,
                       ndim=max(nd, 1), sdtype=DTYPE_CODE[src.dtype], ddtype=DTYPE_CODE[dst.dtype]),
             grid=grid1d(n), inputs=ins, outputs=outs, params={"total": n}))

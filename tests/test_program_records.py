@@ -46,3 +46,18 @@ def test_fields_that_a_saved_program_does_not_know_are_empty():
         for name in ("q_weight", "k_weight", "k_scales", "v_scales", "eps", "pad"):
             del s["args"][name]
     assert program_from_dict(data).steps[0].kernel == prog.steps[0].kernel
+
+
+def test_copies_of_bytes_saved_with_the_kernel_of_all_types_load_as_copies_of_bytes():
+    from irgen.builder import IRBuilder
+
+    for dtype, kernel in (("uint8", "k_copy_bytes"), ("bool", "k_copy_bytes"), ("int32", "k_copy"), ("bfloat16", "k_copy")):
+        b = IRBuilder("Turned")
+        x = b.op("aten.permute.default", [b.input("x", [3, 5], dtype)], {"dims": [1, 0]})
+        b.output(b.op("aten.contiguous.default", [x]))
+        prog = compile_subgraph(b.to_dict())
+        assert [s.kernel for s in prog.steps] == [kernel]
+        data = program_to_dict(prog)
+        for s in _steps(data):
+            s["kernel"] = "k_copy"
+        assert program_from_dict(data) == prog
